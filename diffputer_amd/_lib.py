@@ -17,6 +17,8 @@ DP_DTYPE_BF16 = 1
 DP_ACCUMULATE = 1
 DP_NO_FINAL_LEVEL = 2
 DP_STATIC_SCRATCH_BYTES = 32 << 20
+DP_NORM_MAX = 0
+DP_NORM_L2 = 2
 
 # every symbol include/diffputer.h declares: (restype, argtypes)
 _vp, _i, _i64, _u64, _u32, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_uint32, C.c_float, C.c_size_t
@@ -45,6 +47,13 @@ SIGNATURES = {
     "dp_masked_errors": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
     "dp_mstep_workspace_bytes": (_sz, [_i, _i, _i64]),
     "dp_mstep_fwd_bwd": (_i, [_i, _i, _i64, _vp, _vp, _vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), _vp, _vp, _vp, _sz, _vp]),
+    "dp_gated_linear_pre_bytes": (_sz, [_i64, _i]),
+    "dp_gated_linear_workspace_bytes": (_sz, [_i, _i64, _i, _i, _i]),
+    "dp_gated_linear": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
+    "dp_gated_linear_bwd": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
+    "dp_grad_workspace_bytes": (_sz, [_i]),
+    "dp_grad_norm": (_i, [_i, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(_i), _i, _vp, _vp, _sz, _vp]),
+    "dp_clip_grads": (_i, [_i, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(_i), _i, _f, _vp, _vp, _sz, _vp]),
     "dp_noise_field": (_i, [_vp, _i64, _i, _u64, _u64, _i, _u32, _i, _vp]),
 }
 

@@ -1,0 +1,322 @@
+// Gated projection h = act(x Wg^T + bg) * (x Wu^T + bu) and its backward: the three products that carry it, and the
+// elementwise passes between them.
+//
+//   forward   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u                  x [M, K], W [N, K], h [M, N]
+//   backward  du = dh act(g), dg = dh u act'(g)                               (k_gated_dgu, with the column sums for db)
+//             dx = dg Wg + du Wu          one product over a contraction of 2 N
+//             dWg = dg^T x, dWu = du^T x  two products over the rows
+//
+// All three are C(i, j) = sum_k A(i, k) B(j, k) with each operand either "row" laid out (k contiguous) or "column" laid
+// out (i or j contiguous, as a transposed product finds its operands in memory).
+#pragma once
+#include "dp_util.h"
+
+namespace dp {
+
+enum { GL_FWD = 0, GL_DX = 1, GL_DW = 2 };
+enum { GL_ACT_NONE = 0, GL_ACT_SILU = 1, GL_ACT_GELU = 2 };
+
+// ---- scalar types --------------------------------------------------------------------------------------------------
+template <typename T> struct GlType;
+template <> struct GlType<float> {
+    static __device__ __forceinline__ float get(float v) { return v; }
+    static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct GlType<bf16_t> {
+    static __device__ __forceinline__ float get(bf16_t v) { return bf2f(v); }
+    static __device__ __forceinline__ bf16_t put(float v) { return f2bf(v); }
+};
+
+// ---- activations, float32 ------------------------------------------------------------------------------------------
+// silu(g) = g s(g), s = 1 / (1 + e^-g): e^-g overflows to inf below -88, where s is 0 and the product the right -0;
+// gelu(g) = g Phi(g), Phi = erfc(-g / sqrt 2) / 2 (erfc keeps the relative accuracy of the left tail that 1 + erf loses).
+// At g = -inf both products are 0 * inf = NaN; plain torch expressions give the same.
+__device__ __forceinline__ float gl_sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+__device__ __forceinline__ float gl_phi(float g) { return 0.5f * erfcf(-0.70710678118654752f * g); }
+__device__ __forceinline__ float gl_act(int act, float g) {
+    if (act == GL_ACT_SILU) return g * gl_sigmoid(g);
+    if (act == GL_ACT_GELU) return g * gl_phi(g);
+    return g;
+}
+__device__ __forceinline__ void gl_act_grad(int act, float g, float& a, float& da) {
+    if (act == GL_ACT_SILU) {
+        const float s = gl_sigmoid(g);
+        a = g * s;
+        da = s * (1.0f + g * (1.0f - s));
+    } else if (act == GL_ACT_GELU) {
+        const float p = gl_phi(g);
+        a = g * p;
+        da = p + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    } else {
+        a = g;
+        da = 1.0f;
+    }
+}
+
+// ---- operands ------------------------------------------------------------------------------------------------------
+// row layout:    element (i, k) at p[i * ld + k]     (k contiguous)
+// column layout: element (i, k) at p[k * ld + i]     (i contiguous)
+struct GlOp {
+    const void* p;
+    int64_t ld;
+};
+
+// One product launch.  GL_FWD: A = x (row), B[0] / B[1] = Wg / Wu (row): columns 0..n-1 of the gate and of the up product.
+// GL_DX: A[s] = dg / du planes (row), B[s] = Wg / Wu (column), s = contraction segment.  GL_DW: A[z] = dg / du plane
+// (column), B[0] = x (column), z = which weight.
+// Split launches (splits > 1): slice s takes K-tiles [s, s + 1) * kt_per of the contraction and writes float32 sums to
+// part[s][plane][rows][ldp]; k_gated_join adds the slices in order, so results do not depend on timing.
+struct GlArgs {
+    GlOp A[2], B[2];
+    int64_t I;                 // rows of C
+    int J;                     // columns of C (of one plane)
+    int64_t C;                 // contraction length of one segment
+    int kt_per, splits;        // K-tiles per slice, slices
+    int zfirst;                // GL_DW: first plane of this launch (planes = gridDim.z / splits)
+    // outputs
+    void* out[2];              // GL_FWD: h in out[0]; GL_DX: dx; GL_DW: dWg, dWu
+    int64_t ldo;
+    float* part;               // split launches: partial sums
+    int64_t ldp;
+    float* pre;                // GL_FWD, training: g plane, then u plane, [M][ldpre] float32
+    int64_t ldpre;
+    const void* bias[2];
+    int act;
+};
+
+template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs& p, int64_t m, int n, int cnt, const float* g, const float* u) {
+    T* const h = (T*)p.out[0] + m * p.ldo + n;
+    for (int r = 0; r < cnt; ++r) {
+        float gv = g[r], uv = u[r];
+        if (p.bias[0]) gv += GlType<T>::get(((const T*)p.bias[0])[n + r]);
+        if (p.bias[1]) uv += GlType<T>::get(((const T*)p.bias[1])[n + r]);
+        if (p.pre) {
+            p.pre[m * p.ldpre + n + r] = gv;
+            p.pre[(p.I + m) * p.ldpre + n + r] = uv;
+        }
+        h[r] = GlType<T>::put(gl_act(p.act, gv) * uv);
+    }
+}
+
+// ---- general product: any size, stride and alignment ------------------------------------------------------------------
+// 64 x 64 x 32 tile, 4 waves of 32 x 32, operands through registers into LDS as [row][k] (element loads with bounds checks).
+// GL_FWD: columns 0..31 of the tile are 32 gate columns, 32..63 the up columns of the same places, so that one lane ends
+// with g and u of the same elements.
+constexpr int GG_T = 64, GG_K = 32;
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
+    constexpr bool BF = sizeof(T) == 2;
+    constexpr int LD = BF ? GG_K + 8 : GG_K + 1;
+    constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
+    __shared__ __attribute__((aligned(16))) T sa[GG_T * LD];
+    __shared__ __attribute__((aligned(16))) T sb[GG_T * LD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    const int64_t i0 = (int64_t)blockIdx.x * GG_T;
+    const int j0 = blockIdx.y * (MODE == GL_FWD ? GG_T / 2 : GG_T);
+    const int slice = blockIdx.z % p.splits, plane = p.zfirst + blockIdx.z / p.splits;
+    const int segs = MODE == GL_DX ? 2 : 1;
+    const int64_t nk = ceil_div<int64_t>(p.C, GG_K);
+    const int64_t kt0 = (int64_t)slice * p.kt_per, kt1 = kt0 + p.kt_per < nk * segs ? kt0 + p.kt_per : nk * segs;
+
+    T ra[8], rb[8];
+    auto load8 = [&](T* r, const T* src, int64_t valid) {          // `valid` of the 8 elements exist
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = e < valid ? src[e] : (T)0;
+    };
+    // row layout: thread = (row tid / 4, 8 k's from (tid % 4) * 8); column layout: thread = (k tid / 8, 8 rows from (tid % 8) * 8)
+    auto fetch = [&](int64_t kt) {
+        const int seg = kt >= nk ? 1 : 0;
+        const int64_t k0 = (kt - seg * nk) * GG_K;
+        const GlOp A = p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
+        if (A_ROW) {
+            const int64_t i = i0 + (tid >> 2), k = k0 + (tid & 3) * 8;
+            load8(ra, (const T*)A.p + i * A.ld + k, i < p.I ? p.C - k : 0);
+        } else {
+            const int64_t k = k0 + (tid >> 3), i = i0 + (tid & 7) * 8;
+            load8(ra, (const T*)A.p + k * A.ld + i, k < p.C ? p.I - i : 0);
+        }
+        if (B_ROW) {
+            const int row = tid >> 2, half = row >> 5;
+            const int64_t j = j0 + (row & 31), k = k0 + (tid & 3) * 8;
+            load8(rb, (const T*)p.B[half].p + j * p.B[half].ld + k, j < p.J ? p.C - k : 0);
+        } else {
+            const GlOp B = p.B[MODE == GL_DX ? seg : 0];
+            const int64_t k = k0 + (tid >> 3);
+            const int j = j0 + (tid & 7) * 8;
+            load8(rb, (const T*)B.p + k * B.ld + j, k < p.C ? p.J - j : 0);
+        }
+    };
+    auto put8 = [&](T* s, const T* r, bool row) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (row) s[(tid >> 2) * LD + (tid & 3) * 8 + e] = r[e];
+            else s[((tid & 7) * 8 + e) * LD + (tid >> 3)] = r[e];
+        }
+    };
+
+    f32x4 acc[2][2];                                               // [m-tile][column half]
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (kt0 < kt1) fetch(kt0);
+    for (int64_t kt = kt0; kt < kt1; ++kt) {
+        __syncthreads();
+        put8(sa, ra, A_ROW);
+        put8(sb, rb, B_ROW);
+        __syncthreads();
+        if (kt + 1 < kt1) fetch(kt + 1);
+        const int r = lane & 15, q = lane >> 4;
+        if constexpr (BF) {
+            bf16x8 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = *(const bf16x8*)&sa[(wm * 32 + i * 16 + r) * LD + q * 8];
+                b[i] = *(const bf16x8*)&sb[(i * 32 + wn * 16 + r) * LD + q * 8];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < GG_K / 4; ++kk) {
+                float a[2], b[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    a[i] = sa[(wm * 32 + i * 16 + r) * LD + kk * 4 + q];
+                    b[i] = sb[(i * 32 + wn * 16 + r) * LD + kk * 4 + q];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j], a[i], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+    // lane: row (lane & 15) of each 16 x 16 tile, columns 4 (lane >> 4) + 0..3
+    const int cl = wn * 16 + (lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t m = i0 + wm * 32 + i * 16 + (lane & 15);
+        if (m >= p.I) continue;
+        if (MODE == GL_FWD && p.splits == 1) {
+            const int n = j0 + cl, cnt = p.J - n < 4 ? p.J - n : 4;
+            float g[4], u[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) { g[r] = acc[i][0][r]; u[r] = acc[i][1][r]; }
+            if (cnt > 0) gl_fwd_store<T>(p, m, n, cnt, g, u);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int n = j0 + (MODE == GL_FWD ? 0 : j * 32) + cl;
+            const int pl = MODE == GL_FWD ? j : MODE == GL_DW ? plane : 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n + r < p.J) {
+                    if (p.splits > 1) p.part[(((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n + r] = acc[i][j][r];
+                    else ((T*)p.out[pl])[m * p.ldo + n + r] = GlType<T>::put(acc[i][j][r]);
+                }
+        }
+    }
+}
+
+// Joins the slices of a split launch, in order: 4 columns of one row per thread.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void k_gated_join(GlArgs p, int planes) {
+    const int64_t per_row = ceil_div(p.J, 4), rows = p.I * planes, total = rows * per_row;
+    const int64_t stride = 2 * p.I * p.ldp;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+        const int64_t row = t / per_row;
+        const int n = (int)(t - row * per_row) * 4, cnt = p.J - n < 4 ? p.J - n : 4;
+        const int pl = p.zfirst + (int)(row / p.I);
+        const int64_t m = row % p.I;
+        const float* a = p.part + ((int64_t)pl * p.I + m) * p.ldp + n;
+        f32x4 s0 = *(const f32x4*)a, s1 = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const float* b = a + p.I * p.ldp;                          // GL_FWD: the up plane
+        if (MODE == GL_FWD) s1 = *(const f32x4*)b;
+        for (int s = 1; s < p.splits; ++s) {
+            s0 += *(const f32x4*)(a + s * stride);
+            if (MODE == GL_FWD) s1 += *(const f32x4*)(b + s * stride);
+        }
+        if (MODE == GL_FWD) {
+            float g[4] = {s0[0], s0[1], s0[2], s0[3]}, u[4] = {s1[0], s1[1], s1[2], s1[3]};
+            gl_fwd_store<T>(p, m, n, cnt, g, u);
+        } else {
+            for (int r = 0; r < cnt; ++r) ((T*)p.out[pl])[m * p.ldo + n + r] = GlType<T>::put(s0[r]);
+        }
+    }
+}
+
+// ---- backward, elementwise: du = dh act(g), dg = dh u act'(g), and their column sums ------------------------------------
+// Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows.  dgu: two planes [M][ldg] of T, columns N..ldg - 1
+// zero.  colpart: NULL, or [row block][2][ldg] float32 sums of the unrounded values, joined by k_gated_colsum.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_dgu(const float* pre, int64_t ldpre, const T* dh, int64_t lddh, T* dgu, int64_t ldg,
+                                                   float* colpart, int64_t M, int N, int act, int tx, int rows) {
+    __shared__ f32x4 red[2][256];
+    const int cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
+    const int n = (blockIdx.x * tx + cx) * 4;
+    const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = r0 + rows < M ? r0 + rows : M;
+    f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
+    if (n < ldg) {
+        for (int64_t m = r0 + ry; m < r1; m += ty) {
+            f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
+            if (n < N) {
+                const f32x4 g = *(const f32x4*)(pre + m * ldpre + n), u = *(const f32x4*)(pre + (M + m) * ldpre + n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < N) {
+                        const float d = GlType<T>::get(dh[m * lddh + n + e]);
+                        float a, da;
+                        gl_act_grad(act, g[e], a, da);
+                        du[e] = d * a;
+                        dg[e] = d * u[e] * da;
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dgu[m * ldg + n + e] = GlType<T>::put(dg[e]);
+                dgu[(M + m) * ldg + n + e] = GlType<T>::put(du[e]);
+            }
+            sg += dg;
+            su += du;
+        }
+    }
+    if (colpart == nullptr) return;
+    red[0][threadIdx.x] = sg;
+    red[1][threadIdx.x] = su;
+    __syncthreads();
+    if (ry == 0 && n < ldg) {
+        for (int k = 1; k < ty; ++k) {
+            sg += red[0][k * tx + cx];
+            su += red[1][k * tx + cx];
+        }
+        float* c = colpart + (int64_t)blockIdx.y * 2 * ldg + n;
+        *(f32x4*)c = sg;
+        *(f32x4*)(c + ldg) = su;
+    }
+}
+
+// db[n] = sum of the row blocks' partial sums: 64 columns x 4 lanes per block, lanes joined in order
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_colsum(const float* colpart, int nblk, int64_t ldg, T* dbg, T* dbu, int N) {
+    __shared__ float red[4][64];
+    const int c = threadIdx.x & 63, y = threadIdx.x >> 6;
+    const int n = blockIdx.x * 64 + c, pl = blockIdx.y;
+    float s = 0.f;
+    if (n < N)
+        for (int b = y; b < nblk; b += 4) s += colpart[((int64_t)b * 2 + pl) * ldg + n];
+    red[y][c] = s;
+    __syncthreads();
+    T* const out = pl ? dbu : dbg;
+    if (y == 0 && n < N && out) out[n] = GlType<T>::put(red[0][c] + red[1][c] + red[2][c] + red[3][c]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_zero(T* a, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) a[i] = (T)0;
+}
+
+}  // namespace dp

@@ -1,0 +1,142 @@
+// Global norm of many gradient tensors, and clipping by it.
+//
+//   norm = sqrt(sum over tensors and elements of g^2)   or   max |g|
+//   coef = min(1, limit / (norm + 1e-6)),  g <- g coef  (in place; nothing is written when coef is 1)
+//
+// Two passes over memory: k_grad_norm leaves one partial per workgroup, k_grad_clip reduces the partials (each workgroup
+// for itself, in one fixed order: same bits everywhere) and scales.  Squares and sums are held in float64: a square of any
+// float32 is then exact to 53 bits and neither overflows nor vanishes, and the float64 pipes are idle in a kernel that
+// waits for memory.
+#pragma once
+#include "dp_util.h"
+
+namespace dp {
+
+// One tensor of the table that travels in the kernel's arguments (no upload, nothing a captured graph could outlive).
+struct GradEntry {
+    uint64_t base;             // address rounded down to 16
+    uint64_t bytes;            // from `base` to the end of the tensor
+    uint32_t chunk0;           // first chunk of this tensor
+    uint16_t head;             // bytes between `base` and the first element (< 16)
+    uint16_t bf16;             // element type: 1 = bf16, 0 = float32
+};
+constexpr int GN_MAX = 160;    // entries per launch: 24 bytes each, under the 4 KiB of kernel arguments
+struct GradTable {
+    int n;
+    uint32_t chunks;
+    GradEntry e[GN_MAX];
+};
+constexpr int GN_CHUNK = 32768;                                  // bytes of one chunk: 8 loads of 16 bytes per thread
+constexpr int GN_THREADS = 256;
+constexpr int GN_MAX_BLOCKS = 1024;                              // partials of one launch
+
+// the entry that holds chunk c: entries are in the order of their first chunk
+__device__ __forceinline__ int gn_find(const GradTable& t, uint32_t c) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.e[mid].chunk0 <= c) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double gn_join(int inf, double a, double b) {
+    if (!inf) return a + b;
+    return (b > a || b != b) ? b : a;                            // NaN wins
+}
+__device__ __forceinline__ void gn_take(int inf, double& a, float v) {
+    if (!inf) a = fma((double)v, (double)v, a);
+    else a = gn_join(1, a, (double)fabsf(v));
+}
+
+// sum (or maximum) over the workgroup, valid in every thread
+__device__ __forceinline__ double gn_block(int inf, double v, double* red) {
+    for (int o = 32; o; o >>= 1) v = gn_join(inf, v, __shfl_xor(v, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < GN_THREADS / 64; ++w) v = gn_join(inf, v, red[w]);
+    return v;
+}
+
+__global__ __launch_bounds__(GN_THREADS) void k_grad_norm(GradTable t, double* part, int inf) {
+    __shared__ double red[GN_THREADS / 64];
+    double a = 0.0;
+    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+        const GradEntry e = t.e[gn_find(t, c)];
+        const uint64_t off0 = (uint64_t)(c - e.chunk0) * GN_CHUNK;
+        const char* const base = (const char*)e.base;
+        const int es = e.bf16 ? 2 : 4;
+#pragma unroll 8
+        for (int v = 0; v < GN_CHUNK / 16 / GN_THREADS; ++v) {
+            const uint64_t o = off0 + (uint64_t)(v * GN_THREADS + threadIdx.x) * 16;
+            if (o >= e.head && o + 16 <= e.bytes) {
+                const uint4 q = *(const uint4*)(base + o);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (e.bf16) {
+                        gn_take(inf, a, __builtin_bit_cast(float, w[k] << 16));
+                        gn_take(inf, a, __builtin_bit_cast(float, w[k] & 0xffff0000u));
+                    } else gn_take(inf, a, __builtin_bit_cast(float, w[k]));
+                }
+            } else {
+                for (uint64_t b = o < e.head ? e.head : o; b < o + 16 && b < e.bytes; b += es)
+                    gn_take(inf, a, e.bf16 ? bf2f(*(const bf16_t*)(base + b)) : *(const float*)(base + b));
+            }
+        }
+    }
+    a = gn_block(inf, a, red);
+    if (threadIdx.x == 0) part[blockIdx.x] = a;
+}
+
+__device__ __forceinline__ double gn_total(const double* part, int nparts, int inf, double* red) {
+    double a = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += GN_THREADS) a = gn_join(inf, a, part[i]);
+    a = gn_block(inf, a, red);
+    return inf ? a : sqrt(a);
+}
+
+__global__ __launch_bounds__(GN_THREADS) void k_grad_total(const double* part, int nparts, int inf, float* norm) {
+    __shared__ double red[GN_THREADS / 64];
+    const double total = gn_total(part, nparts, inf, red);
+    if (threadIdx.x == 0) *norm = (float)total;
+}
+
+__global__ __launch_bounds__(GN_THREADS) void k_grad_clip(GradTable t, const double* part, int nparts, int inf, float limit, float* norm) {
+    __shared__ double red[GN_THREADS / 64];
+    const double total = gn_total(part, nparts, inf, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+    const double cd = (double)limit / (total + 1e-6);
+    if (cd >= 1.0) return;                                       // within the limit (a NaN coefficient goes on, and marks every element)
+    const float coef = (float)cd;
+    if (coef == 1.0f) return;
+    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+        const GradEntry e = t.e[gn_find(t, c)];
+        const uint64_t off0 = (uint64_t)(c - e.chunk0) * GN_CHUNK;
+        char* const base = (char*)e.base;
+        const int es = e.bf16 ? 2 : 4;
+#pragma unroll 8
+        for (int v = 0; v < GN_CHUNK / 16 / GN_THREADS; ++v) {
+            const uint64_t o = off0 + (uint64_t)(v * GN_THREADS + threadIdx.x) * 16;
+            if (o >= e.head && o + 16 <= e.bytes) {
+                uint4 q = *(const uint4*)(base + o);
+                uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (e.bf16) w[k] = pack_bf16x2(__builtin_bit_cast(float, w[k] << 16) * coef, __builtin_bit_cast(float, w[k] & 0xffff0000u) * coef);
+                    else w[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[k]) * coef);
+                }
+                *(uint4*)(base + o) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                for (uint64_t b = o < e.head ? e.head : o; b < o + 16 && b < e.bytes; b += es) {
+                    if (e.bf16) *(bf16_t*)(base + b) = f2bf(bf2f(*(const bf16_t*)(base + b)) * coef);
+                    else *(float*)(base + b) *= coef;
+                }
+            }
+        }
+    }
+}
+
+}  // namespace dp

@@ -15,18 +15,25 @@ from dataclasses import dataclass, field
 import torch
 
 from . import estep, formats, prep
+from .grads import clip_grads
 from .model import MLPDiffusion, Model
 
 
 def m_step(train_data: torch.Tensor, hid_dim: int, *, max_epochs: int = 10001, batch_size: int = 4096, lr: float = 1e-4,
-           patience: int = 500, generator: torch.Generator | None = None, log=None, native: bool | None = None):
+           patience: int = 500, generator: torch.Generator | None = None, log=None, native: bool | None = None,
+           max_grad_norm: float | None = None):
     """main.py:92-152: a FRESH MLPDiffusion each EM iteration, Adam(lr 1e-4), ReduceLROnPlateau(0.9, 50), shuffled batches of
     4096, best-epoch-loss checkpoint, early stop after `patience` epochs without improvement.  Returns (model with the best
     weights loaded, best loss).  `train_data` [N, D] float32 on the training device.
 
     native: loss and gradients of a batch from the HIP training step (`mstep.NativeTrainStep`, dp_mstep_fwd_bwd: bf16 hi/lo
     split GEMMs, ~1e-5 of float32 autograd, 1.7-1.8x its speed at H = 1024 / batch 4096) instead of PyTorch autograd; the draws,
-    Adam and the scheduler stay PyTorch's.  Default (None): native on a CUDA device, autograd on CPU."""
+    Adam and the scheduler stay PyTorch's.  Default (None): native on a CUDA device, autograd on CPU.
+
+    max_grad_norm: clip every batch's gradients by their global norm before Adam's step (`grads.clip_grads` where the training
+    step is native, torch.nn.utils.clip_grad_norm_ elsewhere; no counterpart in the reference).  None (default): no clipping."""
+    if max_grad_norm is not None and not max_grad_norm >= 0.0:
+        raise ValueError(f"max_grad_norm has to be a number of at least 0, got {max_grad_norm}")
     dev = train_data.device
     n, d = train_data.shape
     model = Model(denoise_fn=MLPDiffusion(d, hid_dim), hid_dim=d).to(dev)
@@ -47,10 +54,14 @@ def m_step(train_data: torch.Tensor, hid_dim: int, *, max_epochs: int = 10001, b
             x = train_data[perm[b0:b0 + batch_size]]
             if step is not None:
                 loss = step.loss_and_grads(x)              # overwrites every .grad: zero_grad + backward in one call
+                if max_grad_norm is not None:
+                    clip_grads([p.grad for p in step.params], max_grad_norm)
             else:
                 loss = model(x).mean()
                 opt.zero_grad(set_to_none=True)
                 loss.backward()
+                if max_grad_norm is not None:
+                    torch.nn.utils.clip_grad_norm_(model.parameters(), max_grad_norm)
             opt.step()
             tot += loss.detach() * x.shape[0]              # accumulated on the device: one host sync per epoch, not per batch
         cur = float(tot) / n
@@ -120,11 +131,13 @@ class EMResult:
 
 def run_em(X, mask_train, X_test=None, mask_test=None, *, hid_dim: int = 1024, max_iter: int = 10, num_trials: int = 20,
            num_steps: int = 50, device="cuda:0", ckpt_dir: str | None = None, max_epochs: int = 10001, dtype: str | None = None,
-           seed: int = 0, num_num: int | None = None, oos_drop_rows=None, log=print, native_mstep: bool | None = None) -> EMResult:
+           seed: int = 0, num_num: int | None = None, oos_drop_rows=None, log=print, native_mstep: bool | None = None,
+           max_grad_norm: float | None = None) -> EMResult:
     """X, X_test: normalised tables ((x - mean)/std/2, main.py:58,61) holding the TRUE values (used for scoring only, like the
     reference); masks True = missing.
     `oos_drop_rows`: rows of the test table left out of its score (news: [6265], dataset.py:194-197).
     `native_mstep`: see `m_step(native=...)`; None = the HIP training step on a CUDA device, PyTorch autograd on CPU.
+    `max_grad_norm`: see `m_step(max_grad_norm=...)`; None = no clipping, as in the reference.
 
     Under torch.distributed (every rank calls this with the same tables): the M-step runs on rank 0 only -- the reference
     has ONE trainer and GPU training is not bit-reproducible across ranks -- and its best weights are broadcast, so every
@@ -143,7 +156,7 @@ def run_em(X, mask_train, X_test=None, mask_test=None, *, hid_dim: int = 1024, m
     for it in range(max_iter):
         log(f"EM iteration {it}: M-step on {tuple(train_data.shape)}")
         if rank == 0:
-            model, loss = m_step(train_data, hid_dim, max_epochs=max_epochs, generator=gen, log=log, native=native_mstep)
+            model, loss = m_step(train_data, hid_dim, max_epochs=max_epochs, generator=gen, log=log, native=native_mstep, max_grad_norm=max_grad_norm)
         else:
             model, loss = Model(denoise_fn=MLPDiffusion(X.shape[1], hid_dim), hid_dim=X.shape[1]).to(dev).eval(), 0.0
         if distributed:

@@ -272,6 +272,53 @@ int dp_mstep_fwd_bwd(int d_in, int hid, int64_t batch, const float* x, const flo
 int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t row_offset, int trial,
                    uint32_t block, int comp, void* stream);
 
+/*
+ * Gated projection  h = act(x Wg^T + bg) * (x Wu^T + bu):  both products, the activation and the gating in one kernel; the
+ * gated counterpart of dp_linear's act(A W^T + bias) for denoisers built from gated layers.  No counterpart in the reference.
+ *   dtype        DP_DTYPE_BF16 or DP_DTYPE_F32: type of x, w, b, h, dh and of every gradient.  Sums are float32.
+ *   x  [M, K]    row stride ldx elements (>= K);  w_gate, w_up [N, K], row stride ldw (>= K);  b_gate, b_up [N] or NULL
+ *   h  [M, N]    row stride ldh (>= N)
+ *   act          0 = none, 1 = SiLU, 2 = GELU (g Phi(g), not its tanh approximation); a NaN of x or w reaches every element that depends on it
+ *   pre          NULL, or dp_gated_linear_pre_bytes(M, N) bytes (16-byte aligned) that receive both projections in float32
+ *                for the backward pass; the layout is the library's own
+ * Any strides, element-aligned pointers, 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
+ * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
+ * (workspace >= dp_gated_linear_workspace_bytes(.., backward), 256-byte aligned; calls that may overlap in time need
+ * workspaces of their own), and may be captured into a graph.
+ *
+ * dp_gated_linear_bwd: gradients for a given dh [M, N] (row stride lddh).  dx [M, K], dw_gate, dw_up [N, K], db_gate,
+ * db_up [N]: contiguous, overwritten, each may be NULL (not wanted).  M = 0 writes zeros to the weights' gradients.
+ * bf16: dg and du are rounded to bf16 once, as the operands of the three products; bias gradients sum them unrounded.
+ */
+size_t dp_gated_linear_pre_bytes(int64_t M, int N);
+size_t dp_gated_linear_workspace_bytes(int dtype, int64_t M, int N, int K, int backward);
+int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
+                    void* h, int64_t ldh, void* pre, int64_t M, int N, int K, int act, void* workspace, size_t workspace_bytes, void* stream);
+int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,
+                        void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up, int64_t M, int N, int K, int act,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Global norm of n gradient tensors and clipping by it, between the M-step's backward pass and its optimiser step.  No
+ * counterpart in the reference (its M-step does not clip, main.py:124-133).
+ *   g[i], numel[i], dtype[i]   contiguous device tensors (element-aligned; HOST arrays of n entries, read before the call
+ *                              returns); tensors of zero elements and n = 0 are allowed
+ *   norm_type                  DP_NORM_L2: sqrt of the sum of all squares; DP_NORM_MAX: largest absolute value
+ *   norm                       one float32 on the device.  Sums are float64; NaN and infinities propagate.
+ * dp_clip_grads multiplies every tensor in place by min(1, limit / (norm + 1e-6)) (float32 product, rounded to the tensor's
+ * type) and returns the norm from before; nothing is written when the coefficient is 1.  limit >= 0.  A norm of +inf gives
+ * the coefficient 0, a NaN makes every element NaN.  Tensors that share memory are refused (DP_EINVAL).
+ * Deterministic, asynchronous on `stream`, allocates nothing on the device (workspace >= dp_grad_workspace_bytes(n), 8-byte
+ * aligned), may be captured into a graph (the pointers are part of the captured launches).
+ */
+#define DP_NORM_MAX 0
+#define DP_NORM_L2  2
+size_t dp_grad_workspace_bytes(int n);
+int dp_grad_norm(int n, const void* const* g, const int64_t* numel, const int* dtype, int norm_type, float* norm,
+                 void* workspace, size_t workspace_bytes, void* stream);
+int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, float limit, float* norm,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,422 @@
+"""The gated projection (`diffputer_amd.gated`, dp_gated_linear / dp_gated_linear_bwd) on the GPU against its formulas in float64.
+
+Tolerances are componentwise bounds, worked out from the inputs:  a float32 sum of k products is off by at most
+gamma(k) = 2 (k + 4) 2^-24 times the sum of the absolute products (2: the matrix pipes may round inside a step of their
+own), an elementary function or a rounding in float32 by 2^-22 of its value, and a rounding to the tensor's type by
+eps / 2 of it (bf16 2^-8).  |silu'| <= 1.1, |gelu'| <= 1.13, |silu''| <= 0.5, |gelu''| <= 0.8.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F8 = torch.float64
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+E32 = 2.0 ** -22
+TINY = 1e-30
+A1, A2 = 1.13, 0.8
+
+
+def gamma(k):
+    return 2 * (k + 4) * 2.0 ** -24
+
+
+def half_step(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def act_of(g, act):
+    """act(g), act'(g) in float64"""
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if act == "gelu":
+        p = 0.5 * torch.erfc(-g / math.sqrt(2))
+        return g * p, p + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    return g, torch.ones_like(g)
+
+
+def make(M, K, N, dtype, bias=True, seed=0, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    dt = DT[dtype]
+    x = (torch.randn(M, K, generator=gen) * scale).to(dt)
+    w = [(torch.randn(N, K, generator=gen) / math.sqrt(K)).to(dt) for _ in range(2)]
+    b = [torch.randn(N, generator=gen).to(dt) if bias else None for _ in range(2)]
+    dh = torch.randn(M, N, generator=gen).to(dt)
+    return x, w[0], w[1], b[0], b[1], dh
+
+
+class Ref:
+    """Formulas and error bounds in float64 on the CPU."""
+
+    def __init__(self, x, wg, wu, bg, bu, dh, act):
+        dt = x.dtype
+        u_t = half_step(dt)
+        mix = u_t if dt == torch.bfloat16 else 0.0                # dg, du are rounded to bf16 as operands
+        x, wg, wu, dh = (t.detach().cpu().to(F8) for t in (x, wg, wu, dh))
+        N, K = wg.shape
+        M = x.shape[0]
+        zero = torch.zeros(N, dtype=F8)
+        bg, bu = (zero if b is None else b.detach().cpu().to(F8) for b in (bg, bu))
+        g, u = x @ wg.T + bg, x @ wu.T + bu
+        eg, eu = (gamma(K) * (x.abs() @ w.abs().T + b.abs()) for w, b in ((wg, bg), (wu, bu)))
+        a, da = act_of(g, act)
+        ea = A1 * eg + E32 * a.abs()
+        self.h = a * u
+        self.eh = ea * (u.abs() + eu) + a.abs() * eu + (E32 + u_t) * self.h.abs() * 1.01 + TINY
+        du, dg = dh * a, dh * u * da
+        edu = dh.abs() * ea + E32 * du.abs()
+        edg = dh.abs() * (eu * A1 + (u.abs() + eu) * (A2 * eg + 2 * E32 * A1)) + 2 * E32 * dg.abs()
+        rdu, rdg = edu + mix * (du.abs() + edu), edg + mix * (dg.abs() + edg)      # as operands of the products
+        self.dx = dg @ wg + du @ wu
+        mag = (dg.abs() + rdg) @ wg.abs() + (du.abs() + rdu) @ wu.abs()
+        self.edx = rdg @ wg.abs() + rdu @ wu.abs() + gamma(2 * N) * mag + u_t * (self.dx.abs() + rdg @ wg.abs() + rdu @ wu.abs()) + TINY
+        for name, d, r, e in (("g", dg, rdg, edg), ("u", du, rdu, edu)):
+            v = d.T @ x
+            err = r.T @ x.abs() + gamma(M) * ((d.abs() + r).T @ x.abs())
+            setattr(self, "dw" + name, v)
+            setattr(self, "edw" + name, err + u_t * (v.abs() + err) + TINY)
+            s = d.sum(0)
+            err = e.sum(0) + gamma(M) * (d.abs() + e).sum(0)
+            setattr(self, "db" + name, s)
+            setattr(self, "edb" + name, err + u_t * (s.abs() + err) + TINY)
+
+
+def close(got, want, bound, what):
+    assert tuple(got.shape) == tuple(want.shape), (what, got.shape, want.shape)
+    off = (got.detach().cpu().to(F8) - want).abs()
+    assert torch.isfinite(got.detach().cpu().to(F8)).all(), what
+    worst = float((off / bound).max()) if off.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the bound"
+
+
+def check(x, wg, wu, bg, bu, dh, act, train=True):
+    from diffputer_amd.gated import gated_linear
+    ref = Ref(x, wg, wu, bg, bu, dh, act)
+    dev = [None if t is None else t.to(DEV) for t in (x, wg, wu, bg, bu)]
+    close(gated_linear(*dev, act=act), ref.h, ref.eh, "h")
+    if not train:
+        return
+    leaves = [None if t is None else t.requires_grad_() for t in dev]
+    h = gated_linear(*leaves, act=act)
+    close(h, ref.h, ref.eh, "h (training)")
+    given = [t for t in leaves if t is not None]
+    grads = iter(torch.autograd.grad(h, given, dh.to(DEV)))
+    for name in ("x", "wg", "wu", "bg", "bu"):
+        if {"bg": bg, "bu": bu}.get(name, x) is not None:
+            g = next(grads)
+            assert g.dtype == x.dtype
+            close(g, getattr(ref, "d" + name), getattr(ref, "ed" + name), "d" + name)
+
+
+SIZES = [  # M, K, N
+    (1, 1, 1), (1, 64, 64), (1, 256, 520), (2, 7, 3), (3, 8, 16), (15, 9, 64), (16, 64, 32), (17, 65, 33), (31, 130, 31),
+    (33, 72, 100), (64, 128, 128), (65, 63, 129), (100, 200, 65), (130, 320, 260), (257, 100, 40), (300, 33, 257), (1000, 16, 8),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_against_formula(M, K, N, dtype):
+    check(*make(M, K, N, dtype, seed=M * 7 + K + N), act="silu")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("act", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_activations_and_bias(act, bias, dtype):
+    check(*make(70, 96, 72, dtype, bias=bias, seed=3, scale=3.0), act=act)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(512, 1024, 768), (1024, 512, 1000), (2048, 264, 256), (700, 1030, 520)])
+def test_larger(M, K, N, dtype):
+    check(*make(M, K, N, dtype, seed=5), act="silu")
+
+
+def test_one_bias_only():
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = make(20, 40, 24, "f32", seed=8)
+    for b0, b1 in ((bg, None), (None, bu)):
+        ref = Ref(x, wg, wu, b0, b1, dh, "silu")
+        dev = [None if t is None else t.to(DEV).requires_grad_() for t in (x, wg, wu, b0, b1)]
+        h = gated_linear(*dev)
+        close(h, ref.h, ref.eh, "h")
+        given = [t for t in dev if t is not None]
+        db = torch.autograd.grad(h, given, dh.to(DEV))[-1]
+        name = "bg" if b1 is None else "bu"
+        close(db, getattr(ref, "d" + name), getattr(ref, "ed" + name), name)
+
+
+@pytest.mark.parametrize("act,at", [("silu", -200.0), ("silu", 200.0), ("silu", -20.0), ("gelu", -200.0), ("gelu", 200.0), ("gelu", -6.0), ("gelu", -13.0)])
+def test_saturated_gates(act, at):
+    """Gates far out: the exponentials overflow or vanish, values and gradients stay what the formula says."""
+    x, wg, wu, bg, bu, dh = make(40, 16, 24, "f32", seed=9)
+    bg = torch.full_like(bg, at)
+    check(x, wg, wu, bg, bu, dh, act)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_differences(dtype):
+    """The gradients against central differences of the formula in float64 along a random direction."""
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = make(33, 24, 20, dtype, seed=11)
+    ref = Ref(x, wg, wu, bg, bu, dh, "gelu")
+    leaves = [t.to(DEV).requires_grad_() for t in (x, wg, wu, bg, bu)]
+    grads = torch.autograd.grad(gated_linear(*leaves, act="gelu"), leaves, dh.to(DEV))
+    gen = torch.Generator().manual_seed(1)
+    at = [t.to(F8) for t in (x, wg, wu, bg, bu)]
+    v = [torch.randn(t.shape, generator=gen, dtype=F8) for t in at]
+
+    def loss(eps):
+        p = [t + eps * d for t, d in zip(at, v)]
+        return float((act_of(p[0] @ p[1].T + p[3], "gelu")[0] * (p[0] @ p[2].T + p[4]) * dh.to(F8)).sum())
+
+    eps = 1e-4
+    slope = (loss(eps) - loss(-eps)) / (2 * eps)
+    half = (loss(2 * eps) - loss(-2 * eps)) / (4 * eps)
+    truncation = abs(half - slope)                                  # about 3 times the error of `slope` in eps^2
+    ours = sum(float((g.cpu().to(F8) * d).sum()) for g, d in zip(grads, v))
+    bound = sum(float((getattr(ref, "ed" + n) * d.abs()).sum()) for n, d in zip(("x", "wg", "wu", "bg", "bu"), v))
+    assert abs(ours - slope) <= bound + truncation + 1e-6 * abs(slope), (ours, slope, bound, truncation)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_strides_and_layouts(dtype):
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = make(50, 72, 40, dtype, seed=13)
+    want = gated_linear(*[t.to(DEV) for t in (x, wg, wu, bg, bu)])
+    wide = torch.full((50, 100), float("nan"), dtype=x.dtype, device=DEV)
+    for off in (0, 3, 8, 28):                                       # a column range of a wider table
+        wide[:] = float("nan")
+        wide[:, off:off + 72] = x.to(DEV)
+        assert torch.equal(gated_linear(wide[:, off:off + 72], *[t.to(DEV) for t in (wg, wu, bg, bu)]), want), off
+    fused = torch.cat([wg, wu]).to(DEV)                             # both weights as halves of one tensor
+    assert torch.equal(gated_linear(x.to(DEV), fused[:40], fused[40:], bg.to(DEV), bu.to(DEV)), want)
+    pair = torch.stack([wg, wu], 1).to(DEV)                         # rows of both in turn: row stride 2 K
+    assert torch.equal(gated_linear(x.to(DEV), pair[:, 0], pair[:, 1], bg.to(DEV), bu.to(DEV)), want)
+    assert torch.equal(gated_linear(x.to(DEV), pair[:, 0], wu.to(DEV), bg.to(DEV), bu.to(DEV)), want)      # two row strides
+    assert torch.equal(gated_linear(x.t().contiguous().to(DEV).t(), *[t.to(DEV) for t in (wg, wu, bg, bu)]), want)
+    assert torch.equal(gated_linear(x.to(DEV).reshape(5, 2, 5, 72), *[t.to(DEV) for t in (wg, wu, bg, bu)]), want.reshape(5, 2, 5, 40))
+    one = gated_linear(x[0].to(DEV), *[t.to(DEV) for t in (wg, wu, bg, bu)])
+    assert one.shape == (40,)
+    row = gated_linear(x[:1].to(DEV).expand(50, 72), *[t.to(DEV) for t in (wg, wu, bg, bu)])               # one row, broadcast
+    assert torch.equal(row, row[:1].expand_as(row))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_gradients_of_broadcast_and_shared_inputs(dtype):
+    """An expanded x, one weight used as gate and as up weight, and an expanded dh (h.sum().backward())."""
+    from diffputer_amd.gated import gated_linear
+    x, w, _, b, _, _ = make(1, 24, 16, dtype, seed=14)
+    n = 5
+    xs = x.expand(n, 24)
+    ones = torch.ones(n, 16, dtype=x.dtype)
+    ref = Ref(xs, w, w, b, b, ones, "silu")
+    lx, lw, lb = (t.to(DEV).requires_grad_() for t in (x, w, b))
+    gated_linear(lx.expand(n, 24), lw, lw, lb, lb).sum().backward()
+    u = half_step(x.dtype)
+    for got, v, e in ((lx.grad, ref.dx.sum(0, keepdim=True), ref.edx.sum(0, keepdim=True)), (lw.grad, ref.dwg + ref.dwu, ref.edwg + ref.edwu),
+                      (lb.grad, ref.dbg + ref.dbu, ref.edbg + ref.edbu)):
+        close(got, v, e + 2 * n * u * (ref_abs(v) + e), "shared")   # torch adds the parts in the tensor's type
+
+
+def ref_abs(v):
+    return v.abs() + float(v.abs().max())
+
+
+def test_only_the_wanted_gradients():
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = make(30, 20, 12, "f32", seed=15)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    for i, name in enumerate(("x", "wg", "wu", "bg", "bu")):
+        dev = [t.to(DEV) for t in (x, wg, wu, bg, bu)]
+        dev[i].requires_grad_()
+        (g,) = torch.autograd.grad(gated_linear(*dev), [dev[i]], dh.to(DEV))
+        close(g, getattr(ref, "d" + name), getattr(ref, "ed" + name), name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_no_rows(dtype):
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, _ = make(3, 24, 16, dtype)
+    leaves = [t.to(DEV).requires_grad_() for t in (x[:0], wg, wu, bg, bu)]
+    h = gated_linear(*leaves)
+    assert h.shape == (0, 16)
+    grads = torch.autograd.grad(h, leaves, torch.empty_like(h))
+    assert grads[0].shape == (0, 24)
+    assert all(bool((g == 0).all()) for g in grads[1:])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(40, 72, 33), (1, 64, 64), (300, 128, 256)])
+def test_nan_and_inf_stay_in_their_rows(M, K, N, dtype):
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, _ = [t.to(DEV) for t in make(M, K, N, dtype, seed=17)]
+    want = gated_linear(x, wg, wu, bg, bu)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        y = x.clone()
+        y[M // 2, K - 1] = bad
+        h = gated_linear(y, wg, wu, bg, bu)
+        keep = torch.arange(M, device=DEV) != M // 2
+        assert torch.equal(h[keep], want[keep])
+        assert not torch.isfinite(h[M // 2]).any()
+    v = wg.clone()
+    v[N - 1, 0] = float("nan")                                      # a weight row: its column of h
+    h = gated_linear(x, v, wu, bg, bu)
+    assert torch.isnan(h[:, N - 1]).all() and torch.equal(h[:, :N - 1], want[:, :N - 1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,N", [(1, 24), (37, 33), (130, 64), (300, 264)])
+def test_nothing_beside_the_output_is_written(M, N, dtype):
+    """h as a block of a larger buffer through the C ABI: the rows behind the last one and the columns beside it stay."""
+    import ctypes as C
+
+    from diffputer_amd import _lib
+    from diffputer_amd.gated import _DTYPES, gated_linear
+    K = 40
+    x, wg, wu, bg, bu, _ = [t.to(DEV) for t in make(M, K, N, dtype, seed=19)]
+    want = gated_linear(x, wg, wu, bg, bu)
+    lib = _lib.load()
+    buf = torch.full((M + 9, N + 13), 7.0, dtype=x.dtype, device=DEV)
+    need = lib.dp_gated_linear_workspace_bytes(_DTYPES[x.dtype], M, N, K, 0)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    h = buf[3:3 + M, 5:5 + N]
+    rc = lib.dp_gated_linear(_DTYPES[x.dtype], x.data_ptr(), K, wg.data_ptr(), wu.data_ptr(), K, bg.data_ptr(), bu.data_ptr(), h.data_ptr(), N + 13, None,
+                             M, N, K, 1, ws.data_ptr(), need, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0, lib.dp_last_error()
+    assert torch.equal(h, want)
+    h.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_same_bits_twice(dtype):
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(900, 200, 136, dtype, seed=21)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+
+    def once():
+        h = gated_linear(*leaves)
+        return [h.detach(), *torch.autograd.grad(h, leaves, dh)]
+
+    first = once()
+    for _ in range(3):
+        torch.randn(1 << 20, device=DEV)
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
+
+
+def test_side_stream():
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(600, 256, 200, "bf16", seed=22)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    h = gated_linear(*leaves)
+    want = [h.detach(), *torch.autograd.grad(h, leaves, dh)]
+    del h                                                           # its graph: a leaf's accumulation node belongs to one stream
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        h = gated_linear(*leaves)
+        got = [h.detach(), *torch.autograd.grad(h, leaves, dh)]
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype,M", [("bf16", 1), ("bf16", 300), ("f32", 70)])
+def test_captured_and_replayed(dtype, M):
+    """Forward and backward in a graph, replayed with new inputs and eager work between the replays; a second graph of the
+    same operator beside it."""
+    from diffputer_amd.gated import gated_linear
+    K, N = 96, 72
+    sets = [make(M, K, N, dtype, seed=30 + i) for i in range(3)]
+    static = [t.to(DEV) for t in sets[0]]
+    leaves = [t.requires_grad_() for t in static[:5]]
+
+    def once():
+        h = gated_linear(*leaves)
+        return [h.detach(), *torch.autograd.grad(h, leaves, static[5])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = once()
+        graphs.append((g, out))
+    for it in range(6):
+        with torch.no_grad():
+            for t, v in zip(static, sets[it % 3]):
+                t.copy_(v.to(DEV))
+        want = once()
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            g.replay()
+            once()                                                  # eager work of its own in between
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(want, out)), it
+
+
+def test_module_and_denoiser_training_step():
+    """A denoiser of gated layers inside model.Model: loss, gradients, clipping and Adam's step on the GPU against the same
+    modules on the CPU in float64 (the draws replayed)."""
+    from diffputer_amd.gated import GatedLinear
+    from diffputer_amd.grads import clip_grads
+    from diffputer_amd.model import Model, PositionalEmbedding
+
+    class Denoiser(torch.nn.Module):
+        def __init__(self, d, h):
+            super().__init__()
+            self.proj = GatedLinear(d, h)
+            self.map_noise = PositionalEmbedding(num_channels=h)
+            self.mid = GatedLinear(h, 2 * h, act="gelu")
+            self.out = torch.nn.Linear(2 * h, d)
+
+        def forward(self, x, noise_labels, class_labels=None):
+            return self.out(self.mid(self.proj(x) + self.map_noise(noise_labels).to(x.dtype)))
+
+    d, h, n = 9, 64, 200
+    torch.manual_seed(5)
+    cpu = Model(denoise_fn=Denoiser(d, h), hid_dim=d)
+    gpu = Model(denoise_fn=Denoiser(d, h), hid_dim=d)
+    gpu.load_state_dict(cpu.state_dict())
+    assert "denoise_fn_D.denoise_fn_F.mid.gate.weight" in gpu.state_dict()
+    gpu = gpu.to(DEV)
+    x, zs, zn = torch.randn(n, d), torch.randn(n), torch.randn(n, d)
+
+    def step(model, dev, limit):
+        saved = (torch.randn, torch.randn_like)
+        torch.randn = lambda *a, **k: zs.to(dev)
+        torch.randn_like = lambda t, **k: zn.to(dev)
+        try:
+            loss = model(x.to(dev))
+        finally:
+            torch.randn, torch.randn_like = saved
+        params = list(model.parameters())
+        for p in params:
+            p.grad = None
+        loss.backward()
+        before = [p.grad.clone() for p in params]
+        norm = clip_grads([p.grad for p in params], limit) if dev != "cpu" else torch.nn.utils.clip_grad_norm_(params, limit)
+        after = [p.grad.clone() for p in params]
+        torch.optim.Adam(params, lr=1e-3).step()
+        return float(loss.detach()), before, float(norm), after
+
+    ref = step(cpu, "cpu", 0.25)
+    got = step(gpu, DEV, 0.25)
+    assert abs(got[0] - ref[0]) <= 1e-4 * abs(ref[0])
+    assert ref[2] > 0.25, "the limit has to bite"
+    # both sides are float32 with sums of a few hundred terms in different orders: 1e-4 of a tensor's scale is over 1000 half steps
+    for i in (1, 3):
+        for a, b in zip(got[i], ref[i]):
+            assert float((a.cpu() - b).abs().max()) <= 1e-4 * float(b.abs().max()) + 1e-8
+    assert abs(got[2] - ref[2]) <= 1e-4 * ref[2]
+    total = math.sqrt(sum(float(g.double().square().sum()) for g in got[3]))
+    assert abs(total - 0.25) <= 1e-5

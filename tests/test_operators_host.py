@@ -1,0 +1,152 @@
+"""What the gated projection and the gradient clipping refuse, and what they do without a GPU (their C entry points check
+every argument before the first HIP call)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from diffputer_amd import _lib
+from diffputer_amd.gated import GatedLinear, gated_linear
+from diffputer_amd.grads import clip_grads, grad_norm
+
+
+def _err(lib):
+    return lib.dp_last_error().decode()
+
+
+def test_gated_linear_refuses():
+    x, w, b = torch.randn(3, 4), torch.randn(5, 4), torch.randn(5)
+    for args, kw, why in (
+        ((x, w, w), {"act": "relu"}, "act must be"),
+        ((x, w, w[:4]), {}, "expected"),
+        ((x, w[:, :3], w[:, :3]), {}, "expected"),
+        ((torch.randn(()), w, w), {}, "expected"),
+        ((x, w[0], w[0]), {}, "expected"),
+        ((x, w[:0], w[:0]), {}, "at least 1"),
+        ((x[:, :0], w[:, :0], w[:, :0]), {}, "at least 1"),
+        ((x, w, w, b[:4]), {}, "b_gate"),
+        ((x, w, w, None, b.reshape(1, 5)), {}, "b_up"),
+        ((x, w.bfloat16(), w), {}, "float32, or all bfloat16"),
+        ((x.half(), w.half(), w.half()), {}, "float32, or all bfloat16"),
+        ((x.double(), w.double(), w.double()), {}, "float32, or all bfloat16"),
+        ((x, w, w, b.bfloat16()), {}, "b_gate"),
+        ((x, w.to("meta"), w), {}, "is on meta"),
+    ):
+        with pytest.raises(ValueError, match=why):
+            gated_linear(*args, **kw)
+    with pytest.raises(_lib.DiffputerError, match="no CPU fallback"):
+        gated_linear(x, w, w, b, b)
+
+
+def test_grads_refuse():
+    g = torch.randn(4)
+    for call in (grad_norm, lambda t, **k: clip_grads(t, 1.0, **k)):
+        with pytest.raises(_lib.DiffputerError, match="no CPU fallback"):
+            call([g])
+        with pytest.raises(ValueError, match="norm_type"):
+            call([g], norm_type=1.0)
+        with pytest.raises(ValueError, match="no tensors"):
+            call([])
+        with pytest.raises(ValueError, match="float16"):
+            call([g.half()])
+        with pytest.raises(ValueError, match="tensor 1 is on meta"):
+            call([g, g.to("meta")])
+    for limit in (-1.0, math.nan, "x"):
+        with pytest.raises(ValueError):
+            clip_grads([g], limit)
+
+
+def test_module_on_the_cpu():
+    torch.manual_seed(1)
+    for act, f in (("silu", torch.nn.functional.silu), ("gelu", torch.nn.functional.gelu), ("none", lambda t: t)):
+        m = GatedLinear(7, 5, act=act)
+        assert sorted(m.state_dict()) == ["gate.bias", "gate.weight", "up.bias", "up.weight"]
+        x = torch.randn(2, 3, 7)
+        assert torch.allclose(m(x), f(m.gate(x)) * m.up(x))
+    assert GatedLinear(7, 5, bias=False).gate.bias is None
+    with pytest.raises(ValueError):
+        GatedLinear(7, 5, act="tanh")
+
+
+def test_m_step_limit_on_the_cpu():
+    from diffputer_amd import em
+    X = torch.randn(40, 3)
+    with pytest.raises(ValueError):
+        em.m_step(X, 8, max_epochs=1, max_grad_norm=-1.0)
+    torch.manual_seed(0)
+    model, best = em.m_step(X, 8, max_epochs=2, max_grad_norm=1e-3)
+    assert math.isfinite(best)
+
+
+FAKE = 1 << 12                                                     # an aligned address that nothing reads: every call below is refused first
+
+
+def _fwd(lib, dtype=1, x=FAKE, ldx=64, wg=FAKE, wu=FAKE, ldw=64, bg=None, bu=None, h=FAKE, ldh=32, pre=None, M=10, N=32, K=64, act=1, ws=FAKE, ws_bytes=1 << 40):
+    return lib.dp_gated_linear(dtype, x, ldx, wg, wu, ldw, bg, bu, h, ldh, pre, M, N, K, act, ws, ws_bytes, None)
+
+
+def _bwd(lib, dtype=1, x=FAKE, ldx=64, wg=FAKE, wu=FAKE, ldw=64, pre=FAKE, dh=FAKE, lddh=32, dx=FAKE, dwg=FAKE, dwu=FAKE, dbg=None, dbu=None, M=10, N=32, K=64, act=1,
+         ws=FAKE, ws_bytes=1 << 40):
+    return lib.dp_gated_linear_bwd(dtype, x, ldx, wg, wu, ldw, pre, dh, lddh, dx, dwg, dwu, dbg, dbu, M, N, K, act, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("call", [_fwd, _bwd])
+def test_c_entry_refuses(call):
+    lib = _lib.load()
+    bad = [dict(dtype=2), dict(dtype=-1), dict(M=-1), dict(M=1 << 29), dict(N=0), dict(K=0), dict(N=-5), dict(N=(1 << 20) + 1), dict(K=(1 << 20) + 1), dict(act=3), dict(act=-1),
+           dict(x=None), dict(wg=None), dict(wu=None), dict(ldx=63), dict(ldw=63), dict(x=FAKE + 1), dict(wg=FAKE + 1), dict(dtype=0, wu=FAKE + 2)]
+    bad += [dict(h=None), dict(ldh=31), dict(h=FAKE + 1), dict(bg=FAKE + 1), dict(pre=FAKE + 8)] if call is _fwd else \
+           [dict(pre=None), dict(dh=None), dict(lddh=31), dict(dh=FAKE + 1), dict(pre=FAKE + 8), dict(dx=FAKE + 1), dict(dwg=FAKE + 1), dict(dbu=FAKE + 1)]
+    for kw in bad:
+        assert call(lib, **kw) == -1, kw                            # DP_EINVAL
+        assert "dp_gated_linear" in _err(lib), kw
+    for kw in (dict(ws=None), dict(ws_bytes=0), dict(ws=FAKE + 128)):
+        assert call(lib, **kw) == -4, kw                            # DP_EWORKSPACE
+    assert _fwd(lib, M=0, x=None, h=None, ws=None) == 0             # no rows: nothing to do
+
+
+def test_gated_sizes():
+    lib = _lib.load()
+    assert lib.dp_gated_linear_pre_bytes(10, 33) == 10 * 2 * 36 * 4
+    assert lib.dp_gated_linear_pre_bytes(-1, 33) == 0 and lib.dp_gated_linear_pre_bytes(5, 0) == 0
+    for args in ((2, 5, 5, 5, 0), (0, -1, 5, 5, 0), (0, 5, 0, 5, 1), (0, 5, 5, 0, 1)):
+        assert lib.dp_gated_linear_workspace_bytes(*args) == 0
+    for dtype in (0, 1):
+        for M, N, K in ((0, 5, 5), (1, 1, 1), (1, 2048, 1024), (24, 8192, 4096), (16384, 64, 9), (4096, 2048, 1024), ((1 << 29) - 1, 64, 64)):
+            for backward in (0, 1):
+                assert lib.dp_gated_linear_workspace_bytes(dtype, M, N, K, backward) >= 256
+    # a float32 plane of a large batch passes 32 bits
+    assert lib.dp_gated_linear_workspace_bytes(0, 1 << 20, 4096, 64, 1) >= 2 * (1 << 20) * 4096 * 4
+    assert lib.dp_gated_linear_pre_bytes(1 << 20, 4096) == 2 * (1 << 20) * 4096 * 4
+
+
+def _table(ptrs, numel, dtypes):
+    n = len(ptrs)
+    return n, (C.c_void_p * n)(*ptrs), (C.c_int64 * n)(*numel), (C.c_int * n)(*dtypes)
+
+
+def test_c_clip_refuses():
+    lib = _lib.load()
+    big = 1 << 30
+
+    def clip(ptrs=(FAKE,), numel=(8,), dtypes=(0,), kind=2, limit=1.0, norm=FAKE, ws=FAKE, ws_bytes=big, n=None):
+        t = _table(ptrs, numel, dtypes)
+        return lib.dp_clip_grads(t[0] if n is None else n, *t[1:], kind, limit, norm, ws, ws_bytes, None)
+
+    def norm_(ptrs=(FAKE,), numel=(8,), dtypes=(0,), kind=2, norm=FAKE, ws=FAKE, ws_bytes=big, n=None):
+        t = _table(ptrs, numel, dtypes)
+        return lib.dp_grad_norm(t[0] if n is None else n, *t[1:], kind, norm, ws, ws_bytes, None)
+
+    for call, name in ((clip, "dp_clip_grads"), (norm_, "dp_grad_norm")):
+        for kw in (dict(dtypes=(5,)), dict(numel=(-1,)), dict(numel=(1 << 60,)), dict(ptrs=(None,)), dict(ptrs=(FAKE + 2,)), dict(ptrs=(FAKE + 1,), dtypes=(1,)),
+                   dict(kind=1), dict(norm=None), dict(n=-1)):
+            assert call(**kw) == -1, (name, kw)
+            assert name in _err(lib)
+        for kw in (dict(ws=None), dict(ws_bytes=8), dict(ws=FAKE + 4)):
+            assert call(**kw) == -4, (name, kw)
+    for limit in (-0.5, math.nan):
+        assert clip(limit=limit) == -1
+    for ptrs, numel, dtypes in (((FAKE, FAKE), (8, 8), (0, 0)), ((FAKE, FAKE + 28), (8, 8), (0, 1)), ((FAKE + 64, FAKE), (4, 17), (0, 0)),
+                                ((FAKE, FAKE + 4, FAKE + 8), (100, 0, 1), (0, 0, 0))):
+        assert clip(ptrs=ptrs, numel=numel, dtypes=dtypes) == -1 and "share memory" in _err(lib)
