@@ -98,6 +98,7 @@ static std::atomic<int> g_w4_min_k{1024};  // "w4_min_k": smallest K the four-wa
 static std::atomic<int> g_narrow_bm{128};   // "narrow_bm": rows per tile of the simple kernel on layers with N % 256 != 0 (mlp.6 of narrow tables): 128
                                            // (default: 512 tiles of 48 KiB LDS keep three workgroups per CU loading; the layer is bound by reading h3) or 256
 static std::atomic<int> g_fuse_mid{1};     // "fuse_mid": 1 = k_step_mid runs inside the mlp.6 GEMM when d_in = 256 (bf16 plans)
+extern std::atomic<int> g_gated_kernel, g_gated_splits;   // "gated_kernel", "gated_splits": the gated projection's dispatch (diffputer_ops.hip)
 static inline int tune(const std::atomic<int>& v) { return v.load(std::memory_order_relaxed); }
 
 // dp_impute_static's scratch: device memory beyond the caller's tables, held by every GPU the library runs on until the
@@ -987,6 +988,16 @@ int dp_tune(const char* key, int value) {
     if (!strcmp(key, "gemm_variant")) {
         if (value < 1 || value > 3) return fail(DP_EINVAL, "gemm_variant must be 1, 2 or 3");
         g_gemm_variant = value;
+        return DP_OK;
+    }
+    if (!strcmp(key, "gated_kernel")) {
+        if (value != 0 && value != 1 && value != 128 && value != 256) return fail(DP_EINVAL, "gated_kernel must be 0, 1, 128 or 256");
+        g_gated_kernel = value;
+        return DP_OK;
+    }
+    if (!strcmp(key, "gated_splits")) {
+        if (value < 0 || value > 64) return fail(DP_EINVAL, "gated_splits must be 0 (by size) to 64");
+        g_gated_splits = value;
         return DP_OK;
     }
     if (!strcmp(key, "narrow_bm")) {

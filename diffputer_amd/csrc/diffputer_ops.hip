@@ -4,10 +4,13 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <new>
 #include <vector>
 
 #include "dp_gated.h"
+#include "dp_gated_tile.h"
 #include "dp_grads.h"
 #include "dp_util.h"
 
@@ -27,35 +30,99 @@ static int gl_check(const char* who, int dtype, int64_t M, int N, int K, int act
     return DP_OK;
 }
 
-// How a product is cut: tiles over C and slices of the contraction.  A launch with few tiles leaves most of the 256 CUs
-// idle, so the contraction is cut until there are about two workgroups per CU, as long as a slice keeps 8 K-tiles.
-struct GlCut { int kt_per, splits; };
-static GlCut gl_cut(int64_t tiles, int64_t nk, int64_t part_bytes) {
-    int64_t s = std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), nk / 8, (int64_t)(64 << 20) / std::max<int64_t>(part_bytes, 1), 64});
-    if (s <= 1) return {(int)nk, 1};
-    const int64_t per = ceil_div<int64_t>(nk, s);
-    return {(int)per, (int)ceil_div<int64_t>(nk, per)};
+// tuning knobs (dp_tune, defined in diffputer_hip.hip): "gated_kernel" 0 = by the rule below, 1 = the general kernel, 128 / 256 = that tile;
+// "gated_splits" 0 = by the rule, n = that many slices of the contraction (as many as there are K-tiles at most)
+std::atomic<int> g_gated_kernel{0}, g_gated_splits{0};
+
+// dynamic LDS of the tile kernels, once per device
+template <int MODE> static hipError_t gt_attributes() {
+    const void* k[] = {(const void*)k_gated_tile<MODE, 256, false>, (const void*)k_gated_tile<MODE, 256, true>, (const void*)k_gated_tile<MODE, 128, false>, (const void*)k_gated_tile<MODE, 128, true>};
+    for (int i = 0; i < 4; ++i) {
+        const hipError_t e = hipFuncSetAttribute(k[i], hipFuncAttributeMaxDynamicSharedMemorySize, i < 2 ? GtShape<256>::LDS : GtShape<128>::LDS);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+static int gt_ready() {
+    static std::atomic<int> ready[64];
+    static std::mutex mutex;
+    int dev = 0;
+    DP_HIP(hipGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(DP_EHIP, "device index %d", dev);
+    if (ready[dev].load(std::memory_order_acquire)) return DP_OK;
+    std::lock_guard<std::mutex> lock(mutex);
+    DP_HIP(gt_attributes<GL_FWD>());
+    DP_HIP(gt_attributes<GL_DX>());
+    DP_HIP(gt_attributes<GL_DW>());
+    ready[dev].store(1, std::memory_order_release);
+    return DP_OK;
 }
 
+// How a product runs: the general kernel (T = 0) or a tile kernel, and how many slices of the contraction.
 struct GlShape { int mode; int64_t I; int J; int64_t C; int planes; };
+struct GlPlan { int T, kt_per, splits; int64_t ti, tj; };
 static int64_t gl_ldp(int J) { return round_up<int64_t>(J, 4); }
 static size_t gl_part_bytes(const GlShape& s) { return (size_t)2 * s.I * gl_ldp(s.J) * 4; }       // one slice: two planes
-static GlCut gl_plan(const GlShape& s) {
-    const int64_t tiles = ceil_div<int64_t>(s.I, GG_T) * ceil_div<int64_t>(s.J, s.mode == GL_FWD ? GG_T / 2 : GG_T) * s.planes;
-    return gl_cut(tiles, ceil_div<int64_t>(s.C, GG_K) * (s.mode == GL_DX ? 2 : 1), gl_part_bytes(s));
+
+// Cuts the contraction of a launch that has few tiles, until there are about `want` workgroups, as long as a slice keeps
+// `least` K-tiles and the partial sums stay within 64 MiB.
+static void gl_cut(GlPlan& pl, const GlShape& s, int64_t tiles, int64_t nk, int64_t want, int64_t least) {
+    int64_t n = std::min<int64_t>({want / std::max<int64_t>(tiles, 1), nk / least, (int64_t)(64 << 20) / std::max<int64_t>(gl_part_bytes(s), 1), 64});
+    if (const int forced = g_gated_splits.load(std::memory_order_relaxed)) n = std::min<int64_t>(forced, nk);
+    if (n < 1) n = 1;
+    pl.kt_per = (int)ceil_div<int64_t>(nk, n);
+    pl.splits = (int)ceil_div<int64_t>(nk, pl.kt_per);
 }
-static size_t gl_split_bytes(const GlShape& s) {
-    const GlCut c = gl_plan(s);
+static GlPlan gl_plan(const GlShape& s, bool tile) {
+    GlPlan pl;
+    const int segs = s.mode == GL_DX ? 2 : 1;
+    auto shape = [&](int T) {
+        pl.T = T;
+        pl.ti = ceil_div<int64_t>(s.I, T ? T : GG_T);
+        pl.tj = ceil_div<int64_t>(s.J, (T ? T : GG_T) / (s.mode == GL_FWD ? 2 : 1));
+        return pl.ti * pl.tj * s.planes;
+    };
+    const int forced = g_gated_kernel.load(std::memory_order_relaxed);
+    if (tile && forced != 1) {
+        const int64_t nk = ceil_div<int64_t>(s.C, 64) * segs;
+        int64_t tiles = shape(256);
+        if (forced == 128 || (forced == 0 && tiles < 256)) tiles = shape(128);
+        if (tiles < (int64_t)1 << 22) {                           // the grid of a launch
+            gl_cut(pl, s, tiles, nk, pl.T == 256 ? 256 : 512, 4);
+            return pl;
+        }
+    }
+    const int64_t tiles = shape(0);
+    gl_cut(pl, s, tiles, ceil_div<int64_t>(s.C, GG_K) * segs, 512, 8);
+    return pl;
+}
+static size_t gl_split_bytes(const GlShape& s, bool tile) {
+    const GlPlan c = gl_plan(s, tile);
     return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0;
 }
 
+template <int MODE, int T>
+static int gt_launch(const GlArgs& a, const GlPlan& pl, int planes, hipStream_t st) {
+    const GtArgs q = {a, (int)pl.ti, (int)pl.tj, 8};
+    const dim3 grid((unsigned)(pl.ti * pl.tj * planes * pl.splits)), block(GtShape<T>::THREADS);
+    if (pl.splits > 1) hipLaunchKernelGGL((k_gated_tile<MODE, T, true>), grid, block, GtShape<T>::LDS, st, q);
+    else hipLaunchKernelGGL((k_gated_tile<MODE, T, false>), grid, block, GtShape<T>::LDS, st, q);
+    DP_LAUNCH_CHECK("k_gated_tile");
+    return DP_OK;
+}
+
 template <typename T, int MODE>
-static int gl_mm(GlArgs a, const GlShape& s, hipStream_t st) {
-    const GlCut c = gl_plan(s);
+static int gl_mm(GlArgs a, const GlShape& s, bool tile, hipStream_t st) {
+    const GlPlan c = gl_plan(s, tile);
+    int rc;
     a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
-    const int64_t gx = ceil_div<int64_t>(s.I, GG_T), gy = ceil_div<int64_t>(s.J, MODE == GL_FWD ? GG_T / 2 : GG_T);
-    hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)gx, (unsigned)gy, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, a);
-    DP_LAUNCH_CHECK("k_gated_mm");
+    if (c.T == 0) {
+        hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, a);
+        DP_LAUNCH_CHECK("k_gated_mm");
+    } else {
+        if ((rc = gt_ready())) return rc;
+        if ((rc = c.T == 256 ? gt_launch<MODE, 256>(a, c, s.planes, st) : gt_launch<MODE, 128>(a, c, s.planes, st))) return rc;
+    }
     if (c.splits > 1) {
         const int64_t n = s.I * s.planes * ceil_div<int64_t>(s.J, 4);
         const unsigned grid = (unsigned)std::min<int64_t>(ceil_div<int64_t>(n, 256), 4096);
@@ -65,7 +132,72 @@ static int gl_mm(GlArgs a, const GlShape& s, hipStream_t st) {
     return DP_OK;
 }
 
-// backward workspace: the two planes dg, du; partial column sums; partial products (dx and dW use the same bytes in turn)
+// The tile kernels load 16 bytes at a time: an operand is read where it is if its rows start on 16 bytes and end on 8
+// elements.  Others are copied to the workspace (rows padded with zeros) where the product is large enough to pay for it.
+static bool gt_direct(const void* p, int64_t ld, int64_t cols) { return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= 1 << 22; }
+constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
+struct GtOperands { bool tile, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
+static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
+    GtOperands o;
+    o.pack_x = !gt_direct(x, ldx, K);
+    o.pack_w = !gt_direct(wg, ldw, K) || !gt_direct(wu, ldw, K);
+    o.ldk = round_up<int64_t>(K, 8);
+    const int forced = g_gated_kernel.load(std::memory_order_relaxed);
+    o.tile = dtype == DP_DTYPE_BF16 && forced != 1 && (forced || (!o.pack_x && !o.pack_w) || M * N * K >= GT_PACK_LEAST);
+    if (!o.tile) o.pack_x = o.pack_w = false;
+    return o;
+}
+struct Carver {
+    char* base;
+    size_t off = 0;
+    char* take(size_t n) { const size_t o = off; off += round_up<size_t>(n, 256); return base ? base + o : (char*)nullptr; }
+};
+static int gt_pack(GlOp& op, void* to, int64_t ldk, int64_t rows, hipStream_t st) {
+    const int64_t n = rows * (ldk / 8);
+    hipLaunchKernelGGL(k_gated_pack, dim3((unsigned)std::min<int64_t>(ceil_div<int64_t>(n, 256), 8192)), dim3(256), 0, st, (const bf16_t*)op.p, op.ld, (bf16_t*)to, ldk, rows, op.cols);
+    DP_LAUNCH_CHECK("k_gated_pack");
+    op = {to, ldk, ldk};
+    return DP_OK;
+}
+
+// x and both weights as the products read them: where they are, or copied to the workspace
+struct GlIn {
+    GlOp x, wg, wu;
+    int64_t M;
+    int N, K;
+    GtOperands o;
+    char *px, *pw;
+    void carve(Carver& c) {
+        px = o.pack_x ? c.take((size_t)M * o.ldk * 2) : nullptr;
+        pw = o.pack_w ? c.take((size_t)2 * N * o.ldk * 2) : nullptr;
+    }
+    int pack(bool need_x, bool need_w, hipStream_t st) {
+        int rc;
+        if (o.pack_x && need_x && (rc = gt_pack(x, px, o.ldk, M, st))) return rc;
+        if (o.pack_w && need_w && ((rc = gt_pack(wg, pw, o.ldk, N, st)) || (rc = gt_pack(wu, pw + (size_t)N * o.ldk * 2, o.ldk, N, st)))) return rc;
+        return DP_OK;
+    }
+    // contraction length of the forward product: the copies' padding belongs to it (zeros on both sides)
+    int64_t fwd_c() const { return o.pack_x && o.pack_w ? o.ldk : K; }
+};
+static GlIn gl_in(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
+    GlIn in = {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
+    if (K % 8 && in.o.tile) in.o.pack_x = in.o.pack_w = true;
+    return in;
+}
+
+// forward workspace: copies, partial sums
+struct GlFwd { float* part; size_t bytes; };
+static GlFwd gl_fwd_carve(GlIn& in, void* base) {
+    Carver c = {(char*)base};
+    in.carve(c);
+    GlFwd w;
+    w.part = (float*)c.take(gl_split_bytes({GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile));
+    w.bytes = c.off;
+    return w;
+}
+
+// backward workspace: copies; the two planes dg, du; partial column sums; partial products (dx and dW use the same bytes in turn)
 struct GlBwd {
     char* dgu;
     float *colpart, *part;
@@ -73,28 +205,36 @@ struct GlBwd {
     int tx, rows, nblk;
     size_t bytes;
 };
-static GlBwd gl_bwd_carve(int dtype, int64_t M, int N, int K, void* base) {
+static GlBwd gl_bwd_carve(int dtype, GlIn& in, void* base) {
+    const int64_t M = in.M;
+    const int N = in.N, K = in.K;
     GlBwd w;
-    size_t off = 0;
-    auto take = [&](size_t n) { const size_t o = off; off += round_up<size_t>(n, 256); return base ? (char*)base + o : (char*)nullptr; };
+    Carver c = {(char*)base};
+    in.carve(c);
     w.ldg = round_up<int64_t>(N, 64);
-    w.tx = (int)std::min<int64_t>(64, w.ldg / 4);                 // 16, 32, 48 or 64 column groups of 4
+    w.tx = (int)std::min<int64_t>(64, w.ldg / 4);                 // 16, 32 or 64 column groups of 4
     if (w.tx == 48) w.tx = 64;
     const int64_t cols = ceil_div<int64_t>(w.ldg, w.tx * 4);
     const int ty = 256 / w.tx;
     // about 2048 workgroups, at least 4 rows per row lane
     w.rows = (int)std::max<int64_t>(4 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 2048 / cols)));
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
-    w.dgu = take((size_t)2 * M * w.ldg * (dtype == DP_DTYPE_BF16 ? 2 : 4));
-    w.colpart = (float*)take((size_t)w.nblk * 2 * w.ldg * 4);
-    w.part = (float*)take(std::max(gl_split_bytes({GL_DX, M, K, N, 1}), gl_split_bytes({GL_DW, N, K, M, 2})));
-    w.bytes = off;
+    w.dgu = c.take((size_t)2 * M * w.ldg * (dtype == DP_DTYPE_BF16 ? 2 : 4));
+    w.colpart = (float*)c.take((size_t)w.nblk * 2 * w.ldg * 4);
+    w.part = (float*)c.take(std::max(gl_split_bytes({GL_DX, M, K, N, 1}, in.o.tile), gl_split_bytes({GL_DW, N, K, M, 2}, in.o.tile)));
+    w.bytes = c.off;
     return w;
 }
 
 template <typename T>
-static int gl_forward(const GlArgs& a, int64_t M, int N, int K, hipStream_t st) {
-    return gl_mm<T, GL_FWD>(a, {GL_FWD, M, N, K, 1}, st);
+static int gl_forward(GlArgs a, GlIn& in, void* ws, hipStream_t st) {
+    const GlFwd w = gl_fwd_carve(in, ws);
+    int rc;
+    if ((rc = in.pack(true, true, st))) return rc;
+    a.A[0] = in.x;
+    a.B[0] = in.wg; a.B[1] = in.wu;
+    a.part = w.part;
+    return gl_mm<T, GL_FWD>(a, {GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile, st);
 }
 
 template <typename T>
@@ -105,8 +245,9 @@ static int gl_zero(void* p, int64_t n, hipStream_t st) {
 }
 
 template <typename T>
-static int gl_backward(int dtype, const GlOp& x, const GlOp& wg, const GlOp& wu, const float* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2],
-                       int64_t M, int N, int K, int act, void* ws, hipStream_t st) {
+static int gl_backward(int dtype, GlIn& in, const float* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2], int act, void* ws, hipStream_t st) {
+    const int64_t M = in.M;
+    const int N = in.N, K = in.K;
     int rc;
     if (M == 0) {                                                // no rows: the sums are empty
         for (int z = 0; z < 2; ++z) {
@@ -115,9 +256,10 @@ static int gl_backward(int dtype, const GlOp& x, const GlOp& wg, const GlOp& wu,
         }
         return DP_OK;
     }
-    const GlBwd w = gl_bwd_carve(dtype, M, N, K, ws);
+    const GlBwd w = gl_bwd_carve(dtype, in, ws);
     T* const dgu = (T*)w.dgu;
     const bool bias = db[0] || db[1];
+    if ((rc = in.pack(dw[0] || dw[1], dx != nullptr, st))) return rc;
     hipLaunchKernelGGL((k_gated_dgu<T>), dim3((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk), dim3(256), 0, st, pre, gl_ldp(N),
                        (const T*)dh.p, dh.ld, dgu, w.ldg, bias ? w.colpart : (float*)nullptr, M, N, act, w.tx, w.rows);
     DP_LAUNCH_CHECK("k_gated_dgu");
@@ -128,18 +270,18 @@ static int gl_backward(int dtype, const GlOp& x, const GlOp& wg, const GlOp& wu,
     GlArgs a;
     memset(&a, 0, sizeof a);
     a.part = w.part;
-    a.A[0] = {dgu, w.ldg};
-    a.A[1] = {dgu + (size_t)M * w.ldg, w.ldg};
+    a.A[0] = {dgu, w.ldg, w.ldg};
+    a.A[1] = {dgu + (size_t)M * w.ldg, w.ldg, w.ldg};
     if (dx) {
-        a.B[0] = wg; a.B[1] = wu;
+        a.B[0] = in.wg; a.B[1] = in.wu;
         a.out[0] = dx; a.ldo = K;
-        if ((rc = gl_mm<T, GL_DX>(a, {GL_DX, M, K, N, 1}, st))) return rc;
+        if ((rc = gl_mm<T, GL_DX>(a, {GL_DX, M, K, N, 1}, in.o.tile, st))) return rc;
     }
     if (dw[0] || dw[1]) {
-        a.B[0] = x;
+        a.B[0] = in.x;
         a.out[0] = dw[0]; a.out[1] = dw[1]; a.ldo = K;
         a.zfirst = dw[0] ? 0 : 1;
-        if ((rc = gl_mm<T, GL_DW>(a, {GL_DW, N, K, M, dw[0] && dw[1] ? 2 : 1}, st))) return rc;
+        if ((rc = gl_mm<T, GL_DW>(a, {GL_DW, N, K, M, dw[0] && dw[1] ? 2 : 1}, in.o.tile, st))) return rc;
     }
     return DP_OK;
 }
@@ -210,10 +352,11 @@ size_t dp_gated_linear_pre_bytes(int64_t M, int N) {
     return (size_t)std::max<int64_t>(M, 1) * 2 * gl_ldp(N) * 4;
 }
 
-size_t dp_gated_linear_workspace_bytes(int dtype, int64_t M, int N, int K, int backward) {
+size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, int64_t M, int N, int K, int backward) {
     if (gl_check("dp_gated_linear_workspace_bytes", dtype, M, N, K, 0)) return 0;
-    const size_t need = M == 0 ? 0 : backward ? gl_bwd_carve(dtype, M, N, K, nullptr).bytes : gl_split_bytes({GL_FWD, M, N, K, 1});
-    return std::max<size_t>(need, 256);
+    if (M == 0) return 256;
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
+    return std::max<size_t>(backward ? gl_bwd_carve(dtype, in, nullptr).bytes : gl_fwd_carve(in, nullptr).bytes, 256);
 }
 
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
@@ -227,20 +370,17 @@ int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, c
     for (const void* p : {x, w_gate, w_up, b_gate, b_up, (const void*)h})
         if (!aligned(p, es)) return fail(DP_EINVAL, "dp_gated_linear: a pointer is not aligned to its element");
     if (!aligned(pre, 16)) return fail(DP_EINVAL, "dp_gated_linear: pre must be 16-byte aligned");
-    const size_t need = dp_gated_linear_workspace_bytes(dtype, M, N, K, 0);
+    const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, 0);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
     GlArgs a;
     memset(&a, 0, sizeof a);
-    a.A[0] = {x, ldx};
-    a.B[0] = {w_gate, ldw};
-    a.B[1] = {w_up, ldw};
     a.out[0] = h; a.ldo = ldh;
-    a.part = (float*)workspace;
     a.pre = (float*)pre; a.ldpre = gl_ldp(N);
     a.bias[0] = b_gate; a.bias[1] = b_up;
     a.act = act;
     hipStream_t st = (hipStream_t)stream;
-    return dtype == DP_DTYPE_BF16 ? gl_forward<bf16_t>(a, M, N, K, st) : gl_forward<float>(a, M, N, K, st);
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
+    return dtype == DP_DTYPE_BF16 ? gl_forward<bf16_t>(a, in, workspace, st) : gl_forward<float>(a, in, workspace, st);
 }
 
 int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,
@@ -253,19 +393,20 @@ int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gat
         if (!x || !w_gate || !w_up || !pre || !dh) return fail(DP_EINVAL, "dp_gated_linear_bwd: null pointer");
         if (ldx < K || ldw < K || lddh < N) return fail(DP_EINVAL, "dp_gated_linear_bwd: row strides ldx=%lld ldw=%lld lddh=%lld are shorter than a row (K=%d, N=%d)", (long long)ldx, (long long)ldw, (long long)lddh, K, N);
         if (!aligned(pre, 16)) return fail(DP_EINVAL, "dp_gated_linear_bwd: pre must be 16-byte aligned");
-        const size_t need = dp_gated_linear_workspace_bytes(dtype, M, N, K, 1);
+        const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, 1);
         if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear_bwd: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
     }
     for (const void* p : {x, w_gate, w_up, dh, (const void*)dx, (const void*)dw_gate, (const void*)dw_up, (const void*)db_gate, (const void*)db_up})
         if (!aligned(p, es)) return fail(DP_EINVAL, "dp_gated_linear_bwd: a pointer is not aligned to its element");
-    const GlOp ox = {x, ldx}, og = {w_gate, ldw}, ou = {w_up, ldw}, od = {dh, lddh};
+    const GlOp od = {dh, lddh, N};
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == DP_DTYPE_BF16) {
         bf16_t *dw[2] = {(bf16_t*)dw_gate, (bf16_t*)dw_up}, *db[2] = {(bf16_t*)db_gate, (bf16_t*)db_up};
-        return gl_backward<bf16_t>(dtype, ox, og, ou, (const float*)pre, od, (bf16_t*)dx, dw, db, M, N, K, act, workspace, st);
+        return gl_backward<bf16_t>(dtype, in, (const float*)pre, od, (bf16_t*)dx, dw, db, act, workspace, st);
     }
     float *dw[2] = {(float*)dw_gate, (float*)dw_up}, *db[2] = {(float*)db_gate, (float*)db_up};
-    return gl_backward<float>(dtype, ox, og, ou, (const float*)pre, od, (float*)dx, dw, db, M, N, K, act, workspace, st);
+    return gl_backward<float>(dtype, in, (const float*)pre, od, (float*)dx, dw, db, act, workspace, st);
 }
 
 size_t dp_grad_workspace_bytes(int n) { return n < 0 ? 0 : (size_t)(gn_cap(n) * gn_launches(n) + 1) * sizeof(double); }

@@ -59,6 +59,7 @@ __device__ __forceinline__ void gl_act_grad(int act, float g, float& a, float& d
 struct GlOp {
     const void* p;
     int64_t ld;
+    int64_t cols;              // elements of a row that exist
 };
 
 // One product launch.  GL_FWD: A = x (row), B[0] / B[1] = Wg / Wu (row): columns 0..n-1 of the gate and of the up product.

@@ -1,0 +1,393 @@
+// bf16 tile products of the gated projection (dp_gated.h has the three products and their operands): T x T tile of products,
+// 64 deep, T = 256 (8 waves, one workgroup per CU) or 128 (4 waves, two per CU).
+//
+//   * A K-tile is four half-tiles in LDS, A0 A1 B0 B1 (T / 2 rows of A or of B, 64 deep), two K-tiles deep.  Each half-tile
+//     is loaded straight into LDS (buffer loads, 16 bytes a lane) 5 to 6 phases before it is read, and the loads stay in
+//     flight across barriers (counted vmcnt).  Rows or k's that do not exist lie behind the buffer's last byte: the range
+//     check returns zeros for them, which is all the masking that ragged sizes need.
+//   * A K-tile is four phases, one quadrant (A half x B half) of matrix instructions each:
+//       phase   LDS reads                 loads issued         quadrant    landed after the phase's vmcnt
+//       c0      B0(t), A0(t)              -                    A0 B0       -
+//       c1      -                         A1(t+1), B1(t+2)     A0 B1       A1(t)
+//       c2      A1(t)                     A0(t+2)              A1 B1       B1(t+1)
+//       c3      B1(t+1)                   B0(t+2)              A1 B0       A0(t+1), B0(t+1)
+//     A half-tile is read after the vmcnt of every wave and a barrier; its slot is loaded again at least two phases after
+//     its last read, whose lgkmcnt(0) every wave has passed by then.  K-tiles past the end are "loaded" from an empty
+//     buffer (zeros, no traffic), so that every count holds for any number of K-tiles.
+//   * T = 256: the waves of the lower half run one barrier behind, so that one wave of a SIMD multiplies while its partner
+//     reads LDS.  T = 128: the partner is the CU's other workgroup.
+//   * Row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7); fragments by
+//     ds_read_b128.  Column layout (a transposed product's operand): LDS holds the k rows as they are in memory, and
+//     ds_read_b64_tr_b16 turns 4 k's x 16 columns into a fragment's k order while reading, 32-byte slot s of k row k at
+//     s ^ g(k), with g spread so that the 8 rows of a half wave's read lie in 8 different slots.
+//   * GL_FWD: B0 are the gate's rows and B1 the up's rows for the same columns of h: one lane ends with g and u of the
+//     same elements, and the activation and the product are lane-local.
+#pragma once
+#include "dp_gated.h"
+#include "dp_gemm_bf16.h"
+
+namespace dp {
+
+typedef __attribute__((ext_vector_type(4))) short bf16x4;
+
+struct GtArgs {
+    GlArgs g;
+    int nti, ntj;              // tiles along I and J
+    int group;                 // tile rows that are walked together (shared B panels stay in the XCD's L2)
+};
+
+template <int T> struct GtShape {
+    static constexpr int THREADS = T == 256 ? 512 : 256;
+    static constexpr int NW = THREADS / 64, WN = T == 256 ? 4 : 2;         // waves; waves along the columns (2 along the rows)
+    static constexpr int HR = T / 2, HB = HR * 128;                        // rows and bytes of a half-tile
+    static constexpr int MI = HR / 32, NJ = HR / WN / 16;                  // 16 x 16 tiles of a wave's quadrant
+    static constexpr int LDS = 8 * HB;
+};
+
+__device__ __forceinline__ unsigned gt_lds(const void* p) { return (unsigned)(size_t)(DP_LDS_AS const char*)p; }   // LDS byte address
+
+#define GT_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
+
+// byte range [p, end) as a buffer; reads behind it return 0
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t gt_buffer(const char* p, const char* end) {
+    const int64_t n = end - p;
+    const int hi = (int)(n >> 32);
+    const unsigned lo = (unsigned)n;
+    const unsigned bytes = hi < 0 ? 0u : hi > 0 || lo > 0x7fffffffu ? 0x7fffffffu : lo;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00027000);
+}
+
+// Fragments of column-laid-out half-tiles: for every 16-column tile and k-step two reads of 4 k's each, in one statement that
+// ends with their wait (KS, HI: byte offsets of the second k-step and of a fragment's second four k's).
+template <int KS, int HI> __device__ __forceinline__ void gt_tr4(bf16x4 (&a)[2][4][2], const unsigned (&ra)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %16\n\t" "ds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %4, %17\n\t" "ds_read_b64_tr_b16 %5, %17 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %8, %18\n\t" "ds_read_b64_tr_b16 %9, %18 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %12, %19\n\t" "ds_read_b64_tr_b16 %13, %19 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %2, %16 offset:%21\n\t" "ds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %6, %17 offset:%21\n\t" "ds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %10, %18 offset:%21\n\t" "ds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %14, %19 offset:%21\n\t" "ds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
+                   "=&v"(a[1][1][1]), "=&v"(a[0][2][0]), "=&v"(a[0][2][1]), "=&v"(a[1][2][0]), "=&v"(a[1][2][1]), "=&v"(a[0][3][0]), "=&v"(a[0][3][1]),
+                   "=&v"(a[1][3][0]), "=&v"(a[1][3][1])
+                 : "v"(ra[0]), "v"(ra[1]), "v"(ra[2]), "v"(ra[3]), "n"(HI), "n"(KS), "n"(KS + HI)
+                 : "memory");
+}
+template <int KS, int HI> __device__ __forceinline__ void gt_tr2(bf16x4 (&a)[2][2][2], const unsigned (&ra)[2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\t" "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %4, %9\n\t" "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t" "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t" "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]), "=&v"(a[1][1][1])
+                 : "v"(ra[0]), "v"(ra[1]), "n"(HI), "n"(KS), "n"(KS + HI)
+                 : "memory");
+}
+template <int KS, int HI> __device__ __forceinline__ void gt_tr4_2(bf16x4 (&a)[2][4][2], const unsigned (&ra)[4], bf16x4 (&b)[2][2][2], const unsigned (&rb)[2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %24\n\t" "ds_read_b64_tr_b16 %1, %24 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %4, %25\n\t" "ds_read_b64_tr_b16 %5, %25 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %8, %26\n\t" "ds_read_b64_tr_b16 %9, %26 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %12, %27\n\t" "ds_read_b64_tr_b16 %13, %27 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %16, %28\n\t" "ds_read_b64_tr_b16 %17, %28 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %20, %29\n\t" "ds_read_b64_tr_b16 %21, %29 offset:%30\n\t"
+                 "ds_read_b64_tr_b16 %2, %24 offset:%31\n\t" "ds_read_b64_tr_b16 %3, %24 offset:%32\n\t"
+                 "ds_read_b64_tr_b16 %6, %25 offset:%31\n\t" "ds_read_b64_tr_b16 %7, %25 offset:%32\n\t"
+                 "ds_read_b64_tr_b16 %10, %26 offset:%31\n\t" "ds_read_b64_tr_b16 %11, %26 offset:%32\n\t"
+                 "ds_read_b64_tr_b16 %14, %27 offset:%31\n\t" "ds_read_b64_tr_b16 %15, %27 offset:%32\n\t"
+                 "ds_read_b64_tr_b16 %18, %28 offset:%31\n\t" "ds_read_b64_tr_b16 %19, %28 offset:%32\n\t"
+                 "ds_read_b64_tr_b16 %22, %29 offset:%31\n\t" "ds_read_b64_tr_b16 %23, %29 offset:%32\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
+                   "=&v"(a[1][1][1]), "=&v"(a[0][2][0]), "=&v"(a[0][2][1]), "=&v"(a[1][2][0]), "=&v"(a[1][2][1]), "=&v"(a[0][3][0]), "=&v"(a[0][3][1]),
+                   "=&v"(a[1][3][0]), "=&v"(a[1][3][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[0][1][0]),
+                   "=&v"(b[0][1][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
+                 : "v"(ra[0]), "v"(ra[1]), "v"(ra[2]), "v"(ra[3]), "v"(rb[0]), "v"(rb[1]), "n"(HI), "n"(KS), "n"(KS + HI)
+                 : "memory");
+}
+template <int KS, int HI> __device__ __forceinline__ void gt_tr2_2(bf16x4 (&a)[2][2][2], const unsigned (&ra)[2], bf16x4 (&b)[2][2][2], const unsigned (&rb)[2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %16\n\t" "ds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %4, %17\n\t" "ds_read_b64_tr_b16 %5, %17 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %8, %18\n\t" "ds_read_b64_tr_b16 %9, %18 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %12, %19\n\t" "ds_read_b64_tr_b16 %13, %19 offset:%20\n\t"
+                 "ds_read_b64_tr_b16 %2, %16 offset:%21\n\t" "ds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %6, %17 offset:%21\n\t" "ds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %10, %18 offset:%21\n\t" "ds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
+                 "ds_read_b64_tr_b16 %14, %19 offset:%21\n\t" "ds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
+                   "=&v"(a[1][1][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
+                   "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
+                 : "v"(ra[0]), "v"(ra[1]), "v"(rb[0]), "v"(rb[1]), "n"(HI), "n"(KS), "n"(KS + HI)
+                 : "memory");
+}
+__device__ __forceinline__ bf16x8 gt_join(const bf16x4 (&f)[2]) { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); }
+
+template <int MODE, int T, bool SPLIT>
+__device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice, char* smem) {
+    using S = GtShape<T>;
+    constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
+    constexpr int HR = S::HR, HB = S::HB, MI = S::MI, NJ = S::NJ, NW = S::NW, WN = S::WN;
+    constexpr unsigned OUTSIDE = 0x80000000u;                              // an offset behind every buffer
+    const GlArgs& p = q.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // tile -> (row, column): groups of q.group tile rows, column by column within a group
+    const int per_plane = q.nti * q.ntj;
+    const int plane = MODE == GL_DW ? p.zfirst + __builtin_amdgcn_readfirstlane(tile / per_plane) : 0;
+    const int tp = tile % per_plane, gsz = q.group * q.ntj, grp = tp / gsz, in = tp - grp * gsz;
+    const int rows_here = min(q.group, q.nti - grp * q.group);
+    const int ti = __builtin_amdgcn_readfirstlane(grp * q.group + in % rows_here), tj = __builtin_amdgcn_readfirstlane(in / rows_here);
+    const int64_t i0 = (int64_t)ti * T;
+    const int j0 = tj * (MODE == GL_FWD ? HR : T);
+
+    const int nk = (int)((p.C + 63) >> 6);                                 // K-tiles of a segment
+    const int kt0 = SPLIT ? slice * p.kt_per : 0;
+    const int all = nk * (MODE == GL_DX ? 2 : 1), kt1 = SPLIT ? min(kt0 + p.kt_per, all) : all;
+
+    // ---- loads: a wave moves pieces `wave` and `wave + NW` (1 KiB each) of every half-tile ----
+    //   row layout: piece = 8 rows x 128 B; column layout: piece = 1024 / (2 HR) k rows x 2 HR bytes
+    const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
+    constexpr int KR = 1024 / (2 * HR), CH = HR / 8;                       // k rows per piece, 16-byte chunks per k row
+    auto g_of = [](int k) { return HR == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; };
+    unsigned va[2], vb[2];
+    const int r8 = lane >> 3, c8 = (lane & 7) ^ r8;                        // row layout: row of the piece, chunk of memory
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int piece = wave + s * NW;
+        const int k = piece * KR + lane / CH, c = (lane % CH) ^ (2 * g_of(k));
+        va[s] = A_ROW ? (unsigned)((piece * 8 + r8) * lda + c8 * 16) : (unsigned)(k * lda + c * 16);
+        vb[s] = B_ROW ? (unsigned)((piece * 8 + r8) * ldb + c8 * 16) : (unsigned)(k * ldb + c * 16);
+    }
+    // row layout, last K-tile of a contraction that is no multiple of 64: chunks past its end
+    const int tail = B_ROW && (p.C & 63) ? nk - 1 : -1;
+    const bool tail_out = c8 * 8 >= (int)(p.C & 63);
+
+    auto stage = [&](bool is_b, int kt, int h) {
+        const bool row = is_b ? B_ROW : A_ROW;
+        const bool live = kt < kt1;
+        const int seg = MODE == GL_DX && kt >= nk ? 1 : 0;
+        const int64_t kk = kt - seg * nk;
+        const GlOp& op = is_b ? p.B[MODE == GL_FWD ? h : seg] : p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
+        const int64_t ld = is_b ? ldb : lda, size = is_b ? p.J : p.I;
+        const int64_t at = (is_b ? j0 : i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);           // first row / column of the half
+        const char* const base = (const char*)op.p;
+        const char* const from = base + (row ? at * ld + kk * 128 : kk * 64 * ld + at * 2);
+        const char* const end = base + (row ? size - 1 : p.C - 1) * ld + op.cols * 2;
+        const auto buf = gt_buffer(from, live ? end : from);
+        char* const dst = smem + (((kt - kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            unsigned vo = is_b ? vb[s] : va[s];
+            if (row && B_ROW && kt == tail && tail_out) vo = OUTSIDE;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)(dst + s * NW * 1024), 16, (int)vo, 0, 0, 0);
+        }
+    };
+
+    // ---- fragment reads ----
+    //   row layout: row (lane & 15) of a 16-row tile, chunk ks * 4 + lane / 16, swizzled: an address per k-step
+    //   column layout: lane = (k row (lane >> 2) & 3 of four, 8 bytes lane & 3 of the tile's 32): an address per 16-column tile
+    const int foff = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    const int krow = (lane >> 4) * 8 + ((lane >> 2) & 3);
+    unsigned ra[A_ROW ? 2 : MI], rb[B_ROW ? 2 : NJ];
+    if (A_ROW) { ra[0] = wm * (HR / 2) * 128 + foff; ra[1] = ra[0] ^ 64; }
+    else
+#pragma unroll
+        for (int i = 0; i < MI; ++i) ra[i] = krow * HR * 2 + (((wm * MI + i) ^ g_of(krow)) << 5) + (lane & 3) * 8;
+    if (B_ROW) { rb[0] = wn * NJ * 2048 + foff; rb[1] = rb[0] ^ 64; }
+    else
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) rb[j] = krow * HR * 2 + (((wn * NJ + j) ^ g_of(krow)) << 5) + (lane & 3) * 8;
+    constexpr int KS = 32 * HR * 2, HI = 4 * HR * 2;
+    const unsigned lds0 = gt_lds(smem);
+    bf16x8 af[2][MI], b0[2][NJ], b1[2][NJ];
+    // A half `ha` of buffer `buf` into af and / or B half `hb` into d (-1: none); with column-laid-out operands the reads have
+    // landed when this returns, with row-laid-out ones they are in flight
+    auto read = [&](const char* buf, int ha, bf16x8 (*d)[NJ], int hb) {
+        if (A_ROW && ha >= 0)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) af[ks][i] = *(const bf16x8*)(buf + ha * HB + ra[A_ROW ? ks : 0] + i * 2048);
+        if (B_ROW && hb >= 0)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) d[ks][j] = *(const bf16x8*)(buf + (2 + hb) * HB + rb[B_ROW ? ks : 0] + j * 2048);
+        if constexpr (!B_ROW) {
+            const unsigned at = lds0 + (unsigned)(buf - smem);
+            bf16x4 ta[2][MI][2], tb[2][NJ][2];
+            unsigned xa[MI], xb[NJ];
+            if constexpr (!A_ROW)
+                if (ha >= 0)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) xa[i] = at + ha * HB + ra[i];
+            if (hb >= 0)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) xb[j] = at + (2 + hb) * HB + rb[j];
+            if constexpr (A_ROW) {
+                if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
+            } else if (ha >= 0) {
+                if constexpr (MI == 4) {
+                    if (hb >= 0) gt_tr4_2<KS, HI>(ta, xa, tb, xb);
+                    else gt_tr4<KS, HI>(ta, xa);
+                } else {
+                    if (hb >= 0) gt_tr2_2<KS, HI>(ta, xa, tb, xb);
+                    else gt_tr2<KS, HI>(ta, xa);
+                }
+            } else if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (!A_ROW && ha >= 0)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) af[ks][i] = gt_join(ta[ks][i]);
+                if (hb >= 0)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) d[ks][j] = gt_join(tb[ks][j]);
+            }
+        }
+    };
+
+    f32x4 acc[2][MI][2][NJ];                                               // [A half][m-tile][B half][n-tile]
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[a][i][b][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+#define GT_MFMA(ha, hb, bfr)                                                                                    \
+    do {                                                                                                        \
+        __builtin_amdgcn_s_barrier();                                                                           \
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                      \
+        __builtin_amdgcn_sched_barrier(0);                                                                      \
+        __builtin_amdgcn_s_setprio(1);                                                                          \
+        _Pragma("unroll") for (int ks = 0; ks < 2; ++ks) _Pragma("unroll") for (int i = 0; i < MI; ++i)         \
+            _Pragma("unroll") for (int j = 0; j < NJ; ++j)                                                      \
+                acc[ha][i][hb][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[ks][j], af[ks][i], acc[ha][i][hb][j], 0, 0, 0); \
+        __builtin_amdgcn_s_setprio(0);                                                                          \
+        __builtin_amdgcn_sched_barrier(0);                                                                      \
+        if (T == 256) __builtin_amdgcn_s_barrier();                                                             \
+    } while (0)
+
+    stage(true, kt0, 1); stage(false, kt0, 0); stage(true, kt0, 0); stage(false, kt0, 1);
+    stage(true, kt0 + 1, 1); stage(false, kt0 + 1, 0); stage(true, kt0 + 1, 0);
+    GT_VMCNT(8);                                                           // B1, A0, B0 of the first K-tile
+    __builtin_amdgcn_s_barrier();
+    if (T == 256 && wm == 1) __builtin_amdgcn_s_barrier();                 // the lower half runs one barrier behind
+    read(smem, -1, b1, 1);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (T == 256) __builtin_amdgcn_s_barrier();
+#pragma clang loop unroll(disable)
+    for (int kt = kt0; kt < kt1; ++kt) {
+        const char* const buf = smem + ((kt - kt0) & 1) * 4 * HB;
+        const char* const nbuf = smem + ((kt + 1 - kt0) & 1) * 4 * HB;
+        read(buf, 0, b0, 0);                                               // c0
+        GT_MFMA(0, 0, b0);
+        stage(false, kt + 1, 1);                                           // c1
+        stage(true, kt + 2, 1);
+        GT_VMCNT(10);
+        GT_MFMA(0, 1, b1);
+        stage(false, kt + 2, 0);                                           // c2
+        read(buf, 1, nullptr, -1);
+        GT_VMCNT(10);
+        GT_MFMA(1, 1, b1);
+        stage(true, kt + 2, 0);                                            // c3
+        read(nbuf, -1, b1, 1);
+        GT_VMCNT(8);
+        GT_MFMA(1, 0, b0);
+    }
+    if (T == 256 && wm == 0) __builtin_amdgcn_s_barrier();                 // as many barriers as the lower half
+    GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
+#undef GT_MFMA
+
+    // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
+    const int cl = wn * NJ * 16 + (lane >> 4) * 4;
+    const int64_t mrow = i0 + wm * (HR / 2) + (lane & 15);
+    if (SPLIT) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                const int64_t m = mrow + a * HR + i * 16;
+                if (m >= p.I) continue;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const int n = j0 + (MODE == GL_FWD ? 0 : b * HR) + cl + j * 16, pl = MODE == GL_FWD ? b : plane;
+                        // ldp is a multiple of 4: four columns that start inside a row end inside its padding
+                        if (n < p.J) *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = acc[a][i][b][j];
+                    }
+            }
+        return;
+    }
+    const bool vec = (p.ldo & 3) == 0 && ((uintptr_t)p.out[MODE == GL_DW ? plane : 0] & 7) == 0;
+#pragma unroll
+    for (int b = 0; b < (MODE == GL_FWD ? 1 : 2); ++b)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int n = j0 + b * HR + cl + j * 16;
+            if (n >= p.J) continue;
+            const bool whole = vec && n + 4 <= p.J;
+            f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = {0.f, 0.f, 0.f, 0.f};
+            if (MODE == GL_FWD) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (p.bias[0] && n + r < p.J) bg[r] = bf2f(((const bf16_t*)p.bias[0])[n + r]);
+                    if (p.bias[1] && n + r < p.J) bu[r] = bf2f(((const bf16_t*)p.bias[1])[n + r]);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int64_t m = mrow + a * HR + i * 16;
+                    if (m >= p.I) continue;
+                    f32x4 v = acc[a][i][b][j];
+                    if (MODE == GL_FWD) {
+                        const f32x4 g = v + bg, u = acc[a][i][1][j] + bu;
+                        if (p.pre) {                                       // rows of ldpre = J rounded up to 4
+                            *(f32x4*)(p.pre + m * p.ldpre + n) = g;
+                            *(f32x4*)(p.pre + (p.I + m) * p.ldpre + n) = u;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = gl_act(p.act, g[r]) * u[r];
+                    }
+                    bf16_t* const o = (bf16_t*)p.out[MODE == GL_DW ? plane : 0] + m * p.ldo + n;
+                    if (whole) *(uint2*)o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (n + r < p.J) o[r] = f2bf(v[r]);
+                }
+        }
+}
+
+template <int MODE, int T, bool SPLIT>
+__global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile(GtArgs q) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int t = xcd_remap(blockIdx.x, gridDim.x);
+    const int tiles = gridDim.x / q.g.splits;
+    gt_product<MODE, T, SPLIT>(q, SPLIT ? t % tiles : t, SPLIT ? t / tiles : 0, smem);
+}
+
+// copy of a matrix whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero
+__global__ __launch_bounds__(256) void k_gated_pack(const bf16_t* src, int64_t ld, bf16_t* dst, int64_t ldd, int64_t rows, int64_t C) {
+    const int64_t per = ldd / 8, total = rows * per;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+        const int64_t r = t / per, c = (t - r * per) * 8;
+        bf16x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < C ? (short)src[r * ld + c + e] : (short)0;
+        *(bf16x8*)(dst + r * ldd + c) = v;
+    }
+}
+
+}  // namespace dp

@@ -38,11 +38,15 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(lib, dtype, M, N, K, backward, device):
-    need = lib.dp_gated_linear_workspace_bytes(dtype, M, N, K, backward)
+def _workspace(lib, operands, M, N, K, backward, device):
+    need = lib.dp_gated_linear_workspace_bytes(*operands, M, N, K, backward)
     if need == 0:
         _lib.check(-1, "dp_gated_linear_workspace_bytes")
     return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _operands(x, w_gate, w_up):
+    return _DTYPES[x.dtype], x.data_ptr(), _ld(x), w_gate.data_ptr(), w_up.data_ptr(), _ld(w_gate)
 
 
 def _stream(device):
@@ -59,15 +63,16 @@ def _weights(w_gate, w_up):
 
 def _forward(x, w_gate, w_up, b_gate, b_up, act, save):
     lib = _lib.load()
-    (M, K), N, dt = x.shape, w_gate.shape[0], _DTYPES[x.dtype]
+    (M, K), N = x.shape, w_gate.shape[0]
     h = torch.empty((M, N), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
         pre = None
         if save:
             pre = torch.empty(lib.dp_gated_linear_pre_bytes(M, N), dtype=torch.uint8, device=x.device)
         if M:
-            ws = _workspace(lib, dt, M, N, K, 0, x.device)
-            rc = lib.dp_gated_linear(dt, x.data_ptr(), _ld(x), w_gate.data_ptr(), w_up.data_ptr(), _ld(w_gate), _ptr(b_gate), _ptr(b_up),
+            ops = _operands(x, w_gate, w_up)
+            ws = _workspace(lib, ops, M, N, K, 0, x.device)
+            rc = lib.dp_gated_linear(*ops, _ptr(b_gate), _ptr(b_up),
                                      h.data_ptr(), N, _ptr(pre), M, N, K, act, ws.data_ptr(), ws.numel(), _stream(x.device))
             _lib.check(rc, "dp_gated_linear")
     return h, pre
@@ -88,7 +93,7 @@ class _GatedLinear(torch.autograd.Function):
         x, w_gate, w_up, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
         lib = _lib.load()
-        (M, K), N, dt = x.shape, w_gate.shape[0], _DTYPES[x.dtype]
+        (M, K), N = x.shape, w_gate.shape[0]
         dh = _rows(dh)
 
         def out(wanted, *shape):
@@ -98,8 +103,9 @@ class _GatedLinear(torch.autograd.Function):
         dwg, dwu = out(need[1], N, K), out(need[2], N, K)
         dbg, dbu = out(need[3], N), out(need[4], N)
         with torch.cuda.device(x.device):
-            ws = _workspace(lib, dt, M, N, K, 1, x.device)
-            rc = lib.dp_gated_linear_bwd(dt, x.data_ptr(), _ld(x), w_gate.data_ptr(), w_up.data_ptr(), _ld(w_gate), pre.data_ptr(), dh.data_ptr(), _ld(dh),
+            ops = _operands(x, w_gate, w_up)
+            ws = _workspace(lib, ops, M, N, K, 1, x.device)
+            rc = lib.dp_gated_linear_bwd(*ops, pre.data_ptr(), dh.data_ptr(), _ld(dh),
                                          _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), M, N, K, ctx.act, ws.data_ptr(), ws.numel(), _stream(x.device))
         _lib.check(rc, "dp_gated_linear_bwd")
         return dx, dwg, dwu, dbg, dbu, None

@@ -216,6 +216,10 @@ int dp_linear(int dtype, const void* A, const void* W, const float* bias, void* 
  *   "fuse_mid"      1 (default) = for bf16 plans with d_in = 256 the arithmetic after a Heun iteration's first evaluation
  *                   (diffusion_utils.py:100-101) runs in the epilogue of the mlp.6 GEMM instead of a kernel of its own;
  *                   bit-identical results.
+ *   "gated_kernel"  which kernel runs the products of dp_gated_linear and its backward: 0 (default) = by size and alignment, 1 = the
+ *                   general kernel (any size, stride and type), 128 / 256 = the bf16 tile kernels of that tile.
+ *   "gated_splits"  slices of the contraction of those products: 0 (default) = by size, else that many (at most one per K-tile).  The
+ *                   order of sums, and with it the last bits, depend on it.
  */
 int dp_tune(const char* key, int value);
 
@@ -283,15 +287,17 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  *                for the backward pass; the layout is the library's own
  * Any strides, element-aligned pointers, 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
  * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
- * (workspace >= dp_gated_linear_workspace_bytes(.., backward), 256-byte aligned; calls that may overlap in time need
- * workspaces of their own), and may be captured into a graph.
+ * (workspace >= dp_gated_linear_workspace_bytes(.., backward) for the same arguments, 256-byte aligned; calls that may
+ * overlap in time need workspaces of their own), and may be captured into a graph.  bf16 is fastest where x and the weights
+ * have rows that start on 16 bytes and K % 8 == 0: other rows are first copied to the workspace.
  *
  * dp_gated_linear_bwd: gradients for a given dh [M, N] (row stride lddh).  dx [M, K], dw_gate, dw_up [N, K], db_gate,
  * db_up [N]: contiguous, overwritten, each may be NULL (not wanted).  M = 0 writes zeros to the weights' gradients.
  * bf16: dg and du are rounded to bf16 once, as the operands of the three products; bias gradients sum them unrounded.
  */
 size_t dp_gated_linear_pre_bytes(int64_t M, int N);
-size_t dp_gated_linear_workspace_bytes(int dtype, int64_t M, int N, int K, int backward);
+size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw,
+                                       int64_t M, int N, int K, int backward);
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
                     void* h, int64_t ldh, void* pre, int64_t M, int N, int K, int act, void* workspace, size_t workspace_bytes, void* stream);
 int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,

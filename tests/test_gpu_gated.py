@@ -123,6 +123,44 @@ def test_against_formula(M, K, N, dtype):
     check(*make(M, K, N, dtype, seed=M * 7 + K + N), act="silu")
 
 
+@pytest.fixture
+def tune():
+    from diffputer_amd import _lib
+    lib = _lib.load()
+
+    def put(kernel, splits):
+        _lib.check(lib.dp_tune(b"gated_kernel", kernel), "dp_tune")
+        _lib.check(lib.dp_tune(b"gated_splits", splits), "dp_tune")
+
+    yield put
+    put(0, 0)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (40, 64, 64), (70, 200, 40), (129, 64, 65), (257, 72, 129), (300, 136, 264), (513, 1032, 264), (600, 71, 300)])
+@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (128, 0), (128, 3), (256, 0), (256, 2), (256, 5)])
+def test_every_kernel(tune, kernel, splits, M, K, N):
+    tune(kernel, splits)
+    check(*make(M, K, N, "bf16", seed=M + K), act="silu")
+
+
+@pytest.mark.parametrize("kernel", [1, 128, 256])
+def test_every_kernel_strides(tune, kernel):
+    """A column range of a wider table: aligned rows are read where they are (the columns beside them hold NaN), others copied."""
+    from diffputer_amd.gated import gated_linear
+    tune(kernel, 0)
+    x, wg, wu, bg, bu, dh = make(300, 72, 136, "bf16", seed=6)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    for off in (0, 8, 3):
+        wide = torch.full((300, 96), float("nan"), dtype=x.dtype, device=DEV)
+        wide[:, off:off + 72] = x.to(DEV)
+        leaves = [wide[:, off:off + 72], *[t.to(DEV) for t in (wg, wu, bg, bu)]]
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        h = gated_linear(*leaves)
+        close(h, ref.h, ref.eh, "h")
+        for name, g in zip(("x", "wg", "wu", "bg", "bu"), torch.autograd.grad(h, leaves, dh.to(DEV))):
+            close(g, getattr(ref, "d" + name), getattr(ref, "ed" + name), "d" + name)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("act", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("bias", [True, False])
@@ -282,10 +320,11 @@ def test_nothing_beside_the_output_is_written(M, N, dtype):
     want = gated_linear(x, wg, wu, bg, bu)
     lib = _lib.load()
     buf = torch.full((M + 9, N + 13), 7.0, dtype=x.dtype, device=DEV)
-    need = lib.dp_gated_linear_workspace_bytes(_DTYPES[x.dtype], M, N, K, 0)
+    ops = (_DTYPES[x.dtype], x.data_ptr(), K, wg.data_ptr(), wu.data_ptr(), K)
+    need = lib.dp_gated_linear_workspace_bytes(*ops, M, N, K, 0)
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)
     h = buf[3:3 + M, 5:5 + N]
-    rc = lib.dp_gated_linear(_DTYPES[x.dtype], x.data_ptr(), K, wg.data_ptr(), wu.data_ptr(), K, bg.data_ptr(), bu.data_ptr(), h.data_ptr(), N + 13, None,
+    rc = lib.dp_gated_linear(*ops, bg.data_ptr(), bu.data_ptr(), h.data_ptr(), N + 13, None,
                              M, N, K, 1, ws.data_ptr(), need, C.c_void_p(torch.cuda.current_stream().cuda_stream))
     assert rc == 0, lib.dp_last_error()
     assert torch.equal(h, want)

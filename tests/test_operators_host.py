@@ -110,14 +110,20 @@ def test_gated_sizes():
     lib = _lib.load()
     assert lib.dp_gated_linear_pre_bytes(10, 33) == 10 * 2 * 36 * 4
     assert lib.dp_gated_linear_pre_bytes(-1, 33) == 0 and lib.dp_gated_linear_pre_bytes(5, 0) == 0
+
+    def ws(dtype, M, N, K, backward, at=FAKE):
+        return lib.dp_gated_linear_workspace_bytes(dtype, at, K, at, at, K, M, N, K, backward)
+
     for args in ((2, 5, 5, 5, 0), (0, -1, 5, 5, 0), (0, 5, 0, 5, 1), (0, 5, 5, 0, 1)):
-        assert lib.dp_gated_linear_workspace_bytes(*args) == 0
+        assert ws(*args) == 0
     for dtype in (0, 1):
         for M, N, K in ((0, 5, 5), (1, 1, 1), (1, 2048, 1024), (24, 8192, 4096), (16384, 64, 9), (4096, 2048, 1024), ((1 << 29) - 1, 64, 64)):
             for backward in (0, 1):
-                assert lib.dp_gated_linear_workspace_bytes(dtype, M, N, K, backward) >= 256
+                assert ws(dtype, M, N, K, backward) >= 256
     # a float32 plane of a large batch passes 32 bits
-    assert lib.dp_gated_linear_workspace_bytes(0, 1 << 20, 4096, 64, 1) >= 2 * (1 << 20) * 4096 * 4
+    assert ws(0, 1 << 20, 4096, 64, 1) >= 2 * (1 << 20) * 4096 * 4
+    # rows that are not aligned are copied: x and both weights
+    assert ws(1, 4096, 2048, 1024, 0, FAKE + 2) >= (4096 + 2 * 2048) * 1024 * 2 > ws(1, 4096, 2048, 1024, 0)
     assert lib.dp_gated_linear_pre_bytes(1 << 20, 4096) == 2 * (1 << 20) * 4096 * 4
 
 
