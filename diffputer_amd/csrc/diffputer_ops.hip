@@ -10,6 +10,8 @@
 #include <vector>
 
 #include "dp_gated.h"
+#include "dp_gated_f32.h"
+#include "dp_gated_rows.h"
 #include "dp_gated_tile.h"
 #include "dp_grads.h"
 #include "dp_util.h"
@@ -41,6 +43,11 @@ template <int MODE> static hipError_t gt_attributes() {
         const hipError_t e = hipFuncSetAttribute(k[i], hipFuncAttributeMaxDynamicSharedMemorySize, i < 2 ? GtShape<256>::LDS : GtShape<128>::LDS);
         if (e != hipSuccess) return e;
     }
+    const void* f[] = {(const void*)k_gated_f32<MODE, false, false>, (const void*)k_gated_f32<MODE, false, true>, (const void*)k_gated_f32<MODE, true, false>, (const void*)k_gated_f32<MODE, true, true>};
+    for (const void* k1 : f) {
+        const hipError_t e = hipFuncSetAttribute(k1, hipFuncAttributeMaxDynamicSharedMemorySize, GF_LDS);
+        if (e != hipSuccess) return e;
+    }
     return hipSuccess;
 }
 static int gt_ready() {
@@ -58,7 +65,9 @@ static int gt_ready() {
     return DP_OK;
 }
 
-// How a product runs: the general kernel (T = 0) or a tile kernel, and how many slices of the contraction.
+// How a product runs: by the general kernel (T = 0), a bf16 tile kernel (T = 128 or 256), the float32 tile kernel (GF_T) or the
+// kernel for few rows (GL_ROWS, forward only), and how many slices of the contraction.
+constexpr int GL_ROWS = 1;
 struct GlShape { int mode; int64_t I; int J; int64_t C; int planes; };
 struct GlPlan { int T, kt_per, splits; int64_t ti, tj; };
 static int64_t gl_ldp(int J) { return round_up<int64_t>(J, 4); }
@@ -73,7 +82,7 @@ static void gl_cut(GlPlan& pl, const GlShape& s, int64_t tiles, int64_t nk, int6
     pl.kt_per = (int)ceil_div<int64_t>(nk, n);
     pl.splits = (int)ceil_div<int64_t>(nk, pl.kt_per);
 }
-static GlPlan gl_plan(const GlShape& s, bool tile) {
+static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
     GlPlan pl;
     const int segs = s.mode == GL_DX ? 2 : 1;
     auto shape = [&](int T) {
@@ -83,10 +92,12 @@ static GlPlan gl_plan(const GlShape& s, bool tile) {
         return pl.ti * pl.tj * s.planes;
     };
     const int forced = g_gated_kernel.load(std::memory_order_relaxed);
+    if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0) return {GL_ROWS, 0, 1, 1, 1};
     if (tile && forced != 1) {
-        const int64_t nk = ceil_div<int64_t>(s.C, 64) * segs;
-        int64_t tiles = shape(256);
-        if (forced == 128 || (forced == 0 && tiles < 256)) tiles = shape(128);
+        const bool f32 = dtype == DP_DTYPE_F32;
+        const int64_t nk = ceil_div<int64_t>(s.C, f32 ? GF_K : 64) * segs;
+        int64_t tiles = shape(f32 ? GF_T : 256);
+        if (!f32 && (forced == 128 || (forced == 0 && tiles < 256))) tiles = shape(128);
         if (tiles < (int64_t)1 << 22) {                           // the grid of a launch
             gl_cut(pl, s, tiles, nk, pl.T == 256 ? 256 : 512, 4);
             return pl;
@@ -96,8 +107,8 @@ static GlPlan gl_plan(const GlShape& s, bool tile) {
     gl_cut(pl, s, tiles, ceil_div<int64_t>(s.C, GG_K) * segs, 512, 8);
     return pl;
 }
-static size_t gl_split_bytes(const GlShape& s, bool tile) {
-    const GlPlan c = gl_plan(s, tile);
+static size_t gl_split_bytes(const GlShape& s, int dtype, bool tile) {
+    const GlPlan c = gl_plan(s, dtype, tile);
     return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0;
 }
 
@@ -111,17 +122,52 @@ static int gt_launch(const GlArgs& a, const GlPlan& pl, int planes, hipStream_t 
     return DP_OK;
 }
 
+template <int MODE>
+static int gf_launch(const GlArgs& a, const GlPlan& pl, int planes, bool vec, hipStream_t st) {
+    const GtArgs q = {a, (int)pl.ti, (int)pl.tj, 8};
+    const dim3 grid((unsigned)(pl.ti * pl.tj * planes * pl.splits)), block(GF_THREADS);
+    if (pl.splits > 1) {
+        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, true, true>), grid, block, GF_LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_f32<MODE, false, true>), grid, block, GF_LDS, st, q);
+    } else {
+        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, true, false>), grid, block, GF_LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_f32<MODE, false, false>), grid, block, GF_LDS, st, q);
+    }
+    DP_LAUNCH_CHECK("k_gated_f32");
+    return DP_OK;
+}
+
+template <typename T, int MT, int CB>
+static int gr_launch(const GlArgs& a, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)ceil_div(a.J, CB)), block(GR_WAVES * 64);
+    if (vec) hipLaunchKernelGGL((k_gated_rows<T, MT, CB, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_gated_rows<T, MT, CB, false>), grid, block, 0, st, a);
+    DP_LAUNCH_CHECK("k_gated_rows");
+    return DP_OK;
+}
+template <typename T>
+static int gr_rows(const GlArgs& a, bool vec, hipStream_t st) {
+    const bool wide = a.J >= 16 * 256;                            // narrower: 8 columns per workgroup, twice as many workgroups
+    if (a.I <= 16) return wide ? gr_launch<T, 1, 16>(a, vec, st) : gr_launch<T, 1, 8>(a, vec, st);
+    if (a.I <= 32) return wide ? gr_launch<T, 2, 16>(a, vec, st) : gr_launch<T, 2, 8>(a, vec, st);
+    return wide ? gr_launch<T, 4, 16>(a, vec, st) : gr_launch<T, 4, 8>(a, vec, st);
+}
+
 template <typename T, int MODE>
-static int gl_mm(GlArgs a, const GlShape& s, bool tile, hipStream_t st) {
-    const GlPlan c = gl_plan(s, tile);
+static int gl_mm(GlArgs a, const GlShape& s, bool tile, bool vec, hipStream_t st) {
+    constexpr int DT = sizeof(T) == 2 ? DP_DTYPE_BF16 : DP_DTYPE_F32;
+    const GlPlan c = gl_plan(s, DT, tile);
     int rc;
     a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
+    if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(a, vec, st) : DP_EINVAL;
     if (c.T == 0) {
         hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, a);
         DP_LAUNCH_CHECK("k_gated_mm");
     } else {
         if ((rc = gt_ready())) return rc;
-        if ((rc = c.T == 256 ? gt_launch<MODE, 256>(a, c, s.planes, st) : gt_launch<MODE, 128>(a, c, s.planes, st))) return rc;
+        if (DT == DP_DTYPE_F32) rc = gf_launch<MODE>(a, c, s.planes, vec, st);
+        else rc = c.T == 256 ? gt_launch<MODE, 256>(a, c, s.planes, st) : gt_launch<MODE, 128>(a, c, s.planes, st);
+        if (rc) return rc;
     }
     if (c.splits > 1) {
         const int64_t n = s.I * s.planes * ceil_div<int64_t>(s.J, 4);
@@ -132,19 +178,32 @@ static int gl_mm(GlArgs a, const GlShape& s, bool tile, hipStream_t st) {
     return DP_OK;
 }
 
-// The tile kernels load 16 bytes at a time: an operand is read where it is if its rows start on 16 bytes and end on 8
-// elements.  Others are copied to the workspace (rows padded with zeros) where the product is large enough to pay for it.
-static bool gt_direct(const void* p, int64_t ld, int64_t cols) { return aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= 1 << 22; }
+// 16-byte loads need rows that start on 16 bytes and end on a whole chunk.  The bf16 tile kernels know no others: such operands
+// are copied to the workspace (rows padded with zeros) where the product is large enough to pay for it, and smaller ones run
+// on the general kernel.  The float32 tile kernel and the kernel for few rows have a form with narrower loads.
+static bool gt_direct(const void* p, int64_t ld, int64_t cols, int chunk) { return aligned(p, 16) && ld % chunk == 0 && cols % chunk == 0; }
 constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
-struct GtOperands { bool tile, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
+constexpr int64_t GT_MAX_LD = 1 << 21;                           // 128 rows of float32 stay within 2^30 bytes
+struct GtOperands { bool tile, vec, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
 static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
     GtOperands o;
-    o.pack_x = !gt_direct(x, ldx, K);
-    o.pack_w = !gt_direct(wg, ldw, K) || !gt_direct(wu, ldw, K);
-    o.ldk = round_up<int64_t>(K, 8);
+    const bool bf = dtype == DP_DTYPE_BF16;
+    const int chunk = bf ? 8 : 4;
+    const bool x_in = gt_direct(x, ldx, K, chunk), w_in = gt_direct(wg, ldw, K, chunk) && gt_direct(wu, ldw, K, chunk);
+    const bool short_rows = ldx <= GT_MAX_LD && ldw <= GT_MAX_LD;
     const int forced = g_gated_kernel.load(std::memory_order_relaxed);
-    o.tile = dtype == DP_DTYPE_BF16 && forced != 1 && (forced || (!o.pack_x && !o.pack_w) || M * N * K >= GT_PACK_LEAST);
-    if (!o.tile) o.pack_x = o.pack_w = false;
+    o.vec = x_in && w_in;
+    o.pack_x = o.pack_w = false;
+    o.ldk = round_up<int64_t>(K, 8);
+    if (!bf) {
+        o.tile = short_rows && forced != 1;
+        return o;
+    }
+    o.tile = forced != 1 && (forced || (o.vec && short_rows) || M * N * K >= GT_PACK_LEAST);
+    if (o.tile) {
+        o.pack_x = !x_in || ldx > GT_MAX_LD || K % 8;
+        o.pack_w = !w_in || ldw > GT_MAX_LD || K % 8;
+    }
     return o;
 }
 struct Carver {
@@ -181,18 +240,17 @@ struct GlIn {
     int64_t fwd_c() const { return o.pack_x && o.pack_w ? o.ldk : K; }
 };
 static GlIn gl_in(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
-    GlIn in = {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
-    if (K % 8 && in.o.tile) in.o.pack_x = in.o.pack_w = true;
-    return in;
+    return {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
 }
 
 // forward workspace: copies, partial sums
 struct GlFwd { float* part; size_t bytes; };
-static GlFwd gl_fwd_carve(GlIn& in, void* base) {
+static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
+    if (gl_plan({GL_FWD, in.M, in.N, in.K, 1}, dtype, in.o.tile).T == GL_ROWS) in.o.pack_x = in.o.pack_w = false;
     Carver c = {(char*)base};
     in.carve(c);
     GlFwd w;
-    w.part = (float*)c.take(gl_split_bytes({GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile));
+    w.part = (float*)c.take(gl_split_bytes({GL_FWD, in.M, in.N, in.fwd_c(), 1}, dtype, in.o.tile));
     w.bytes = c.off;
     return w;
 }
@@ -221,20 +279,20 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, void* base) {
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
     w.dgu = c.take((size_t)2 * M * w.ldg * (dtype == DP_DTYPE_BF16 ? 2 : 4));
     w.colpart = (float*)c.take((size_t)w.nblk * 2 * w.ldg * 4);
-    w.part = (float*)c.take(std::max(gl_split_bytes({GL_DX, M, K, N, 1}, in.o.tile), gl_split_bytes({GL_DW, N, K, M, 2}, in.o.tile)));
+    w.part = (float*)c.take(std::max(gl_split_bytes({GL_DX, M, K, N, 1}, dtype, in.o.tile), gl_split_bytes({GL_DW, N, K, M, 2}, dtype, in.o.tile)));
     w.bytes = c.off;
     return w;
 }
 
 template <typename T>
 static int gl_forward(GlArgs a, GlIn& in, void* ws, hipStream_t st) {
-    const GlFwd w = gl_fwd_carve(in, ws);
+    const GlFwd w = gl_fwd_carve(sizeof(T) == 2 ? DP_DTYPE_BF16 : DP_DTYPE_F32, in, ws);
     int rc;
     if ((rc = in.pack(true, true, st))) return rc;
     a.A[0] = in.x;
     a.B[0] = in.wg; a.B[1] = in.wu;
     a.part = w.part;
-    return gl_mm<T, GL_FWD>(a, {GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile, st);
+    return gl_mm<T, GL_FWD>(a, {GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile, in.o.vec, st);
 }
 
 template <typename T>
@@ -275,13 +333,13 @@ static int gl_backward(int dtype, GlIn& in, const float* pre, const GlOp& dh, T*
     if (dx) {
         a.B[0] = in.wg; a.B[1] = in.wu;
         a.out[0] = dx; a.ldo = K;
-        if ((rc = gl_mm<T, GL_DX>(a, {GL_DX, M, K, N, 1}, in.o.tile, st))) return rc;
+        if ((rc = gl_mm<T, GL_DX>(a, {GL_DX, M, K, N, 1}, in.o.tile, in.o.vec, st))) return rc;
     }
     if (dw[0] || dw[1]) {
         a.B[0] = in.x;
         a.out[0] = dw[0]; a.out[1] = dw[1]; a.ldo = K;
         a.zfirst = dw[0] ? 0 : 1;
-        if ((rc = gl_mm<T, GL_DW>(a, {GL_DW, N, K, M, dw[0] && dw[1] ? 2 : 1}, in.o.tile, st))) return rc;
+        if ((rc = gl_mm<T, GL_DW>(a, {GL_DW, N, K, M, dw[0] && dw[1] ? 2 : 1}, in.o.tile, in.o.vec, st))) return rc;
     }
     return DP_OK;
 }
@@ -356,7 +414,7 @@ size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, co
     if (gl_check("dp_gated_linear_workspace_bytes", dtype, M, N, K, 0)) return 0;
     if (M == 0) return 256;
     GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
-    return std::max<size_t>(backward ? gl_bwd_carve(dtype, in, nullptr).bytes : gl_fwd_carve(in, nullptr).bytes, 256);
+    return std::max<size_t>(backward ? gl_bwd_carve(dtype, in, nullptr).bytes : gl_fwd_carve(dtype, in, nullptr).bytes, 256);
 }
 
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,

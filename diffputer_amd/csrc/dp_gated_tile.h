@@ -57,6 +57,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t gt_buffer(const char* p, const
     return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00027000);
 }
 
+// EL bytes per lane from the buffer's byte `off` on into LDS, lane after lane from `dst` on
+template <int EL> __device__ __forceinline__ void gt_load(__amdgpu_buffer_rsrc_t buf, char* dst, unsigned off) {
+    if constexpr (EL == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 16, (int)off, 0, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 4, (int)off, 0, 0, 0);
+}
+
 // Fragments of column-laid-out half-tiles: for every 16-column tile and k-step two reads of 4 k's each, in one statement that
 // ends with their wait (KS, HI: byte offsets of the second k-step and of a fragment's second four k's).
 template <int KS, int HI> __device__ __forceinline__ void gt_tr4(bf16x4 (&a)[2][4][2], const unsigned (&ra)[4]) {
@@ -124,6 +130,22 @@ template <int KS, int HI> __device__ __forceinline__ void gt_tr2_2(bf16x4 (&a)[2
 }
 __device__ __forceinline__ bf16x8 gt_join(const bf16x4 (&f)[2]) { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// workgroup -> (slice, tile): neighbouring tiles on one XCD
+template <bool SPLIT> __device__ __forceinline__ int gt_slice(const GlArgs& p, int& slice) {
+    const int t = xcd_remap(blockIdx.x, gridDim.x), tiles = gridDim.x / p.splits;
+    slice = SPLIT ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
+    return SPLIT ? __builtin_amdgcn_readfirstlane(t % tiles) : t;
+}
+// tile -> (plane, row, column): groups of q.group tile rows, column by column within a group
+template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int tile, int& plane, int& ti, int& tj) {
+    const int per_plane = q.nti * q.ntj;
+    plane = MODE == GL_DW ? q.g.zfirst + __builtin_amdgcn_readfirstlane(tile / per_plane) : 0;
+    const int tp = tile % per_plane, gsz = q.group * q.ntj, grp = tp / gsz, in = tp - grp * gsz;
+    const int rows_here = min(q.group, q.nti - grp * q.group);
+    ti = __builtin_amdgcn_readfirstlane(grp * q.group + in % rows_here);
+    tj = __builtin_amdgcn_readfirstlane(in / rows_here);
+}
+
 template <int MODE, int T, bool SPLIT>
 __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice, char* smem) {
     using S = GtShape<T>;
@@ -135,12 +157,8 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    // tile -> (row, column): groups of q.group tile rows, column by column within a group
-    const int per_plane = q.nti * q.ntj;
-    const int plane = MODE == GL_DW ? p.zfirst + __builtin_amdgcn_readfirstlane(tile / per_plane) : 0;
-    const int tp = tile % per_plane, gsz = q.group * q.ntj, grp = tp / gsz, in = tp - grp * gsz;
-    const int rows_here = min(q.group, q.nti - grp * q.group);
-    const int ti = __builtin_amdgcn_readfirstlane(grp * q.group + in % rows_here), tj = __builtin_amdgcn_readfirstlane(in / rows_here);
+    int plane, ti, tj;
+    gt_tile<MODE>(q, tile, plane, ti, tj);
     const int64_t i0 = (int64_t)ti * T;
     const int j0 = tj * (MODE == GL_FWD ? HR : T);
 
@@ -183,7 +201,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
         for (int s = 0; s < 2; ++s) {
             unsigned vo = is_b ? vb[s] : va[s];
             if (row && B_ROW && kt == tail && tail_out) vo = OUTSIDE;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)(dst + s * NW * 1024), 16, (int)vo, 0, 0, 0);
+            gt_load<16>(buf, dst + s * NW * 1024, vo);
         }
     };
 
@@ -373,9 +391,9 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
 template <int MODE, int T, bool SPLIT>
 __global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile(GtArgs q) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int t = xcd_remap(blockIdx.x, gridDim.x);
-    const int tiles = gridDim.x / q.g.splits;
-    gt_product<MODE, T, SPLIT>(q, SPLIT ? t % tiles : t, SPLIT ? t / tiles : 0, smem);
+    int slice;
+    const int tile = gt_slice<SPLIT>(q.g, slice);
+    gt_product<MODE, T, SPLIT>(q, tile, slice, smem);
 }
 
 // copy of a matrix whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero

@@ -10,7 +10,8 @@ other modules of a denoiser do.
 """
 from __future__ import annotations
 
-import ctypes as C
+import contextlib
+import functools
 import math
 
 import torch
@@ -21,11 +22,12 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.DP_DTYPE_F32, torch.bfloat16: _lib.DP_DTYPE_BF16}
 _ACTS = {"none": 0, "silu": 1, "gelu": 2}
+_EWORKSPACE = -4
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] with contiguous rows that do not overlap: `t` itself, or a copy."""
-    if t.shape[0] == 0 or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1)):
+    if t.is_contiguous() or t.shape[0] == 0 or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1)):
         return t
     return t.contiguous()
 
@@ -38,50 +40,49 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(lib, operands, M, N, K, backward, device):
-    need = lib.dp_gated_linear_workspace_bytes(*operands, M, N, K, backward)
+@functools.lru_cache(maxsize=4096)
+def _need(dtype, ox, ldx, og, ou, ldw, M, N, K, backward):
+    """Workspace bytes of a call: by its sizes, strides and the pointers' alignment (their last 4 bits), nothing else."""
+    lib = _lib.load()
+    need = lib.dp_gated_linear_workspace_bytes(dtype, 16 + ox, ldx, 16 + og, 16 + ou, ldw, M, N, K, backward)
     if need == 0:
         _lib.check(-1, "dp_gated_linear_workspace_bytes")
-    return torch.empty(need, dtype=torch.uint8, device=device)
+    return need
 
 
-def _operands(x, w_gate, w_up):
-    return _DTYPES[x.dtype], x.data_ptr(), _ld(x), w_gate.data_ptr(), w_up.data_ptr(), _ld(w_gate)
-
-
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-def _weights(w_gate, w_up):
-    """Both weights with one row stride."""
-    w_gate, w_up = _rows(w_gate), _rows(w_up)
-    if w_gate.shape[0] > 1 and w_gate.stride(0) != w_up.stride(0):
-        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
-    return w_gate, w_up
+def _call(name, x, w_gate, w_up, rest, M, N, K, act, backward):
+    """One call of the C entry `name` on the current stream of x's device, with a workspace of its own."""
+    lib = _lib.load()
+    dt, px, pg, pu, ldx, ldw = _DTYPES[x.dtype], x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ld(x), _ld(w_gate)
+    index = x.device.index
+    key = (dt, px & 15, ldx, pg & 15, pu & 15, ldw, M, N, K, backward)
+    guard = torch.cuda.device(index) if torch.cuda.current_device() != index else contextlib.nullcontext()
+    with guard:
+        for attempt in range(2):
+            need = _need(*key)
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            rc = getattr(lib, name)(dt, px, ldx, pg, pu, ldw, *rest, M, N, K, act, ws.data_ptr(), need, torch.cuda.current_stream(index).cuda_stream)
+            if rc != _EWORKSPACE or attempt:
+                break
+            _need.cache_clear()                               # a dp_tune setting changed what the kernels need
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def _forward(x, w_gate, w_up, b_gate, b_up, act, save):
-    lib = _lib.load()
     (M, K), N = x.shape, w_gate.shape[0]
-    h = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        pre = None
-        if save:
-            pre = torch.empty(lib.dp_gated_linear_pre_bytes(M, N), dtype=torch.uint8, device=x.device)
-        if M:
-            ops = _operands(x, w_gate, w_up)
-            ws = _workspace(lib, ops, M, N, K, 0, x.device)
-            rc = lib.dp_gated_linear(*ops, _ptr(b_gate), _ptr(b_up),
-                                     h.data_ptr(), N, _ptr(pre), M, N, K, act, ws.data_ptr(), ws.numel(), _stream(x.device))
-            _lib.check(rc, "dp_gated_linear")
+    h = x.new_empty((M, N))
+    pre = None
+    if save:
+        pre = torch.empty(_lib.load().dp_gated_linear_pre_bytes(M, N), dtype=torch.uint8, device=x.device)
+    if M:
+        _call("dp_gated_linear", x, w_gate, w_up, (_ptr(b_gate), _ptr(b_up), h.data_ptr(), N, _ptr(pre)), M, N, K, act, 0)
     return h, pre
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
-        w_gate, w_up = _weights(w_gate, w_up)
         h, pre = _forward(x, w_gate, w_up, b_gate, b_up, act, True)
         ctx.save_for_backward(x, w_gate, w_up, pre)
         ctx.act = act
@@ -92,23 +93,36 @@ class _GatedLinear(torch.autograd.Function):
     def backward(ctx, dh):
         x, w_gate, w_up, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
-        lib = _lib.load()
         (M, K), N = x.shape, w_gate.shape[0]
         dh = _rows(dh)
-
-        def out(wanted, *shape):
-            return torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None
-
-        dx = out(need[0], M, K)
-        dwg, dwu = out(need[1], N, K), out(need[2], N, K)
-        dbg, dbu = out(need[3], N), out(need[4], N)
-        with torch.cuda.device(x.device):
-            ops = _operands(x, w_gate, w_up)
-            ws = _workspace(lib, ops, M, N, K, 1, x.device)
-            rc = lib.dp_gated_linear_bwd(*ops, pre.data_ptr(), dh.data_ptr(), _ld(dh),
-                                         _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu), M, N, K, ctx.act, ws.data_ptr(), ws.numel(), _stream(x.device))
-        _lib.check(rc, "dp_gated_linear_bwd")
+        dx = x.new_empty((M, K)) if need[0] else None
+        dwg = x.new_empty((N, K)) if need[1] else None
+        dwu = x.new_empty((N, K)) if need[2] else None
+        dbg = x.new_empty(N) if need[3] else None
+        dbu = x.new_empty(N) if need[4] else None
+        _call("dp_gated_linear_bwd", x, w_gate, w_up, (pre.data_ptr(), dh.data_ptr(), _ld(dh), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dbg), _ptr(dbu)), M, N, K, ctx.act, 1)
         return dx, dwg, dwu, dbg, dbu, None
+
+
+def _refuse(x, w_gate, w_up, b_gate, b_up, act):
+    """The error of a call that gated_linear does not take."""
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
+    if x.ndim < 1 or w_gate.ndim != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}: expected [..., K], [N, K], [N, K]")
+    N, K = w_gate.shape
+    if N < 1 or K < 1:
+        raise ValueError(f"w_gate {tuple(w_gate.shape)}: N and K have to be at least 1")
+    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)):
+        if t is None:
+            continue
+        if name.startswith("b_") and tuple(t.shape) != (N,):
+            raise ValueError(f"{name} {tuple(t.shape)} does not match N = {N}")
+        if t.dtype != x.dtype or t.dtype not in _DTYPES:
+            raise ValueError(f"{name} is {t.dtype}: all tensors have to be float32, or all bfloat16")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    raise _lib.DiffputerError("gated_linear needs tensors on a CUDA (ROCm) device; there is no CPU fallback")
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: torch.Tensor | None = None,
@@ -118,33 +132,33 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     x [..., K]; w_gate, w_up [N, K]; b_gate, b_up [N] or None each; all of one dtype (float32 or bfloat16) on one CUDA (ROCm)
     device.  act: "silu", "gelu" (g Phi(g), not its tanh approximation) or "none".  Row strides are used as they are (a column range
     of a wider table is not copied); other layouts are copied.  Runs on torch's current stream of x's device; first
-    derivatives only.  A row's result does not depend on the rows beside it."""
-    if act not in _ACTS:
-        raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
-    if x.ndim < 1 or w_gate.ndim != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
-        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}: expected [..., K], [N, K], [N, K]")
-    N, K = w_gate.shape
-    if N < 1 or K < 1:
-        raise ValueError(f"w_gate {tuple(w_gate.shape)}: N and K have to be at least 1")
-    given = [("x", x), ("w_gate", w_gate), ("w_up", w_up), ("b_gate", b_gate), ("b_up", b_up)]
-    for name, t in given:
-        if t is None:
-            continue
-        if name.startswith("b_") and tuple(t.shape) != (N,):
-            raise ValueError(f"{name} {tuple(t.shape)} does not match N = {N}")
-        if t.dtype != x.dtype or t.dtype not in _DTYPES:
-            raise ValueError(f"{name} is {t.dtype}: all tensors have to be float32, or all bfloat16")
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    if not x.is_cuda:
-        raise _lib.DiffputerError("gated_linear needs tensors on a CUDA (ROCm) device; there is no CPU fallback")
-    x2 = _rows(x.reshape(math.prod(x.shape[:-1]), K))
-    b_gate, b_up = (None if b is None else b.contiguous() for b in (b_gate, b_up))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for _, t in given):
-        h = _GatedLinear.apply(x2, w_gate, w_up, b_gate, b_up, _ACTS[act])
+    derivatives only.  A row of h depends on its own row of x only."""
+    code, dt, dev, shape = _ACTS.get(act), x.dtype, x.device, w_gate.shape
+    ok = code is not None and x.is_cuda and dt in _DTYPES and len(shape) == 2 and w_up.shape == shape and x.ndim >= 1 and x.shape[-1] == shape[1] and shape.numel() > 0
+    grad = x.requires_grad
+    if ok:
+        for t in (w_gate, w_up):
+            ok = ok and t.dtype == dt and t.device == dev
+            grad = grad or t.requires_grad
+        for t in (b_gate, b_up):
+            if t is not None:
+                ok = ok and t.dtype == dt and t.device == dev and t.ndim == 1 and t.shape[0] == shape[0]
+                grad = grad or t.requires_grad
+    if not ok:
+        _refuse(x, w_gate, w_up, b_gate, b_up, act)
+    x2 = _rows(x if x.ndim == 2 else x.reshape(math.prod(x.shape[:-1]), shape[1]))
+    w_gate, w_up = _rows(w_gate), _rows(w_up)
+    if shape[0] > 1 and w_gate.stride(0) != w_up.stride(0):   # the kernels take both weights with one row stride
+        w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    if b_gate is not None and not b_gate.is_contiguous():
+        b_gate = b_gate.contiguous()
+    if b_up is not None and not b_up.is_contiguous():
+        b_up = b_up.contiguous()
+    if grad and torch.is_grad_enabled():
+        h = _GatedLinear.apply(x2, w_gate, w_up, b_gate, b_up, code)
     else:
-        h = _forward(x2, *_weights(w_gate, w_up), b_gate, b_up, _ACTS[act], False)[0]
-    return h.reshape(*x.shape[:-1], N)
+        h = _forward(x2, w_gate, w_up, b_gate, b_up, code, False)[0]
+    return h if x.ndim == 2 else h.reshape(*x.shape[:-1], shape[0])
 
 
 class GatedLinear(nn.Module):

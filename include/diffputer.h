@@ -217,7 +217,7 @@ int dp_linear(int dtype, const void* A, const void* W, const float* bias, void* 
  *                   (diffusion_utils.py:100-101) runs in the epilogue of the mlp.6 GEMM instead of a kernel of its own;
  *                   bit-identical results.
  *   "gated_kernel"  which kernel runs the products of dp_gated_linear and its backward: 0 (default) = by size and alignment, 1 = the
- *                   general kernel (any size, stride and type), 128 / 256 = the bf16 tile kernels of that tile.
+ *                   general kernel (any size, stride and type), 128 / 256 = the tile kernels (bf16: of that tile; float32 has one).
  *   "gated_splits"  slices of the contraction of those products: 0 (default) = by size, else that many (at most one per K-tile).  The
  *                   order of sums, and with it the last bits, depend on it.
  */

@@ -113,7 +113,7 @@ def check(x, wg, wu, bg, bu, dh, act, train=True):
 
 SIZES = [  # M, K, N
     (1, 1, 1), (1, 64, 64), (1, 256, 520), (2, 7, 3), (3, 8, 16), (15, 9, 64), (16, 64, 32), (17, 65, 33), (31, 130, 31),
-    (33, 72, 100), (64, 128, 128), (65, 63, 129), (100, 200, 65), (130, 320, 260), (257, 100, 40), (300, 33, 257), (1000, 16, 8),
+    (33, 72, 100), (64, 128, 128), (1, 1000, 4100), (20, 520, 4100), (50, 1032, 300), (64, 2050, 4096), (65, 63, 129), (100, 200, 65), (130, 320, 260), (257, 100, 40), (300, 33, 257), (1000, 16, 8),
 ]
 
 
@@ -141,6 +141,13 @@ def tune():
 def test_every_kernel(tune, kernel, splits, M, K, N):
     tune(kernel, splits)
     check(*make(M, K, N, "bf16", seed=M + K), act="silu")
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (40, 64, 64), (70, 200, 40), (129, 64, 65), (257, 73, 129), (300, 136, 264), (513, 1032, 264), (200, 31, 66)])
+@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (128, 0), (128, 3), (128, 7)])
+def test_every_kernel_f32(tune, kernel, splits, M, K, N):
+    tune(kernel, splits)
+    check(*make(M, K, N, "f32", seed=M + K), act="silu")
 
 
 @pytest.mark.parametrize("kernel", [1, 128, 256])
