@@ -991,7 +991,7 @@ int dp_tune(const char* key, int value) {
         return DP_OK;
     }
     if (!strcmp(key, "gated_kernel")) {
-        if (value != 0 && value != 1 && value != 128 && value != 256) return fail(DP_EINVAL, "gated_kernel must be 0, 1, 128 or 256");
+        if (value != 0 && value != 1 && value != 64 && value != 128 && value != 256) return fail(DP_EINVAL, "gated_kernel must be 0, 1, 64, 128 or 256");
         g_gated_kernel = value;
         return DP_OK;
     }

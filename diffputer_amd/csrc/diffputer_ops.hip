@@ -32,20 +32,21 @@ static int gl_check(const char* who, int dtype, int64_t M, int N, int K, int act
     return DP_OK;
 }
 
-// tuning knobs (dp_tune, defined in diffputer_hip.hip): "gated_kernel" 0 = by the rule below, 1 = the general kernel, 128 / 256 = that tile;
-// "gated_splits" 0 = by the rule, n = that many slices of the contraction (as many as there are K-tiles at most)
+// tuning knobs (dp_tune, defined in diffputer_hip.hip): "gated_kernel" 0 = by the rule below, 1 = the general kernel, 64 / 128 / 256 = the
+// tile kernel of that tile (the nearest one that the type has); "gated_splits" 0 = by the rule, n = that many slices of the
+// contraction (as many as there are K-tiles at most)
 std::atomic<int> g_gated_kernel{0}, g_gated_splits{0};
+static int forced_kernel() { return g_gated_kernel.load(std::memory_order_relaxed); }
 
 // dynamic LDS of the tile kernels, once per device
 template <int MODE> static hipError_t gt_attributes() {
-    const void* k[] = {(const void*)k_gated_tile<MODE, 256, false>, (const void*)k_gated_tile<MODE, 256, true>, (const void*)k_gated_tile<MODE, 128, false>, (const void*)k_gated_tile<MODE, 128, true>};
-    for (int i = 0; i < 4; ++i) {
-        const hipError_t e = hipFuncSetAttribute(k[i], hipFuncAttributeMaxDynamicSharedMemorySize, i < 2 ? GtShape<256>::LDS : GtShape<128>::LDS);
-        if (e != hipSuccess) return e;
-    }
-    const void* f[] = {(const void*)k_gated_f32<MODE, false, false>, (const void*)k_gated_f32<MODE, false, true>, (const void*)k_gated_f32<MODE, true, false>, (const void*)k_gated_f32<MODE, true, true>};
-    for (const void* k1 : f) {
-        const hipError_t e = hipFuncSetAttribute(k1, hipFuncAttributeMaxDynamicSharedMemorySize, GF_LDS);
+    const struct { const void* k; int lds; } all[] = {
+        {(const void*)k_gated_tile<MODE, 256>, GtShape<256>::LDS}, {(const void*)k_gated_tile<MODE, 128>, GtShape<128>::LDS},
+        {(const void*)k_gated_f32<MODE, 128, false>, GfShape<128>::LDS}, {(const void*)k_gated_f32<MODE, 128, true>, GfShape<128>::LDS},
+        {(const void*)k_gated_tile_both<256>, GtShape<256>::LDS}, {(const void*)k_gated_tile_both<128>, GtShape<128>::LDS},
+        {(const void*)k_gated_f32_both<128, false>, GfShape<128>::LDS}, {(const void*)k_gated_f32_both<128, true>, GfShape<128>::LDS}};
+    for (const auto& a : all) {
+        const hipError_t e = hipFuncSetAttribute(a.k, hipFuncAttributeMaxDynamicSharedMemorySize, a.lds);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -65,77 +66,121 @@ static int gt_ready() {
     return DP_OK;
 }
 
-// How a product runs: by the general kernel (T = 0), a bf16 tile kernel (T = 128 or 256), the float32 tile kernel (GF_T) or the
-// kernel for few rows (GL_ROWS, forward only), and how many slices of the contraction.
+// ---- how a product runs: by the general kernel (T = 0), a tile kernel (T = 64, 128 or 256) or the kernel for few rows
+// (GL_ROWS, forward only), and in how many slices of the contraction ----
 constexpr int GL_ROWS = 1;
 struct GlShape { int mode; int64_t I; int J; int64_t C; int planes; };
-struct GlPlan { int T, kt_per, splits; int64_t ti, tj; };
+struct GlPlan { int T, kt_per, splits; int64_t ti, tj, wgs; };
 static int64_t gl_ldp(int J) { return round_up<int64_t>(J, 4); }
 static size_t gl_part_bytes(const GlShape& s) { return (size_t)2 * s.I * gl_ldp(s.J) * 4; }       // one slice: two planes
 
-// Cuts the contraction of a launch that has few tiles, until there are about `want` workgroups, as long as a slice keeps
-// `least` K-tiles and the partial sums stay within 64 MiB.
-static void gl_cut(GlPlan& pl, const GlShape& s, int64_t tiles, int64_t nk, int64_t want, int64_t least) {
-    int64_t n = std::min<int64_t>({want / std::max<int64_t>(tiles, 1), nk / least, (int64_t)(64 << 20) / std::max<int64_t>(gl_part_bytes(s), 1), 64});
-    if (const int forced = g_gated_splits.load(std::memory_order_relaxed)) n = std::min<int64_t>(forced, nk);
-    if (n < 1) n = 1;
-    pl.kt_per = (int)ceil_div<int64_t>(nk, n);
-    pl.splits = (int)ceil_div<int64_t>(nk, pl.kt_per);
-}
-static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
+static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
     GlPlan pl;
-    const int segs = s.mode == GL_DX ? 2 : 1;
-    auto shape = [&](int T) {
-        pl.T = T;
-        pl.ti = ceil_div<int64_t>(s.I, T ? T : GG_T);
-        pl.tj = ceil_div<int64_t>(s.J, (T ? T : GG_T) / (s.mode == GL_FWD ? 2 : 1));
-        return pl.ti * pl.tj * s.planes;
-    };
-    const int forced = g_gated_kernel.load(std::memory_order_relaxed);
-    if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0) return {GL_ROWS, 0, 1, 1, 1};
-    if (tile && forced != 1) {
-        const bool f32 = dtype == DP_DTYPE_F32;
-        const int64_t nk = ceil_div<int64_t>(s.C, f32 ? GF_K : 64) * segs;
-        int64_t tiles = shape(f32 ? GF_T : 256);
-        if (!f32 && (forced == 128 || (forced == 0 && tiles < 256))) tiles = shape(128);
-        if (tiles < (int64_t)1 << 22) {                           // the grid of a launch
-            gl_cut(pl, s, tiles, nk, pl.T == 256 ? 256 : 512, 4);
-            return pl;
-        }
-    }
-    const int64_t tiles = shape(0);
-    gl_cut(pl, s, tiles, ceil_div<int64_t>(s.C, GG_K) * segs, 512, 8);
+    const int t = T ? T : GG_T;
+    const int64_t nk = ceil_div<int64_t>(s.C, kdepth) * (s.mode == GL_DX ? 2 : 1);
+    pl.T = T;
+    pl.ti = ceil_div<int64_t>(s.I, t);
+    pl.tj = ceil_div<int64_t>(s.J, s.mode == GL_FWD ? t / 2 : t);
+    if (const int f = g_gated_splits.load(std::memory_order_relaxed)) want = f;
+    pl.kt_per = (int)ceil_div<int64_t>(nk, std::max<int64_t>(1, std::min<int64_t>(want, nk)));
+    pl.splits = (int)ceil_div<int64_t>(nk, pl.kt_per);
+    pl.wgs = pl.ti * pl.tj * s.planes * pl.splits;
     return pl;
 }
-static size_t gl_split_bytes(const GlShape& s, int dtype, bool tile) {
-    const GlPlan c = gl_plan(s, dtype, tile);
-    return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0;
+
+// Microseconds of a launch of up to two products, by what the kernels measured (bf16: 64 deep K-tiles, float32: 32 deep).  A K-tile takes
+// `one` where a workgroup has its CU to itself and `full` where the CU holds `per_cu` of them; both from launches that
+// fill the chip and launches that do not (K-loops of 64 K-tiles).  A split launch pays for its partial sums: written and read at
+// about 3 TB/s, and a launch more.
+struct GlRate { int T, per_cu; double one, full; };
+static const GlRate GL_RATES_BF16[] = {{256, 1, 1.70, 1.70}, {128, 2, 0.70, 1.04}};
+static const GlRate GL_RATES_F32[] = {{128, 2, 1.90, 3.50}, {64, 4, 0.60, 1.85}};
+static double gl_cost(const GlRate& r, const GlPlan* pl, const GlShape* s, int n) {
+    double wgs = 0, work = 0, longest = 0, join = 0;
+    for (int i = 0; i < n; ++i) {
+        wgs += (double)pl[i].wgs;
+        work += (double)pl[i].wgs * pl[i].kt_per;
+        longest = std::max(longest, (double)pl[i].kt_per);
+        if (pl[i].splits > 1) join = std::max(join, 5.0) + (double)s[i].I * s[i].J * (s[i].mode == GL_DX ? 1 : 2) * 4 * 2 * pl[i].splits / 3.0e6;
+    }
+    const double slots = 256.0 * r.per_cu;
+    const double step = wgs <= 256 ? r.one : wgs >= slots ? r.full : r.one + (r.full - r.one) * (wgs - 256) / (slots - 256);
+    const double rounds = wgs <= slots ? longest : std::max(work / slots + 0.5 * longest * (fmod(wgs, slots) != 0), longest);
+    return rounds * step + join;
 }
 
-template <int MODE, int T>
-static int gt_launch(const GlArgs& a, const GlPlan& pl, int planes, hipStream_t st) {
-    const GtArgs q = {a, (int)pl.ti, (int)pl.tj, 8};
-    const dim3 grid((unsigned)(pl.ti * pl.tj * planes * pl.splits)), block(GtShape<T>::THREADS);
-    if (pl.splits > 1) hipLaunchKernelGGL((k_gated_tile<MODE, T, true>), grid, block, GtShape<T>::LDS, st, q);
-    else hipLaunchKernelGGL((k_gated_tile<MODE, T, false>), grid, block, GtShape<T>::LDS, st, q);
-    DP_LAUNCH_CHECK("k_gated_tile");
-    return DP_OK;
+// The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass).
+static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
+    const bool bf = dtype == DP_DTYPE_BF16;
+    const int forced = forced_kernel(), kdepth = bf ? 64 : GF_K;
+    static const int slices[] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
+    double least = 1e300;
+    for (int k = 0; k < 2; ++k) {
+        const GlRate& r = bf ? GL_RATES_BF16[k] : GL_RATES_F32[k];
+        if (forced > 1 && r.T != (bf ? std::max(forced, 128) : std::min(forced, 128))) continue;
+        for (int a : slices)
+            for (int b : slices) {
+                if (n == 1 && b > 1) break;
+                GlPlan pl[2] = {gl_shape(s[0], r.T, kdepth, a), n > 1 ? gl_shape(s[1], r.T, kdepth, b) : GlPlan{}};
+                bool fits = true;
+                for (int i = 0; i < n; ++i) fits = fits && (pl[i].splits == 1 || gl_part_bytes(s[i]) * pl[i].splits <= (size_t)128 << 20);
+                if (!fits && (a > 1 || b > 1)) continue;
+                const double c = gl_cost(r, pl, s, n);
+                if (c < least) {
+                    least = c;
+                    for (int i = 0; i < n; ++i) best[i] = pl[i];
+                }
+            }
+    }
 }
+static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < (int64_t)1 << 22; }
+
+static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
+    const int forced = forced_kernel();
+    if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0) return {GL_ROWS, 0, 1, 1, 1, 1};
+    if (tile && forced != 1) {
+        GlPlan pl;
+        gl_choose(&s, 1, dtype, &pl);
+        if (gl_grid_ok(pl)) return pl;
+    }
+    // general kernel: slices until there are about two workgroups per CU, as long as a slice keeps 8 K-tiles
+    const int64_t nk = ceil_div<int64_t>(s.C, GG_K) * (s.mode == GL_DX ? 2 : 1), tiles = gl_shape(s, 0, GG_K, 1).wgs;
+    const int64_t want = std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), nk / 8, (int64_t)(64 << 20) / std::max<int64_t>(gl_part_bytes(s), 1), 64});
+    return gl_shape(s, 0, GG_K, (int)std::max<int64_t>(want, 1));
+}
+// both backward products: in one launch on a tile kernel, or two plans of their own
+static bool gl_plan_both(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
+    if (tile && forced_kernel() != 1) {
+        gl_choose(s, 2, dtype, pl);
+        if (gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]) && pl[0].wgs + pl[1].wgs < (int64_t)1 << 22) return true;
+    }
+    for (int i = 0; i < 2; ++i) pl[i] = gl_plan(s[i], dtype, tile);
+    return false;
+}
+static size_t gl_split_bytes(const GlShape& s, const GlPlan& c) { return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0; }
 
 template <int MODE>
-static int gf_launch(const GlArgs& a, const GlPlan& pl, int planes, bool vec, hipStream_t st) {
-    const GtArgs q = {a, (int)pl.ti, (int)pl.tj, 8};
-    const dim3 grid((unsigned)(pl.ti * pl.tj * planes * pl.splits)), block(GF_THREADS);
-    if (pl.splits > 1) {
-        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, true, true>), grid, block, GF_LDS, st, q);
-        else hipLaunchKernelGGL((k_gated_f32<MODE, false, true>), grid, block, GF_LDS, st, q);
+static int gt_launch(const GtArgs& q, const GlPlan& pl, bool bf, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)pl.wgs);
+    if (bf) {
+        if (pl.T == 256) hipLaunchKernelGGL((k_gated_tile<MODE, 256>), grid, dim3(GtShape<256>::THREADS), GtShape<256>::LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_tile<MODE, 128>), grid, dim3(GtShape<128>::THREADS), GtShape<128>::LDS, st, q);
+    } else if (pl.T == 128) {
+        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, 128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_f32<MODE, 128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, q);
     } else {
-        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, true, false>), grid, block, GF_LDS, st, q);
-        else hipLaunchKernelGGL((k_gated_f32<MODE, false, false>), grid, block, GF_LDS, st, q);
+        if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, 64, true>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_f32<MODE, 64, false>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, q);
     }
-    DP_LAUNCH_CHECK("k_gated_f32");
+    DP_LAUNCH_CHECK("gated tile kernel");
     return DP_OK;
 }
+
+static GtArgs gl_args(GlArgs a, const GlShape& s, const GlPlan& c) {
+    a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
+    return {a, (int)c.ti, (int)c.tj, 8};
+}
+static unsigned gl_join_grid(const GlShape& s) { return (unsigned)std::min<int64_t>(ceil_div<int64_t>(s.I * s.planes * ceil_div<int64_t>(s.J, 4), 256), 4096); }
 
 template <typename T, int MT, int CB>
 static int gr_launch(const GlArgs& a, bool vec, hipStream_t st) {
@@ -154,26 +199,44 @@ static int gr_rows(const GlArgs& a, bool vec, hipStream_t st) {
 }
 
 template <typename T, int MODE>
-static int gl_mm(GlArgs a, const GlShape& s, bool tile, bool vec, hipStream_t st) {
-    constexpr int DT = sizeof(T) == 2 ? DP_DTYPE_BF16 : DP_DTYPE_F32;
-    const GlPlan c = gl_plan(s, DT, tile);
+static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, hipStream_t st) {
+    const GtArgs q = gl_args(a, s, c);
     int rc;
-    a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
-    if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(a, vec, st) : DP_EINVAL;
+    if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(q.g, vec, st) : DP_EINVAL;
     if (c.T == 0) {
-        hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, q.g);
         DP_LAUNCH_CHECK("k_gated_mm");
-    } else {
-        if ((rc = gt_ready())) return rc;
-        if (DT == DP_DTYPE_F32) rc = gf_launch<MODE>(a, c, s.planes, vec, st);
-        else rc = c.T == 256 ? gt_launch<MODE, 256>(a, c, s.planes, st) : gt_launch<MODE, 128>(a, c, s.planes, st);
-        if (rc) return rc;
-    }
+    } else if ((rc = gt_ready()) || (rc = gt_launch<MODE>(q, c, sizeof(T) == 2, vec, st))) return rc;
     if (c.splits > 1) {
-        const int64_t n = s.I * s.planes * ceil_div<int64_t>(s.J, 4);
-        const unsigned grid = (unsigned)std::min<int64_t>(ceil_div<int64_t>(n, 256), 4096);
-        hipLaunchKernelGGL((k_gated_join<T, MODE>), dim3(grid), dim3(256), 0, st, a, s.planes);
+        hipLaunchKernelGGL((k_gated_join<T, MODE>), dim3(gl_join_grid(s)), dim3(256), 0, st, q.g, s.planes);
         DP_LAUNCH_CHECK("k_gated_join");
+    }
+    return DP_OK;
+}
+
+// both backward products in one launch: the longer contraction's workgroups start first
+template <typename T>
+static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], bool vec, hipStream_t st) {
+    int rc;
+    if ((rc = gt_ready())) return rc;
+    const GtArgs dx = gl_args(a[0], s[0], c[0]), dw = gl_args(a[1], s[1], c[1]);
+    const int dx_first = c[0].kt_per >= c[1].kt_per, n0 = (int)c[dx_first ? 0 : 1].wgs;
+    const dim3 grid((unsigned)(c[0].wgs + c[1].wgs));
+    if (sizeof(T) == 2) {
+        if (c[0].T == 256) hipLaunchKernelGGL((k_gated_tile_both<256>), grid, dim3(GtShape<256>::THREADS), GtShape<256>::LDS, st, dx, dw, n0, dx_first);
+        else hipLaunchKernelGGL((k_gated_tile_both<128>), grid, dim3(GtShape<128>::THREADS), GtShape<128>::LDS, st, dx, dw, n0, dx_first);
+    } else if (c[0].T == 128) {
+        if (vec) hipLaunchKernelGGL((k_gated_f32_both<128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
+        else hipLaunchKernelGGL((k_gated_f32_both<128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
+    } else {
+        if (vec) hipLaunchKernelGGL((k_gated_f32_both<64, true>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first);
+        else hipLaunchKernelGGL((k_gated_f32_both<64, false>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first);
+    }
+    DP_LAUNCH_CHECK("gated tile kernel");
+    const unsigned jx = c[0].splits > 1 ? gl_join_grid(s[0]) : 0, jw = c[1].splits > 1 ? gl_join_grid(s[1]) : 0;
+    if (jx + jw) {
+        hipLaunchKernelGGL((k_gated_join_both<T>), dim3(jx + jw), dim3(256), 0, st, dx.g, dw.g, (int)jx);
+        DP_LAUNCH_CHECK("k_gated_join_both");
     }
     return DP_OK;
 }
@@ -191,7 +254,7 @@ static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void*
     const int chunk = bf ? 8 : 4;
     const bool x_in = gt_direct(x, ldx, K, chunk), w_in = gt_direct(wg, ldw, K, chunk) && gt_direct(wu, ldw, K, chunk);
     const bool short_rows = ldx <= GT_MAX_LD && ldw <= GT_MAX_LD;
-    const int forced = g_gated_kernel.load(std::memory_order_relaxed);
+    const int forced = forced_kernel();
     o.vec = x_in && w_in;
     o.pack_x = o.pack_w = false;
     o.ldk = round_up<int64_t>(K, 8);
@@ -244,26 +307,34 @@ static GlIn gl_in(int dtype, const void* x, int64_t ldx, const void* wg, const v
 }
 
 // forward workspace: copies, partial sums
-struct GlFwd { float* part; size_t bytes; };
+struct GlFwd { GlShape s; GlPlan plan; float* part; size_t bytes; };
 static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
-    if (gl_plan({GL_FWD, in.M, in.N, in.K, 1}, dtype, in.o.tile).T == GL_ROWS) in.o.pack_x = in.o.pack_w = false;
+    GlFwd w;
+    w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1};
+    w.plan = gl_plan(w.s, dtype, in.o.tile);
+    if (w.plan.T == GL_ROWS) {                                    // reads rows of any alignment
+        in.o.pack_x = in.o.pack_w = false;
+        w.s.C = in.K;
+    }
     Carver c = {(char*)base};
     in.carve(c);
-    GlFwd w;
-    w.part = (float*)c.take(gl_split_bytes({GL_FWD, in.M, in.N, in.fwd_c(), 1}, dtype, in.o.tile));
+    w.part = (float*)c.take(gl_split_bytes(w.s, w.plan));
     w.bytes = c.off;
     return w;
 }
 
-// backward workspace: copies; the two planes dg, du; partial column sums; partial products (dx and dW use the same bytes in turn)
+// backward workspace: copies; the two planes dg, du; partial column sums; partial products
 struct GlBwd {
     char* dgu;
-    float *colpart, *part;
+    float *colpart, *part[2];
+    GlShape s[2];              // dx, dW
+    GlPlan plan[2];
+    bool both;                 // in one launch
     int64_t ldg;
     int tx, rows, nblk;
     size_t bytes;
 };
-static GlBwd gl_bwd_carve(int dtype, GlIn& in, void* base) {
+static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* base) {
     const int64_t M = in.M;
     const int N = in.N, K = in.K;
     GlBwd w;
@@ -274,12 +345,17 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, void* base) {
     if (w.tx == 48) w.tx = 64;
     const int64_t cols = ceil_div<int64_t>(w.ldg, w.tx * 4);
     const int ty = 256 / w.tx;
-    // about 2048 workgroups, at least 4 rows per row lane
-    w.rows = (int)std::max<int64_t>(4 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 2048 / cols)));
+    // about 1024 workgroups, at least 4 rows per row lane
+    w.rows = (int)std::max<int64_t>(4 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 1024 / cols)));
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
     w.dgu = c.take((size_t)2 * M * w.ldg * (dtype == DP_DTYPE_BF16 ? 2 : 4));
-    w.colpart = (float*)c.take((size_t)w.nblk * 2 * w.ldg * 4);
-    w.part = (float*)c.take(std::max(gl_split_bytes({GL_DX, M, K, N, 1}, dtype, in.o.tile), gl_split_bytes({GL_DW, N, K, M, 2}, dtype, in.o.tile)));
+    w.colpart = (float*)c.take(w.nblk > 1 ? (size_t)w.nblk * 2 * w.ldg * 4 : 0);
+    w.s[0] = {GL_DX, M, K, N, 1};
+    w.s[1] = {GL_DW, N, K, M, planes ? planes : 2};
+    w.both = false;
+    if (want_dx && planes == 2) w.both = gl_plan_both(w.s, dtype, in.o.tile, w.plan);
+    else for (int i = 0; i < 2; ++i) w.plan[i] = gl_plan(w.s[i], dtype, in.o.tile);
+    for (int i = 0; i < 2; ++i) w.part[i] = (float*)c.take((i ? planes > 0 : want_dx) ? gl_split_bytes(w.s[i], w.plan[i]) : 0);
     w.bytes = c.off;
     return w;
 }
@@ -292,7 +368,7 @@ static int gl_forward(GlArgs a, GlIn& in, void* ws, hipStream_t st) {
     a.A[0] = in.x;
     a.B[0] = in.wg; a.B[1] = in.wu;
     a.part = w.part;
-    return gl_mm<T, GL_FWD>(a, {GL_FWD, in.M, in.N, in.fwd_c(), 1}, in.o.tile, in.o.vec, st);
+    return gl_mm<T, GL_FWD>(a, w.s, w.plan, in.o.vec, st);
 }
 
 template <typename T>
@@ -314,33 +390,33 @@ static int gl_backward(int dtype, GlIn& in, const float* pre, const GlOp& dh, T*
         }
         return DP_OK;
     }
-    const GlBwd w = gl_bwd_carve(dtype, in, ws);
+    const int planes = (dw[0] != nullptr) + (dw[1] != nullptr);
+    const GlBwd w = gl_bwd_carve(dtype, in, planes, dx != nullptr, ws);
     T* const dgu = (T*)w.dgu;
-    const bool bias = db[0] || db[1];
-    if ((rc = in.pack(dw[0] || dw[1], dx != nullptr, st))) return rc;
-    hipLaunchKernelGGL((k_gated_dgu<T>), dim3((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk), dim3(256), 0, st, pre, gl_ldp(N),
-                       (const T*)dh.p, dh.ld, dgu, w.ldg, bias ? w.colpart : (float*)nullptr, M, N, act, w.tx, w.rows);
+    if ((rc = in.pack(planes > 0, dx != nullptr, st))) return rc;
+    const GlDgu e = {pre, dh.p, dgu, w.colpart, {db[0], db[1]}, gl_ldp(N), dh.ld, w.ldg, M, N, act, w.tx, w.rows};
+    hipLaunchKernelGGL((k_gated_dgu<T>), dim3((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk), dim3(256), 0, st, e);
     DP_LAUNCH_CHECK("k_gated_dgu");
-    if (bias) {
+    if ((db[0] || db[1]) && w.nblk > 1) {
         hipLaunchKernelGGL((k_gated_colsum<T>), dim3((unsigned)ceil_div(N, 64), 2), dim3(256), 0, st, w.colpart, w.nblk, w.ldg, db[0], db[1], N);
         DP_LAUNCH_CHECK("k_gated_colsum");
     }
-    GlArgs a;
-    memset(&a, 0, sizeof a);
-    a.part = w.part;
-    a.A[0] = {dgu, w.ldg, w.ldg};
-    a.A[1] = {dgu + (size_t)M * w.ldg, w.ldg, w.ldg};
-    if (dx) {
-        a.B[0] = in.wg; a.B[1] = in.wu;
-        a.out[0] = dx; a.ldo = K;
-        if ((rc = gl_mm<T, GL_DX>(a, {GL_DX, M, K, N, 1}, in.o.tile, in.o.vec, st))) return rc;
+    GlArgs a[2];
+    memset(a, 0, sizeof a);
+    for (int i = 0; i < 2; ++i) {
+        a[i].part = w.part[i];
+        a[i].A[0] = {dgu, w.ldg, w.ldg};
+        a[i].A[1] = {dgu + (size_t)M * w.ldg, w.ldg, w.ldg};
+        a[i].ldo = K;
     }
-    if (dw[0] || dw[1]) {
-        a.B[0] = in.x;
-        a.out[0] = dw[0]; a.out[1] = dw[1]; a.ldo = K;
-        a.zfirst = dw[0] ? 0 : 1;
-        if ((rc = gl_mm<T, GL_DW>(a, {GL_DW, N, K, M, dw[0] && dw[1] ? 2 : 1}, in.o.tile, in.o.vec, st))) return rc;
-    }
+    a[0].B[0] = in.wg; a[0].B[1] = in.wu;
+    a[0].out[0] = dx;
+    a[1].B[0] = in.x;
+    a[1].out[0] = dw[0]; a[1].out[1] = dw[1];
+    a[1].zfirst = dw[0] ? 0 : 1;
+    if (w.both) return gl_both<T>(a, w.s, w.plan, in.o.vec, st);
+    if (dx && (rc = gl_mm<T, GL_DX>(a[0], w.s[0], w.plan[0], in.o.vec, st))) return rc;
+    if (planes && (rc = gl_mm<T, GL_DW>(a[1], w.s[1], w.plan[1], in.o.vec, st))) return rc;
     return DP_OK;
 }
 
@@ -414,7 +490,11 @@ size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, co
     if (gl_check("dp_gated_linear_workspace_bytes", dtype, M, N, K, 0)) return 0;
     if (M == 0) return 256;
     GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
-    return std::max<size_t>(backward ? gl_bwd_carve(dtype, in, nullptr).bytes : gl_fwd_carve(dtype, in, nullptr).bytes, 256);
+    if (!backward) return std::max<size_t>(gl_fwd_carve(dtype, in, nullptr).bytes, 256);
+    size_t most = 256;                                            // whichever gradients a call asks for
+    for (int planes = 0; planes < 3; ++planes)
+        for (int dx = 0; dx < 2; ++dx) most = std::max(most, gl_bwd_carve(dtype, in, planes, dx, nullptr).bytes);
+    return most;
 }
 
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,

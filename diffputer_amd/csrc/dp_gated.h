@@ -9,6 +9,8 @@
 // All three are C(i, j) = sum_k A(i, k) B(j, k) with each operand either "row" laid out (k contiguous) or "column" laid
 // out (i or j contiguous, as a transposed product finds its operands in memory).
 #pragma once
+#include <type_traits>
+
 #include "dp_util.h"
 
 namespace dp {
@@ -31,26 +33,41 @@ template <> struct GlType<bf16_t> {
 // silu(g) = g s(g), s = 1 / (1 + e^-g): e^-g overflows to inf below -88, where s is 0 and the product the right -0;
 // gelu(g) = g Phi(g), Phi = erfc(-g / sqrt 2) / 2 (erfc keeps the relative accuracy of the left tail that 1 + erf loses).
 // At g = -inf both products are 0 * inf = NaN; plain torch expressions give the same.
-__device__ __forceinline__ float gl_sigmoid(float g) { return 1.0f / (1.0f + expf(-g)); }
+// float32 results take expf and a division; for bf16 results the hardware's 2^x and reciprocal do (|g| 2^-24 + 2^-22 of s: at
+// most 2^-17 where s is not 0, against half a step of 2^-9): what a 256-tile launch takes beyond its K-tiles fell from 18.9 to
+// 11.4 us with them.
+template <typename T> __device__ __forceinline__ float gl_sigmoid(float g) {
+    if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f));
+}
+template <typename T> __device__ __forceinline__ float gl_exp(float x) {
+    return sizeof(T) == 4 ? expf(x) : __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+}
 __device__ __forceinline__ float gl_phi(float g) { return 0.5f * erfcf(-0.70710678118654752f * g); }
-__device__ __forceinline__ float gl_act(int act, float g) {
-    if (act == GL_ACT_SILU) return g * gl_sigmoid(g);
-    if (act == GL_ACT_GELU) return g * gl_phi(g);
+template <typename T, int ACT> __device__ __forceinline__ float gl_act(float g) {
+    if (ACT == GL_ACT_SILU) return g * gl_sigmoid<T>(g);
+    if (ACT == GL_ACT_GELU) return g * gl_phi(g);
     return g;
 }
-__device__ __forceinline__ void gl_act_grad(int act, float g, float& a, float& da) {
-    if (act == GL_ACT_SILU) {
-        const float s = gl_sigmoid(g);
+template <typename T, int ACT> __device__ __forceinline__ void gl_act_grad(float g, float& a, float& da) {
+    if (ACT == GL_ACT_SILU) {
+        const float s = gl_sigmoid<T>(g);
         a = g * s;
         da = s * (1.0f + g * (1.0f - s));
-    } else if (act == GL_ACT_GELU) {
+    } else if (ACT == GL_ACT_GELU) {
         const float p = gl_phi(g);
         a = g * p;
-        da = p + g * (0.39894228040143268f * expf(-0.5f * g * g));
+        da = p + g * (0.39894228040143268f * gl_exp<T>(-0.5f * g * g));
     } else {
         a = g;
         da = 1.0f;
     }
+}
+// calls f with the activation as a constant
+template <typename F> __device__ __forceinline__ void gl_with_act(int act, F f) {
+    if (act == GL_ACT_SILU) f(std::integral_constant<int, GL_ACT_SILU>{});
+    else if (act == GL_ACT_GELU) f(std::integral_constant<int, GL_ACT_GELU>{});
+    else f(std::integral_constant<int, GL_ACT_NONE>{});
 }
 
 // ---- operands ------------------------------------------------------------------------------------------------------
@@ -85,18 +102,54 @@ struct GlArgs {
     int act;
 };
 
-template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs& p, int64_t m, int n, int cnt, const float* g, const float* u) {
-    T* const h = (T*)p.out[0] + m * p.ldo + n;
-    for (int r = 0; r < cnt; ++r) {
-        float gv = g[r], uv = u[r];
-        if (p.bias[0]) gv += GlType<T>::get(((const T*)p.bias[0])[n + r]);
-        if (p.bias[1]) uv += GlType<T>::get(((const T*)p.bias[1])[n + r]);
-        if (p.pre) {
-            p.pre[m * p.ldpre + n + r] = gv;
-            p.pre[(p.I + m) * p.ldpre + n + r] = uv;
-        }
-        h[r] = GlType<T>::put(gl_act(p.act, gv) * uv);
+// four columns of one row: whole and aligned, or element by element
+template <typename T> struct GlVec;
+template <> struct GlVec<float> { typedef f32x4 V; static __device__ __forceinline__ V put(f32x4 v) { return v; } static __device__ __forceinline__ f32x4 get(V v) { return v; } };
+template <> struct GlVec<bf16_t> {
+    typedef uint2 V;
+    static __device__ __forceinline__ V put(f32x4 v) { return make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])); }
+    static __device__ __forceinline__ f32x4 get(V v) {
+        return (f32x4){__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u), __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u)};
     }
+};
+template <typename T> __device__ __forceinline__ bool gl_whole(const T* base, int64_t ld) { return (ld & 3) == 0 && ((uintptr_t)base & (4 * sizeof(T) - 1)) == 0; }
+template <typename T> __device__ __forceinline__ void gl_put4(T* o, f32x4 v, int cnt, bool whole) {
+    if (whole && cnt >= 4) *(typename GlVec<T>::V*)o = GlVec<T>::put(v);
+    else
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < cnt) o[r] = GlType<T>::put(v[r]);
+}
+template <typename T> __device__ __forceinline__ f32x4 gl_get4(const T* o, int cnt, bool whole) {
+    if (whole && cnt >= 4) return GlVec<T>::get(*(const typename GlVec<T>::V*)o);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (r < cnt) v[r] = GlType<T>::get(o[r]);
+    return v;
+}
+// the biases of columns n .. n + cnt - 1
+template <typename T> __device__ __forceinline__ void gl_bias(const GlArgs& p, int n, int cnt, f32x4& bg, f32x4& bu) {
+    bg = bu = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (p.bias[0]) bg = gl_get4((const T*)p.bias[0] + n, cnt, gl_whole((const T*)p.bias[0], 0));
+    if (p.bias[1]) bu = gl_get4((const T*)p.bias[1] + n, cnt, gl_whole((const T*)p.bias[1], 0));
+}
+// h of row m, columns n .. n + cnt - 1 (n a multiple of 4), from both finished projections
+template <typename T, int ACT> __device__ __forceinline__ void gl_fwd_put(const GlArgs& p, int64_t m, int n, int cnt, f32x4 g, f32x4 u) {
+    if (p.pre) {                                                 // rows of ldpre = N rounded up to 4
+        *(f32x4*)(p.pre + m * p.ldpre + n) = g;
+        *(f32x4*)(p.pre + (p.I + m) * p.ldpre + n) = u;
+    }
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = gl_act<T, ACT>(g[r]) * u[r];
+    T* const h = (T*)p.out[0];
+    gl_put4(h + m * p.ldo + n, v, cnt, gl_whole(h, p.ldo));
+}
+template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs& p, int64_t m, int n, int cnt, f32x4 g, f32x4 u) {
+    f32x4 bg, bu;
+    gl_bias<T>(p, n, cnt, bg, bu);
+    gl_with_act(p.act, [&](auto act) { gl_fwd_put<T, decltype(act)::value>(p, m, n, cnt, g + bg, u + bu); });
 }
 
 // ---- general product: any size, stride and alignment ------------------------------------------------------------------
@@ -203,10 +256,7 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
         if (m >= p.I) continue;
         if (MODE == GL_FWD && p.splits == 1) {
             const int n = j0 + cl, cnt = p.J - n < 4 ? p.J - n : 4;
-            float g[4], u[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) { g[r] = acc[i][0][r]; u[r] = acc[i][1][r]; }
-            if (cnt > 0) gl_fwd_store<T>(p, m, n, cnt, g, u);
+            if (cnt > 0) gl_fwd_store<T>(p, m, n, cnt, acc[i][0], acc[i][1]);
             continue;
         }
 #pragma unroll
@@ -223,12 +273,12 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
     }
 }
 
-// Joins the slices of a split launch, in order: 4 columns of one row per thread.
+// Joins the slices of a split launch, in order: 4 columns of one row per step.
 template <typename T, int MODE>
-__global__ __launch_bounds__(256) void k_gated_join(GlArgs p, int planes) {
+__device__ __forceinline__ void gl_join(const GlArgs& p, int planes, int64_t first, int64_t step) {
     const int64_t per_row = ceil_div(p.J, 4), rows = p.I * planes, total = rows * per_row;
     const int64_t stride = 2 * p.I * p.ldp;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    for (int64_t t = first; t < total; t += step) {
         const int64_t row = t / per_row;
         const int n = (int)(t - row * per_row) * 4, cnt = p.J - n < 4 ? p.J - n : 4;
         const int pl = p.zfirst + (int)(row / p.I);
@@ -241,78 +291,103 @@ __global__ __launch_bounds__(256) void k_gated_join(GlArgs p, int planes) {
             s0 += *(const f32x4*)(a + s * stride);
             if (MODE == GL_FWD) s1 += *(const f32x4*)(b + s * stride);
         }
-        if (MODE == GL_FWD) {
-            float g[4] = {s0[0], s0[1], s0[2], s0[3]}, u[4] = {s1[0], s1[1], s1[2], s1[3]};
-            gl_fwd_store<T>(p, m, n, cnt, g, u);
-        } else {
-            for (int r = 0; r < cnt; ++r) ((T*)p.out[pl])[m * p.ldo + n + r] = GlType<T>::put(s0[r]);
-        }
+        if (MODE == GL_FWD) gl_fwd_store<T>(p, m, n, cnt, s0, s1);
+        else gl_put4((T*)p.out[pl] + m * p.ldo + n, s0, cnt, gl_whole((T*)p.out[pl], p.ldo));
     }
+}
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void k_gated_join(GlArgs p, int planes) {
+    gl_join<T, MODE>(p, planes, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+// both backward products of one launch: the first `n_dx` workgroups dx, the others dW
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_join_both(GlArgs dx, GlArgs dw, int n_dx) {
+    const int b = blockIdx.x;
+    if (b < n_dx) gl_join<T, GL_DX>(dx, 1, (int64_t)b * 256 + threadIdx.x, (int64_t)n_dx * 256);
+    else gl_join<T, GL_DW>(dw, 2, (int64_t)(b - n_dx) * 256 + threadIdx.x, (int64_t)(gridDim.x - n_dx) * 256);
 }
 
 // ---- backward, elementwise: du = dh act(g), dg = dh u act'(g), and their column sums ------------------------------------
 // Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows.  dgu: two planes [M][ldg] of T, columns N..ldg - 1
-// zero.  colpart: NULL, or [row block][2][ldg] float32 sums of the unrounded values, joined by k_gated_colsum.
+// zero.  db: the column sums of the unrounded values: written here if one block has all rows, else left as partial sums
+// colpart [row block][2][ldg] for k_gated_colsum.
+struct GlDgu {
+    const float* pre;
+    const void* dh;
+    void* dgu;
+    float* colpart;
+    void* db[2];
+    int64_t ldpre, lddh, ldg, M;
+    int N, act, tx, rows;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_dgu(const float* pre, int64_t ldpre, const T* dh, int64_t lddh, T* dgu, int64_t ldg,
-                                                   float* colpart, int64_t M, int N, int act, int tx, int rows) {
+__global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
     __shared__ f32x4 red[2][256];
-    const int cx = threadIdx.x % tx, ry = threadIdx.x / tx, ty = 256 / tx;
-    const int n = (blockIdx.x * tx + cx) * 4;
-    const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = r0 + rows < M ? r0 + rows : M;
+    const int cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
+    const int n = (blockIdx.x * p.tx + cx) * 4, cnt = p.N - n;
+    const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
+    const bool whole = gl_whole((const T*)p.dh, p.lddh);
+    T* const dgu = (T*)p.dgu;
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
-    if (n < ldg) {
+    if (n < p.ldg) gl_with_act(p.act, [&](auto act) {
+#pragma unroll 4
         for (int64_t m = r0 + ry; m < r1; m += ty) {
             f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
-            if (n < N) {
-                const f32x4 g = *(const f32x4*)(pre + m * ldpre + n), u = *(const f32x4*)(pre + (M + m) * ldpre + n);
+            if (cnt > 0) {
+                const f32x4 g = *(const f32x4*)(p.pre + m * p.ldpre + n), u = *(const f32x4*)(p.pre + (p.M + m) * p.ldpre + n);
+                const f32x4 d = gl_get4((const T*)p.dh + m * p.lddh + n, cnt, whole);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (n + e < N) {
-                        const float d = GlType<T>::get(dh[m * lddh + n + e]);
+                    if (e < cnt) {
                         float a, da;
-                        gl_act_grad(act, g[e], a, da);
-                        du[e] = d * a;
-                        dg[e] = d * u[e] * da;
+                        gl_act_grad<T, decltype(act)::value>(g[e], a, da);
+                        du[e] = d[e] * a;
+                        dg[e] = d[e] * u[e] * da;
                     }
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dgu[m * ldg + n + e] = GlType<T>::put(dg[e]);
-                dgu[(M + m) * ldg + n + e] = GlType<T>::put(du[e]);
-            }
+            *(typename GlVec<T>::V*)(dgu + m * p.ldg + n) = GlVec<T>::put(dg);
+            *(typename GlVec<T>::V*)(dgu + (p.M + m) * p.ldg + n) = GlVec<T>::put(du);
             sg += dg;
             su += du;
         }
-    }
-    if (colpart == nullptr) return;
+    });
+    if (!p.db[0] && !p.db[1]) return;
     red[0][threadIdx.x] = sg;
     red[1][threadIdx.x] = su;
     __syncthreads();
-    if (ry == 0 && n < ldg) {
+    if (ry == 0 && n < p.ldg) {
         for (int k = 1; k < ty; ++k) {
-            sg += red[0][k * tx + cx];
-            su += red[1][k * tx + cx];
+            sg += red[0][k * p.tx + cx];
+            su += red[1][k * p.tx + cx];
         }
-        float* c = colpart + (int64_t)blockIdx.y * 2 * ldg + n;
-        *(f32x4*)c = sg;
-        *(f32x4*)(c + ldg) = su;
+        if (gridDim.y == 1) {
+            if (p.db[0] && cnt > 0) gl_put4((T*)p.db[0] + n, sg, cnt, gl_whole((T*)p.db[0], 0));
+            if (p.db[1] && cnt > 0) gl_put4((T*)p.db[1] + n, su, cnt, gl_whole((T*)p.db[1], 0));
+        } else {
+            float* c = p.colpart + (int64_t)blockIdx.y * 2 * p.ldg + n;
+            *(f32x4*)c = sg;
+            *(f32x4*)(c + p.ldg) = su;
+        }
     }
 }
 
-// db[n] = sum of the row blocks' partial sums: 64 columns x 4 lanes per block, lanes joined in order
+// db[n] = sum of the row blocks' partial sums: 64 columns (16 groups of 4) x 16 lanes per block, lanes joined in order
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_colsum(const float* colpart, int nblk, int64_t ldg, T* dbg, T* dbu, int N) {
-    __shared__ float red[4][64];
-    const int c = threadIdx.x & 63, y = threadIdx.x >> 6;
-    const int n = blockIdx.x * 64 + c, pl = blockIdx.y;
-    float s = 0.f;
-    if (n < N)
-        for (int b = y; b < nblk; b += 4) s += colpart[((int64_t)b * 2 + pl) * ldg + n];
+    __shared__ f32x4 red[16][16];
+    const int c = threadIdx.x & 15, y = threadIdx.x >> 4;
+    const int n = blockIdx.x * 64 + c * 4, pl = blockIdx.y, cnt = N - n;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (cnt > 0)
+#pragma unroll 8
+        for (int b = y; b < nblk; b += 16) s += *(const f32x4*)(colpart + ((int64_t)b * 2 + pl) * ldg + n);
     red[y][c] = s;
     __syncthreads();
     T* const out = pl ? dbu : dbg;
-    if (y == 0 && n < N && out) out[n] = GlType<T>::put(red[0][c] + red[1][c] + red[2][c] + red[3][c]);
+    if (y == 0 && cnt > 0 && out) {
+        for (int k = 1; k < 16; ++k) s += red[k][c];
+        gl_put4(out + n, s, cnt, gl_whole(out, 0));
+    }
 }
 
 template <typename T>

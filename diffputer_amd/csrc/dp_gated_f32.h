@@ -1,44 +1,58 @@
-// float32 tile products of the gated projection (dp_gated.h has the three products and their operands): 128 x 128 tile of
-// products, 32 deep, 4 waves of 64 x 64, v_mfma_f32_32x32x2_f32 (a k-ordered chain of float32 fused multiply-adds).
+// float32 tile products of the gated projection (dp_gated.h has the three products and their operands): T x T tile of products,
+// 32 deep, 4 waves of T / 2 x T / 2 by v_mfma_f32_32x32x2_f32 (T = 128) or v_mfma_f32_16x16x4_f32 (T = 64): k-ordered chains
+// of float32 fused multiply-adds.
 //
-// The float32 matrix pipe takes 64 cycles for 4096 products, 16 times the bf16 one: a K-tile is 4096 cycles of it per wave
-// against 32 KiB of loads and 64 LDS reads, so one K-tile of loads in flight and one barrier per K-tile keep it fed, and two
-// workgroups share a CU.  Operands go straight into LDS as in the bf16 tile kernels (rows that do not exist lie behind the
-// buffer's end and arrive as zeros), 16 bytes a lane where rows start on 16 bytes, else 4: element-wise loads are four times
-// the instructions and still fit under the products.
-//   row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7); a lane reads four k's of its
-//     row at once, lanes 0..31 the k's 8 q .. 8 q + 3 and lanes 32..63 the next four: step s of the four multiplies the
-//     k's 8 q + s and 8 q + 4 + s (both operands agree on that, and a sum over k does not ask for more).
-//   column layout: LDS holds k rows of 512 bytes as they are in memory, a lane reads one k of its column; rows with
-//     (k & 4) are stored with the two 128-byte parts of every 256 swapped, so that the two k's of a read use all banks.
+// The float32 matrix pipe takes 64 cycles for 4096 products, 16 times the bf16 one: a K-tile of T = 128 is 4096 cycles of it
+// per wave against 32 KiB of loads and 64 LDS reads, so one K-tile of loads in flight and one barrier per K-tile keep it
+// fed, and two workgroups share a CU.  T = 64 is for products with too few tiles of 128 to fill the chip.  Operands go
+// straight into LDS as in the bf16 tile kernels (rows that do not exist lie behind the buffer's end and arrive as zeros), 16
+// bytes a lane where rows start on 16 bytes, else 4: element-wise loads are four times the instructions and still fit under
+// the products.
+//   With G = 64 / (T / 4) lane groups of T / 4 lanes, a lane reads four k's of its row or column, the group's 4 (G g + group) ..
+//   + 3: step s of the four multiplies the G k's 4 (G g + group) + s (both operands agree on that, and a sum over k does not
+//   ask for more).
+//   row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7), one ds_read_b128;
+//   column layout: LDS holds k rows of 4 T bytes as they are in memory, four ds_read_b32; the bytes of k row k are stored with
+//   their place xor'ed by T * ((k / 4) % G), so that the G k's of a read use all banks.
 #pragma once
 #include "dp_gated_tile.h"
 
 namespace dp {
 
-constexpr int GF_T = 128, GF_K = 32, GF_THREADS = 256;
-constexpr int GF_OP = GF_T * GF_K * 4;                           // bytes of one operand's K-tile
-constexpr int GF_LDS = 4 * GF_OP;
+constexpr int GF_K = 32, GF_THREADS = 256;
+template <int T> struct GfShape {
+    static constexpr int TS = T / 4, G = 64 / TS;                // matrix tile, lane groups
+    static constexpr int OP = T * GF_K * 4, LDS = 4 * OP;        // bytes of one operand's K-tile; two buffers
+};
+template <int TS> struct GfAcc;
+template <> struct GfAcc<32> {
+    typedef f32x16 V;
+    static __device__ __forceinline__ V mul(float b, float a, V c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(b, a, c, 0, 0, 0); }
+};
+template <> struct GfAcc<16> {
+    typedef f32x4 V;
+    static __device__ __forceinline__ V mul(float b, float a, V c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(b, a, c, 0, 0, 0); }
+};
 
-template <int MODE, bool VEC, bool SPLIT>
-__global__ __launch_bounds__(GF_THREADS) void k_gated_f32(GtArgs q) {
+template <int MODE, int T, bool VEC>
+__device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, char* smem) {
+    using S = GfShape<T>;
+    using Acc = GfAcc<S::TS>;
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
     constexpr unsigned OUTSIDE = 0x80000000u;
+    constexpr int TS = S::TS, G = S::G, OP = S::OP;
     constexpr int EL = VEC ? 16 : 4;                             // bytes per lane and load
-    constexpr int NL = GF_OP / (64 * EL) / 4;                    // loads per wave, operand and K-tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int NL = OP / (64 * EL) / 4;                       // loads per wave, operand and K-tile
     const GlArgs& p = q.g;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
-    int slice;
-    const int tile = gt_slice<SPLIT>(p, slice);
-    int plane, ti, tj;
-    gt_tile<MODE>(q, tile, plane, ti, tj);
-    const int64_t i0 = (int64_t)ti * GF_T;
-    const int j0 = tj * (MODE == GL_FWD ? GF_T / 2 : GF_T);
+    const bool split = p.splits > 1;
+    int slice, plane, ti, tj;
+    gt_tile<MODE>(q, b, count, slice, plane, ti, tj);
+    const int64_t i0 = (int64_t)ti * T;
+    const int j0 = tj * (MODE == GL_FWD ? T / 2 : T);
     const int nk = (int)((p.C + GF_K - 1) / GF_K);
-    const int all = nk * (MODE == GL_DX ? 2 : 1);
-    const int kt0 = SPLIT ? slice * p.kt_per : 0, kt1 = SPLIT ? min(kt0 + p.kt_per, all) : all;
+    const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
 
     // load `n` of a wave covers bytes (wave * NL + n) * 64 * EL .. of the operand's image; this lane's EL of them
     const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 4, ldb = p.B[0].ld * 4;
@@ -49,17 +63,16 @@ __global__ __launch_bounds__(GF_THREADS) void k_gated_f32(GtArgs q) {
     for (int n = 0; n < NL; ++n) {
         const int byte = (wave * NL + n) * 64 * EL + lane * EL;
         const int r = byte >> 7, in_r = (((byte >> 4) & 7) ^ (r & 7)) * 16 + (byte & 15);      // row layout: row, byte within the row
-        const int k = byte >> 9, in_k = (byte & 511) ^ (((k >> 2) & 1) << 7);                  // column layout: k, byte within the k row
-        // FWD: rows 0..63 of the B image are gate rows, 64..127 up rows: handled by base and row below
+        const int k = byte / (4 * T), in_k = (byte % (4 * T)) ^ (((k >> 2) & (G - 1)) * T);    // column layout: k, byte within the k row
         va[n] = A_ROW ? (unsigned)(r * lda + in_r) : (unsigned)(k * lda + in_k);
-        vb[n] = B_ROW ? (unsigned)((r & (MODE == GL_FWD ? 63 : 127)) * ldb + in_r) : (unsigned)(k * ldb + in_k);
+        vb[n] = B_ROW ? (unsigned)((r & (MODE == GL_FWD ? T / 2 - 1 : T - 1)) * ldb + in_r) : (unsigned)(k * ldb + in_k);
         tail_out[n] = in_r / 4 >= left;
     }
     auto stage = [&](int kt) {
         const int seg = MODE == GL_DX && kt >= nk ? 1 : 0;
         const int64_t kk = kt - seg * nk;
         const bool last = kk == nk - 1;
-        char* const dst = smem + ((kt - kt0) & 1) * 2 * GF_OP + wave * NL * 64 * EL;
+        char* const dst = smem + ((kt - kt0) & 1) * 2 * OP + wave * NL * 64 * EL;
         {
             const GlOp& op = p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
             const char* const base = (const char*)op.p;
@@ -74,84 +87,94 @@ __global__ __launch_bounds__(GF_THREADS) void k_gated_f32(GtArgs q) {
         const auto buf = gt_buffer(base + (B_ROW ? j0 * ldb + kk * (GF_K * 4) : kk * GF_K * ldb + (int64_t)j0 * 4), base + (B_ROW ? p.J - 1 : p.C - 1) * ldb + op.cols * 4);
 #pragma unroll
         for (int n = 0; n < NL; ++n)
-            gt_load<EL>(buf, dst + GF_OP + n * 64 * EL, B_ROW && last && tail_out[n] ? OUTSIDE : vb[n]);
+            gt_load<EL>(buf, dst + OP + n * 64 * EL, B_ROW && last && tail_out[n] ? OUTSIDE : vb[n]);
     };
 
-    const int r32 = lane & 31, half = lane >> 5;
-    f32x16 acc[2][2];                                            // [rows wm * 64 + 32 i][columns 64 b + wn * 32]
+    const int r = lane % TS, grp = lane / TS;
+    typename Acc::V acc[2][2];                                   // [rows wm * T / 2 + TS i][columns b * T / 2 + wn * TS]
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][b][e] = 0.f;
+            for (int e = 0; e < TS * TS / 64; ++e) acc[i][h][e] = 0.f;
 
     stage(kt0);
     GT_VMCNT(0);
     __builtin_amdgcn_s_barrier();
 #pragma clang loop unroll(disable)
     for (int kt = kt0; kt < kt1; ++kt) {
-        const char* const sa = smem + ((kt - kt0) & 1) * 2 * GF_OP;
-        const char* const sb = sa + GF_OP;
+        const char* const sa = smem + ((kt - kt0) & 1) * 2 * OP;
+        const char* const sb = sa + OP;
         if (kt + 1 < kt1) stage(kt + 1);
 #pragma unroll
-        for (int g = 0; g < GF_K / 8; ++g) {
-            f32x4 a[2], b[2];
+        for (int g = 0; g < GF_K / (4 * G); ++g) {
+            f32x4 av[2], bv[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (A_ROW) a[i] = *(const f32x4*)(sa + (wm * 64 + i * 32 + r32) * 128 + (((2 * g + half) ^ (r32 & 7)) << 4));
+                const int ra = wm * (T / 2) + i * TS + r, rb = i * (T / 2) + wn * TS + r;
+                if (A_ROW) av[i] = *(const f32x4*)(sa + ra * 128 + (((G * g + grp) ^ (r & 7)) << 4));
                 else
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) a[i][s] = *(const float*)(sa + (8 * g + 4 * half + s) * 512 + (((wm * 64 + i * 32 + r32) * 4) ^ (half << 7)));
-                if (B_ROW) b[i] = *(const f32x4*)(sb + (i * 64 + wn * 32 + r32) * 128 + (((2 * g + half) ^ (r32 & 7)) << 4));
+                    for (int s = 0; s < 4; ++s) av[i][s] = *(const float*)(sa + (4 * (G * g + grp) + s) * (4 * T) + ((ra * 4) ^ (grp * T)));
+                if (B_ROW) bv[i] = *(const f32x4*)(sb + rb * 128 + (((G * g + grp) ^ (r & 7)) << 4));
                 else
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) b[i][s] = *(const float*)(sb + (8 * g + 4 * half + s) * 512 + (((i * 64 + wn * 32 + r32) * 4) ^ (half << 7)));
+                    for (int s = 0; s < 4; ++s) bv[i][s] = *(const float*)(sb + (4 * (G * g + grp) + s) * (4 * T) + ((rb * 4) ^ (grp * T)));
             }
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j][s], a[i][s], acc[i][j], 0, 0, 0);
+                    for (int h = 0; h < 2; ++h) acc[i][h] = Acc::mul(bv[h][s], av[i][s], acc[i][h]);
         }
         GT_VMCNT(0);
         __builtin_amdgcn_s_barrier();
     }
 
-    // lane: row (lane & 31), columns 8 e + 4 half + 0..3 of each 32 x 32 tile
+    // lane: row r, columns 8 e + 4 grp + 0..3 of each TS x TS tile
+    float* const out = (float*)p.out[MODE == GL_DW ? plane : 0];
+    const bool whole = gl_whole(out, p.ldo);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t m = i0 + wm * 64 + i * 32 + r32;
-        if (m >= p.I) continue;
+    for (int e = 0; e < TS * TS / 256; ++e) {
+        const int cl = wn * TS + 8 * e + 4 * grp;
+        f32x4 bg, bu;
+        if (MODE == GL_FWD && !split && j0 + cl < p.J) gl_bias<float>(p, j0 + cl, p.J - j0 - cl, bg, bu);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int cl = wn * 32 + 8 * e + 4 * half;
-            if (MODE == GL_FWD && !SPLIT) {
-                const int n = j0 + cl, cnt = p.J - n < 4 ? p.J - n : 4;
-                const float g[4] = {acc[i][0][4 * e], acc[i][0][4 * e + 1], acc[i][0][4 * e + 2], acc[i][0][4 * e + 3]};
-                const float u[4] = {acc[i][1][4 * e], acc[i][1][4 * e + 1], acc[i][1][4 * e + 2], acc[i][1][4 * e + 3]};
-                if (cnt > 0) gl_fwd_store<float>(p, m, n, cnt, g, u);
+        for (int i = 0; i < 2; ++i) {
+            const int64_t m = i0 + wm * (T / 2) + i * TS + r;
+            if (m >= p.I) continue;
+            f32x4 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v[h] = (f32x4){acc[i][h][4 * e], acc[i][h][4 * e + 1], acc[i][h][4 * e + 2], acc[i][h][4 * e + 3]};
+            if (MODE == GL_FWD && !split) {
+                if (j0 + cl < p.J)
+                    gl_with_act(p.act, [&](auto act) { gl_fwd_put<float, decltype(act)::value>(p, m, j0 + cl, p.J - j0 - cl, v[0] + bg, v[1] + bu); });
                 continue;
             }
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int n = j0 + (MODE == GL_FWD ? 0 : b * 64) + cl, pl = MODE == GL_FWD ? b : plane;
+            for (int h = 0; h < 2; ++h) {
+                const int n = j0 + (MODE == GL_FWD ? 0 : h * (T / 2)) + cl, pl = MODE == GL_FWD ? h : plane;
                 if (n >= p.J) continue;
-                const f32x4 v = {acc[i][b][4 * e], acc[i][b][4 * e + 1], acc[i][b][4 * e + 2], acc[i][b][4 * e + 3]};
-                if (SPLIT) {
-                    *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = v;
-                } else {
-                    float* const o = (float*)p.out[MODE == GL_DW ? plane : 0] + m * p.ldo + n;
-                    if ((p.ldo & 3) == 0 && ((uintptr_t)o & 15) == 0 && n + 4 <= p.J) *(f32x4*)o = v;
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (n + r < p.J) o[r] = v[r];
-                }
+                if (split) *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = v[h];
+                else gl_put4(out + m * p.ldo + n, v[h], p.J - n, whole);
             }
         }
     }
+}
+
+template <int MODE, int T, bool VEC>
+__global__ __launch_bounds__(GF_THREADS) void k_gated_f32(GtArgs q) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    gf_product<MODE, T, VEC>(q, blockIdx.x, gridDim.x, smem);
+}
+template <int T, bool VEC>
+__global__ __launch_bounds__(GF_THREADS) void k_gated_f32_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
+    if (first == dx_first) gf_product<GL_DX, T, VEC>(dx, at, count, smem);
+    else gf_product<GL_DW, T, VEC>(dw, at, count, smem);
 }
 
 }  // namespace dp

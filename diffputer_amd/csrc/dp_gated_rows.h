@@ -114,8 +114,7 @@ __global__ __launch_bounds__(GR_WAVES * 64) void k_gated_rows(GlArgs p) {
             g += red[v][0][t][l];
             u += F == 2 ? red[v][F - 1][t][l] : red[v][0][t][l + 32];
         }
-        const float ga[4] = {g[0], g[1], g[2], g[3]}, ua[4] = {u[0], u[1], u[2], u[3]};
-        gl_fwd_store<T>(p, m, n, cnt, ga, ua);
+        gl_fwd_store<T>(p, m, n, cnt, g, u);
     }
 }
 

@@ -130,14 +130,10 @@ template <int KS, int HI> __device__ __forceinline__ void gt_tr2_2(bf16x4 (&a)[2
 }
 __device__ __forceinline__ bf16x8 gt_join(const bf16x4 (&f)[2]) { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// workgroup -> (slice, tile): neighbouring tiles on one XCD
-template <bool SPLIT> __device__ __forceinline__ int gt_slice(const GlArgs& p, int& slice) {
-    const int t = xcd_remap(blockIdx.x, gridDim.x), tiles = gridDim.x / p.splits;
-    slice = SPLIT ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
-    return SPLIT ? __builtin_amdgcn_readfirstlane(t % tiles) : t;
-}
-// tile -> (plane, row, column): groups of q.group tile rows, column by column within a group
-template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int tile, int& plane, int& ti, int& tj) {
+// workgroup -> slice, and tile -> (plane, row, column): groups of q.group tile rows, column by column within a group
+template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int b, int count, int& slice, int& plane, int& ti, int& tj) {
+    const int t = xcd_remap(b, count), tiles = count / q.g.splits, tile = t % tiles;
+    slice = __builtin_amdgcn_readfirstlane(t / tiles);
     const int per_plane = q.nti * q.ntj;
     plane = MODE == GL_DW ? q.g.zfirst + __builtin_amdgcn_readfirstlane(tile / per_plane) : 0;
     const int tp = tile % per_plane, gsz = q.group * q.ntj, grp = tp / gsz, in = tp - grp * gsz;
@@ -146,8 +142,9 @@ template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int
     tj = __builtin_amdgcn_readfirstlane(in / rows_here);
 }
 
-template <int MODE, int T, bool SPLIT>
-__device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice, char* smem) {
+// workgroup `b` of the launch's `count` that run this product: its tile and slice, neighbouring tiles on one XCD
+template <int MODE, int T>
+__device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, char* smem) {
     using S = GtShape<T>;
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
     constexpr int HR = S::HR, HB = S::HB, MI = S::MI, NJ = S::NJ, NW = S::NW, WN = S::WN;
@@ -157,14 +154,14 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
 
-    int plane, ti, tj;
-    gt_tile<MODE>(q, tile, plane, ti, tj);
+    const bool split = p.splits > 1;
+    int slice, plane, ti, tj;
+    gt_tile<MODE>(q, b, count, slice, plane, ti, tj);
     const int64_t i0 = (int64_t)ti * T;
     const int j0 = tj * (MODE == GL_FWD ? HR : T);
 
     const int nk = (int)((p.C + 63) >> 6);                                 // K-tiles of a segment
-    const int kt0 = SPLIT ? slice * p.kt_per : 0;
-    const int all = nk * (MODE == GL_DX ? 2 : 1), kt1 = SPLIT ? min(kt0 + p.kt_per, all) : all;
+    const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
 
     // ---- loads: a wave moves pieces `wave` and `wave + NW` (1 KiB each) of every half-tile ----
     //   row layout: piece = 8 rows x 128 B; column layout: piece = 1024 / (2 HR) k rows x 2 HR bytes
@@ -328,7 +325,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
     // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
     const int cl = wn * NJ * 16 + (lane >> 4) * 4;
     const int64_t mrow = i0 + wm * (HR / 2) + (lane & 15);
-    if (SPLIT) {
+    if (split) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -346,54 +343,55 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int tile, int slice,
             }
         return;
     }
-    const bool vec = (p.ldo & 3) == 0 && ((uintptr_t)p.out[MODE == GL_DW ? plane : 0] & 7) == 0;
+    if constexpr (MODE == GL_FWD) {
+        gl_with_act(p.act, [&](auto act) {
 #pragma unroll
-    for (int b = 0; b < (MODE == GL_FWD ? 1 : 2); ++b)
+            for (int j = 0; j < NJ; ++j) {
+                const int n = j0 + cl + j * 16, cnt = p.J - n;
+                if (cnt <= 0) continue;
+                f32x4 bg, bu;
+                gl_bias<bf16_t>(p, n, cnt, bg, bu);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int n = j0 + b * HR + cl + j * 16;
-            if (n >= p.J) continue;
-            const bool whole = vec && n + 4 <= p.J;
-            f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = {0.f, 0.f, 0.f, 0.f};
-            if (MODE == GL_FWD) {
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (p.bias[0] && n + r < p.J) bg[r] = bf2f(((const bf16_t*)p.bias[0])[n + r]);
-                    if (p.bias[1] && n + r < p.J) bu[r] = bf2f(((const bf16_t*)p.bias[1])[n + r]);
-                }
-            }
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    const int64_t m = mrow + a * HR + i * 16;
-                    if (m >= p.I) continue;
-                    f32x4 v = acc[a][i][b][j];
-                    if (MODE == GL_FWD) {
-                        const f32x4 g = v + bg, u = acc[a][i][1][j] + bu;
-                        if (p.pre) {                                       // rows of ldpre = J rounded up to 4
-                            *(f32x4*)(p.pre + m * p.ldpre + n) = g;
-                            *(f32x4*)(p.pre + (p.I + m) * p.ldpre + n) = u;
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = gl_act(p.act, g[r]) * u[r];
+                    for (int i = 0; i < MI; ++i) {
+                        const int64_t m = mrow + a * HR + i * 16;
+                        if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[a][i][0][j] + bg, acc[a][i][1][j] + bu);
                     }
-                    bf16_t* const o = (bf16_t*)p.out[MODE == GL_DW ? plane : 0] + m * p.ldo + n;
-                    if (whole) *(uint2*)o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-                    else
+            }
+        });
+    } else {
+        bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? plane : 0];
+        const bool whole = gl_whole(out, p.ldo);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (n + r < p.J) o[r] = f2bf(v[r]);
-                }
-        }
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = j0 + b * HR + cl + j * 16, cnt = p.J - n;
+                if (cnt <= 0) continue;
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) {
+                        const int64_t m = mrow + a * HR + i * 16;
+                        if (m < p.I) gl_put4(out + m * p.ldo + n, acc[a][i][b][j], cnt, whole);
+                    }
+            }
+    }
 }
 
-template <int MODE, int T, bool SPLIT>
+template <int MODE, int T>
 __global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile(GtArgs q) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int slice;
-    const int tile = gt_slice<SPLIT>(q.g, slice);
-    gt_product<MODE, T, SPLIT>(q, tile, slice, smem);
+    gt_product<MODE, T>(q, blockIdx.x, gridDim.x, smem);
+}
+// both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, [n0, gridDim) the other
+template <int T>
+__global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
+    if (first == dx_first) gt_product<GL_DX, T>(dx, at, count, smem);
+    else gt_product<GL_DW, T>(dw, at, count, smem);
 }
 
 // copy of a matrix whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero

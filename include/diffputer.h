@@ -217,7 +217,8 @@ int dp_linear(int dtype, const void* A, const void* W, const float* bias, void* 
  *                   (diffusion_utils.py:100-101) runs in the epilogue of the mlp.6 GEMM instead of a kernel of its own;
  *                   bit-identical results.
  *   "gated_kernel"  which kernel runs the products of dp_gated_linear and its backward: 0 (default) = by size and alignment, 1 = the
- *                   general kernel (any size, stride and type), 128 / 256 = the tile kernels (bf16: of that tile; float32 has one).
+ *                   general kernel (any size, stride and type), 64 / 128 / 256 = the tile kernel of that tile
+ *                   (bf16 has 128 and 256, float32 64 and 128: the nearest).
  *   "gated_splits"  slices of the contraction of those products: 0 (default) = by size, else that many (at most one per K-tile).  The
  *                   order of sums, and with it the last bits, depend on it.
  */

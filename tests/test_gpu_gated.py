@@ -137,25 +137,26 @@ def tune():
 
 
 @pytest.mark.parametrize("M,K,N", [(1, 8, 8), (40, 64, 64), (70, 200, 40), (129, 64, 65), (257, 72, 129), (300, 136, 264), (513, 1032, 264), (600, 71, 300)])
-@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (128, 0), (128, 3), (256, 0), (256, 2), (256, 5)])
+@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (128, 0), (128, 1), (128, 3), (256, 0), (256, 1), (256, 5)])
 def test_every_kernel(tune, kernel, splits, M, K, N):
     tune(kernel, splits)
     check(*make(M, K, N, "bf16", seed=M + K), act="silu")
 
 
 @pytest.mark.parametrize("M,K,N", [(1, 8, 8), (40, 64, 64), (70, 200, 40), (129, 64, 65), (257, 73, 129), (300, 136, 264), (513, 1032, 264), (200, 31, 66)])
-@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (128, 0), (128, 3), (128, 7)])
+@pytest.mark.parametrize("kernel,splits", [(1, 0), (1, 3), (64, 0), (64, 1), (64, 4), (128, 0), (128, 1), (128, 3)])
 def test_every_kernel_f32(tune, kernel, splits, M, K, N):
     tune(kernel, splits)
     check(*make(M, K, N, "f32", seed=M + K), act="silu")
 
 
-@pytest.mark.parametrize("kernel", [1, 128, 256])
-def test_every_kernel_strides(tune, kernel):
-    """A column range of a wider table: aligned rows are read where they are (the columns beside them hold NaN), others copied."""
+@pytest.mark.parametrize("kernel,dtype", [(1, "bf16"), (128, "bf16"), (256, "bf16"), (1, "f32"), (64, "f32"), (128, "f32")])
+def test_every_kernel_strides(tune, kernel, dtype):
+    """A column range of a wider table (the columns beside it hold NaN): aligned rows are read where they are, others copied or
+    read by narrower loads."""
     from diffputer_amd.gated import gated_linear
     tune(kernel, 0)
-    x, wg, wu, bg, bu, dh = make(300, 72, 136, "bf16", seed=6)
+    x, wg, wu, bg, bu, dh = make(300, 72, 136, dtype, seed=6)
     ref = Ref(x, wg, wu, bg, bu, dh, "silu")
     for off in (0, 8, 3):
         wide = torch.full((300, 96), float("nan"), dtype=x.dtype, device=DEV)
@@ -166,6 +167,23 @@ def test_every_kernel_strides(tune, kernel):
         close(h, ref.h, ref.eh, "h")
         for name, g in zip(("x", "wg", "wu", "bg", "bu"), torch.autograd.grad(h, leaves, dh.to(DEV))):
             close(g, getattr(ref, "d" + name), getattr(ref, "ed" + name), "d" + name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kernel", [0, 1, 128])
+def test_some_gradients_on_every_kernel(tune, kernel, dtype):
+    """dx alone, one weight's gradient alone, both: the products run in other launches than all together."""
+    from diffputer_amd.gated import gated_linear
+    tune(kernel, 0)
+    x, wg, wu, bg, bu, dh = make(300, 72, 136, dtype, seed=7)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    names = ("x", "wg", "wu", "bg", "bu")
+    for want in ((0,), (1,), (2,), (1, 2), (0, 2), (3,), (0, 1, 2)):
+        dev = [t.to(DEV) for t in (x, wg, wu, bg, bu)]
+        for i in want:
+            dev[i].requires_grad_()
+        for i, g in zip(want, torch.autograd.grad(gated_linear(*dev), [dev[i] for i in want], dh.to(DEV))):
+            close(g, getattr(ref, "d" + names[i]), getattr(ref, "ed" + names[i]), "d" + names[i])
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
