@@ -11,6 +11,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libdiffputer_hip.so")
+TORCH_PATH = os.path.join(_HERE, "csrc", "dp_torch.so")
 
 DP_DTYPE_F32 = 0
 DP_DTYPE_BF16 = 1
@@ -83,6 +84,28 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch_side = None
+
+
+def torch_side():
+    """The Python module csrc/dp_torch.so (tensors in, tensors out; it calls the library's C ABI); loaded once, raises if it has
+    not been built."""
+    global _torch_side
+    if _torch_side is None:
+        load()
+        if not os.path.exists(TORCH_PATH):
+            raise DiffputerError(f"{TORCH_PATH} not found: the HIP extension is not built. Run `python -c 'import __graft_entry__ as g; g.build()'`.")
+        import importlib.machinery
+        import importlib.util
+        loader = importlib.machinery.ExtensionFileLoader("dp_torch", TORCH_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("dp_torch", loader))
+        loader.exec_module(module)
+        import torch
+        module.set_errors(DiffputerError, torch.OutOfMemoryError)
+        _torch_side = module
+    return _torch_side
 
 
 def check(rc: int, what: str):

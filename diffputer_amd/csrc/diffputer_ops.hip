@@ -118,24 +118,33 @@ static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
     for (int k = 0; k < 2; ++k) {
         const GlRate& r = bf ? GL_RATES_BF16[k] : GL_RATES_F32[k];
         if (forced > 1 && r.T != (bf ? std::max(forced, 128) : std::min(forced, 128))) continue;
-        for (int a : slices)
-            for (int b : slices) {
-                if (n == 1 && b > 1) break;
-                GlPlan pl[2] = {gl_shape(s[0], r.T, kdepth, a), n > 1 ? gl_shape(s[1], r.T, kdepth, b) : GlPlan{}};
-                bool fits = true;
-                for (int i = 0; i < n; ++i) fits = fits && (pl[i].splits == 1 || gl_part_bytes(s[i]) * pl[i].splits <= (size_t)128 << 20);
-                if (!fits && (a > 1 || b > 1)) continue;
-                const double c = gl_cost(r, pl, s, n);
-                if (c < least) {
-                    least = c;
-                    for (int i = 0; i < n; ++i) best[i] = pl[i];
-                }
+        GlPlan whole[2];
+        int64_t longest = 1;
+        for (int i = 0; i < n; ++i) {
+            whole[i] = gl_shape(s[i], r.T, kdepth, 1);
+            longest = std::max<int64_t>(longest, whole[i].kt_per);
+        }
+        for (int a : slices) {                                    // the longer contraction in `a` slices, the other in slices as long
+            if (a > 1 && longest < 2 * a) break;
+            const int64_t per = ceil_div<int64_t>(longest, a);
+            GlPlan pl[2];
+            bool fits = true;
+            for (int i = 0; i < n; ++i) {
+                pl[i] = gl_shape(s[i], r.T, kdepth, (int)ceil_div<int64_t>(whole[i].kt_per, per));
+                fits = fits && (pl[i].splits == 1 || gl_part_bytes(s[i]) * pl[i].splits <= (size_t)128 << 20);
             }
+            if (!fits && a > 1) continue;
+            const double c = gl_cost(r, pl, s, n);
+            if (c < least) {
+                least = c;
+                for (int i = 0; i < n; ++i) best[i] = pl[i];
+            }
+        }
     }
 }
 static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < (int64_t)1 << 22; }
 
-static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
+static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
     const int forced = forced_kernel();
     if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0) return {GL_ROWS, 0, 1, 1, 1, 1};
     if (tile && forced != 1) {
@@ -149,13 +158,52 @@ static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
     return gl_shape(s, 0, GG_K, (int)std::max<int64_t>(want, 1));
 }
 // both backward products: in one launch on a tile kernel, or two plans of their own
-static bool gl_plan_both(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
+static GlPlan gl_plan(const GlShape& s, int dtype, bool tile);
+static bool gl_plan_both_new(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
     if (tile && forced_kernel() != 1) {
         gl_choose(s, 2, dtype, pl);
         if (gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]) && pl[0].wgs + pl[1].wgs < (int64_t)1 << 22) return true;
     }
     for (int i = 0; i < 2; ++i) pl[i] = gl_plan(s[i], dtype, tile);
     return false;
+}
+// A choice takes a microsecond or two and is asked for several times per call (workspace query, check, launch): the last ones are
+// remembered by everything that they depend on, sizes and settings.
+struct GlKey {
+    int64_t I, C;
+    int J, mode, planes, dtype, tile, kernel, splits, both;
+    bool operator==(const GlKey& o) const {
+        return I == o.I && C == o.C && J == o.J && mode == o.mode && planes == o.planes && dtype == o.dtype && tile == o.tile && kernel == o.kernel && splits == o.splits && both == o.both;
+    }
+};
+struct GlMemo { GlKey key; GlPlan pl[2]; bool one; };
+static GlMemo& gl_memo(const GlShape& s, int dtype, bool tile, int both, bool& known) {
+    static thread_local GlMemo memo[64];
+    const GlKey k = {s.I, s.C, s.J, s.mode + 1, s.planes, dtype, tile, forced_kernel(), g_gated_splits.load(std::memory_order_relaxed), both};
+    GlMemo& m = memo[((uint64_t)(s.I * 31 + s.C) * 31 + (uint64_t)s.J * 7 + (uint64_t)(s.mode * 5 + both * 3 + dtype)) % 64];
+    known = m.key == k;
+    m.key = k;
+    return m;
+}
+static GlPlan gl_plan(const GlShape& s, int dtype, bool tile) {
+    bool known;
+    GlMemo& m = gl_memo(s, dtype, tile, 0, known);
+    if (!known) m.pl[0] = gl_plan_new(s, dtype, tile);
+    return m.pl[0];
+}
+// (the second product's shape follows from the first's)
+static bool gl_plan_both(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
+    bool known;
+    GlMemo& m = gl_memo(s[0], dtype, tile, 1, known);
+    if (!known) {
+        GlPlan p[2];
+        const bool one = gl_plan_both_new(s, dtype, tile, p);     // may use the memo itself
+        GlMemo& again = gl_memo(s[0], dtype, tile, 1, known);
+        again.pl[0] = p[0]; again.pl[1] = p[1];
+        again.one = one;
+    }
+    pl[0] = m.pl[0]; pl[1] = m.pl[1];
+    return m.one;
 }
 static size_t gl_split_bytes(const GlShape& s, const GlPlan& c) { return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0; }
 
@@ -486,15 +534,13 @@ size_t dp_gated_linear_pre_bytes(int64_t M, int N) {
     return (size_t)std::max<int64_t>(M, 1) * 2 * gl_ldp(N) * 4;
 }
 
-size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, int64_t M, int N, int K, int backward) {
+size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, int64_t M, int N, int K, int grads) {
     if (gl_check("dp_gated_linear_workspace_bytes", dtype, M, N, K, 0)) return 0;
+    if (grads < 0 || grads > 15) { fail(DP_EINVAL, "dp_gated_linear_workspace_bytes: grads %d", grads); return 0; }
     if (M == 0) return 256;
     GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
-    if (!backward) return std::max<size_t>(gl_fwd_carve(dtype, in, nullptr).bytes, 256);
-    size_t most = 256;                                            // whichever gradients a call asks for
-    for (int planes = 0; planes < 3; ++planes)
-        for (int dx = 0; dx < 2; ++dx) most = std::max(most, gl_bwd_carve(dtype, in, planes, dx, nullptr).bytes);
-    return most;
+    if (grads == DP_GATED_FORWARD) return std::max<size_t>(gl_fwd_carve(dtype, in, nullptr).bytes, 256);
+    return std::max<size_t>(gl_bwd_carve(dtype, in, ((grads & DP_GATED_DW_GATE) != 0) + ((grads & DP_GATED_DW_UP) != 0), (grads & DP_GATED_DX) != 0, nullptr).bytes, 256);
 }
 
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
@@ -531,7 +577,8 @@ int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gat
         if (!x || !w_gate || !w_up || !pre || !dh) return fail(DP_EINVAL, "dp_gated_linear_bwd: null pointer");
         if (ldx < K || ldw < K || lddh < N) return fail(DP_EINVAL, "dp_gated_linear_bwd: row strides ldx=%lld ldw=%lld lddh=%lld are shorter than a row (K=%d, N=%d)", (long long)ldx, (long long)ldw, (long long)lddh, K, N);
         if (!aligned(pre, 16)) return fail(DP_EINVAL, "dp_gated_linear_bwd: pre must be 16-byte aligned");
-        const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, 1);
+        const int grads = (dx ? DP_GATED_DX : 0) | (dw_gate ? DP_GATED_DW_GATE : 0) | (dw_up ? DP_GATED_DW_UP : 0) | DP_GATED_DB;
+        const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, grads);
         if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear_bwd: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
     }
     for (const void* p : {x, w_gate, w_up, dh, (const void*)dx, (const void*)dw_gate, (const void*)dw_up, (const void*)db_gate, (const void*)db_up})

@@ -288,7 +288,7 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  *                for the backward pass; the layout is the library's own
  * Any strides, element-aligned pointers, 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
  * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
- * (workspace >= dp_gated_linear_workspace_bytes(.., backward) for the same arguments, 256-byte aligned; calls that may
+ * (workspace >= dp_gated_linear_workspace_bytes(.., grads) for the same arguments, grads = DP_GATED_FORWARD, or the DP_GATED_D.. that dp_gated_linear_bwd is asked for, 256-byte aligned; calls that may
  * overlap in time need workspaces of their own), and may be captured into a graph.  bf16 is fastest where x and the weights
  * have rows that start on 16 bytes and K % 8 == 0: other rows are first copied to the workspace.
  *
@@ -296,9 +296,14 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  * db_up [N]: contiguous, overwritten, each may be NULL (not wanted).  M = 0 writes zeros to the weights' gradients.
  * bf16: dg and du are rounded to bf16 once, as the operands of the three products; bias gradients sum them unrounded.
  */
+#define DP_GATED_FORWARD 0
+#define DP_GATED_DX      1
+#define DP_GATED_DW_GATE 2
+#define DP_GATED_DW_UP   4
+#define DP_GATED_DB      8   /* either bias gradient */
 size_t dp_gated_linear_pre_bytes(int64_t M, int N);
 size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw,
-                                       int64_t M, int N, int K, int backward);
+                                       int64_t M, int N, int K, int grads);
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
                     void* h, int64_t ldh, void* pre, int64_t M, int N, int K, int act, void* workspace, size_t workspace_bytes, void* stream);
 int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,

@@ -301,6 +301,30 @@ def test_only_the_wanted_gradients():
         close(g, getattr(ref, "d" + name), getattr(ref, "ed" + name), name)
 
 
+def test_first_derivatives_only():
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = make(20, 12, 8, "f32", seed=16)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, wg, wu, bg, bu)]
+    plain = torch.autograd.grad(gated_linear(*leaves), leaves, dh.to(DEV))
+    grads = torch.autograd.grad(gated_linear(*leaves), leaves, dh.to(DEV), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    with pytest.raises(RuntimeError):                               # the second graph does not lead to a leaf
+        torch.autograd.grad(grads[0].sum(), leaves[1], retain_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives only"):
+        grads[0].sum().backward()
+
+
+def test_changed_inputs_are_noticed():
+    """autograd refuses a backward pass whose saved inputs were overwritten in between."""
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(20, 12, 8, "f32", seed=16)]
+    wg.requires_grad_()
+    h = gated_linear(x, wg, wu, bg, bu)
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, wg, dh)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_no_rows(dtype):
     from diffputer_amd.gated import gated_linear

@@ -120,6 +120,9 @@ def test_gated_sizes():
         for M, N, K in ((0, 5, 5), (1, 1, 1), (1, 2048, 1024), (24, 8192, 4096), (16384, 64, 9), (4096, 2048, 1024), ((1 << 29) - 1, 64, 64)):
             for backward in (0, 1):
                 assert ws(dtype, M, N, K, backward) >= 256
+    assert ws(0, 10, 10, 10, 16) == 0 and ws(0, 10, 10, 10, -1) == 0
+    for grads in range(1, 16):
+        assert ws(1, 300, 200, 100, grads) >= 2 * 300 * 256 * 2
     # a float32 plane of a large batch passes 32 bits
     assert ws(0, 1 << 20, 4096, 64, 1) >= 2 * (1 << 20) * 4096 * 4
     # rows that are not aligned are copied: x and both weights
