@@ -11,6 +11,7 @@
 
 #include "dp_gated.h"
 #include "dp_gated_f32.h"
+#include "dp_gated_ring.h"
 #include "dp_gated_rows.h"
 #include "dp_gated_tile.h"
 #include "dp_grads.h"
@@ -41,9 +42,9 @@ static int forced_kernel() { return g_gated_kernel.load(std::memory_order_relaxe
 // dynamic LDS of the tile kernels, once per device
 template <int MODE> static hipError_t gt_attributes() {
     const struct { const void* k; int lds; } all[] = {
-        {(const void*)k_gated_tile<MODE, 256>, GtShape<256>::LDS}, {(const void*)k_gated_tile<MODE, 128>, GtShape<128>::LDS},
+        {(const void*)k_gated_tile<MODE>, GT_LDS}, {(const void*)k_gated_ring<MODE>, GS_LDS},
         {(const void*)k_gated_f32<MODE, 128, false>, GfShape<128>::LDS}, {(const void*)k_gated_f32<MODE, 128, true>, GfShape<128>::LDS},
-        {(const void*)k_gated_tile_both<256>, GtShape<256>::LDS}, {(const void*)k_gated_tile_both<128>, GtShape<128>::LDS},
+        {(const void*)k_gated_tile_both, GT_LDS}, {(const void*)k_gated_ring_both, GS_LDS},
         {(const void*)k_gated_f32_both<128, false>, GfShape<128>::LDS}, {(const void*)k_gated_f32_both<128, true>, GfShape<128>::LDS}};
     for (const auto& a : all) {
         const hipError_t e = hipFuncSetAttribute(a.k, hipFuncAttributeMaxDynamicSharedMemorySize, a.lds);
@@ -88,36 +89,37 @@ static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
     return pl;
 }
 
-// Microseconds of a launch of up to two products, by what the kernels measured (bf16: 64 deep K-tiles, float32: 32 deep).  A K-tile takes
-// `one` where a workgroup has its CU to itself and `full` where the CU holds `per_cu` of them; both from launches that
-// fill the chip and launches that do not (K-loops of 64 K-tiles).  A split launch pays for its partial sums: written and read at
-// about 3 TB/s, and a launch more.
-struct GlRate { int T, per_cu; double one, full; };
-static const GlRate GL_RATES_BF16[] = {{256, 1, 1.70, 1.70}, {128, 2, 0.70, 1.04}};
-static const GlRate GL_RATES_F32[] = {{128, 2, 1.90, 3.50}, {64, 4, 0.60, 1.85}};
+// Microseconds of a launch of up to two products, from what the kernels measured with 64 to 4096 workgroups and K-loops of 16 and
+// 64 K-tiles: a K-step of `depth` takes `one` where a workgroup has its CU to itself and `full` where the CU holds `per_cu` of
+// them; `fixed` is what a launch takes beyond its K-steps, `round` what every further round of workgroups adds to that.  A split launch
+// pays for its partial sums, written and read at about 4.5 TB/s, and a launch more.
+struct GlRate { int T, depth, per_cu; double one, full, fixed, round; };
+static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.49, 1.49, 10.4, 8.0}, {128, 32, 2, 0.29, 0.62, 6.0, 1.0}};
+static const GlRate GL_RATES_F32[] = {{128, GF_K, 2, 2.10, 3.80, 9.0, 4.0}, {64, GF_K, 4, 0.70, 2.05, 4.0, 1.0}};
 static double gl_cost(const GlRate& r, const GlPlan* pl, const GlShape* s, int n) {
     double wgs = 0, work = 0, longest = 0, join = 0;
     for (int i = 0; i < n; ++i) {
         wgs += (double)pl[i].wgs;
         work += (double)pl[i].wgs * pl[i].kt_per;
         longest = std::max(longest, (double)pl[i].kt_per);
-        if (pl[i].splits > 1) join = std::max(join, 5.0) + (double)s[i].I * s[i].J * (s[i].mode == GL_DX ? 1 : 2) * 4 * 2 * pl[i].splits / 3.0e6;
+        if (pl[i].splits > 1) join = std::max(join, 5.0) + (double)s[i].I * s[i].J * (s[i].mode == GL_DX ? 1 : 2) * 4 * 2 * pl[i].splits / 4.5e6;
     }
     const double slots = 256.0 * r.per_cu;
     const double step = wgs <= 256 ? r.one : wgs >= slots ? r.full : r.one + (r.full - r.one) * (wgs - 256) / (slots - 256);
     const double rounds = wgs <= slots ? longest : std::max(work / slots + 0.5 * longest * (fmod(wgs, slots) != 0), longest);
-    return rounds * step + join;
+    return r.fixed + r.round * std::max(0.0, ceil(wgs / slots) - 1.0) + rounds * step + join;
 }
 
 // The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass).
 static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
     const bool bf = dtype == DP_DTYPE_BF16;
-    const int forced = forced_kernel(), kdepth = bf ? 64 : GF_K;
+    const int forced = forced_kernel();
     static const int slices[] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
     double least = 1e300;
     for (int k = 0; k < 2; ++k) {
         const GlRate& r = bf ? GL_RATES_BF16[k] : GL_RATES_F32[k];
         if (forced > 1 && r.T != (bf ? std::max(forced, 128) : std::min(forced, 128))) continue;
+        const int kdepth = r.depth;
         GlPlan whole[2];
         int64_t longest = 1;
         for (int i = 0; i < n; ++i) {
@@ -211,8 +213,8 @@ template <int MODE>
 static int gt_launch(const GtArgs& q, const GlPlan& pl, bool bf, bool vec, hipStream_t st) {
     const dim3 grid((unsigned)pl.wgs);
     if (bf) {
-        if (pl.T == 256) hipLaunchKernelGGL((k_gated_tile<MODE, 256>), grid, dim3(GtShape<256>::THREADS), GtShape<256>::LDS, st, q);
-        else hipLaunchKernelGGL((k_gated_tile<MODE, 128>), grid, dim3(GtShape<128>::THREADS), GtShape<128>::LDS, st, q);
+        if (pl.T == 256) hipLaunchKernelGGL((k_gated_tile<MODE>), grid, dim3(GT_THREADS), GT_LDS, st, q);
+        else hipLaunchKernelGGL((k_gated_ring<MODE>), grid, dim3(GS_THREADS), GS_LDS, st, q);
     } else if (pl.T == 128) {
         if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, 128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, q);
         else hipLaunchKernelGGL((k_gated_f32<MODE, 128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, q);
@@ -271,8 +273,8 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], boo
     const int dx_first = c[0].kt_per >= c[1].kt_per, n0 = (int)c[dx_first ? 0 : 1].wgs;
     const dim3 grid((unsigned)(c[0].wgs + c[1].wgs));
     if (sizeof(T) == 2) {
-        if (c[0].T == 256) hipLaunchKernelGGL((k_gated_tile_both<256>), grid, dim3(GtShape<256>::THREADS), GtShape<256>::LDS, st, dx, dw, n0, dx_first);
-        else hipLaunchKernelGGL((k_gated_tile_both<128>), grid, dim3(GtShape<128>::THREADS), GtShape<128>::LDS, st, dx, dw, n0, dx_first);
+        if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, grid, dim3(GT_THREADS), GT_LDS, st, dx, dw, n0, dx_first);
+        else hipLaunchKernelGGL(k_gated_ring_both, grid, dim3(GS_THREADS), GS_LDS, st, dx, dw, n0, dx_first);
     } else if (c[0].T == 128) {
         if (vec) hipLaunchKernelGGL((k_gated_f32_both<128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
         else hipLaunchKernelGGL((k_gated_f32_both<128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
@@ -322,14 +324,6 @@ struct Carver {
     size_t off = 0;
     char* take(size_t n) { const size_t o = off; off += round_up<size_t>(n, 256); return base ? base + o : (char*)nullptr; }
 };
-static int gt_pack(GlOp& op, void* to, int64_t ldk, int64_t rows, hipStream_t st) {
-    const int64_t n = rows * (ldk / 8);
-    hipLaunchKernelGGL(k_gated_pack, dim3((unsigned)std::min<int64_t>(ceil_div<int64_t>(n, 256), 8192)), dim3(256), 0, st, (const bf16_t*)op.p, op.ld, (bf16_t*)to, ldk, rows, op.cols);
-    DP_LAUNCH_CHECK("k_gated_pack");
-    op = {to, ldk, ldk};
-    return DP_OK;
-}
-
 // x and both weights as the products read them: where they are, or copied to the workspace
 struct GlIn {
     GlOp x, wg, wu;
@@ -342,9 +336,21 @@ struct GlIn {
         pw = o.pack_w ? c.take((size_t)2 * N * o.ldk * 2) : nullptr;
     }
     int pack(bool need_x, bool need_w, hipStream_t st) {
-        int rc;
-        if (o.pack_x && need_x && (rc = gt_pack(x, px, o.ldk, M, st))) return rc;
-        if (o.pack_w && need_w && ((rc = gt_pack(wg, pw, o.ldk, N, st)) || (rc = gt_pack(wu, pw + (size_t)N * o.ldk * 2, o.ldk, N, st)))) return rc;
+        GlPack p = {{}, o.ldk, K, 0};
+        int64_t rows = 0;
+        auto add = [&](GlOp& op, char* to, int64_t n) {
+            p.m[p.n++] = {(const bf16_t*)op.p, (bf16_t*)to, op.ld, n};
+            rows += n;
+            op = {to, o.ldk, o.ldk};
+        };
+        if (o.pack_x && need_x) add(x, px, M);
+        if (o.pack_w && need_w) {
+            add(wg, pw, N);
+            add(wu, pw + (size_t)N * o.ldk * 2, N);
+        }
+        if (p.n == 0) return DP_OK;
+        hipLaunchKernelGGL(k_gated_pack, dim3((unsigned)std::min<int64_t>(ceil_div<int64_t>(rows * (o.ldk / 8), 256), 8192)), dim3(256), 0, st, p);
+        DP_LAUNCH_CHECK("k_gated_pack");
         return DP_OK;
     }
     // contraction length of the forward product: the copies' padding belongs to it (zeros on both sides)

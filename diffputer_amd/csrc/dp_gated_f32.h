@@ -15,7 +15,7 @@
 //   column layout: LDS holds k rows of 4 T bytes as they are in memory, four ds_read_b32; the bytes of k row k are stored with
 //   their place xor'ed by T * ((k / 4) % G), so that the G k's of a read use all banks.
 #pragma once
-#include "dp_gated_tile.h"
+#include "dp_gated_lds.h"
 
 namespace dp {
 

@@ -1,0 +1,264 @@
+// bf16 products of the gated projection with fewer than 256 tiles of 256 x 256 (dp_gated.h has the three products and their
+// operands): 128 x 128 tile, 4 waves of 64 x 64, K-steps of 32 in a ring of five LDS slots, two workgroups per CU.
+//
+// Such launches give a CU one or two workgroups and are bound by the latency of a K-step, not by the matrix pipes: nothing of a
+// step waits for itself.  While a step's products run, the fragments of the next one are read into a second set of registers
+// and the loads of the step five ahead go out, interleaved with the products; the only waits are one per step, for loads
+// that went out four steps before and for reads whose latency the products have covered, and one barrier.  Against the
+// four-phase schedule of the 256 x 256 kernel at this tile: 64 k's take 0.51 instead of 0.92 us with one workgroup on a CU in
+// four, 0.59 instead of 1.02 with one on each, 1.24 instead of 1.20 with two on each (64-byte row segments: half a cache line per request).
+//   step s:   { load step s + 5 into the slot of step s ; read fragments of s + 1 ; products of s ; wait ; barrier }
+//   RAW  step s + 1 was loaded in step s - 4 and waited for (all but the three newest steps' loads) at the end of step s - 1;
+//   WAR  the slot of step s was read in step s - 1, whose end every wave has passed with its reads done.
+// Steps past the end are "loaded" with no bytes (zeros, no traffic): every count holds for any number of steps.
+// Masking as in the 256 x 256 kernel: what does not exist lies behind the buffer's end, or is asked for there.
+// GL_FWD: the first 64 B rows are gate rows, the others the up rows of the same columns: one lane ends with g and u of the same
+// elements.
+#pragma once
+#include "dp_gated_lds.h"
+
+namespace dp {
+
+constexpr int GS_T = 128, GS_THREADS = 256;
+constexpr int GS_NB = 5, GS_STEP = GS_T * 128, GS_LDS = GS_NB * GS_STEP;   // ring slots; bytes of a slot (A, then B)
+constexpr int GS_MI = GS_T / 32, GS_NJ = GS_T / 64, GS_NP = GS_T / 64;     // m-tiles; n-tiles of a half; loads of a wave, operand and step
+
+// 16 bytes per lane from byte `off` of [base, base + records) to LDS byte `lds` on; zeros where a lane is outside.  In assembly so
+// that the compiler does not wait for loads in flight before every LDS read (there is no register result: the waits for what
+// arrives in LDS are the counted ones below).
+__device__ __forceinline__ void gs_load(const char* base, unsigned records, unsigned off, unsigned lds) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const uint64_t b = (uint64_t)base;
+    const u32x4 rs = {(unsigned)b, (unsigned)(b >> 32) & 0xffffu, records, 0x00027000u};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rs) : "memory");
+}
+__device__ __forceinline__ unsigned gs_clip(int64_t n) { return n <= 0 ? 0u : n > 0x7fffffff ? 0x7fffffffu : (unsigned)n; }
+
+template <int MODE>
+__device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, char* smem) {
+    constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
+    constexpr int T = GS_T, NB = GS_NB, STEP = GS_STEP, MI = GS_MI, NJ = GS_NJ, NP = GS_NP, NI = 2 * NP;
+    constexpr unsigned OUTSIDE = 0x80000000u;
+    const GlArgs& p = q.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const bool split = p.splits > 1;
+    int slice, plane, ti, tj;
+    gt_tile<MODE>(q, b, count, slice, plane, ti, tj);
+    const int64_t i0 = (int64_t)ti * T;
+    const int j0 = tj * (MODE == GL_FWD ? T / 2 : T);
+    const int nk = (int)((p.C + 31) >> 5);                                 // K-steps of a segment
+    const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
+
+    // ---- loads: a wave moves pieces wave, wave + 4, .. (1 KiB) of each operand's T x 32 image ----
+    //   row layout: piece = 16 rows x 64 B, 16-byte chunk c of row r at c ^ ((r >> 2) & 3)
+    //   column layout: k rows of 2 T bytes, piece = 512 / T of them, 32-byte slot s of k row k at s ^ g(k)
+    const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
+    constexpr int KR = 512 / T, CH = T / 8;                                // k rows of a piece, 16-byte chunks of a k row
+    auto g_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
+    const int r16 = lane >> 2, c4 = (lane & 3) ^ ((lane >> 4) & 3);
+    unsigned va[NP], vb[NP];
+#pragma unroll
+    for (int s = 0; s < NP; ++s) {
+        const int piece = wave + s * 4;
+        const int k = piece * KR + lane / CH, c = (lane % CH) ^ (2 * g_of(k));
+        const int rb = MODE == GL_FWD ? (piece * 16 + r16) & (T / 2 - 1) : piece * 16 + r16;   // FWD: row within the gate's or the up's half
+        va[s] = A_ROW ? (unsigned)((piece * 16 + r16) * lda + c4 * 16) : (unsigned)(k * lda + c * 16);
+        vb[s] = B_ROW ? (unsigned)(rb * ldb + c4 * 16) : (unsigned)(k * ldb + c * 16);
+    }
+    const bool tail_out = B_ROW && (p.C & 31) && c4 * 8 >= (int)(p.C & 31);                    // chunks past the contraction's end, last K-step
+
+    // A stream walks an operand K-step by K-step.  Row layout: rows that do not exist lie behind `full` bytes whatever the step.
+    // Column layout: a step has 32 k rows, the segment's last one `last` bytes.
+    struct Stream { const char* at; unsigned full, last; };
+    auto open = [&](const GlOp& op, bool row, int64_t first, int64_t size, int64_t kk) {
+        const int64_t ld = op.ld * 2;
+        Stream st;
+        st.at = (const char*)op.p + (row ? first * ld + kk * 64 : kk * 32 * ld + first * 2);
+        st.full = gs_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 31 * ld + (op.cols - first) * 2);
+        st.last = row ? st.full : gs_clip((p.C - 1 - (int64_t)(nk - 1) * 32) * ld + (op.cols - first) * 2);
+        return st;
+    };
+    auto seg_of = [&](int kt) { return MODE == GL_DX && kt >= nk ? 1 : 0; };
+    auto open_a = [&](int kt) { return open(p.A[MODE == GL_DX ? seg_of(kt) : MODE == GL_DW ? plane : 0], A_ROW, i0, p.I, kt - seg_of(kt) * nk); };
+    auto open_b = [&](int kt, int half) { return open(p.B[MODE == GL_FWD ? half : seg_of(kt)], B_ROW, j0, p.J, kt - seg_of(kt) * nk); };
+    Stream sa = open_a(kt0), sb = open_b(kt0, 0), su = sb;
+    if (MODE == GL_FWD) su = open_b(kt0, 1);
+    const int64_t step_a = A_ROW ? 64 : 32 * lda, step_b = B_ROW ? 64 : 32 * ldb;
+    int skt = kt0;                                                         // next K-step to load
+    unsigned slot_in = gt_lds(smem);                                       // its slot
+    const unsigned lds0 = slot_in;
+    unsigned rec_a, rec_b, rec_u;
+    bool s_tail;
+    auto stage_begin = [&]() {
+        const int kk = skt - seg_of(skt) * nk;
+        const bool live = skt < kt1, last = kk == nk - 1;
+        rec_a = !live ? 0u : last ? sa.last : sa.full;
+        rec_b = !live ? 0u : last ? sb.last : sb.full;
+        rec_u = !live ? 0u : su.full;
+        s_tail = last;
+    };
+    auto stage_one = [&](int i) {                                          // load i of NI
+        const bool is_b = i >= NP;
+        const int s = is_b ? i - NP : i;
+        unsigned vo = is_b ? vb[s] : va[s];
+        if (B_ROW && s_tail && tail_out) vo = OUTSIDE;
+        const unsigned dst = slot_in + (is_b ? STEP / 2 : 0) + (wave + s * 4) * 1024;
+        if (!is_b) gs_load(sa.at, rec_a, vo, dst);
+        else if (MODE == GL_FWD && s >= NP / 2) gs_load(su.at, rec_u, vo, dst);
+        else gs_load(sb.at, rec_b, vo, dst);
+    };
+    auto stage_end = [&]() {
+        ++skt;
+        sa.at += step_a;
+        sb.at += step_b;
+        if (MODE == GL_FWD) su.at += step_b;
+        if (MODE == GL_DX && skt == nk) { sa = open_a(skt); sb = open_b(skt, 0); }
+        slot_in += STEP;
+        if (slot_in == lds0 + NB * STEP) slot_in = lds0;
+    };
+
+    // ---- fragment reads: LDS byte addresses; column layout: the tile's number is xor'ed into the slot bits ----
+    const unsigned fa = A_ROW ? wm * MI * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4) : 0;              // row layout: + 1024 per 16 rows
+    const unsigned fb = B_ROW ? wn * NJ * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4) : 0;
+    const int krow = (lane >> 4) * 8 + ((lane >> 2) & 3);
+    const unsigned fc = krow * T * 2 + (g_of(krow) << 5) + (lane & 3) * 8;
+    auto tr = [&](unsigned at) {
+        typedef DP_LDS_AS bf16x4* ptr;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(at + 4 * T * 2));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    struct Frags { bf16x8 a[MI], b[2 * NJ]; };
+    unsigned slot_out = lds0;                                              // slot of the K-step to read next
+    auto read_one = [&](Frags& f, int n) {                                 // fragment n of MI + 2 NJ
+        typedef const DP_LDS_AS bf16x8* ptr;
+        if (n < MI) f.a[n] = A_ROW ? *(ptr)(uintptr_t)(slot_out + fa + n * 1024) : tr((slot_out + fc) ^ ((wm * MI + n) << 5));
+        else {
+            const int j = n - MI, t = (j / NJ) * (T / 32) + j % NJ;
+            f.b[j] = B_ROW ? *(ptr)(uintptr_t)(slot_out + STEP / 2 + fb + t * 1024) : tr((slot_out + STEP / 2 + fc) ^ ((wn * NJ + t) << 5));
+        }
+    };
+    auto read_end = [&]() {
+        slot_out += STEP;
+        if (slot_out == lds0 + NB * STEP) slot_out = lds0;
+    };
+
+    f32x4 acc[MI][2 * NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2 * NJ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    // all but the newest `n` loads into LDS and every LDS read of this wave done, in all waves (a wait that the compiler knows, so
+    // that it does not wait again for the fragments)
+#define GS_SYNC(n)                                                                                              \
+    do {                                                                                                        \
+        asm volatile("" ::: "memory");                                                                          \
+        __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | (7 << 4));                                 \
+        __builtin_amdgcn_s_barrier();                                                                           \
+        asm volatile("" ::: "memory");                                                                          \
+    } while (0)
+    // one K-step: in NI groups, a load of the step NB ahead, fragments of the next step, products of this one
+    auto step = [&](const Frags& cur, Frags& next) {
+        stage_begin();
+#pragma unroll
+        for (int g = 0; g < NI; ++g) {
+            stage_one(g);
+#pragma unroll
+            for (int n = g * (MI + 2 * NJ) / NI; n < (g + 1) * (MI + 2 * NJ) / NI; ++n) read_one(next, n);
+#pragma unroll
+            for (int m = g * MI * 2 * NJ / NI; m < (g + 1) * MI * 2 * NJ / NI; ++m)
+                acc[m / (2 * NJ)][m % (2 * NJ)] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cur.b[m % (2 * NJ)], cur.a[m / (2 * NJ)], acc[m / (2 * NJ)][m % (2 * NJ)], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage_end();
+        read_end();
+        GS_SYNC((NB - 2) * NI);
+    };
+    Frags f0, f1;
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {
+        stage_begin();
+#pragma unroll
+        for (int g = 0; g < NI; ++g) stage_one(g);
+        stage_end();
+    }
+    GS_SYNC((NB - 1) * NI);
+#pragma unroll
+    for (int n = 0; n < MI + 2 * NJ; ++n) read_one(f0, n);
+    read_end();
+    GS_SYNC((NB - 2) * NI);
+    int kt = kt0;
+#pragma clang loop unroll(disable)
+    for (; kt + 1 < kt1; kt += 2) {
+        step(f0, f1);
+        step(f1, f0);
+    }
+    if (kt < kt1) step(f0, f1);
+    GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
+#undef GS_SYNC
+
+    // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
+    const int cl = wn * NJ * 16 + (lane >> 4) * 4;
+    const int64_t mrow = i0 + wm * (T / 2) + (lane & 15);
+    if (split) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int64_t m = mrow + i * 16;
+            if (m >= p.I) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = j0 + (MODE == GL_FWD ? 0 : h * (T / 2)) + cl + j * 16, pl = MODE == GL_FWD ? h : plane;
+                    // ldp is a multiple of 4: four columns that start inside a row end inside its padding
+                    if (n < p.J) *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = acc[i][h * NJ + j];
+                }
+        }
+    } else if constexpr (MODE == GL_FWD) {
+        gl_with_act(p.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = j0 + cl + j * 16, cnt = p.J - n;
+                if (cnt <= 0) continue;
+                f32x4 bg, bu;
+                gl_bias<bf16_t>(p, n, cnt, bg, bu);
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int64_t m = mrow + i * 16;
+                    if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[i][j] + bg, acc[i][NJ + j] + bu);
+                }
+            }
+        });
+    } else {
+        bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? plane : 0];
+        const bool whole = gl_whole(out, p.ldo);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int n = j0 + h * (T / 2) + cl + j * 16, cnt = p.J - n;
+                if (cnt <= 0) continue;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int64_t m = mrow + i * 16;
+                    if (m < p.I) gl_put4(out + m * p.ldo + n, acc[i][h * NJ + j], cnt, whole);
+                }
+            }
+    }
+}
+
+template <int MODE>
+__global__ __launch_bounds__(GS_THREADS, 2) void k_gated_ring(GtArgs q) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    gs_product<MODE>(q, blockIdx.x, gridDim.x, smem);
+}
+// both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, [n0, gridDim) the other
+__global__ __launch_bounds__(GS_THREADS, 2) static void k_gated_ring_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
+    if (first == dx_first) gs_product<GL_DX>(dx, at, count, smem);
+    else gs_product<GL_DW>(dw, at, count, smem);
+}
+
+}  // namespace dp

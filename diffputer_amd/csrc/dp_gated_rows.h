@@ -8,7 +8,7 @@
 // CB = 16: 16 gate and 16 up rows, two fragments; CB = 8 (narrow layers, twice the workgroups): 8 gate and 8 up rows in one.
 // x is read by every workgroup, from the L2.
 #pragma once
-#include "dp_gated_tile.h"
+#include "dp_gated_lds.h"
 
 namespace dp {
 

@@ -1,7 +1,7 @@
-// bf16 tile products of the gated projection (dp_gated.h has the three products and their operands): T x T tile of products,
-// 64 deep, T = 256 (8 waves, one workgroup per CU) or 128 (4 waves, two per CU).
+// bf16 products of the gated projection that fill the chip with 256 x 256 tiles (dp_gated.h has the three products and their
+// operands): 64 deep, 8 waves of 128 x 64, one workgroup per CU.
 //
-//   * A K-tile is four half-tiles in LDS, A0 A1 B0 B1 (T / 2 rows of A or of B, 64 deep), two K-tiles deep.  Each half-tile
+//   * A K-tile is four half-tiles in LDS, A0 A1 B0 B1 (128 rows of A or of B, 64 deep), two K-tiles deep.  Each half-tile
 //     is loaded straight into LDS (buffer loads, 16 bytes a lane) 5 to 6 phases before it is read, and the loads stay in
 //     flight across barriers (counted vmcnt).  Rows or k's that do not exist lie behind the buffer's last byte: the range
 //     check returns zeros for them, which is all the masking that ragged sizes need.
@@ -14,8 +14,7 @@
 //     A half-tile is read after the vmcnt of every wave and a barrier; its slot is loaded again at least two phases after
 //     its last read, whose lgkmcnt(0) every wave has passed by then.  K-tiles past the end are "loaded" from an empty
 //     buffer (zeros, no traffic), so that every count holds for any number of K-tiles.
-//   * T = 256: the waves of the lower half run one barrier behind, so that one wave of a SIMD multiplies while its partner
-//     reads LDS.  T = 128: the partner is the CU's other workgroup.
+//   * The waves of the lower half run one barrier behind, so that one wave of a SIMD multiplies while its partner reads LDS.
 //   * Row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7); fragments by
 //     ds_read_b128.  Column layout (a transposed product's operand): LDS holds the k rows as they are in memory, and
 //     ds_read_b64_tr_b16 turns 4 k's x 16 columns into a fragment's k order while reading, 32-byte slot s of k row k at
@@ -23,45 +22,15 @@
 //   * GL_FWD: B0 are the gate's rows and B1 the up's rows for the same columns of h: one lane ends with g and u of the
 //     same elements, and the activation and the product are lane-local.
 #pragma once
-#include "dp_gated.h"
-#include "dp_gemm_bf16.h"
+#include "dp_gated_lds.h"
 
 namespace dp {
 
-typedef __attribute__((ext_vector_type(4))) short bf16x4;
-
-struct GtArgs {
-    GlArgs g;
-    int nti, ntj;              // tiles along I and J
-    int group;                 // tile rows that are walked together (shared B panels stay in the XCD's L2)
-};
-
-template <int T> struct GtShape {
-    static constexpr int THREADS = T == 256 ? 512 : 256;
-    static constexpr int NW = THREADS / 64, WN = T == 256 ? 4 : 2;         // waves; waves along the columns (2 along the rows)
-    static constexpr int HR = T / 2, HB = HR * 128;                        // rows and bytes of a half-tile
-    static constexpr int MI = HR / 32, NJ = HR / WN / 16;                  // 16 x 16 tiles of a wave's quadrant
-    static constexpr int LDS = 8 * HB;
-};
-
-__device__ __forceinline__ unsigned gt_lds(const void* p) { return (unsigned)(size_t)(DP_LDS_AS const char*)p; }   // LDS byte address
-
-#define GT_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
-
-// byte range [p, end) as a buffer; reads behind it return 0
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t gt_buffer(const char* p, const char* end) {
-    const int64_t n = end - p;
-    const int hi = (int)(n >> 32);
-    const unsigned lo = (unsigned)n;
-    const unsigned bytes = hi < 0 ? 0u : hi > 0 || lo > 0x7fffffffu ? 0x7fffffffu : lo;
-    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00027000);
-}
-
-// EL bytes per lane from the buffer's byte `off` on into LDS, lane after lane from `dst` on
-template <int EL> __device__ __forceinline__ void gt_load(__amdgpu_buffer_rsrc_t buf, char* dst, unsigned off) {
-    if constexpr (EL == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 16, (int)off, 0, 0, 0);
-    else __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 4, (int)off, 0, 0, 0);
-}
+constexpr int GT_T = 256, GT_THREADS = 512;
+constexpr int GT_NW = 8, GT_WN = 4;                                        // waves; waves along the columns (2 along the rows)
+constexpr int GT_HR = GT_T / 2, GT_HB = GT_HR * 128;                       // rows and bytes of a half-tile
+constexpr int GT_MI = GT_HR / 32, GT_NJ = GT_HR / GT_WN / 16;              // 16 x 16 tiles of a wave's quadrant
+constexpr int GT_LDS = 8 * GT_HB;
 
 // Fragments of column-laid-out half-tiles: for every 16-column tile and k-step two reads of 4 k's each, in one statement that
 // ends with their wait (KS, HI: byte offsets of the second k-step and of a fragment's second four k's).
@@ -112,42 +81,13 @@ template <int KS, int HI> __device__ __forceinline__ void gt_tr4_2(bf16x4 (&a)[2
                  : "v"(ra[0]), "v"(ra[1]), "v"(ra[2]), "v"(ra[3]), "v"(rb[0]), "v"(rb[1]), "n"(HI), "n"(KS), "n"(KS + HI)
                  : "memory");
 }
-template <int KS, int HI> __device__ __forceinline__ void gt_tr2_2(bf16x4 (&a)[2][2][2], const unsigned (&ra)[2], bf16x4 (&b)[2][2][2], const unsigned (&rb)[2]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %16\n\t" "ds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %4, %17\n\t" "ds_read_b64_tr_b16 %5, %17 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %8, %18\n\t" "ds_read_b64_tr_b16 %9, %18 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %12, %19\n\t" "ds_read_b64_tr_b16 %13, %19 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %2, %16 offset:%21\n\t" "ds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %6, %17 offset:%21\n\t" "ds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %10, %18 offset:%21\n\t" "ds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %14, %19 offset:%21\n\t" "ds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
-                   "=&v"(a[1][1][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[0][1][0]), "=&v"(b[0][1][1]),
-                   "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
-                 : "v"(ra[0]), "v"(ra[1]), "v"(rb[0]), "v"(rb[1]), "n"(HI), "n"(KS), "n"(KS + HI)
-                 : "memory");
-}
 __device__ __forceinline__ bf16x8 gt_join(const bf16x4 (&f)[2]) { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// workgroup -> slice, and tile -> (plane, row, column): groups of q.group tile rows, column by column within a group
-template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int b, int count, int& slice, int& plane, int& ti, int& tj) {
-    const int t = xcd_remap(b, count), tiles = count / q.g.splits, tile = t % tiles;
-    slice = __builtin_amdgcn_readfirstlane(t / tiles);
-    const int per_plane = q.nti * q.ntj;
-    plane = MODE == GL_DW ? q.g.zfirst + __builtin_amdgcn_readfirstlane(tile / per_plane) : 0;
-    const int tp = tile % per_plane, gsz = q.group * q.ntj, grp = tp / gsz, in = tp - grp * gsz;
-    const int rows_here = min(q.group, q.nti - grp * q.group);
-    ti = __builtin_amdgcn_readfirstlane(grp * q.group + in % rows_here);
-    tj = __builtin_amdgcn_readfirstlane(in / rows_here);
-}
-
 // workgroup `b` of the launch's `count` that run this product: its tile and slice, neighbouring tiles on one XCD
-template <int MODE, int T>
+template <int MODE>
 __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, char* smem) {
-    using S = GtShape<T>;
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
-    constexpr int HR = S::HR, HB = S::HB, MI = S::MI, NJ = S::NJ, NW = S::NW, WN = S::WN;
+    constexpr int HR = GT_HR, HB = GT_HB, MI = GT_MI, NJ = GT_NJ, NW = GT_NW, WN = GT_WN;
     constexpr unsigned OUTSIDE = 0x80000000u;                              // an offset behind every buffer
     const GlArgs& p = q.g;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -157,8 +97,8 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     const bool split = p.splits > 1;
     int slice, plane, ti, tj;
     gt_tile<MODE>(q, b, count, slice, plane, ti, tj);
-    const int64_t i0 = (int64_t)ti * T;
-    const int j0 = tj * (MODE == GL_FWD ? HR : T);
+    const int64_t i0 = (int64_t)ti * GT_T;
+    const int j0 = tj * (MODE == GL_FWD ? HR : GT_T);
 
     const int nk = (int)((p.C + 63) >> 6);                                 // K-tiles of a segment
     const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
@@ -167,7 +107,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     //   row layout: piece = 8 rows x 128 B; column layout: piece = 1024 / (2 HR) k rows x 2 HR bytes
     const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
     constexpr int KR = 1024 / (2 * HR), CH = HR / 8;                       // k rows per piece, 16-byte chunks per k row
-    auto g_of = [](int k) { return HR == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; };
+    auto g_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
     unsigned va[2], vb[2];
     const int r8 = lane >> 3, c8 = (lane & 7) ^ r8;                        // row layout: row of the piece, chunk of memory
 #pragma unroll
@@ -246,13 +186,8 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
             if constexpr (A_ROW) {
                 if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
             } else if (ha >= 0) {
-                if constexpr (MI == 4) {
-                    if (hb >= 0) gt_tr4_2<KS, HI>(ta, xa, tb, xb);
-                    else gt_tr4<KS, HI>(ta, xa);
-                } else {
-                    if (hb >= 0) gt_tr2_2<KS, HI>(ta, xa, tb, xb);
-                    else gt_tr2<KS, HI>(ta, xa);
-                }
+                if (hb >= 0) gt_tr4_2<KS, HI>(ta, xa, tb, xb);
+                else gt_tr4<KS, HI>(ta, xa);
             } else if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -287,18 +222,18 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
                 acc[ha][i][hb][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[ks][j], af[ks][i], acc[ha][i][hb][j], 0, 0, 0); \
         __builtin_amdgcn_s_setprio(0);                                                                          \
         __builtin_amdgcn_sched_barrier(0);                                                                      \
-        if (T == 256) __builtin_amdgcn_s_barrier();                                                             \
+        __builtin_amdgcn_s_barrier();                                                             \
     } while (0)
 
     stage(true, kt0, 1); stage(false, kt0, 0); stage(true, kt0, 0); stage(false, kt0, 1);
     stage(true, kt0 + 1, 1); stage(false, kt0 + 1, 0); stage(true, kt0 + 1, 0);
     GT_VMCNT(8);                                                           // B1, A0, B0 of the first K-tile
     __builtin_amdgcn_s_barrier();
-    if (T == 256 && wm == 1) __builtin_amdgcn_s_barrier();                 // the lower half runs one barrier behind
+    if (wm == 1) __builtin_amdgcn_s_barrier();                 // the lower half runs one barrier behind
     read(smem, -1, b1, 1);
     __builtin_amdgcn_s_barrier();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (T == 256) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_barrier();
 #pragma clang loop unroll(disable)
     for (int kt = kt0; kt < kt1; ++kt) {
         const char* const buf = smem + ((kt - kt0) & 1) * 4 * HB;
@@ -318,7 +253,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         GT_VMCNT(8);
         GT_MFMA(1, 0, b0);
     }
-    if (T == 256 && wm == 0) __builtin_amdgcn_s_barrier();                 // as many barriers as the lower half
+    if (wm == 0) __builtin_amdgcn_s_barrier();                 // as many barriers as the lower half
     GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
 #undef GT_MFMA
 
@@ -380,30 +315,17 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     }
 }
 
-template <int MODE, int T>
-__global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile(GtArgs q) {
+template <int MODE>
+__global__ __launch_bounds__(GT_THREADS) void k_gated_tile(GtArgs q) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    gt_product<MODE, T>(q, blockIdx.x, gridDim.x, smem);
+    gt_product<MODE>(q, blockIdx.x, gridDim.x, smem);
 }
 // both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, [n0, gridDim) the other
-template <int T>
-__global__ __launch_bounds__(GtShape<T>::THREADS) void k_gated_tile_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+__global__ __launch_bounds__(GT_THREADS) static void k_gated_tile_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
-    if (first == dx_first) gt_product<GL_DX, T>(dx, at, count, smem);
-    else gt_product<GL_DW, T>(dw, at, count, smem);
-}
-
-// copy of a matrix whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero
-__global__ __launch_bounds__(256) void k_gated_pack(const bf16_t* src, int64_t ld, bf16_t* dst, int64_t ldd, int64_t rows, int64_t C) {
-    const int64_t per = ldd / 8, total = rows * per;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-        const int64_t r = t / per, c = (t - r * per) * 8;
-        bf16x8 v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < C ? (short)src[r * ld + c + e] : (short)0;
-        *(bf16x8*)(dst + r * ldd + c) = v;
-    }
+    if (first == dx_first) gt_product<GL_DX>(dx, at, count, smem);
+    else gt_product<GL_DW>(dw, at, count, smem);
 }
 
 }  // namespace dp
