@@ -48,7 +48,7 @@ SIGNATURES = {
     "dp_masked_errors": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _vp, _vp]),
     "dp_mstep_workspace_bytes": (_sz, [_i, _i, _i64]),
     "dp_mstep_fwd_bwd": (_i, [_i, _i, _i64, _vp, _vp, _vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), _vp, _vp, _vp, _sz, _vp]),
-    "dp_gated_linear_pre_bytes": (_sz, [_i64, _i]),
+    "dp_gated_linear_pre_bytes": (_sz, [_i, _i64, _i]),
     "dp_gated_linear_workspace_bytes": (_sz, [_i, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _i]),
     "dp_gated_linear": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "dp_gated_linear_bwd": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),

@@ -433,7 +433,7 @@ static int gl_zero(void* p, int64_t n, hipStream_t st) {
 }
 
 template <typename T>
-static int gl_backward(int dtype, GlIn& in, const float* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2], int act, void* ws, hipStream_t st) {
+static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2], int act, void* ws, hipStream_t st) {
     const int64_t M = in.M;
     const int N = in.N, K = in.K;
     int rc;
@@ -448,7 +448,7 @@ static int gl_backward(int dtype, GlIn& in, const float* pre, const GlOp& dh, T*
     const GlBwd w = gl_bwd_carve(dtype, in, planes, dx != nullptr, ws);
     T* const dgu = (T*)w.dgu;
     if ((rc = in.pack(planes > 0, dx != nullptr, st))) return rc;
-    const GlDgu e = {pre, dh.p, dgu, w.colpart, {db[0], db[1]}, gl_ldp(N), dh.ld, w.ldg, M, N, act, w.tx, w.rows};
+    const GlDgu e = {pre, dh.p, dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows};
     hipLaunchKernelGGL((k_gated_dgu<T>), dim3((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk), dim3(256), 0, st, e);
     DP_LAUNCH_CHECK("k_gated_dgu");
     if ((db[0] || db[1]) && w.nblk > 1) {
@@ -491,11 +491,11 @@ static int gn_check(const char* who, int n, void* const* g, const int64_t* numel
     return DP_OK;
 }
 
-// next table of at most GN_MAX entries from tensor `i` on (which moves on)
-static bool gn_next(GradTable& t, int& i, int n, void* const* g, const int64_t* numel, const int* dtype) {
+// next table of at most GN_MAX entries from tensor `i` on (which moves on, forwards or backwards)
+static bool gn_next(GradTable& t, int& i, int step, int n, void* const* g, const int64_t* numel, const int* dtype) {
     t.n = 0;
     t.chunks = 0;
-    for (; i < n && t.n < GN_MAX; ++i) {
+    for (; i >= 0 && i < n && t.n < GN_MAX; i += step) {
         if (numel[i] == 0) continue;
         const int64_t es = dtype[i] == DP_DTYPE_BF16 ? 2 : 4;
         const uint64_t p = (uint64_t)g[i], base = p & ~(uint64_t)15;
@@ -519,7 +519,7 @@ static int gn_norm(int n, void* const* g, const int64_t* numel, const int* dtype
     int i = 0;
     *nparts = *launches = 0;
     const int cap = gn_cap(n);
-    while (gn_next(t, i, n, g, numel, dtype)) {
+    while (gn_next(t, i, 1, n, g, numel, dtype)) {
         const int grid = gn_blocks(t.chunks, cap);
         hipLaunchKernelGGL(k_grad_norm, dim3(grid), dim3(GN_THREADS), 0, st, t, part + *nparts, norm_type == DP_NORM_MAX);
         DP_LAUNCH_CHECK("k_grad_norm");
@@ -535,9 +535,10 @@ using namespace dp;
 
 extern "C" {
 
-size_t dp_gated_linear_pre_bytes(int64_t M, int N) {
-    if (M < 0 || M >= GL_MAX_ROWS || N < 1 || N > GL_MAX_DIM) { fail(DP_EINVAL, "dp_gated_linear_pre_bytes: M=%lld N=%d", (long long)M, N); return 0; }
-    return (size_t)std::max<int64_t>(M, 1) * 2 * gl_ldp(N) * 4;
+size_t dp_gated_linear_pre_bytes(int dtype, int64_t M, int N) {
+    if ((dtype != DP_DTYPE_F32 && dtype != DP_DTYPE_BF16) || M < 0 || M >= GL_MAX_ROWS || N < 1 || N > GL_MAX_DIM) { fail(DP_EINVAL, "dp_gated_linear_pre_bytes: dtype=%d M=%lld N=%d", dtype, (long long)M, N); return 0; }
+    M = std::max<int64_t>(M, 1);
+    return (size_t)(dtype == DP_DTYPE_BF16 ? GlPre<bf16_t>::bytes(M, ceil_div(N, 4)) : GlPre<float>::bytes(M, ceil_div(N, 4)));
 }
 
 size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, int64_t M, int N, int K, int grads) {
@@ -565,7 +566,7 @@ int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, c
     GlArgs a;
     memset(&a, 0, sizeof a);
     a.out[0] = h; a.ldo = ldh;
-    a.pre = (float*)pre; a.ldpre = gl_ldp(N);
+    a.pre = pre;
     a.bias[0] = b_gate; a.bias[1] = b_up;
     a.act = act;
     hipStream_t st = (hipStream_t)stream;
@@ -594,10 +595,10 @@ int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gat
     hipStream_t st = (hipStream_t)stream;
     if (dtype == DP_DTYPE_BF16) {
         bf16_t *dw[2] = {(bf16_t*)dw_gate, (bf16_t*)dw_up}, *db[2] = {(bf16_t*)db_gate, (bf16_t*)db_up};
-        return gl_backward<bf16_t>(dtype, in, (const float*)pre, od, (bf16_t*)dx, dw, db, act, workspace, st);
+        return gl_backward<bf16_t>(dtype, in, pre, od, (bf16_t*)dx, dw, db, act, workspace, st);
     }
     float *dw[2] = {(float*)dw_gate, (float*)dw_up}, *db[2] = {(float*)db_gate, (float*)db_up};
-    return gl_backward<float>(dtype, in, (const float*)pre, od, (float*)dx, dw, db, act, workspace, st);
+    return gl_backward<float>(dtype, in, pre, od, (float*)dx, dw, db, act, workspace, st);
 }
 
 size_t dp_grad_workspace_bytes(int n) { return n < 0 ? 0 : (size_t)(gn_cap(n) * gn_launches(n) + 1) * sizeof(double); }
@@ -636,12 +637,12 @@ int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype,
     int nparts, launches;
     if ((rc = gn_norm(n, g, numel, dtype, norm_type, (double*)workspace, &nparts, &launches, st))) return rc;
     GradTable t;
-    int i = 0;
+    int i = n - 1;
     if (launches == 0) {
         hipLaunchKernelGGL(k_grad_total, dim3(1), dim3(GN_THREADS), 0, st, part, 0, inf, norm);
         DP_LAUNCH_CHECK("k_grad_total");
     }
-    for (int k = 0; gn_next(t, i, n, g, numel, dtype); ++k) {
+    for (int k = 0; gn_next(t, i, -1, n, g, numel, dtype); ++k) {
         hipLaunchKernelGGL(k_grad_clip, dim3(gn_blocks(t.chunks, 2048)), dim3(GN_THREADS), 0, st, t, part, nparts, inf, limit, k == 0 ? norm : nullptr);
         DP_LAUNCH_CHECK("k_grad_clip");
     }

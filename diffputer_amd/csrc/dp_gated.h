@@ -96,8 +96,7 @@ struct GlArgs {
     int64_t ldo;
     float* part;               // split launches: partial sums
     int64_t ldp;
-    float* pre;                // GL_FWD, training: g plane, then u plane, [M][ldpre] float32
-    int64_t ldpre;
+    void* pre;                 // GL_FWD, training: g and u for the backward pass (GlPre)
     const void* bias[2];
     int act;
 };
@@ -134,12 +133,61 @@ template <typename T> __device__ __forceinline__ void gl_bias(const GlArgs& p, i
     if (p.bias[0]) bg = gl_get4((const T*)p.bias[0] + n, cnt, gl_whole((const T*)p.bias[0], 0));
     if (p.bias[1]) bu = gl_get4((const T*)p.bias[1] + n, cnt, gl_whole((const T*)p.bias[1], 0));
 }
+// The projections g and u as the forward pass leaves them for the backward pass, by groups of 4 columns (G = N / 4 rounded up):
+//   float32   g[4], u[4]: two planes [M][G] of 16 bytes
+//   bf16      20 bits of each (sign, exponent, 11 bits of the fraction; rounded, half away from zero): a plane [M][G] of 16 bytes with the
+//             upper 16 bits of g[4] and u[4], and a plane [M][G] of 4 bytes with the next 4 bits of each.
+// Half a step of 20 bits is 2^-12: dg = dh u act'(g) is off by a sixteenth of the rounding to bf16 that it gets as an operand
+// anyway, and neither range nor inf and NaN are lost, as they would be in 16 bits of either kind.  Against float32 planes the
+// forward pass writes and the backward pass reads 20 instead of 32 bytes per group.
+template <typename T> struct GlPre;
+template <> struct GlPre<float> {
+    static __host__ __device__ int64_t bytes(int64_t M, int64_t G) { return M * G * 32; }
+    static __device__ __forceinline__ void put(void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4 g, f32x4 u) {
+        f32x4* const p = (f32x4*)pre + m * G + (n >> 2);
+        p[0] = g;
+        p[M * G] = u;
+    }
+    static __device__ __forceinline__ void get(const void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4& g, f32x4& u) {
+        const f32x4* const p = (const f32x4*)pre + m * G + (n >> 2);
+        g = p[0];
+        u = p[M * G];
+    }
+};
+template <> struct GlPre<bf16_t> {
+    static __host__ __device__ int64_t bytes(int64_t M, int64_t G) { return M * G * 20; }
+    static __device__ __forceinline__ void put(void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4 g, f32x4 u) {
+        uint32_t b[8], low = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            b[e] = __builtin_bit_cast(uint32_t, e < 4 ? g[e] : u[e - 4]) + 0x800u;             // carries into the exponent as a rounding does
+            low |= ((b[e] >> 12) & 15u) << (4 * e);
+        }
+        const int64_t at = m * G + (n >> 2);
+        uint4 hi;
+        hi.x = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
+        hi.y = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
+        hi.z = __builtin_amdgcn_perm(b[5], b[4], 0x07060302u);
+        hi.w = __builtin_amdgcn_perm(b[7], b[6], 0x07060302u);
+        ((uint4*)pre)[at] = hi;
+        ((uint32_t*)((char*)pre + M * G * 16))[at] = low;
+    }
+    static __device__ __forceinline__ void get(const void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4& g, f32x4& u) {
+        const int64_t at = m * G + (n >> 2);
+        const uint4 hi = ((const uint4*)pre)[at];
+        const uint32_t low = ((const uint32_t*)((const char*)pre + M * G * 16))[at];
+        const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t b = (e & 1 ? h[e >> 1] & 0xffff0000u : h[e >> 1] << 16) | ((low >> (4 * e)) & 15u) << 12;
+            if (e < 4) g[e] = __builtin_bit_cast(float, b);
+            else u[e - 4] = __builtin_bit_cast(float, b);
+        }
+    }
+};
 // h of row m, columns n .. n + cnt - 1 (n a multiple of 4), from both finished projections
 template <typename T, int ACT> __device__ __forceinline__ void gl_fwd_put(const GlArgs& p, int64_t m, int n, int cnt, f32x4 g, f32x4 u) {
-    if (p.pre) {                                                 // rows of ldpre = N rounded up to 4
-        *(f32x4*)(p.pre + m * p.ldpre + n) = g;
-        *(f32x4*)(p.pre + (p.I + m) * p.ldpre + n) = u;
-    }
+    if (p.pre) GlPre<T>::put(p.pre, p.I, (p.J + 3) >> 2, m, n, g, u);
     f32x4 v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = gl_act<T, ACT>(g[r]) * u[r];
@@ -312,12 +360,12 @@ __global__ __launch_bounds__(256) void k_gated_join_both(GlArgs dx, GlArgs dw, i
 // zero.  db: the column sums of the unrounded values: written here if one block has all rows, else left as partial sums
 // colpart [row block][2][ldg] for k_gated_colsum.
 struct GlDgu {
-    const float* pre;
+    const void* pre;
     const void* dh;
     void* dgu;
     float* colpart;
     void* db[2];
-    int64_t ldpre, lddh, ldg, M;
+    int64_t lddh, ldg, M;
     int N, act, tx, rows;
 };
 template <typename T>
@@ -334,7 +382,8 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
         for (int64_t m = r0 + ry; m < r1; m += ty) {
             f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
             if (cnt > 0) {
-                const f32x4 g = *(const f32x4*)(p.pre + m * p.ldpre + n), u = *(const f32x4*)(p.pre + (p.M + m) * p.ldpre + n);
+                f32x4 g, u;
+                GlPre<T>::get(p.pre, p.M, (p.N + 3) >> 2, m, n, g, u);
                 const f32x4 d = gl_get4((const T*)p.dh + m * p.lddh + n, cnt, whole);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)

@@ -56,11 +56,11 @@ template <bool VEC> struct GrLoad<float, VEC> {
 };
 
 template <typename T, int MT, int CB, bool VEC>
-__global__ __launch_bounds__(GR_WAVES * 64) void k_gated_rows(GlArgs p) {
+__global__ __launch_bounds__(GR_WAVES * 64, MT > 2 ? 2 : 4) void k_gated_rows(GlArgs p) {
     using L = GrLoad<T, VEC>;
     using V = typename L::V;
     constexpr int F = CB / 8;                                    // weight fragments: gate and up, or one with both
-    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = 4;       // elements of a lane's load, of a fragment's; fragments of a round
+    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = MT == 1 ? 4 : 2;       // elements of a lane's load, of a fragment's; fragments of a round
     __shared__ f32x4 red[GR_WAVES][F][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * CB, K = (int)p.C, M = (int)p.I;

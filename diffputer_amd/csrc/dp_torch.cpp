@@ -65,7 +65,7 @@ Tensor forward_of(const Tensor& x, const Tensor& wg, const Tensor& wu, const Ten
     const int64_t M = x.size(0), K = x.size(1), N = wg.size(0);
     const c10::DeviceGuard guard(x.device());
     Tensor h = at::empty({M, N}, x.options().requires_grad(false));
-    if (pre) *pre = bytes_like(x, dp_gated_linear_pre_bytes(M, (int)N));
+    if (pre) *pre = bytes_like(x, dp_gated_linear_pre_bytes(code_of(x), M, (int)N));
     if (M == 0) return h;
     const int dt = code_of(x);
     const size_t need = dp_gated_linear_workspace_bytes(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), M, (int)N, (int)K, 0);

@@ -284,8 +284,8 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  *   x  [M, K]    row stride ldx elements (>= K);  w_gate, w_up [N, K], row stride ldw (>= K);  b_gate, b_up [N] or NULL
  *   h  [M, N]    row stride ldh (>= N)
  *   act          0 = none, 1 = SiLU, 2 = GELU (g Phi(g), not its tanh approximation); a NaN of x or w reaches every element that depends on it
- *   pre          NULL, or dp_gated_linear_pre_bytes(M, N) bytes (16-byte aligned) that receive both projections in float32
- *                for the backward pass; the layout is the library's own
+ *   pre          NULL, or dp_gated_linear_pre_bytes(dtype, M, N) bytes (16-byte aligned) that receive both projections for the
+ *                backward pass (float32; for bf16 20 bits of it each); the layout is the library's own
  * Any strides, element-aligned pointers, 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
  * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
  * (workspace >= dp_gated_linear_workspace_bytes(.., grads) for the same arguments, grads = DP_GATED_FORWARD, or the DP_GATED_D.. that dp_gated_linear_bwd is asked for, 256-byte aligned; calls that may
@@ -301,7 +301,7 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
 #define DP_GATED_DW_GATE 2
 #define DP_GATED_DW_UP   4
 #define DP_GATED_DB      8   /* either bias gradient */
-size_t dp_gated_linear_pre_bytes(int64_t M, int N);
+size_t dp_gated_linear_pre_bytes(int dtype, int64_t M, int N);
 size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw,
                                        int64_t M, int N, int K, int grads);
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,

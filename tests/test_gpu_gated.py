@@ -3,7 +3,7 @@
 Tolerances are componentwise bounds, worked out from the inputs:  a float32 sum of k products is off by at most
 gamma(k) = 2 (k + 4) 2^-24 times the sum of the absolute products (2: the matrix pipes may round inside a step of their
 own), an elementary function or a rounding in float32 by 2^-22 of its value, and a rounding to the tensor's type by
-eps / 2 of it (bf16 2^-8).  |silu'| <= 1.1, |gelu'| <= 1.13, |silu''| <= 0.5, |gelu''| <= 0.8.
+eps / 2 of it (bf16 2^-8); bf16 keeps the projections for the backward pass in 20 bits (2^-12).  |silu'| <= 1.1, |gelu'| <= 1.13, |silu''| <= 0.5, |gelu''| <= 0.8.
 """
 import math
 
@@ -55,6 +55,7 @@ class Ref:
         dt = x.dtype
         u_t = half_step(dt)
         mix = u_t if dt == torch.bfloat16 else 0.0                # dg, du are rounded to bf16 as operands
+        kept = 2.0 ** -12 if dt == torch.bfloat16 else 0.0        # the saved projections
         x, wg, wu, dh = (t.detach().cpu().to(F8) for t in (x, wg, wu, dh))
         N, K = wg.shape
         M = x.shape[0]
@@ -67,6 +68,8 @@ class Ref:
         self.h = a * u
         self.eh = ea * (u.abs() + eu) + a.abs() * eu + (E32 + u_t) * self.h.abs() * 1.01 + TINY
         du, dg = dh * a, dh * u * da
+        eg, eu = eg + kept * (g.abs() + eg), eu + kept * (u.abs() + eu)
+        ea = A1 * eg + E32 * a.abs()
         edu = dh.abs() * ea + E32 * du.abs()
         edg = dh.abs() * (eu * A1 + (u.abs() + eu) * (A2 * eg + 2 * E32 * A1)) + 2 * E32 * dg.abs()
         rdu, rdg = edu + mix * (du.abs() + edu), edg + mix * (dg.abs() + edg)      # as operands of the products

@@ -108,8 +108,9 @@ def test_c_entry_refuses(call):
 
 def test_gated_sizes():
     lib = _lib.load()
-    assert lib.dp_gated_linear_pre_bytes(10, 33) == 10 * 2 * 36 * 4
-    assert lib.dp_gated_linear_pre_bytes(-1, 33) == 0 and lib.dp_gated_linear_pre_bytes(5, 0) == 0
+    assert lib.dp_gated_linear_pre_bytes(0, 10, 33) == 10 * 2 * 36 * 4
+    assert lib.dp_gated_linear_pre_bytes(1, 10, 33) == 10 * 2 * 36 * 5 // 2
+    assert lib.dp_gated_linear_pre_bytes(0, -1, 33) == 0 and lib.dp_gated_linear_pre_bytes(0, 5, 0) == 0 and lib.dp_gated_linear_pre_bytes(2, 5, 5) == 0
 
     def ws(dtype, M, N, K, backward, at=FAKE):
         return lib.dp_gated_linear_workspace_bytes(dtype, at, K, at, at, K, M, N, K, backward)
@@ -127,7 +128,7 @@ def test_gated_sizes():
     assert ws(0, 1 << 20, 4096, 64, 1) >= 2 * (1 << 20) * 4096 * 4
     # rows that are not aligned are copied: x and both weights
     assert ws(1, 4096, 2048, 1024, 0, FAKE + 2) >= (4096 + 2 * 2048) * 1024 * 2 > ws(1, 4096, 2048, 1024, 0)
-    assert lib.dp_gated_linear_pre_bytes(1 << 20, 4096) == 2 * (1 << 20) * 4096 * 4
+    assert lib.dp_gated_linear_pre_bytes(0, 1 << 20, 4096) == 2 * (1 << 20) * 4096 * 4
 
 
 def _table(ptrs, numel, dtypes):
