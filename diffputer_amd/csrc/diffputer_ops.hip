@@ -233,26 +233,24 @@ static GtArgs gl_args(GlArgs a, const GlShape& s, const GlPlan& c) {
 static unsigned gl_join_grid(const GlShape& s) { return (unsigned)std::min<int64_t>(ceil_div<int64_t>(s.I * s.planes * ceil_div<int64_t>(s.J, 4), 256), 4096); }
 
 template <typename T, int MT, int CB>
-static int gr_launch(const GlArgs& a, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div(a.J, CB)), block(GR_WAVES * 64);
-    if (vec) hipLaunchKernelGGL((k_gated_rows<T, MT, CB, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_gated_rows<T, MT, CB, false>), grid, block, 0, st, a);
+static int gr_launch(const GlArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_gated_rows<T, MT, CB>), dim3((unsigned)ceil_div(a.J, CB)), dim3(GR_WAVES * 64), 0, st, a);
     DP_LAUNCH_CHECK("k_gated_rows");
     return DP_OK;
 }
 template <typename T>
-static int gr_rows(const GlArgs& a, bool vec, hipStream_t st) {
+static int gr_rows(const GlArgs& a, hipStream_t st) {
     const bool wide = a.J >= 16 * 256;                            // narrower: 8 columns per workgroup, twice as many workgroups
-    if (a.I <= 16) return wide ? gr_launch<T, 1, 16>(a, vec, st) : gr_launch<T, 1, 8>(a, vec, st);
-    if (a.I <= 32) return wide ? gr_launch<T, 2, 16>(a, vec, st) : gr_launch<T, 2, 8>(a, vec, st);
-    return wide ? gr_launch<T, 4, 16>(a, vec, st) : gr_launch<T, 4, 8>(a, vec, st);
+    if (a.I <= 16) return wide ? gr_launch<T, 1, 16>(a, st) : gr_launch<T, 1, 8>(a, st);
+    if (a.I <= 32) return wide ? gr_launch<T, 2, 16>(a, st) : gr_launch<T, 2, 8>(a, st);
+    return wide ? gr_launch<T, 4, 16>(a, st) : gr_launch<T, 4, 8>(a, st);
 }
 
 template <typename T, int MODE>
 static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, hipStream_t st) {
     const GtArgs q = gl_args(a, s, c);
     int rc;
-    if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(q.g, vec, st) : DP_EINVAL;
+    if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(q.g, st) : DP_EINVAL;
     if (c.T == 0) {
         hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, q.g);
         DP_LAUNCH_CHECK("k_gated_mm");
@@ -511,7 +509,8 @@ static bool gn_next(GradTable& t, int& i, int step, int n, void* const* g, const
 }
 
 static int gn_launches(int n) { return std::max(1, ceil_div(n, GN_MAX)); }
-static int gn_cap(int n) { return std::max(1, GN_MAX_BLOCKS / ceil_div(std::max(n, 1), GN_MAX)); }     // blocks per launch
+// blocks per launch: four per CU, fewer where there are so many launches that their partials would be slow to join
+static int gn_cap(int n) { return std::max(16, std::min(GN_MAX_BLOCKS, 4096 / gn_launches(n))); }
 
 // partials of all tensors; returns how many there are
 static int gn_norm(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, double* part, int* nparts, int* launches, hipStream_t st) {

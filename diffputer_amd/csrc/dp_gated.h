@@ -101,7 +101,7 @@ struct GlArgs {
     int act;
 };
 
-// four columns of one row: whole and aligned, or element by element
+// four columns of one row, at any alignment of their elements (the loads and stores of this chip take it)
 template <typename T> struct GlVec;
 template <> struct GlVec<float> { typedef f32x4 V; static __device__ __forceinline__ V put(f32x4 v) { return v; } static __device__ __forceinline__ f32x4 get(V v) { return v; } };
 template <> struct GlVec<bf16_t> {
@@ -111,16 +111,21 @@ template <> struct GlVec<bf16_t> {
         return (f32x4){__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u), __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u)};
     }
 };
-template <typename T> __device__ __forceinline__ bool gl_whole(const T* base, int64_t ld) { return (ld & 3) == 0 && ((uintptr_t)base & (4 * sizeof(T) - 1)) == 0; }
-template <typename T> __device__ __forceinline__ void gl_put4(T* o, f32x4 v, int cnt, bool whole) {
-    if (whole && cnt >= 4) *(typename GlVec<T>::V*)o = GlVec<T>::put(v);
-    else
+template <typename T> __device__ __forceinline__ void gl_put4(T* o, f32x4 v, int cnt) {
+    if (cnt >= 4) {
+        const typename GlVec<T>::V q = GlVec<T>::put(v);
+        __builtin_memcpy(o, &q, sizeof q);
+    } else
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (r < cnt) o[r] = GlType<T>::put(v[r]);
 }
-template <typename T> __device__ __forceinline__ f32x4 gl_get4(const T* o, int cnt, bool whole) {
-    if (whole && cnt >= 4) return GlVec<T>::get(*(const typename GlVec<T>::V*)o);
+template <typename T> __device__ __forceinline__ f32x4 gl_get4(const T* o, int cnt) {
+    if (cnt >= 4) {
+        typename GlVec<T>::V q;
+        __builtin_memcpy(&q, o, sizeof q);
+        return GlVec<T>::get(q);
+    }
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -130,8 +135,8 @@ template <typename T> __device__ __forceinline__ f32x4 gl_get4(const T* o, int c
 // the biases of columns n .. n + cnt - 1
 template <typename T> __device__ __forceinline__ void gl_bias(const GlArgs& p, int n, int cnt, f32x4& bg, f32x4& bu) {
     bg = bu = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (p.bias[0]) bg = gl_get4((const T*)p.bias[0] + n, cnt, gl_whole((const T*)p.bias[0], 0));
-    if (p.bias[1]) bu = gl_get4((const T*)p.bias[1] + n, cnt, gl_whole((const T*)p.bias[1], 0));
+    if (p.bias[0]) bg = gl_get4((const T*)p.bias[0] + n, cnt);
+    if (p.bias[1]) bu = gl_get4((const T*)p.bias[1] + n, cnt);
 }
 // The projections g and u as the forward pass leaves them for the backward pass, by groups of 4 columns (G = N / 4 rounded up):
 //   float32   g[4], u[4]: two planes [M][G] of 16 bytes
@@ -192,7 +197,7 @@ template <typename T, int ACT> __device__ __forceinline__ void gl_fwd_put(const 
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = gl_act<T, ACT>(g[r]) * u[r];
     T* const h = (T*)p.out[0];
-    gl_put4(h + m * p.ldo + n, v, cnt, gl_whole(h, p.ldo));
+    gl_put4(h + m * p.ldo + n, v, cnt);
 }
 template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs& p, int64_t m, int n, int cnt, f32x4 g, f32x4 u) {
     f32x4 bg, bu;
@@ -222,6 +227,10 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
 
     T ra[8], rb[8];
     auto load8 = [&](T* r, const T* src, int64_t valid) {          // `valid` of the 8 elements exist
+        if (valid >= 8) {
+            __builtin_memcpy(r, src, 8 * sizeof(T));
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] = e < valid ? src[e] : (T)0;
     };
@@ -340,7 +349,7 @@ __device__ __forceinline__ void gl_join(const GlArgs& p, int planes, int64_t fir
             if (MODE == GL_FWD) s1 += *(const f32x4*)(b + s * stride);
         }
         if (MODE == GL_FWD) gl_fwd_store<T>(p, m, n, cnt, s0, s1);
-        else gl_put4((T*)p.out[pl] + m * p.ldo + n, s0, cnt, gl_whole((T*)p.out[pl], p.ldo));
+        else gl_put4((T*)p.out[pl] + m * p.ldo + n, s0, cnt);
     }
 }
 template <typename T, int MODE>
@@ -374,7 +383,6 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
     const int cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
     const int n = (blockIdx.x * p.tx + cx) * 4, cnt = p.N - n;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
-    const bool whole = gl_whole((const T*)p.dh, p.lddh);
     T* const dgu = (T*)p.dgu;
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
     if (n < p.ldg) gl_with_act(p.act, [&](auto act) {
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
             if (cnt > 0) {
                 f32x4 g, u;
                 GlPre<T>::get(p.pre, p.M, (p.N + 3) >> 2, m, n, g, u);
-                const f32x4 d = gl_get4((const T*)p.dh + m * p.lddh + n, cnt, whole);
+                const f32x4 d = gl_get4((const T*)p.dh + m * p.lddh + n, cnt);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (e < cnt) {
@@ -410,8 +418,8 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
             su += red[1][k * p.tx + cx];
         }
         if (gridDim.y == 1) {
-            if (p.db[0] && cnt > 0) gl_put4((T*)p.db[0] + n, sg, cnt, gl_whole((T*)p.db[0], 0));
-            if (p.db[1] && cnt > 0) gl_put4((T*)p.db[1] + n, su, cnt, gl_whole((T*)p.db[1], 0));
+            if (p.db[0] && cnt > 0) gl_put4((T*)p.db[0] + n, sg, cnt);
+            if (p.db[1] && cnt > 0) gl_put4((T*)p.db[1] + n, su, cnt);
         } else {
             float* c = p.colpart + (int64_t)blockIdx.y * 2 * p.ldg + n;
             *(f32x4*)c = sg;
@@ -435,7 +443,7 @@ __global__ __launch_bounds__(256) void k_gated_colsum(const float* colpart, int 
     T* const out = pl ? dbu : dbg;
     if (y == 0 && cnt > 0 && out) {
         for (int k = 1; k < 16; ++k) s += red[k][c];
-        gl_put4(out + n, s, cnt, gl_whole(out, 0));
+        gl_put4(out + n, s, cnt);
     }
 }
 

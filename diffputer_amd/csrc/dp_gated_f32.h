@@ -135,7 +135,6 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
 
     // lane: row r, columns 8 e + 4 grp + 0..3 of each TS x TS tile
     float* const out = (float*)p.out[MODE == GL_DW ? plane : 0];
-    const bool whole = gl_whole(out, p.ldo);
 #pragma unroll
     for (int e = 0; e < TS * TS / 256; ++e) {
         const int cl = wn * TS + 8 * e + 4 * grp;
@@ -158,7 +157,7 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
                 const int n = j0 + (MODE == GL_FWD ? 0 : h * (T / 2)) + cl, pl = MODE == GL_FWD ? h : plane;
                 if (n >= p.J) continue;
                 if (split) *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = v[h];
-                else gl_put4(out + m * p.ldo + n, v[h], p.J - n, whole);
+                else gl_put4(out + m * p.ldo + n, v[h], p.J - n);
             }
         }
     }

@@ -62,8 +62,10 @@ __global__ __launch_bounds__(256) static void k_gated_pack(GlPack p) {
         while (r >= p.m[i].rows) r -= p.m[i++].rows;
         const bf16_t* const src = p.m[i].src + r * p.m[i].ld + c;
         bf16x8 v;
+        if (c + 8 <= p.C) __builtin_memcpy(&v, src, 16);
+        else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < p.C ? (short)src[e] : (short)0;
+            for (int e = 0; e < 8; ++e) v[e] = c + e < p.C ? (short)src[e] : (short)0;
         *(bf16x8*)(p.m[i].dst + r * p.ldd + c) = v;
     }
 }

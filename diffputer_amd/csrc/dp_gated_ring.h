@@ -232,7 +232,6 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         });
     } else {
         bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? plane : 0];
-        const bool whole = gl_whole(out, p.ldo);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -242,7 +241,7 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
                     const int64_t m = mrow + i * 16;
-                    if (m < p.I) gl_put4(out + m * p.ldo + n, acc[i][h * NJ + j], cnt, whole);
+                    if (m < p.I) gl_put4(out + m * p.ldo + n, acc[i][h * NJ + j], cnt);
                 }
             }
     }

@@ -14,53 +14,40 @@ namespace dp {
 
 constexpr int GR_WAVES = 8, GR_MAX_ROWS = 64;
 
-// 16 bytes of row `p` from element k on; elements at `end` and behind are zeros
-template <typename T, bool VEC> struct GrLoad;
-template <bool VEC> struct GrLoad<bf16_t, VEC> {
+// 16 bytes of a row from element k on, at any alignment; with END, elements at `end` and behind are zeros
+template <typename T> struct GrLoad;
+template <> struct GrLoad<bf16_t> {
     typedef bf16x8 V;
-    static __device__ __forceinline__ V get(const bf16_t* p, int k, int end) {
-        if (VEC) {                                               // end % 8 == 0: all or nothing
-            const bool in = k < end;
-            V v = *(const V*)(p + (in ? k : 0));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = in ? v[e] : (short)0;
-            return v;
-        }
-        V v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = k + e < end ? (short)p[k + e] : (short)0;
-        return v;
-    }
     static __device__ __forceinline__ f32x4 mul(V w, V x, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0); }
 };
-template <bool VEC> struct GrLoad<float, VEC> {
+template <> struct GrLoad<float> {
     typedef f32x4 V;
-    static __device__ __forceinline__ V get(const float* p, int k, int end) {
-        if (VEC) {                                               // end % 4 == 0
-            const bool in = k < end;
-            V v = *(const V*)(p + (in ? k : 0));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = in ? v[e] : 0.f;
-            return v;
-        }
-        V v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < end ? p[k + e] : 0.f;
-        return v;
-    }
     static __device__ __forceinline__ f32x4 mul(V w, V x, f32x4 c) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(w[s], x[s], c, 0, 0, 0);
         return c;
     }
 };
+template <typename T, bool END> __device__ __forceinline__ typename GrLoad<T>::V gr_get(const T* p, int k, int end) {
+    constexpr int E = 16 / sizeof(T);
+    typename GrLoad<T>::V v;
+    if (!END || k + E <= end) __builtin_memcpy(&v, p + k, 16);
+    else
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            T t = 0;
+            if (k + e < end) t = p[k + e];
+            v[e] = t;
+        }
+    return v;
+}
 
-template <typename T, int MT, int CB, bool VEC>
+template <typename T, int MT, int CB>
 __global__ __launch_bounds__(GR_WAVES * 64, MT > 2 ? 2 : 4) void k_gated_rows(GlArgs p) {
-    using L = GrLoad<T, VEC>;
+    using L = GrLoad<T>;
     using V = typename L::V;
     constexpr int F = CB / 8;                                    // weight fragments: gate and up, or one with both
-    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = MT == 1 ? 4 : 2;       // elements of a lane's load, of a fragment's; fragments of a round
+    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = MT == 1 && F == 1 ? 4 : 2;       // elements of a lane's load, of a fragment's; fragments of a round
     __shared__ f32x4 red[GR_WAVES][F][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * CB, K = (int)p.C, M = (int)p.I;
@@ -80,23 +67,41 @@ __global__ __launch_bounds__(GR_WAVES * 64, MT > 2 ? 2 : 4) void k_gated_rows(Gl
     for (int f = 0; f < F; ++f)
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[f][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    // a round: U fragments of each row, two and two next to each other
-    for (int k0 = wave * 2 * STEP; k0 < K; k0 += GR_WAVES * U * STEP) {
-        V wf[U][F], xf[U][MT];
+    // a round: U fragments of each row, two and two next to each other; the next round's weights are in flight under this one's products
+    constexpr int ROUND = GR_WAVES * U * STEP;
+    auto k_of = [&](int k0, int s) { return k0 + (s & 1) * STEP + (s >> 1) * (GR_WAVES * 2 * STEP) + q * E; };
+    constexpr int SPAN = (U / 2 - 1) * (GR_WAVES * 2 * STEP) + 2 * STEP;      // a wave's round reads within [k0, k0 + SPAN)
+    V wf[2][U][F], xf[U][MT];
+    auto load = [&](auto end, V (*wd)[F], V (*xd)[MT], int k0) {
 #pragma unroll
         for (int s = 0; s < U; ++s) {
-            const int k = k0 + (s & 1) * STEP + (s >> 1) * (GR_WAVES * 2 * STEP) + q * E;
+            if (wd)
 #pragma unroll
-            for (int f = 0; f < F; ++f) wf[s][f] = L::get(w[f], k, K);
+                for (int f = 0; f < F; ++f) wd[s][f] = gr_get<T, decltype(end)::value>(w[f], k_of(k0, s), K);
+            if (xd)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xf[s][t] = L::get(x[t], k, K);
+                for (int t = 0; t < MT; ++t) xd[s][t] = gr_get<T, decltype(end)::value>(x[t], k_of(k0, s), K);
         }
+    };
+    auto load_at = [&](V (*wd)[F], V (*xd)[MT], int k0) {
+        if (k0 + SPAN <= K) load(std::false_type{}, wd, xd, k0);
+        else load(std::true_type{}, wd, xd, k0);
+    };
+    auto round = [&](const V (&cur)[U][F], V (&next)[U][F], int k0) {
+        load_at(nullptr, xf, k0);
+        if (k0 + ROUND < K) load_at(next, nullptr, k0 + ROUND);
 #pragma unroll
         for (int s = 0; s < U; ++s)
 #pragma unroll
             for (int f = 0; f < F; ++f)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) acc[f][t] = L::mul(wf[s][f], xf[s][t], acc[f][t]);
+                for (int t = 0; t < MT; ++t) acc[f][t] = L::mul(cur[s][f], xf[s][t], acc[f][t]);
+    };
+    int k0 = wave * 2 * STEP;
+    if (k0 < K) load_at(wf[0], nullptr, k0);
+    for (; k0 < K; k0 += 2 * ROUND) {
+        round(wf[0], wf[1], k0);
+        if (k0 + ROUND < K) round(wf[1], wf[0], k0 + ROUND);
     }
 #pragma unroll
     for (int f = 0; f < F; ++f)

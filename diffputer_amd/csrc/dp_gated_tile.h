@@ -297,7 +297,6 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         });
     } else {
         bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? plane : 0];
-        const bool whole = gl_whole(out, p.ldo);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -309,7 +308,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
                     for (int i = 0; i < MI; ++i) {
                         const int64_t m = mrow + a * HR + i * 16;
-                        if (m < p.I) gl_put4(out + m * p.ldo + n, acc[a][i][b][j], cnt, whole);
+                        if (m < p.I) gl_put4(out + m * p.ldo + n, acc[a][i][b][j], cnt);
                     }
             }
     }

@@ -4,9 +4,10 @@
 //   coef = min(1, limit / (norm + 1e-6)),  g <- g coef  (in place; nothing is written when coef is 1)
 //
 // Two passes over memory: k_grad_norm leaves one partial per workgroup, k_grad_clip reduces the partials (each workgroup
-// for itself, in one fixed order: same bits everywhere) and scales.  Squares and sums are held in float64: a square of any
-// float32 is then exact to 53 bits and neither overflows nor vanishes, and the float64 pipes are idle in a kernel that
-// waits for memory.
+// for itself, in one fixed order: same bits everywhere) and scales.  Sums are float64; squares are added up in float32 within pairs
+// (float32) or fours (bf16, whose squares are exact), two roundings at most, and only those go to float64: one conversion per
+// element held the kernel to 1.25 elements per ps, 2.5 TB/s in bf16.  A group outside [2^-96, inf) takes the long way, element
+// by element in float64: no square overflows or vanishes.
 #pragma once
 #include "dp_util.h"
 
@@ -49,6 +50,25 @@ __device__ __forceinline__ void gn_take(int inf, double& a, float v) {
     else a = gn_join(1, a, (double)fabsf(v));
 }
 
+// sum of the squares (or the maximum) of 16 bytes
+__device__ __forceinline__ void gn_take16(int inf, bool bf, double& a, const uint32_t (&w)[4]) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[2 * k] = __builtin_bit_cast(float, bf ? w[k] << 16 : w[k]);
+        x[2 * k + 1] = __builtin_bit_cast(float, w[k] & 0xffff0000u);
+    }
+    const float g0 = bf ? fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]) : fmaf(x[0], x[0], x[2] * x[2]);
+    const float g1 = bf ? fmaf(x[4], x[4], x[5] * x[5]) + fmaf(x[6], x[6], x[7] * x[7]) : fmaf(x[4], x[4], x[6] * x[6]);
+    const float lo = 0x1p-96f, hi = 0x1.fffffep127f;
+    if (!inf && g0 >= lo && g1 >= lo && g0 <= hi && g1 <= hi) {
+        a += (double)g0;
+        a += (double)g1;
+    } else if ((w[0] | w[1] | w[2] | w[3]) & (bf ? 0x7fff7fffu : 0x7fffffffu)) {              // not all zeros
+        for (int k = 0; k < (bf ? 8 : 4); ++k) gn_take(inf, a, bf ? x[k] : x[2 * k]);
+    }
+}
+
 // sum (or maximum) over the workgroup, valid in every thread
 __device__ __forceinline__ double gn_block(int inf, double v, double* red) {
     for (int o = 32; o; o >>= 1) v = gn_join(inf, v, __shfl_xor(v, o));
@@ -74,13 +94,7 @@ __global__ __launch_bounds__(GN_THREADS) void k_grad_norm(GradTable t, double* p
             if (o >= e.head && o + 16 <= e.bytes) {
                 const uint4 q = *(const uint4*)(base + o);
                 const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (e.bf16) {
-                        gn_take(inf, a, __builtin_bit_cast(float, w[k] << 16));
-                        gn_take(inf, a, __builtin_bit_cast(float, w[k] & 0xffff0000u));
-                    } else gn_take(inf, a, __builtin_bit_cast(float, w[k]));
-                }
+                gn_take16(inf, e.bf16, a, w);
             } else {
                 for (uint64_t b = o < e.head ? e.head : o; b < o + 16 && b < e.bytes; b += es)
                     gn_take(inf, a, e.bf16 ? bf2f(*(const bf16_t*)(base + b)) : *(const float*)(base + b));
