@@ -96,18 +96,24 @@ static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
 struct GlRate { int T, depth, per_cu; double one, full, fixed, round; };
 static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.49, 1.49, 10.4, 8.0}, {128, 32, 2, 0.29, 0.62, 6.0, 1.0}};
 static const GlRate GL_RATES_F32[] = {{128, GF_K, 2, 2.10, 3.80, 9.0, 4.0}, {64, GF_K, 4, 0.70, 2.05, 4.0, 1.0}};
+static double gl_step(const GlRate& r, double wgs) {
+    const double slots = 256.0 * r.per_cu;
+    return wgs <= 256 ? r.one : wgs >= slots ? r.full : r.one + (r.full - r.one) * (wgs - 256) / (slots - 256);
+}
 static double gl_cost(const GlRate& r, const GlPlan* pl, const GlShape* s, int n) {
-    double wgs = 0, work = 0, longest = 0, join = 0;
+    double wgs = 0, work = 0, join = 0;
+    int longer = 0;
     for (int i = 0; i < n; ++i) {
         wgs += (double)pl[i].wgs;
         work += (double)pl[i].wgs * pl[i].kt_per;
-        longest = std::max(longest, (double)pl[i].kt_per);
+        if (pl[i].kt_per > pl[longer].kt_per) longer = i;
         if (pl[i].splits > 1) join = std::max(join, 5.0) + (double)s[i].I * s[i].J * (s[i].mode == GL_DX ? 1 : 2) * 4 * 2 * pl[i].splits / 4.5e6;
     }
-    const double slots = 256.0 * r.per_cu;
-    const double step = wgs <= 256 ? r.one : wgs >= slots ? r.full : r.one + (r.full - r.one) * (wgs - 256) / (slots - 256);
-    const double rounds = wgs <= slots ? longest : std::max(work / slots + 0.5 * longest * (fmod(wgs, slots) != 0), longest);
-    return r.fixed + r.round * std::max(0.0, ceil(wgs / slots) - 1.0) + rounds * step + join;
+    const double slots = 256.0 * r.per_cu, most = pl[longer].kt_per, least = n > 1 ? pl[1 - longer].kt_per : most;
+    double t;
+    if (wgs <= slots) t = least * gl_step(r, wgs) + (most - least) * gl_step(r, (double)pl[longer].wgs);     // all at once; the longer ones go on alone
+    else t = std::max((work / slots + 0.5 * least * (fmod(wgs, slots) != 0)) * r.full, most * r.one);
+    return r.fixed + r.round * std::max(0.0, ceil(wgs / slots) - 1.0) + t + join;
 }
 
 // The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass).
@@ -289,31 +295,30 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], boo
     return DP_OK;
 }
 
-// 16-byte loads need rows that start on 16 bytes and end on a whole chunk.  The bf16 tile kernels know no others: such operands
-// are copied to the workspace (rows padded with zeros) where the product is large enough to pay for it, and smaller ones run
-// on the general kernel.  The float32 tile kernel and the kernel for few rows have a form with narrower loads.
+// 16-byte loads into LDS need rows that start on 16 bytes and end on a whole chunk.  Other operands are copied to the workspace
+// (rows padded with zeros) where the product is large enough to pay for it (float32, 4096 x 1025 x 2048 backward: 774 us with
+// 4-byte loads of rows that start anywhere, 540 with copies).  Smaller products run on the general kernel in bf16, and with 4-byte
+// loads in float32.  The kernel for few rows takes rows of any alignment.
 static bool gt_direct(const void* p, int64_t ld, int64_t cols, int chunk) { return aligned(p, 16) && ld % chunk == 0 && cols % chunk == 0; }
 constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
 constexpr int64_t GT_MAX_LD = 1 << 21;                           // 128 rows of float32 stay within 2^30 bytes
-struct GtOperands { bool tile, vec, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
+struct GtOperands { bool tile, vec, short_rows, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
 static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
     GtOperands o;
     const bool bf = dtype == DP_DTYPE_BF16;
     const int chunk = bf ? 8 : 4;
     const bool x_in = gt_direct(x, ldx, K, chunk), w_in = gt_direct(wg, ldw, K, chunk) && gt_direct(wu, ldw, K, chunk);
-    const bool short_rows = ldx <= GT_MAX_LD && ldw <= GT_MAX_LD;
+    const bool short_rows = o.short_rows = ldx <= GT_MAX_LD && ldw <= GT_MAX_LD;
     const int forced = forced_kernel();
     o.vec = x_in && w_in;
     o.pack_x = o.pack_w = false;
-    o.ldk = round_up<int64_t>(K, 8);
-    if (!bf) {
-        o.tile = short_rows && forced != 1;
-        return o;
-    }
-    o.tile = forced != 1 && (forced || (o.vec && short_rows) || M * N * K >= GT_PACK_LEAST);
-    if (o.tile) {
-        o.pack_x = !x_in || ldx > GT_MAX_LD || K % 8;
-        o.pack_w = !w_in || ldw > GT_MAX_LD || K % 8;
+    o.ldk = round_up<int64_t>(K, chunk);
+    const bool large = M * N * K >= GT_PACK_LEAST;
+    o.tile = forced != 1 && (bf ? forced || (o.vec && short_rows) || large : short_rows || large);
+    if (o.tile && (bf || large || !short_rows)) {
+        o.pack_x = !x_in || ldx > GT_MAX_LD || K % chunk;
+        o.pack_w = !w_in || ldw > GT_MAX_LD || K % chunk;
+        o.vec = true;
     }
     return o;
 }
@@ -327,27 +332,30 @@ struct GlIn {
     GlOp x, wg, wu;
     int64_t M;
     int N, K;
+    size_t es;
     GtOperands o;
     char *px, *pw;
     void carve(Carver& c) {
-        px = o.pack_x ? c.take((size_t)M * o.ldk * 2) : nullptr;
-        pw = o.pack_w ? c.take((size_t)2 * N * o.ldk * 2) : nullptr;
+        px = o.pack_x ? c.take((size_t)M * o.ldk * es) : nullptr;
+        pw = o.pack_w ? c.take((size_t)2 * N * o.ldk * es) : nullptr;
     }
     int pack(bool need_x, bool need_w, hipStream_t st) {
         GlPack p = {{}, o.ldk, K, 0};
         int64_t rows = 0;
         auto add = [&](GlOp& op, char* to, int64_t n) {
-            p.m[p.n++] = {(const bf16_t*)op.p, (bf16_t*)to, op.ld, n};
+            p.m[p.n++] = {op.p, to, op.ld, n};
             rows += n;
             op = {to, o.ldk, o.ldk};
         };
         if (o.pack_x && need_x) add(x, px, M);
         if (o.pack_w && need_w) {
             add(wg, pw, N);
-            add(wu, pw + (size_t)N * o.ldk * 2, N);
+            add(wu, pw + (size_t)N * o.ldk * es, N);
         }
         if (p.n == 0) return DP_OK;
-        hipLaunchKernelGGL(k_gated_pack, dim3((unsigned)std::min<int64_t>(ceil_div<int64_t>(rows * (o.ldk / 8), 256), 8192)), dim3(256), 0, st, p);
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div<int64_t>(rows * (o.ldk * (int64_t)es / 16), 256), 8192));
+        if (es == 2) hipLaunchKernelGGL(k_gated_pack<bf16_t>, grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(k_gated_pack<float>, grid, dim3(256), 0, st, p);
         DP_LAUNCH_CHECK("k_gated_pack");
         return DP_OK;
     }
@@ -355,13 +363,15 @@ struct GlIn {
     int64_t fwd_c() const { return o.pack_x && o.pack_w ? o.ldk : K; }
 };
 static GlIn gl_in(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
-    return {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
+    return {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, dtype == DP_DTYPE_BF16 ? (size_t)2 : (size_t)4, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
 }
 
 // forward workspace: copies, partial sums
 struct GlFwd { GlShape s; GlPlan plan; float* part; size_t bytes; };
 static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
     GlFwd w;
+    // the float32 forward product (both operands row laid out) loses 5 to 10 % to 4-byte loads, less than copies take
+    if (dtype == DP_DTYPE_F32 && in.o.short_rows && (in.o.pack_x || in.o.pack_w)) in.o.pack_x = in.o.pack_w = in.o.vec = false;
     w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1};
     w.plan = gl_plan(w.s, dtype, in.o.tile);
     if (w.plan.T == GL_ROWS) {                                    // reads rows of any alignment

@@ -33,6 +33,27 @@ template <int EL> __device__ __forceinline__ void gt_load(__amdgpu_buffer_rsrc_t
     else __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 4, (int)off, 0, 0, 0);
 }
 
+// 16 bytes per lane from byte `off` of [base, base + records) to LDS byte `lds` on; zeros where a lane is outside.  In assembly so
+// that the compiler does not wait for loads in flight before every LDS read (there is no register result: the waits for what
+// arrives in LDS are the counted ones below).
+__device__ __forceinline__ void gl_load_lds(const char* base, unsigned records, unsigned off, unsigned lds) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const uint64_t b = (uint64_t)base;
+    const u32x4 rs = {(unsigned)b, (unsigned)(b >> 32) & 0xffffu, records, 0x00027000u};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rs) : "memory");
+}
+__device__ __forceinline__ unsigned gl_clip(int64_t n) { return n <= 0 ? 0u : n > 0x7fffffff ? 0x7fffffffu : (unsigned)n; }
+
+    // all but the newest `n` loads into LDS and every LDS read of this wave done, in all waves (a wait that the compiler knows, so
+    // that it does not wait again for the fragments)
+#define GL_SYNC(n)                                                                                              \
+    do {                                                                                                        \
+        asm volatile("" ::: "memory");                                                                          \
+        __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | (7 << 4));                                 \
+        __builtin_amdgcn_s_barrier();                                                                           \
+        asm volatile("" ::: "memory");                                                                          \
+    } while (0)
+
 // workgroup -> slice, and tile -> (plane, row, column): groups of q.group tile rows, column by column within a group
 template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int b, int count, int& slice, int& plane, int& ti, int& tj) {
     const int t = xcd_remap(b, count), tiles = count / q.g.splits, tile = t % tiles;
@@ -47,26 +68,28 @@ template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int
 
 // copies of up to three matrices whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero
 struct GlPack {
-    struct { const bf16_t* src; bf16_t* dst; int64_t ld, rows; } m[3];
+    struct { const void* src; void* dst; int64_t ld, rows; } m[3];
     int64_t ldd;
     int C, n;
 };
-__global__ __launch_bounds__(256) static void k_gated_pack(GlPack p) {
-    const int64_t per = p.ldd / 8;
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_pack(GlPack p) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t per = p.ldd / E;
     int64_t total = 0;
     for (int i = 0; i < p.n; ++i) total += p.m[i].rows * per;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
         int64_t r = t / per;
-        const int64_t c = (t - r * per) * 8;
+        const int64_t c = (t - r * per) * E;
         int i = 0;
         while (r >= p.m[i].rows) r -= p.m[i++].rows;
-        const bf16_t* const src = p.m[i].src + r * p.m[i].ld + c;
-        bf16x8 v;
-        if (c + 8 <= p.C) __builtin_memcpy(&v, src, 16);
+        const T* const src = (const T*)p.m[i].src + r * p.m[i].ld + c;
+        T v[E];
+        if (c + E <= p.C) __builtin_memcpy(v, src, 16);
         else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < p.C ? (short)src[e] : (short)0;
-        *(bf16x8*)(p.m[i].dst + r * p.ldd + c) = v;
+            for (int e = 0; e < E; ++e) v[e] = c + e < p.C ? src[e] : (T)0;
+        __builtin_memcpy(__builtin_assume_aligned((T*)p.m[i].dst + r * p.ldd + c, 16), v, 16);
     }
 }
 

@@ -23,17 +23,6 @@ constexpr int GS_T = 128, GS_THREADS = 256;
 constexpr int GS_NB = 5, GS_STEP = GS_T * 128, GS_LDS = GS_NB * GS_STEP;   // ring slots; bytes of a slot (A, then B)
 constexpr int GS_MI = GS_T / 32, GS_NJ = GS_T / 64, GS_NP = GS_T / 64;     // m-tiles; n-tiles of a half; loads of a wave, operand and step
 
-// 16 bytes per lane from byte `off` of [base, base + records) to LDS byte `lds` on; zeros where a lane is outside.  In assembly so
-// that the compiler does not wait for loads in flight before every LDS read (there is no register result: the waits for what
-// arrives in LDS are the counted ones below).
-__device__ __forceinline__ void gs_load(const char* base, unsigned records, unsigned off, unsigned lds) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const uint64_t b = (uint64_t)base;
-    const u32x4 rs = {(unsigned)b, (unsigned)(b >> 32) & 0xffffu, records, 0x00027000u};
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rs) : "memory");
-}
-__device__ __forceinline__ unsigned gs_clip(int64_t n) { return n <= 0 ? 0u : n > 0x7fffffff ? 0x7fffffffu : (unsigned)n; }
-
 template <int MODE>
 __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, char* smem) {
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
@@ -75,8 +64,8 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         const int64_t ld = op.ld * 2;
         Stream st;
         st.at = (const char*)op.p + (row ? first * ld + kk * 64 : kk * 32 * ld + first * 2);
-        st.full = gs_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 31 * ld + (op.cols - first) * 2);
-        st.last = row ? st.full : gs_clip((p.C - 1 - (int64_t)(nk - 1) * 32) * ld + (op.cols - first) * 2);
+        st.full = gl_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 31 * ld + (op.cols - first) * 2);
+        st.last = row ? st.full : gl_clip((p.C - 1 - (int64_t)(nk - 1) * 32) * ld + (op.cols - first) * 2);
         return st;
     };
     auto seg_of = [&](int kt) { return MODE == GL_DX && kt >= nk ? 1 : 0; };
@@ -104,9 +93,9 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         unsigned vo = is_b ? vb[s] : va[s];
         if (B_ROW && s_tail && tail_out) vo = OUTSIDE;
         const unsigned dst = slot_in + (is_b ? STEP / 2 : 0) + (wave + s * 4) * 1024;
-        if (!is_b) gs_load(sa.at, rec_a, vo, dst);
-        else if (MODE == GL_FWD && s >= NP / 2) gs_load(su.at, rec_u, vo, dst);
-        else gs_load(sb.at, rec_b, vo, dst);
+        if (!is_b) gl_load_lds(sa.at, rec_a, vo, dst);
+        else if (MODE == GL_FWD && s >= NP / 2) gl_load_lds(su.at, rec_u, vo, dst);
+        else gl_load_lds(sb.at, rec_b, vo, dst);
     };
     auto stage_end = [&]() {
         ++skt;
@@ -118,24 +107,25 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         if (slot_in == lds0 + NB * STEP) slot_in = lds0;
     };
 
-    // ---- fragment reads: LDS byte addresses; column layout: the tile's number is xor'ed into the slot bits ----
-    const unsigned fa = A_ROW ? wm * MI * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4) : 0;              // row layout: + 1024 per 16 rows
-    const unsigned fb = B_ROW ? wn * NJ * 1024 + (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4) : 0;
+    // ---- fragment reads: an LDS byte address (column layout: the tile's number is xor'ed into the slot bits), and constant offsets ----
+    const unsigned foff = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4);
     const int krow = (lane >> 4) * 8 + ((lane >> 2) & 3);
     const unsigned fc = krow * T * 2 + (g_of(krow) << 5) + (lane & 3) * 8;
-    auto tr = [&](unsigned at) {
-        typedef DP_LDS_AS bf16x4* ptr;
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(at + 4 * T * 2));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    const unsigned fa = A_ROW ? foff + wm * MI * 1024 : fc ^ (wm * MI << 5), fb = B_ROW ? foff + wn * NJ * 1024 : fc ^ (wn * NJ << 5);
+    typedef const DP_LDS_AS char* LdsAt;
+    auto frag = [&](bool row, unsigned at, int off, int t) {
+        if (row) return *(const DP_LDS_AS bf16x8*)((LdsAt)(uintptr_t)at + (off + t * 1024));
+        const LdsAt c = (LdsAt)(uintptr_t)(at ^ (t << 5)) + off;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DP_LDS_AS bf16x4*)c), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DP_LDS_AS bf16x4*)(c + 4 * T * 2));
+        return (bf16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     struct Frags { bf16x8 a[MI], b[2 * NJ]; };
     unsigned slot_out = lds0;                                              // slot of the K-step to read next
     auto read_one = [&](Frags& f, int n) {                                 // fragment n of MI + 2 NJ
-        typedef const DP_LDS_AS bf16x8* ptr;
-        if (n < MI) f.a[n] = A_ROW ? *(ptr)(uintptr_t)(slot_out + fa + n * 1024) : tr((slot_out + fc) ^ ((wm * MI + n) << 5));
+        if (n < MI) f.a[n] = frag(A_ROW, slot_out + fa, 0, n);
         else {
-            const int j = n - MI, t = (j / NJ) * (T / 32) + j % NJ;
-            f.b[j] = B_ROW ? *(ptr)(uintptr_t)(slot_out + STEP / 2 + fb + t * 1024) : tr((slot_out + STEP / 2 + fc) ^ ((wn * NJ + t) << 5));
+            const int j = n - MI;
+            f.b[j] = frag(B_ROW, slot_out + fb, STEP / 2, (j / NJ) * (T / 32) + j % NJ);
         }
     };
     auto read_end = [&]() {
@@ -149,15 +139,6 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
         for (int j = 0; j < 2 * NJ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    // all but the newest `n` loads into LDS and every LDS read of this wave done, in all waves (a wait that the compiler knows, so
-    // that it does not wait again for the fragments)
-#define GS_SYNC(n)                                                                                              \
-    do {                                                                                                        \
-        asm volatile("" ::: "memory");                                                                          \
-        __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | (7 << 4));                                 \
-        __builtin_amdgcn_s_barrier();                                                                           \
-        asm volatile("" ::: "memory");                                                                          \
-    } while (0)
     // one K-step: in NI groups, a load of the step NB ahead, fragments of the next step, products of this one
     auto step = [&](const Frags& cur, Frags& next) {
         stage_begin();
@@ -173,7 +154,7 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         }
         stage_end();
         read_end();
-        GS_SYNC((NB - 2) * NI);
+        GL_SYNC((NB - 2) * NI);
     };
     Frags f0, f1;
 #pragma unroll
@@ -183,11 +164,11 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         for (int g = 0; g < NI; ++g) stage_one(g);
         stage_end();
     }
-    GS_SYNC((NB - 1) * NI);
+    GL_SYNC((NB - 1) * NI);
 #pragma unroll
     for (int n = 0; n < MI + 2 * NJ; ++n) read_one(f0, n);
     read_end();
-    GS_SYNC((NB - 2) * NI);
+    GL_SYNC((NB - 2) * NI);
     int kt = kt0;
 #pragma clang loop unroll(disable)
     for (; kt + 1 < kt1; kt += 2) {
@@ -196,7 +177,6 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
     }
     if (kt < kt1) step(f0, f1);
     GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
-#undef GS_SYNC
 
     // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
     const int cl = wn * NJ * 16 + (lane >> 4) * 4;

@@ -32,57 +32,6 @@ constexpr int GT_HR = GT_T / 2, GT_HB = GT_HR * 128;                       // ro
 constexpr int GT_MI = GT_HR / 32, GT_NJ = GT_HR / GT_WN / 16;              // 16 x 16 tiles of a wave's quadrant
 constexpr int GT_LDS = 8 * GT_HB;
 
-// Fragments of column-laid-out half-tiles: for every 16-column tile and k-step two reads of 4 k's each, in one statement that
-// ends with their wait (KS, HI: byte offsets of the second k-step and of a fragment's second four k's).
-template <int KS, int HI> __device__ __forceinline__ void gt_tr4(bf16x4 (&a)[2][4][2], const unsigned (&ra)[4]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %16\n\t" "ds_read_b64_tr_b16 %1, %16 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %4, %17\n\t" "ds_read_b64_tr_b16 %5, %17 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %8, %18\n\t" "ds_read_b64_tr_b16 %9, %18 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %12, %19\n\t" "ds_read_b64_tr_b16 %13, %19 offset:%20\n\t"
-                 "ds_read_b64_tr_b16 %2, %16 offset:%21\n\t" "ds_read_b64_tr_b16 %3, %16 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %6, %17 offset:%21\n\t" "ds_read_b64_tr_b16 %7, %17 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %10, %18 offset:%21\n\t" "ds_read_b64_tr_b16 %11, %18 offset:%22\n\t"
-                 "ds_read_b64_tr_b16 %14, %19 offset:%21\n\t" "ds_read_b64_tr_b16 %15, %19 offset:%22\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
-                   "=&v"(a[1][1][1]), "=&v"(a[0][2][0]), "=&v"(a[0][2][1]), "=&v"(a[1][2][0]), "=&v"(a[1][2][1]), "=&v"(a[0][3][0]), "=&v"(a[0][3][1]),
-                   "=&v"(a[1][3][0]), "=&v"(a[1][3][1])
-                 : "v"(ra[0]), "v"(ra[1]), "v"(ra[2]), "v"(ra[3]), "n"(HI), "n"(KS), "n"(KS + HI)
-                 : "memory");
-}
-template <int KS, int HI> __device__ __forceinline__ void gt_tr2(bf16x4 (&a)[2][2][2], const unsigned (&ra)[2]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %8\n\t" "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
-                 "ds_read_b64_tr_b16 %4, %9\n\t" "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
-                 "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t" "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
-                 "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t" "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]), "=&v"(a[1][1][1])
-                 : "v"(ra[0]), "v"(ra[1]), "n"(HI), "n"(KS), "n"(KS + HI)
-                 : "memory");
-}
-template <int KS, int HI> __device__ __forceinline__ void gt_tr4_2(bf16x4 (&a)[2][4][2], const unsigned (&ra)[4], bf16x4 (&b)[2][2][2], const unsigned (&rb)[2]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %24\n\t" "ds_read_b64_tr_b16 %1, %24 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %4, %25\n\t" "ds_read_b64_tr_b16 %5, %25 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %8, %26\n\t" "ds_read_b64_tr_b16 %9, %26 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %12, %27\n\t" "ds_read_b64_tr_b16 %13, %27 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %16, %28\n\t" "ds_read_b64_tr_b16 %17, %28 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %20, %29\n\t" "ds_read_b64_tr_b16 %21, %29 offset:%30\n\t"
-                 "ds_read_b64_tr_b16 %2, %24 offset:%31\n\t" "ds_read_b64_tr_b16 %3, %24 offset:%32\n\t"
-                 "ds_read_b64_tr_b16 %6, %25 offset:%31\n\t" "ds_read_b64_tr_b16 %7, %25 offset:%32\n\t"
-                 "ds_read_b64_tr_b16 %10, %26 offset:%31\n\t" "ds_read_b64_tr_b16 %11, %26 offset:%32\n\t"
-                 "ds_read_b64_tr_b16 %14, %27 offset:%31\n\t" "ds_read_b64_tr_b16 %15, %27 offset:%32\n\t"
-                 "ds_read_b64_tr_b16 %18, %28 offset:%31\n\t" "ds_read_b64_tr_b16 %19, %28 offset:%32\n\t"
-                 "ds_read_b64_tr_b16 %22, %29 offset:%31\n\t" "ds_read_b64_tr_b16 %23, %29 offset:%32\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(a[0][0][0]), "=&v"(a[0][0][1]), "=&v"(a[1][0][0]), "=&v"(a[1][0][1]), "=&v"(a[0][1][0]), "=&v"(a[0][1][1]), "=&v"(a[1][1][0]),
-                   "=&v"(a[1][1][1]), "=&v"(a[0][2][0]), "=&v"(a[0][2][1]), "=&v"(a[1][2][0]), "=&v"(a[1][2][1]), "=&v"(a[0][3][0]), "=&v"(a[0][3][1]),
-                   "=&v"(a[1][3][0]), "=&v"(a[1][3][1]), "=&v"(b[0][0][0]), "=&v"(b[0][0][1]), "=&v"(b[1][0][0]), "=&v"(b[1][0][1]), "=&v"(b[0][1][0]),
-                   "=&v"(b[0][1][1]), "=&v"(b[1][1][0]), "=&v"(b[1][1][1])
-                 : "v"(ra[0]), "v"(ra[1]), "v"(ra[2]), "v"(ra[3]), "v"(rb[0]), "v"(rb[1]), "n"(HI), "n"(KS), "n"(KS + HI)
-                 : "memory");
-}
-__device__ __forceinline__ bf16x8 gt_join(const bf16x4 (&f)[2]) { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); }
-
 // workgroup `b` of the launch's `count` that run this product: its tile and slice, neighbouring tiles on one XCD
 template <int MODE>
 __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, char* smem) {
@@ -104,101 +53,81 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
 
     // ---- loads: a wave moves pieces `wave` and `wave + NW` (1 KiB each) of every half-tile ----
-    //   row layout: piece = 8 rows x 128 B; column layout: piece = 1024 / (2 HR) k rows x 2 HR bytes
+    //   row layout: piece = 8 rows x 128 B; column layout: piece = 4 k rows x 256 B
     const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
-    constexpr int KR = 1024 / (2 * HR), CH = HR / 8;                       // k rows per piece, 16-byte chunks per k row
     auto g_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
-    unsigned va[2], vb[2];
     const int r8 = lane >> 3, c8 = (lane & 7) ^ r8;                        // row layout: row of the piece, chunk of memory
+    unsigned va[2], vb[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-        const int piece = wave + s * NW;
-        const int k = piece * KR + lane / CH, c = (lane % CH) ^ (2 * g_of(k));
+        const int piece = wave + s * NW, k = piece * 4 + (lane >> 4), c = (lane & 15) ^ (2 * g_of(k));
         va[s] = A_ROW ? (unsigned)((piece * 8 + r8) * lda + c8 * 16) : (unsigned)(k * lda + c * 16);
         vb[s] = B_ROW ? (unsigned)((piece * 8 + r8) * ldb + c8 * 16) : (unsigned)(k * ldb + c * 16);
     }
-    // row layout, last K-tile of a contraction that is no multiple of 64: chunks past its end
-    const int tail = B_ROW && (p.C & 63) ? nk - 1 : -1;
-    const bool tail_out = c8 * 8 >= (int)(p.C & 63);
+    const bool tail_out = B_ROW && (p.C & 63) && c8 * 8 >= (int)(p.C & 63);                    // chunks past the contraction's end, last K-tile
 
-    auto stage = [&](bool is_b, int kt, int h) {
+    // A half-tile's stream walks its rows or columns K-tile by K-tile.  Row layout: rows that do not exist lie behind `full` bytes whatever
+    // the K-tile.  Column layout: a K-tile has 64 k rows, the segment's last one `last` bytes.
+    struct Stream { const char* at; unsigned full, last; int kt; };
+    auto seg_of = [&](int kt) { return MODE == GL_DX && kt >= nk ? 1 : 0; };
+    auto open = [&](bool is_b, int h, int kt) {
         const bool row = is_b ? B_ROW : A_ROW;
-        const bool live = kt < kt1;
-        const int seg = MODE == GL_DX && kt >= nk ? 1 : 0;
-        const int64_t kk = kt - seg * nk;
+        const int seg = seg_of(kt);
         const GlOp& op = is_b ? p.B[MODE == GL_FWD ? h : seg] : p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
-        const int64_t ld = is_b ? ldb : lda, size = is_b ? p.J : p.I;
-        const int64_t at = (is_b ? j0 : i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);           // first row / column of the half
-        const char* const base = (const char*)op.p;
-        const char* const from = base + (row ? at * ld + kk * 128 : kk * 64 * ld + at * 2);
-        const char* const end = base + (row ? size - 1 : p.C - 1) * ld + op.cols * 2;
-        const auto buf = gt_buffer(from, live ? end : from);
-        char* const dst = smem + (((kt - kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024;
+        const int64_t ld = op.ld * 2, size = is_b ? p.J : p.I, kk = kt - seg * nk;
+        const int64_t first = (is_b ? j0 : i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);        // first row / column of the half
+        Stream st;
+        st.at = (const char*)op.p + (row ? first * ld + kk * 128 : kk * 64 * ld + first * 2);
+        st.full = gl_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 63 * ld + (op.cols - first) * 2);
+        if (first >= (row ? size : op.cols)) st.full = 0;
+        st.last = row || st.full == 0 ? st.full : gl_clip((p.C - 1 - (int64_t)(nk - 1) * 64) * ld + (op.cols - first) * 2);
+        st.kt = kt;
+        return st;
+    };
+    Stream sa[2] = {open(false, 0, kt0), open(false, 1, kt0)}, sb[2] = {open(true, 0, kt0), open(true, 1, kt0)};
+    const int64_t step_a = A_ROW ? 128 : 64 * lda, step_b = B_ROW ? 128 : 64 * ldb;
+    const unsigned lds0 = gt_lds(smem);
+    auto stage = [&](bool is_b, int h) {                                   // the next K-tile of a half; past the last one: no bytes
+        Stream& st = is_b ? sb[h] : sa[h];
+        const bool last = st.kt - seg_of(st.kt) * nk == nk - 1;
+        const unsigned rec = st.kt >= kt1 ? 0u : last ? st.last : st.full;
+        const unsigned dst = lds0 + (unsigned)((((st.kt - kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             unsigned vo = is_b ? vb[s] : va[s];
-            if (row && B_ROW && kt == tail && tail_out) vo = OUTSIDE;
-            gt_load<16>(buf, dst + s * NW * 1024, vo);
+            if (B_ROW && last && tail_out) vo = OUTSIDE;
+            gl_load_lds(st.at, rec, vo, dst + s * NW * 1024);
         }
+        ++st.kt;
+        st.at += is_b ? step_b : step_a;
+        if (MODE == GL_DX && st.kt == nk) st = open(is_b, h, st.kt);
     };
 
-    // ---- fragment reads ----
-    //   row layout: row (lane & 15) of a 16-row tile, chunk ks * 4 + lane / 16, swizzled: an address per k-step
-    //   column layout: lane = (k row (lane >> 2) & 3 of four, 8 bytes lane & 3 of the tile's 32): an address per 16-column tile
-    const int foff = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+    // ---- fragment reads: an LDS byte address per k-step (row layout) or per 16 columns (column layout: the tile's number is xor'ed
+    // into the slot bits), and constant offsets ----
+    const unsigned foff = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
     const int krow = (lane >> 4) * 8 + ((lane >> 2) & 3);
-    unsigned ra[A_ROW ? 2 : MI], rb[B_ROW ? 2 : NJ];
-    if (A_ROW) { ra[0] = wm * (HR / 2) * 128 + foff; ra[1] = ra[0] ^ 64; }
-    else
-#pragma unroll
-        for (int i = 0; i < MI; ++i) ra[i] = krow * HR * 2 + (((wm * MI + i) ^ g_of(krow)) << 5) + (lane & 3) * 8;
-    if (B_ROW) { rb[0] = wn * NJ * 2048 + foff; rb[1] = rb[0] ^ 64; }
-    else
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) rb[j] = krow * HR * 2 + (((wn * NJ + j) ^ g_of(krow)) << 5) + (lane & 3) * 8;
-    constexpr int KS = 32 * HR * 2, HI = 4 * HR * 2;
-    const unsigned lds0 = gt_lds(smem);
+    const unsigned fc = krow * 256 + (g_of(krow) << 5) + (lane & 3) * 8;
+    const unsigned fa = A_ROW ? foff + wm * MI * 2048 : fc ^ (wm * MI << 5), fb = B_ROW ? foff + wn * NJ * 2048 : fc ^ (wn * NJ << 5);
+    typedef const DP_LDS_AS char* LdsAt;
+    auto frag = [&](bool row, unsigned at, int off, int ks, int t) {       // k-step ks, 16-row tile t of the wave's, half-tile at byte `off`
+        if (row) return *(const DP_LDS_AS bf16x8*)((LdsAt)(uintptr_t)(at ^ (ks * 64)) + (off + t * 2048));
+        const LdsAt c = (LdsAt)(uintptr_t)(at ^ (t << 5)) + (off + ks * 8192);
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DP_LDS_AS bf16x4*)c), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((DP_LDS_AS bf16x4*)(c + 1024));
+        return (bf16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
     bf16x8 af[2][MI], b0[2][NJ], b1[2][NJ];
-    // A half `ha` of buffer `buf` into af and / or B half `hb` into d (-1: none); with column-laid-out operands the reads have
-    // landed when this returns, with row-laid-out ones they are in flight
-    auto read = [&](const char* buf, int ha, bf16x8 (*d)[NJ], int hb) {
-        if (A_ROW && ha >= 0)
+    auto read_a = [&](unsigned buf, int h) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int i = 0; i < MI; ++i) af[ks][i] = *(const bf16x8*)(buf + ha * HB + ra[A_ROW ? ks : 0] + i * 2048);
-        if (B_ROW && hb >= 0)
+            for (int i = 0; i < MI; ++i) af[ks][i] = frag(A_ROW, buf + fa, h * HB, ks, i);
+    };
+    auto read_b = [&](bf16x8 (&d)[2][NJ], unsigned buf, int h) {
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) d[ks][j] = *(const bf16x8*)(buf + (2 + hb) * HB + rb[B_ROW ? ks : 0] + j * 2048);
-        if constexpr (!B_ROW) {
-            const unsigned at = lds0 + (unsigned)(buf - smem);
-            bf16x4 ta[2][MI][2], tb[2][NJ][2];
-            unsigned xa[MI], xb[NJ];
-            if constexpr (!A_ROW)
-                if (ha >= 0)
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) xa[i] = at + ha * HB + ra[i];
-            if (hb >= 0)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) xb[j] = at + (2 + hb) * HB + rb[j];
-            if constexpr (A_ROW) {
-                if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
-            } else if (ha >= 0) {
-                if (hb >= 0) gt_tr4_2<KS, HI>(ta, xa, tb, xb);
-                else gt_tr4<KS, HI>(ta, xa);
-            } else if (hb >= 0) gt_tr2<KS, HI>(tb, xb);
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (!A_ROW && ha >= 0)
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) af[ks][i] = gt_join(ta[ks][i]);
-                if (hb >= 0)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) d[ks][j] = gt_join(tb[ks][j]);
-            }
-        }
+            for (int j = 0; j < NJ; ++j) d[ks][j] = frag(B_ROW, buf + fb, (2 + h) * HB, ks, j);
     };
 
     f32x4 acc[2][MI][2][NJ];                                               // [A half][m-tile][B half][n-tile]
@@ -213,8 +142,9 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
 
 #define GT_MFMA(ha, hb, bfr)                                                                                    \
     do {                                                                                                        \
+        asm volatile("" ::: "memory");                                                                          \
         __builtin_amdgcn_s_barrier();                                                                           \
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                      \
+        __builtin_amdgcn_s_waitcnt(0xc07f);      /* lgkmcnt(0) */                                               \
         __builtin_amdgcn_sched_barrier(0);                                                                      \
         __builtin_amdgcn_s_setprio(1);                                                                          \
         _Pragma("unroll") for (int ks = 0; ks < 2; ++ks) _Pragma("unroll") for (int i = 0; i < MI; ++i)         \
@@ -222,34 +152,39 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
                 acc[ha][i][hb][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfr[ks][j], af[ks][i], acc[ha][i][hb][j], 0, 0, 0); \
         __builtin_amdgcn_s_setprio(0);                                                                          \
         __builtin_amdgcn_sched_barrier(0);                                                                      \
-        __builtin_amdgcn_s_barrier();                                                             \
+        __builtin_amdgcn_s_barrier();                                                                           \
+        asm volatile("" ::: "memory");                                                                          \
     } while (0)
 
-    stage(true, kt0, 1); stage(false, kt0, 0); stage(true, kt0, 0); stage(false, kt0, 1);
-    stage(true, kt0 + 1, 1); stage(false, kt0 + 1, 0); stage(true, kt0 + 1, 0);
+    stage(true, 1); stage(false, 0); stage(true, 0); stage(false, 1);
+    stage(true, 1); stage(false, 0); stage(true, 0);
     GT_VMCNT(8);                                                           // B1, A0, B0 of the first K-tile
     __builtin_amdgcn_s_barrier();
-    if (wm == 1) __builtin_amdgcn_s_barrier();                 // the lower half runs one barrier behind
-    read(smem, -1, b1, 1);
+    if (wm == 1) __builtin_amdgcn_s_barrier();                             // the lower half runs one barrier behind
+    asm volatile("" ::: "memory");
+    read_b(b1, lds0, 1);
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    unsigned par = 0;
 #pragma clang loop unroll(disable)
-    for (int kt = kt0; kt < kt1; ++kt) {
-        const char* const buf = smem + ((kt - kt0) & 1) * 4 * HB;
-        const char* const nbuf = smem + ((kt + 1 - kt0) & 1) * 4 * HB;
-        read(buf, 0, b0, 0);                                               // c0
+    for (int kt = kt0; kt < kt1; ++kt, par ^= 4 * HB) {
+        const unsigned buf = lds0 + par, nbuf = lds0 + (par ^ 4 * HB);
+        read_b(b0, buf, 0);                                                // c0
+        read_a(buf, 0);
         GT_MFMA(0, 0, b0);
-        stage(false, kt + 1, 1);                                           // c1
-        stage(true, kt + 2, 1);
+        stage(false, 1);                                                   // c1: A1(t+1), B1(t+2)
+        stage(true, 1);
         GT_VMCNT(10);
         GT_MFMA(0, 1, b1);
-        stage(false, kt + 2, 0);                                           // c2
-        read(buf, 1, nullptr, -1);
+        read_a(buf, 1);                                                    // c2
+        stage(false, 0);
         GT_VMCNT(10);
         GT_MFMA(1, 1, b1);
-        stage(true, kt + 2, 0);                                            // c3
-        read(nbuf, -1, b1, 1);
+        read_b(b1, nbuf, 1);                                               // c3
+        stage(true, 0);
         GT_VMCNT(8);
         GT_MFMA(1, 0, b0);
     }
