@@ -94,7 +94,7 @@ static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
 // them; `fixed` is what a launch takes beyond its K-steps, `round` what every further round of workgroups adds to that.  A split launch
 // pays for its partial sums, written and read at about 4.5 TB/s, and a launch more.
 struct GlRate { int T, depth, per_cu; double one, full, fixed, round; };
-static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.49, 1.49, 10.4, 8.0}, {128, 32, 2, 0.29, 0.62, 6.0, 1.0}};
+static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.36, 1.36, 11.0, 5.0}, {128, 32, 2, 0.28, 0.58, 5.5, 1.0}};
 static const GlRate GL_RATES_F32[] = {{128, GF_K, 2, 2.10, 3.80, 9.0, 4.0}, {64, GF_K, 4, 0.70, 2.05, 4.0, 1.0}};
 static double gl_step(const GlRate& r, double wgs) {
     const double slots = 256.0 * r.per_cu;
@@ -252,13 +252,16 @@ static int gr_rows(const GlArgs& a, hipStream_t st) {
     return wide ? gr_launch<T, 4, 16>(a, st) : gr_launch<T, 4, 8>(a, st);
 }
 
+// type of the general kernel's A: the planes dg, du are float32 there
+template <typename T, int MODE> struct GlPlane { typedef float V; };
+template <typename T> struct GlPlane<T, GL_FWD> { typedef T V; };
 template <typename T, int MODE>
 static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, hipStream_t st) {
     const GtArgs q = gl_args(a, s, c);
     int rc;
     if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(q.g, st) : DP_EINVAL;
     if (c.T == 0) {
-        hipLaunchKernelGGL((k_gated_mm<T, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, q.g);
+        hipLaunchKernelGGL((k_gated_mm<T, typename GlPlane<T, MODE>::V, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, q.g);
         DP_LAUNCH_CHECK("k_gated_mm");
     } else if ((rc = gt_ready()) || (rc = gt_launch<MODE>(q, c, sizeof(T) == 2, vec, st))) return rc;
     if (c.splits > 1) {
@@ -300,6 +303,7 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], boo
 // 4-byte loads of rows that start anywhere, 540 with copies).  Smaller products run on the general kernel in bf16, and with 4-byte
 // loads in float32.  The kernel for few rows takes rows of any alignment.
 static bool gt_direct(const void* p, int64_t ld, int64_t cols, int chunk) { return aligned(p, 16) && ld % chunk == 0 && cols % chunk == 0; }
+constexpr int64_t GL_EXACT_BELOW = 8192;                         // M N
 constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
 constexpr int64_t GT_MAX_LD = 1 << 21;                           // 128 rows of float32 stay within 2^30 bytes
 struct GtOperands { bool tile, vec, short_rows, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
@@ -392,6 +396,7 @@ struct GlBwd {
     GlShape s[2];              // dx, dW
     GlPlan plan[2];
     bool both;                 // in one launch
+    int plane;                 // type of the planes
     int64_t ldg;
     int tx, rows, nblk;
     size_t bytes;
@@ -400,6 +405,9 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     const int64_t M = in.M;
     const int N = in.N, K = in.K;
     GlBwd w;
+    // small layers take the general kernel, whose dg and du are not rounded: with few of them their roundings do not average out
+    if (dtype == DP_DTYPE_BF16 && M * N < GL_EXACT_BELOW && forced_kernel() == 0) in.o.tile = in.o.pack_x = in.o.pack_w = false;
+    w.plane = in.o.tile ? dtype : DP_DTYPE_F32;
     Carver c = {(char*)base};
     in.carve(c);
     w.ldg = round_up<int64_t>(N, 64);
@@ -410,7 +418,7 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     // about 1024 workgroups, at least 4 rows per row lane
     w.rows = (int)std::max<int64_t>(4 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 1024 / cols)));
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
-    w.dgu = c.take((size_t)2 * M * w.ldg * (dtype == DP_DTYPE_BF16 ? 2 : 4));
+    w.dgu = c.take((size_t)2 * M * w.ldg * (w.plane == DP_DTYPE_BF16 ? 2 : 4));
     w.colpart = (float*)c.take(w.nblk > 1 ? (size_t)w.nblk * 2 * w.ldg * 4 : 0);
     w.s[0] = {GL_DX, M, K, N, 1};
     w.s[1] = {GL_DW, N, K, M, planes ? planes : 2};
@@ -454,10 +462,11 @@ static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* 
     }
     const int planes = (dw[0] != nullptr) + (dw[1] != nullptr);
     const GlBwd w = gl_bwd_carve(dtype, in, planes, dx != nullptr, ws);
-    T* const dgu = (T*)w.dgu;
     if ((rc = in.pack(planes > 0, dx != nullptr, st))) return rc;
-    const GlDgu e = {pre, dh.p, dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows};
-    hipLaunchKernelGGL((k_gated_dgu<T>), dim3((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk), dim3(256), 0, st, e);
+    const GlDgu e = {pre, dh.p, w.dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows};
+    const dim3 grid((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk);
+    if (w.plane == dtype) hipLaunchKernelGGL((k_gated_dgu<T, T>), grid, dim3(256), 0, st, e);
+    else hipLaunchKernelGGL((k_gated_dgu<T, float>), grid, dim3(256), 0, st, e);
     DP_LAUNCH_CHECK("k_gated_dgu");
     if ((db[0] || db[1]) && w.nblk > 1) {
         hipLaunchKernelGGL((k_gated_colsum<T>), dim3((unsigned)ceil_div(N, 64), 2), dim3(256), 0, st, w.colpart, w.nblk, w.ldg, db[0], db[1], N);
@@ -467,8 +476,8 @@ static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* 
     memset(a, 0, sizeof a);
     for (int i = 0; i < 2; ++i) {
         a[i].part = w.part[i];
-        a[i].A[0] = {dgu, w.ldg, w.ldg};
-        a[i].A[1] = {dgu + (size_t)M * w.ldg, w.ldg, w.ldg};
+        a[i].A[0] = {w.dgu, w.ldg, w.ldg};
+        a[i].A[1] = {w.dgu + (size_t)M * w.ldg * (w.plane == DP_DTYPE_BF16 ? 2 : 4), w.ldg, w.ldg};
         a[i].ldo = K;
     }
     a[0].B[0] = in.wg; a[0].B[1] = in.wu;

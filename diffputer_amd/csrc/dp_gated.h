@@ -209,14 +209,17 @@ template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs&
 // 64 x 64 x 32 tile, 4 waves of 32 x 32, operands through registers into LDS as [row][k] (element loads with bounds checks).
 // GL_FWD: columns 0..31 of the tile are 32 gate columns, 32..63 the up columns of the same places, so that one lane ends
 // with g and u of the same elements.
+// TA: type of A.  bf16 layers' dg and du are float32 here and multiplied as bf16 hi + lo, two products: small layers, where
+// one product or two is the same time, then have no rounding between the gradient of h and the sums.
 constexpr int GG_T = 64, GG_K = 32;
-template <typename T, int MODE>
+template <typename T, typename TA, int MODE>
 __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
-    constexpr bool BF = sizeof(T) == 2;
+    constexpr bool BF = sizeof(T) == 2, HILO = BF && sizeof(TA) == 4;
     constexpr int LD = BF ? GG_K + 8 : GG_K + 1;
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
     __shared__ __attribute__((aligned(16))) T sa[GG_T * LD];
     __shared__ __attribute__((aligned(16))) T sb[GG_T * LD];
+    __shared__ __attribute__((aligned(16))) T slo[HILO ? GG_T * LD : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
     const int64_t i0 = (int64_t)blockIdx.x * GG_T;
     const int j0 = blockIdx.y * (MODE == GL_FWD ? GG_T / 2 : GG_T);
@@ -225,14 +228,18 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
     const int64_t nk = ceil_div<int64_t>(p.C, GG_K);
     const int64_t kt0 = (int64_t)slice * p.kt_per, kt1 = kt0 + p.kt_per < nk * segs ? kt0 + p.kt_per : nk * segs;
 
-    T ra[8], rb[8];
-    auto load8 = [&](T* r, const T* src, int64_t valid) {          // `valid` of the 8 elements exist
+    TA ra[8];
+    T rb[8];
+    auto load8 = [&](auto* r, const auto* src, int64_t valid) {    // `valid` of the 8 elements exist
         if (valid >= 8) {
-            __builtin_memcpy(r, src, 8 * sizeof(T));
+            __builtin_memcpy(r, src, 8 * sizeof *r);
             return;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = e < valid ? src[e] : (T)0;
+        for (int e = 0; e < 8; ++e) {
+            r[e] = 0;
+            if (e < valid) r[e] = src[e];
+        }
     };
     // row layout: thread = (row tid / 4, 8 k's from (tid % 4) * 8); column layout: thread = (k tid / 8, 8 rows from (tid % 8) * 8)
     auto fetch = [&](int64_t kt) {
@@ -241,10 +248,10 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
         const GlOp A = p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
         if (A_ROW) {
             const int64_t i = i0 + (tid >> 2), k = k0 + (tid & 3) * 8;
-            load8(ra, (const T*)A.p + i * A.ld + k, i < p.I ? p.C - k : 0);
+            load8(ra, (const TA*)A.p + i * A.ld + k, i < p.I ? p.C - k : 0);
         } else {
             const int64_t k = k0 + (tid >> 3), i = i0 + (tid & 7) * 8;
-            load8(ra, (const T*)A.p + k * A.ld + i, k < p.C ? p.I - i : 0);
+            load8(ra, (const TA*)A.p + k * A.ld + i, k < p.C ? p.I - i : 0);
         }
         if (B_ROW) {
             const int row = tid >> 2, half = row >> 5;
@@ -273,7 +280,17 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
     if (kt0 < kt1) fetch(kt0);
     for (int64_t kt = kt0; kt < kt1; ++kt) {
         __syncthreads();
-        put8(sa, ra, A_ROW);
+        if constexpr (HILO) {
+            T hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                hi[e] = f2bf(ra[e]);
+                const float left = ra[e] - bf2f(hi[e]);
+                lo[e] = __builtin_isfinite(left) ? f2bf(left) : (T)0;          // inf and NaN are in hi
+            }
+            put8(sa, hi, A_ROW);
+            put8(slo, lo, A_ROW);
+        } else put8(sa, ra, A_ROW);
         put8(sb, rb, B_ROW);
         __syncthreads();
         if (kt + 1 < kt1) fetch(kt + 1);
@@ -289,6 +306,14 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+            if constexpr (HILO) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8 l = *(const bf16x8*)&slo[(wm * 32 + i * 16 + r) * LD + q * 8];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], l, acc[i][j], 0, 0, 0);
+                }
+            }
         } else {
 #pragma unroll
             for (int kk = 0; kk < GG_K / 4; ++kk) {
@@ -344,6 +369,7 @@ __device__ __forceinline__ void gl_join(const GlArgs& p, int planes, int64_t fir
         f32x4 s0 = *(const f32x4*)a, s1 = (f32x4){0.f, 0.f, 0.f, 0.f};
         const float* b = a + p.I * p.ldp;                          // GL_FWD: the up plane
         if (MODE == GL_FWD) s1 = *(const f32x4*)b;
+#pragma unroll 8
         for (int s = 1; s < p.splits; ++s) {
             s0 += *(const f32x4*)(a + s * stride);
             if (MODE == GL_FWD) s1 += *(const f32x4*)(b + s * stride);
@@ -365,7 +391,7 @@ __global__ __launch_bounds__(256) void k_gated_join_both(GlArgs dx, GlArgs dw, i
 }
 
 // ---- backward, elementwise: du = dh act(g), dg = dh u act'(g), and their column sums ------------------------------------
-// Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows.  dgu: two planes [M][ldg] of T, columns N..ldg - 1
+// Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows.  dgu: two planes [M][ldg] of TD, columns N..ldg - 1
 // zero.  db: the column sums of the unrounded values: written here if one block has all rows, else left as partial sums
 // colpart [row block][2][ldg] for k_gated_colsum.
 struct GlDgu {
@@ -377,13 +403,13 @@ struct GlDgu {
     int64_t lddh, ldg, M;
     int N, act, tx, rows;
 };
-template <typename T>
+template <typename T, typename TD>
 __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
     __shared__ f32x4 red[2][256];
     const int cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
     const int n = (blockIdx.x * p.tx + cx) * 4, cnt = p.N - n;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
-    T* const dgu = (T*)p.dgu;
+    TD* const dgu = (TD*)p.dgu;
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
     if (n < p.ldg) gl_with_act(p.act, [&](auto act) {
 #pragma unroll 4
@@ -402,8 +428,8 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
                         dg[e] = d[e] * u[e] * da;
                     }
             }
-            *(typename GlVec<T>::V*)(dgu + m * p.ldg + n) = GlVec<T>::put(dg);
-            *(typename GlVec<T>::V*)(dgu + (p.M + m) * p.ldg + n) = GlVec<T>::put(du);
+            *(typename GlVec<TD>::V*)(dgu + m * p.ldg + n) = GlVec<TD>::put(dg);
+            *(typename GlVec<TD>::V*)(dgu + (p.M + m) * p.ldg + n) = GlVec<TD>::put(du);
             sg += dg;
             su += du;
         }

@@ -33,13 +33,18 @@ template <int EL> __device__ __forceinline__ void gt_load(__amdgpu_buffer_rsrc_t
     else __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (DP_LDS_AS void*)dst, 4, (int)off, 0, 0, 0);
 }
 
-// 16 bytes per lane from byte `off` of [base, base + records) to LDS byte `lds` on; zeros where a lane is outside.  In assembly so
-// that the compiler does not wait for loads in flight before every LDS read (there is no register result: the waits for what
-// arrives in LDS are the counted ones below).
-__device__ __forceinline__ void gl_load_lds(const char* base, unsigned records, unsigned off, unsigned lds) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const uint64_t b = (uint64_t)base;
-    const u32x4 rs = {(unsigned)b, (unsigned)(b >> 32) & 0xffffu, records, 0x00027000u};
+// A buffer's descriptor in four scalar registers: base, bytes, type.  Kept whole so that walking on is an addition in place.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4 gl_buffer(const char* base) { return (u32x4){(unsigned)(uint64_t)base, (unsigned)((uint64_t)base >> 32) & 0xffffu, 0u, 0x00027000u}; }
+__device__ __forceinline__ void gl_advance(u32x4& rs, int64_t bytes) {     // addresses have 48 bits: nothing carries into the upper half of the second word
+    const uint64_t b = ((uint64_t)rs[1] << 32 | rs[0]) + (uint64_t)bytes;
+    rs[0] = (unsigned)b;
+    rs[1] = (unsigned)(b >> 32);
+}
+// 16 bytes per lane from byte `off` of the buffer to LDS byte `lds` on; zeros where a lane is outside.  In assembly so that the
+// compiler does not wait for loads in flight before every LDS read (there is no register result: the waits for what arrives in
+// LDS are the counted ones below).
+__device__ __forceinline__ void gl_load_lds(u32x4 rs, unsigned off, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rs) : "memory");
 }
 __device__ __forceinline__ unsigned gl_clip(int64_t n) { return n <= 0 ? 0u : n > 0x7fffffff ? 0x7fffffffu : (unsigned)n; }

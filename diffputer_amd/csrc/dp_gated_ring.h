@@ -59,11 +59,11 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
 
     // A stream walks an operand K-step by K-step.  Row layout: rows that do not exist lie behind `full` bytes whatever the step.
     // Column layout: a step has 32 k rows, the segment's last one `last` bytes.
-    struct Stream { const char* at; unsigned full, last; };
+    struct Stream { u32x4 at; unsigned full, last; };
     auto open = [&](const GlOp& op, bool row, int64_t first, int64_t size, int64_t kk) {
         const int64_t ld = op.ld * 2;
         Stream st;
-        st.at = (const char*)op.p + (row ? first * ld + kk * 64 : kk * 32 * ld + first * 2);
+        st.at = gl_buffer((const char*)op.p + (row ? first * ld + kk * 64 : kk * 32 * ld + first * 2));
         st.full = gl_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 31 * ld + (op.cols - first) * 2);
         st.last = row ? st.full : gl_clip((p.C - 1 - (int64_t)(nk - 1) * 32) * ld + (op.cols - first) * 2);
         return st;
@@ -77,14 +77,13 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
     int skt = kt0;                                                         // next K-step to load
     unsigned slot_in = gt_lds(smem);                                       // its slot
     const unsigned lds0 = slot_in;
-    unsigned rec_a, rec_b, rec_u;
     bool s_tail;
     auto stage_begin = [&]() {
         const int kk = skt - seg_of(skt) * nk;
         const bool live = skt < kt1, last = kk == nk - 1;
-        rec_a = !live ? 0u : last ? sa.last : sa.full;
-        rec_b = !live ? 0u : last ? sb.last : sb.full;
-        rec_u = !live ? 0u : su.full;
+        sa.at[2] = !live ? 0u : last ? sa.last : sa.full;
+        sb.at[2] = !live ? 0u : last ? sb.last : sb.full;
+        if (MODE == GL_FWD) su.at[2] = !live ? 0u : su.full;
         s_tail = last;
     };
     auto stage_one = [&](int i) {                                          // load i of NI
@@ -93,16 +92,20 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
         unsigned vo = is_b ? vb[s] : va[s];
         if (B_ROW && s_tail && tail_out) vo = OUTSIDE;
         const unsigned dst = slot_in + (is_b ? STEP / 2 : 0) + (wave + s * 4) * 1024;
-        if (!is_b) gl_load_lds(sa.at, rec_a, vo, dst);
-        else if (MODE == GL_FWD && s >= NP / 2) gl_load_lds(su.at, rec_u, vo, dst);
-        else gl_load_lds(sb.at, rec_b, vo, dst);
+        if (!is_b) gl_load_lds(sa.at, vo, dst);
+        else if (MODE == GL_FWD && s >= NP / 2) gl_load_lds(su.at, vo, dst);
+        else gl_load_lds(sb.at, vo, dst);
     };
     auto stage_end = [&]() {
         ++skt;
-        sa.at += step_a;
-        sb.at += step_b;
-        if (MODE == GL_FWD) su.at += step_b;
-        if (MODE == GL_DX && skt == nk) { sa = open_a(skt); sb = open_b(skt, 0); }
+        gl_advance(sa.at, step_a);
+        gl_advance(sb.at, step_b);
+        if (MODE == GL_FWD) gl_advance(su.at, step_b);
+        if (MODE == GL_DX && __builtin_expect(skt == nk, 0)) {
+            asm volatile("");                                              // a branch, not a selection computed every time
+            sa = open_a(skt);
+            sb = open_b(skt, 0);
+        }
         slot_in += STEP;
         if (slot_in == lds0 + NB * STEP) slot_in = lds0;
     };

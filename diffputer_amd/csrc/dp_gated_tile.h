@@ -68,7 +68,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
 
     // A half-tile's stream walks its rows or columns K-tile by K-tile.  Row layout: rows that do not exist lie behind `full` bytes whatever
     // the K-tile.  Column layout: a K-tile has 64 k rows, the segment's last one `last` bytes.
-    struct Stream { const char* at; unsigned full, last; int kt; };
+    struct Stream { u32x4 at; unsigned full, last; int kt; };
     auto seg_of = [&](int kt) { return MODE == GL_DX && kt >= nk ? 1 : 0; };
     auto open = [&](bool is_b, int h, int kt) {
         const bool row = is_b ? B_ROW : A_ROW;
@@ -77,7 +77,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         const int64_t ld = op.ld * 2, size = is_b ? p.J : p.I, kk = kt - seg * nk;
         const int64_t first = (is_b ? j0 : i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);        // first row / column of the half
         Stream st;
-        st.at = (const char*)op.p + (row ? first * ld + kk * 128 : kk * 64 * ld + first * 2);
+        st.at = gl_buffer((const char*)op.p + (row ? first * ld + kk * 128 : kk * 64 * ld + first * 2));
         st.full = gl_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 63 * ld + (op.cols - first) * 2);
         if (first >= (row ? size : op.cols)) st.full = 0;
         st.last = row || st.full == 0 ? st.full : gl_clip((p.C - 1 - (int64_t)(nk - 1) * 64) * ld + (op.cols - first) * 2);
@@ -90,17 +90,20 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     auto stage = [&](bool is_b, int h) {                                   // the next K-tile of a half; past the last one: no bytes
         Stream& st = is_b ? sb[h] : sa[h];
         const bool last = st.kt - seg_of(st.kt) * nk == nk - 1;
-        const unsigned rec = st.kt >= kt1 ? 0u : last ? st.last : st.full;
+        st.at[2] = st.kt >= kt1 ? 0u : last ? st.last : st.full;
         const unsigned dst = lds0 + (unsigned)((((st.kt - kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             unsigned vo = is_b ? vb[s] : va[s];
             if (B_ROW && last && tail_out) vo = OUTSIDE;
-            gl_load_lds(st.at, rec, vo, dst + s * NW * 1024);
+            gl_load_lds(st.at, vo, dst + s * NW * 1024);
         }
         ++st.kt;
-        st.at += is_b ? step_b : step_a;
-        if (MODE == GL_DX && st.kt == nk) st = open(is_b, h, st.kt);
+        gl_advance(st.at, is_b ? step_b : step_a);
+        if (MODE == GL_DX && __builtin_expect(st.kt == nk, 0)) {
+            asm volatile("");                                              // a branch, not a selection computed every time
+            st = open(is_b, h, st.kt);
+        }
     };
 
     // ---- fragment reads: an LDS byte address per k-step (row layout) or per 16 columns (column layout: the tile's number is xor'ed

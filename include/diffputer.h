@@ -294,7 +294,8 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  *
  * dp_gated_linear_bwd: gradients for a given dh [M, N] (row stride lddh).  dx [M, K], dw_gate, dw_up [N, K], db_gate,
  * db_up [N]: contiguous, overwritten, each may be NULL (not wanted).  M = 0 writes zeros to the weights' gradients.
- * bf16: dg and du are rounded to bf16 once, as the operands of the three products; bias gradients sum them unrounded.
+ * bf16: dg and du are rounded to bf16 once, as the operands of the three products (not in small layers, M N < 8192); bias
+ * gradients sum them unrounded.
  */
 #define DP_GATED_FORWARD 0
 #define DP_GATED_DX      1

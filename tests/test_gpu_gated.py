@@ -384,6 +384,62 @@ def test_nothing_beside_the_output_is_written(M, N, dtype):
     assert bool((buf == 7.0).all())
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements of h: the last rows against the formula, and weight gradients that only they contribute to."""
+    from diffputer_amd.gated import gated_linear
+    M, K, N, tail = 270_000, 64, 8192, 70
+    x, wg, wu, bg, bu, dh = make(tail, K, N, "bf16", seed=23)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    big = torch.full((M, K), 0.5, dtype=torch.bfloat16, device=DEV)
+    big[-tail:] = x.to(DEV)
+    leaves = [big.requires_grad_(), *[t.to(DEV).requires_grad_() for t in (wg, wu, bg, bu)]]
+    h = gated_linear(*leaves)
+    close(h[-tail:], ref.h, ref.eh, "h")
+    d = torch.zeros((M, N), dtype=torch.bfloat16, device=DEV)
+    d[-tail:] = dh.to(DEV)
+    grads = torch.autograd.grad(h, leaves, d)
+    close(grads[0][-tail:], ref.dx, ref.edx, "dx")
+    assert not grads[0][:-tail].any()
+    for name, g in zip(("wg", "wu", "bg", "bu"), grads[1:]):
+        # sums of M terms, all but `tail` of them zero: the bound counts additions, of zeros too
+        more = gamma(M) / gamma(tail)
+        close(g, getattr(ref, "d" + name), more * getattr(ref, "ed" + name), "d" + name)
+    del h, d, grads, big, leaves
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_threads(dtype):
+    """Two threads, each with a stream of its own, at the same time."""
+    import threading
+
+    from diffputer_amd.gated import gated_linear
+    sets = [[t.to(DEV) for t in make(200 + 100 * i, 136, 96, dtype, seed=40 + i)] for i in range(2)]
+    want = [gated_linear(*s[:5]) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    leaves = [t.detach().requires_grad_() for t in sets[i][:5]]
+                    h = gated_linear(*leaves)
+                    torch.autograd.grad(h, leaves, sets[i][5])
+                got[i] = h.detach()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_same_bits_twice(dtype):
     from diffputer_amd.gated import gated_linear

@@ -139,6 +139,21 @@ def test_shared_memory_is_refused():
     assert abs(float(grad_norm([g, g])) - norm_of([g, g])) <= 1e-5 * norm_of([g, g])       # reading it twice is fine
 
 
+def test_more_than_32_bits_of_bytes():
+    """A tensor of 4.8 GB (and odd ones beside it): every element once, none twice."""
+    from diffputer_amd.grads import clip_grads
+    n = 1_200_000_007
+    g = [torch.full((n,), 2.0, device=DEV), torch.full((5,), 2.0, device=DEV), torch.full((3_000_001,), 2.0, dtype=BF, device=DEV)]
+    count = sum(t.numel() for t in g)
+    norm = float(clip_grads(g, math.sqrt(count)))                    # to a half, but for the 1e-6 and two roundings
+    assert abs(norm - 2 * math.sqrt(count)) <= 2.0 ** -23 * norm
+    for t in g:
+        assert float(t.amin()) == float(t.amax())
+        assert abs(float(t[-1]) - 1.0) <= torch.finfo(t.dtype).eps / 2 + 2.0 ** -21
+    del g
+    torch.cuda.empty_cache()
+
+
 def test_same_bits_twice_and_within_the_limit():
     from diffputer_amd.grads import clip_grads
     one, two = tensors([999_999, 12345], [F32, BF], seed=6), tensors([999_999, 12345], [F32, BF], seed=6)
