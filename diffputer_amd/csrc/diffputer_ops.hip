@@ -528,7 +528,7 @@ static bool gn_next(GradTable& t, int& i, int step, int n, void* const* g, const
 }
 
 static int gn_launches(int n) { return std::max(1, ceil_div(n, GN_MAX)); }
-// blocks per launch: four per CU, fewer where there are so many launches that their partials would be slow to join
+// blocks per launch: eight per CU, fewer where there are so many launches that their partials would be slow to join
 static int gn_cap(int n) { return std::max(16, std::min(GN_MAX_BLOCKS, 4096 / gn_launches(n))); }
 
 // partials of all tensors; returns how many there are
@@ -661,7 +661,7 @@ int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype,
         DP_LAUNCH_CHECK("k_grad_total");
     }
     for (int k = 0; gn_next(t, i, -1, n, g, numel, dtype); ++k) {
-        hipLaunchKernelGGL(k_grad_clip, dim3(gn_blocks(t.chunks, 2048)), dim3(GN_THREADS), 0, st, t, part, nparts, inf, limit, k == 0 ? norm : nullptr);
+        hipLaunchKernelGGL(k_grad_clip, dim3(gn_blocks(t.chunks, GN_MAX_BLOCKS)), dim3(GN_THREADS), 0, st, t, part, nparts, inf, limit, k == 0 ? norm : nullptr);
         DP_LAUNCH_CHECK("k_grad_clip");
     }
     return DP_OK;
