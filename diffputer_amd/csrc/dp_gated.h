@@ -33,9 +33,10 @@ template <> struct GlType<bf16_t> {
 // silu(g) = g s(g), s = 1 / (1 + e^-g): e^-g overflows to inf below -88, where s is 0 and the product the right -0;
 // gelu(g) = g Phi(g), Phi = erfc(-g / sqrt 2) / 2 (erfc keeps the relative accuracy of the left tail that 1 + erf loses).
 // At g = -inf both products are 0 * inf = NaN; plain torch expressions give the same.
-// float32 results take expf and a division; for bf16 results the hardware's 2^x and reciprocal do (|g| 2^-24 + 2^-22 of s: at
+// float32 results take erfcf, expf and a division; for bf16 results the hardware's 2^x and reciprocal do (|g| 2^-24 + 2^-22 of s: at
 // most 2^-17 where s is not 0, against half a step of 2^-9): what a 256-tile launch takes beyond its K-tiles fell from 18.9 to
-// 11.4 us with them.
+// 11.4 us with them.  Phi is e^(-g^2 / 2) t P(t) there, t = 1 / (1 + 0.3076 |g|), for g < 0 (1 - that for g > 0), P fitted to
+// the function's tail e^(x^2) erfc(x) by least relative maximum: 2^-18 of it, 2^-16.7 of Phi with the exponential, down to -13.4.
 template <typename T> __device__ __forceinline__ float gl_sigmoid(float g) {
     if (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f));
@@ -43,10 +44,22 @@ template <typename T> __device__ __forceinline__ float gl_sigmoid(float g) {
 template <typename T> __device__ __forceinline__ float gl_exp(float x) {
     return sizeof(T) == 4 ? expf(x) : __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
 }
-__device__ __forceinline__ float gl_phi(float g) { return 0.5f * erfcf(-0.70710678118654752f * g); }
+// Phi(g), with e = e^(-g^2 / 2)
+template <typename T> __device__ __forceinline__ float gl_phi(float g, float e) {
+    if (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678118654752f * g);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.30759145f, fabsf(g), 1.0f));
+    float q = -0.075778842f;
+    q = fmaf(q, t, 0.19164754f);
+    q = fmaf(q, t, 0.0053418200f);
+    q = fmaf(q, t, 0.13728017f);
+    q = fmaf(q, t, 0.11853294f);
+    q = fmaf(q, t, 0.12297484f);
+    q *= e * t;
+    return g < 0.0f ? q : 1.0f - q;
+}
 template <typename T, int ACT> __device__ __forceinline__ float gl_act(float g) {
     if (ACT == GL_ACT_SILU) return g * gl_sigmoid<T>(g);
-    if (ACT == GL_ACT_GELU) return g * gl_phi(g);
+    if (ACT == GL_ACT_GELU) return g * gl_phi<T>(g, gl_exp<T>(-0.5f * g * g));
     return g;
 }
 template <typename T, int ACT> __device__ __forceinline__ void gl_act_grad(float g, float& a, float& da) {
@@ -55,9 +68,9 @@ template <typename T, int ACT> __device__ __forceinline__ void gl_act_grad(float
         a = g * s;
         da = s * (1.0f + g * (1.0f - s));
     } else if (ACT == GL_ACT_GELU) {
-        const float p = gl_phi(g);
+        const float e = gl_exp<T>(-0.5f * g * g), p = gl_phi<T>(g, e);
         a = g * p;
-        da = p + g * (0.39894228040143268f * gl_exp<T>(-0.5f * g * g));
+        da = p + g * (0.39894228040143268f * e);
     } else {
         a = g;
         da = 1.0f;
@@ -412,26 +425,38 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
     TD* const dgu = (TD*)p.dgu;
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
     if (n < p.ldg) gl_with_act(p.act, [&](auto act) {
-#pragma unroll 4
-        for (int64_t m = r0 + ry; m < r1; m += ty) {
-            f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
-            if (cnt > 0) {
-                f32x4 g, u;
-                GlPre<T>::get(p.pre, p.M, (p.N + 3) >> 2, m, n, g, u);
-                const f32x4 d = gl_get4((const T*)p.dh + m * p.lddh + n, cnt);
+        // R rows at a time, all their loads before the first store (which could hit what is loaded, as far as the compiler knows)
+        constexpr int R = 4;
+        for (int64_t m0 = r0 + ry; m0 < r1; m0 += R * ty) {
+            f32x4 g[R], u[R], d[R];
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const int64_t m = m0 + k * ty;
+                g[k] = u[k] = d[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                if (m < r1 && cnt > 0) {
+                    GlPre<T>::get(p.pre, p.M, (p.N + 3) >> 2, m, n, g[k], u[k]);
+                    d[k] = gl_get4((const T*)p.dh + m * p.lddh + n, cnt);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const int64_t m = m0 + k * ty;
+                f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (e < cnt) {
                         float a, da;
-                        gl_act_grad<T, decltype(act)::value>(g[e], a, da);
-                        du[e] = d[e] * a;
-                        dg[e] = d[e] * u[e] * da;
+                        gl_act_grad<T, decltype(act)::value>(g[k][e], a, da);
+                        du[e] = d[k][e] * a;
+                        dg[e] = d[k][e] * u[k][e] * da;
                     }
+                if (m < r1) {
+                    *(typename GlVec<TD>::V*)(dgu + m * p.ldg + n) = GlVec<TD>::put(dg);
+                    *(typename GlVec<TD>::V*)(dgu + (p.M + m) * p.ldg + n) = GlVec<TD>::put(du);
+                    sg += dg;
+                    su += du;
+                }
             }
-            *(typename GlVec<TD>::V*)(dgu + m * p.ldg + n) = GlVec<TD>::put(dg);
-            *(typename GlVec<TD>::V*)(dgu + (p.M + m) * p.ldg + n) = GlVec<TD>::put(du);
-            sg += dg;
-            su += du;
         }
     });
     if (!p.db[0] && !p.db[1]) return;

@@ -33,11 +33,24 @@ constexpr int GN_THREADS = 256;
 // change nothing there and lose 1 to 2 us at 0.3 MB and 42 MB.
 constexpr int GN_MAX_BLOCKS = 2048;
 
-// the entry that holds chunk c, from entry `at` on: a workgroup's chunks come in ascending order, and so do the entries' first chunks
-__device__ __forceinline__ int gn_find(const GradTable& t, int at, uint32_t c) {
-    while (at + 1 < t.n && t.e[at + 1].chunk0 <= c) ++at;
-    return at;
-}
+// The entry that holds a chunk: lane l keeps the first chunks of entries l, l + 64 and l + 128 and the wave counts those that are not
+// behind it.
+struct GnFirst {
+    uint32_t c[(GN_MAX + 63) / 64];
+    __device__ __forceinline__ explicit GnFirst(const GradTable& t) {
+#pragma unroll
+        for (int k = 0; k < (GN_MAX + 63) / 64; ++k) {
+            const int i = k * 64 + (threadIdx.x & 63);
+            c[k] = i < t.n ? t.e[i].chunk0 : ~0u;
+        }
+    }
+    __device__ __forceinline__ int find(uint32_t chunk) const {
+        int n = -1;
+#pragma unroll
+        for (int k = 0; k < (GN_MAX + 63) / 64; ++k) n += __popcll(__ballot(c[k] <= chunk));
+        return n;
+    }
+};
 
 __device__ __forceinline__ double gn_join(int inf, double a, double b) {
     if (!inf) return a + b;
@@ -81,10 +94,9 @@ __device__ __forceinline__ double gn_block(int inf, double v, double* red) {
 __global__ __launch_bounds__(GN_THREADS) void k_grad_norm(GradTable t, double* part, int inf) {
     __shared__ double red[GN_THREADS / 64];
     double a = 0.0;
-    int at = 0;
+    const GnFirst first(t);
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        at = gn_find(t, at, c);
-        const GradEntry e = t.e[at];
+        const GradEntry e = t.e[first.find(c)];
         const uint64_t off0 = (uint64_t)(c - e.chunk0) * GN_CHUNK;
         const char* const base = (const char*)e.base;
         const int es = e.bf16 ? 2 : 4;
@@ -122,16 +134,15 @@ __global__ __launch_bounds__(GN_THREADS) void k_grad_total(const double* part, i
 // k_grad_norm read is what the caches still hold.
 __global__ __launch_bounds__(GN_THREADS) void k_grad_clip(GradTable t, const double* part, int nparts, int inf, float limit, float* norm) {
     __shared__ double red[GN_THREADS / 64];
+    const GnFirst first(t);
     const double total = gn_total(part, nparts, inf, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
     const double cd = (double)limit / (total + 1e-6);
     if (cd >= 1.0) return;                                       // within the limit (a NaN coefficient goes on, and marks every element)
     const float coef = (float)cd;
     if (coef == 1.0f) return;
-    int at = 0;
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        at = gn_find(t, at, c);
-        const GradEntry e = t.e[at];
+        const GradEntry e = t.e[first.find(c)];
         const uint64_t off0 = (uint64_t)((uint32_t)((e.bytes - 1) / GN_CHUNK) - (c - e.chunk0)) * GN_CHUNK;
         char* const base = (char*)e.base;
         const int es = e.bf16 ? 2 : 4;

@@ -567,3 +567,28 @@ def test_module_and_denoiser_training_step():
     assert abs(got[2] - ref[2]) <= 1e-4 * ref[2]
     total = math.sqrt(sum(float(g.double().square().sum()) for g in got[3]))
     assert abs(total - 0.25) <= 1e-5
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("kernel", [0, 128, 256])
+def test_every_bf16_gate(kernel, act, tune):
+    """act and act' at every finite bf16 number of at most 100: x = g, Wg = 1, u = bu = 1, dh = 1, so that h = act(g),
+    dbu's terms are act(g) and dx = act'(g).
+
+    Beside the bounds above: the hardware's 2^x and reciprocal (2^-17 of sigmoid), Phi's fit and exponential (2^-16 of it); gates are
+    kept in 20 bits exactly.  dx is rounded twice, as the product's operand and as the output.  Behind |g| = 13 gelu's left tail is below 1e-37, and
+    results below float32's smallest normal number, 1.2e-38, may be 0."""
+    from diffputer_amd.gated import gated_linear
+    tune(kernel, 0)
+    g = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    g = g[g.abs() <= 100].reshape(-1, 1)
+    one, zero = torch.ones(1, 1, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.bfloat16)
+    leaves = [t.to(DEV).requires_grad_() for t in (g, one, zero, zero[0], one[0])]
+    h = gated_linear(*leaves, act=act)
+    dx = torch.autograd.grad(h, leaves, torch.ones_like(h))[0]
+    a, da = act_of(g.to(F8), act)
+    e, tail = 2.0 ** -16, 2e-37 * (1 + g.to(F8).abs())
+    step = half_step(torch.bfloat16)
+    close(h, a, (e + step) * 1.01 * a.abs() + tail, "h")
+    eda = e * (1 + g.to(F8).abs() * (1 - torch.sigmoid(g.to(F8)).clamp(max=1))) * torch.sigmoid(g.to(F8)) if act == "silu" else e * (0.5 * torch.erfc(-g.to(F8) / math.sqrt(2)) + g.to(F8).abs() * torch.exp(-g.to(F8) ** 2 / 2))
+    close(dx, da, (eda + 2 * step * da.abs()) * 1.02 + tail, "dx")
