@@ -272,23 +272,23 @@ static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, h
     return DP_OK;
 }
 
-// both backward products in one launch: the longer contraction's workgroups start first
+// both backward products and the column sums in one launch: the longer contraction's workgroups start first
 template <typename T>
-static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], bool vec, hipStream_t st) {
+static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], const GlColsum& cs, bool vec, hipStream_t st) {
     int rc;
     if ((rc = gt_ready())) return rc;
     const GtArgs dx = gl_args(a[0], s[0], c[0]), dw = gl_args(a[1], s[1], c[1]);
     const int dx_first = c[0].kt_per >= c[1].kt_per, n0 = (int)c[dx_first ? 0 : 1].wgs;
-    const dim3 grid((unsigned)(c[0].wgs + c[1].wgs));
+    const dim3 grid((unsigned)(c[0].wgs + c[1].wgs + cs.n));
     if (sizeof(T) == 2) {
-        if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, grid, dim3(GT_THREADS), GT_LDS, st, dx, dw, n0, dx_first);
-        else hipLaunchKernelGGL(k_gated_ring_both, grid, dim3(GS_THREADS), GS_LDS, st, dx, dw, n0, dx_first);
+        if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, grid, dim3(GT_THREADS), GT_LDS, st, dx, dw, n0, dx_first, cs);
+        else hipLaunchKernelGGL(k_gated_ring_both, grid, dim3(GS_THREADS), GS_LDS, st, dx, dw, n0, dx_first, cs);
     } else if (c[0].T == 128) {
-        if (vec) hipLaunchKernelGGL((k_gated_f32_both<128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
-        else hipLaunchKernelGGL((k_gated_f32_both<128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first);
+        if (vec) hipLaunchKernelGGL((k_gated_f32_both<128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first, cs);
+        else hipLaunchKernelGGL((k_gated_f32_both<128, false>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first, cs);
     } else {
-        if (vec) hipLaunchKernelGGL((k_gated_f32_both<64, true>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first);
-        else hipLaunchKernelGGL((k_gated_f32_both<64, false>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first);
+        if (vec) hipLaunchKernelGGL((k_gated_f32_both<64, true>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first, cs);
+        else hipLaunchKernelGGL((k_gated_f32_both<64, false>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first, cs);
     }
     DP_LAUNCH_CHECK("gated tile kernel");
     const unsigned jx = c[0].splits > 1 ? gl_join_grid(s[0]) : 0, jw = c[1].splits > 1 ? gl_join_grid(s[1]) : 0;
@@ -344,7 +344,8 @@ struct GlIn {
         px = o.pack_x ? c.take((size_t)M * o.ldk * es) : nullptr;
         pw = o.pack_w ? c.take((size_t)2 * N * o.ldk * es) : nullptr;
     }
-    int pack(bool need_x, bool need_w, hipStream_t st) {
+    // the copies to make, and how many workgroups make them
+    GlPack copies(bool need_x, bool need_w, int* blocks) {
         GlPack p = {{}, o.ldk, K, 0};
         int64_t rows = 0;
         auto add = [&](GlOp& op, char* to, int64_t n) {
@@ -357,12 +358,8 @@ struct GlIn {
             add(wg, pw, N);
             add(wu, pw + (size_t)N * o.ldk * es, N);
         }
-        if (p.n == 0) return DP_OK;
-        const dim3 grid((unsigned)std::min<int64_t>(ceil_div<int64_t>(rows * (o.ldk * (int64_t)es / 16), 256), 8192));
-        if (es == 2) hipLaunchKernelGGL(k_gated_pack<bf16_t>, grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL(k_gated_pack<float>, grid, dim3(256), 0, st, p);
-        DP_LAUNCH_CHECK("k_gated_pack");
-        return DP_OK;
+        *blocks = (int)std::min<int64_t>(ceil_div<int64_t>(rows * (o.ldk * (int64_t)es / 16), 256), 8192);
+        return p;
     }
     // contraction length of the forward product: the copies' padding belongs to it (zeros on both sides)
     int64_t fwd_c() const { return o.pack_x && o.pack_w ? o.ldk : K; }
@@ -434,8 +431,12 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
 template <typename T>
 static int gl_forward(GlArgs a, GlIn& in, void* ws, hipStream_t st) {
     const GlFwd w = gl_fwd_carve(sizeof(T) == 2 ? DP_DTYPE_BF16 : DP_DTYPE_F32, in, ws);
-    int rc;
-    if ((rc = in.pack(true, true, st))) return rc;
+    int blocks;
+    const GlPack copies = in.copies(true, true, &blocks);
+    if (blocks) {
+        hipLaunchKernelGGL((k_gated_pack<T>), dim3((unsigned)blocks), dim3(256), 0, st, copies);
+        DP_LAUNCH_CHECK("k_gated_pack");
+    }
     a.A[0] = in.x;
     a.B[0] = in.wg; a.B[1] = in.wu;
     a.part = w.part;
@@ -463,14 +464,17 @@ static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* 
     }
     const int planes = (dw[0] != nullptr) + (dw[1] != nullptr);
     const GlBwd w = gl_bwd_carve(dtype, in, planes, dx != nullptr, ws);
-    if ((rc = in.pack(planes > 0, dx != nullptr, st))) return rc;
-    const GlDgu e = {pre, dh.p, w.dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows};
-    const dim3 grid((unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4), (unsigned)w.nblk);
-    if (w.plane == dtype) hipLaunchKernelGGL((k_gated_dgu<T, T>), grid, dim3(256), 0, st, e);
-    else hipLaunchKernelGGL((k_gated_dgu<T, float>), grid, dim3(256), 0, st, e);
+    int blocks;
+    const GlPack copies = in.copies(planes > 0, dx != nullptr, &blocks);
+    const GlDgu e = {pre, dh.p, w.dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows, w.nblk};
+    const unsigned across = (unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4);
+    const dim3 grid(across, (unsigned)(w.nblk + ceil_div<int64_t>(blocks, across)));
+    if (w.plane == dtype) hipLaunchKernelGGL((k_gated_dgu<T, T>), grid, dim3(256), 0, st, e, copies);
+    else hipLaunchKernelGGL((k_gated_dgu<T, float>), grid, dim3(256), 0, st, e, copies);
     DP_LAUNCH_CHECK("k_gated_dgu");
-    if ((db[0] || db[1]) && w.nblk > 1) {
-        hipLaunchKernelGGL((k_gated_colsum<T>), dim3((unsigned)ceil_div(N, 64), 2), dim3(256), 0, st, w.colpart, w.nblk, w.ldg, db[0], db[1], N);
+    GlColsum cs = {w.colpart, {db[0], db[1]}, w.ldg, w.nblk, N, (db[0] || db[1]) && w.nblk > 1 ? 2 * ceil_div(N, 64) : 0};
+    if (cs.n && !w.both) {
+        hipLaunchKernelGGL((k_gated_colsum<T>), dim3((unsigned)cs.n), dim3(256), 0, st, cs);
         DP_LAUNCH_CHECK("k_gated_colsum");
     }
     GlArgs a[2];
@@ -486,7 +490,7 @@ static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* 
     a[1].B[0] = in.x;
     a[1].out[0] = dw[0]; a[1].out[1] = dw[1];
     a[1].zfirst = dw[0] ? 0 : 1;
-    if (w.both) return gl_both<T>(a, w.s, w.plan, in.o.vec, st);
+    if (w.both) return gl_both<T>(a, w.s, w.plan, cs, in.o.vec, st);
     if (dx && (rc = gl_mm<T, GL_DX>(a[0], w.s[0], w.plan[0], in.o.vec, st))) return rc;
     if (planes && (rc = gl_mm<T, GL_DW>(a[1], w.s[1], w.plan[1], in.o.vec, st))) return rc;
     return DP_OK;

@@ -403,10 +403,41 @@ __global__ __launch_bounds__(256) void k_gated_join_both(GlArgs dx, GlArgs dw, i
     else gl_join<T, GL_DW>(dw, 2, (int64_t)(b - n_dx) * 256 + threadIdx.x, (int64_t)(gridDim.x - n_dx) * 256);
 }
 
+// copies of up to three matrices whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero
+struct GlPack {
+    struct { const void* src; void* dst; int64_t ld, rows; } m[3];
+    int64_t ldd;
+    int C, n;
+};
+template <typename T> __device__ __forceinline__ void gl_pack(const GlPack& p, int64_t b, int64_t blocks) {
+    constexpr int E = 16 / sizeof(T);
+    const int64_t per = p.ldd / E;
+    const int64_t n0 = p.m[0].rows, n1 = n0 + p.m[1].rows, total = (n1 + p.m[2].rows) * per;
+    for (int64_t t = b * 256 + threadIdx.x; t < total; t += blocks * 256) {
+        int64_t r = t / per;
+        const int64_t c = (t - r * per) * E;
+        // (selections: a table that is indexed at run time would be copied to private memory first)
+        const T* src = (const T*)(r < n0 ? p.m[0].src : r < n1 ? p.m[1].src : p.m[2].src);
+        T* const dst = (T*)(r < n0 ? p.m[0].dst : r < n1 ? p.m[1].dst : p.m[2].dst);
+        const int64_t ld = r < n0 ? p.m[0].ld : r < n1 ? p.m[1].ld : p.m[2].ld;
+        r -= r < n0 ? 0 : r < n1 ? n0 : n1;
+        src += r * ld + c;
+        T v[E];
+        if (c + E <= p.C) __builtin_memcpy(v, src, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = c + e < p.C ? src[e] : (T)0;
+        __builtin_memcpy(__builtin_assume_aligned(dst + r * p.ldd + c, 16), v, 16);
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_pack(GlPack p) { gl_pack<T>(p, blockIdx.x, gridDim.x); }
+
 // ---- backward, elementwise: du = dh act(g), dg = dh u act'(g), and their column sums ------------------------------------
-// Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows.  dgu: two planes [M][ldg] of TD, columns N..ldg - 1
+// Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows; blocks behind the last row block make the copies that the
+// products read (one launch for both: 1537 x 777 x 1203 in bf16, copies in a launch of their own, 5.8 us).  dgu: two planes [M][ldg] of TD, columns N..ldg - 1
 // zero.  db: the column sums of the unrounded values: written here if one block has all rows, else left as partial sums
-// colpart [row block][2][ldg] for k_gated_colsum.
+// colpart [row block][2][ldg] (gl_colsum).
 struct GlDgu {
     const void* pre;
     const void* dh;
@@ -414,11 +445,15 @@ struct GlDgu {
     float* colpart;
     void* db[2];
     int64_t lddh, ldg, M;
-    int N, act, tx, rows;
+    int N, act, tx, rows, nblk;
 };
 template <typename T, typename TD>
-__global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
+__global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p, GlPack pack) {
     __shared__ f32x4 red[2][256];
+    if ((int)blockIdx.y >= p.nblk) {
+        gl_pack<T>(pack, (int64_t)(blockIdx.y - p.nblk) * gridDim.x + blockIdx.x, (int64_t)(gridDim.y - p.nblk) * gridDim.x);
+        return;
+    }
     const int cx = threadIdx.x % p.tx, ry = threadIdx.x / p.tx, ty = 256 / p.tx;
     const int n = (blockIdx.x * p.tx + cx) * 4, cnt = p.N - n;
     const int64_t r0 = (int64_t)blockIdx.y * p.rows, r1 = r0 + p.rows < p.M ? r0 + p.rows : p.M;
@@ -468,7 +503,7 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
             sg += red[0][k * p.tx + cx];
             su += red[1][k * p.tx + cx];
         }
-        if (gridDim.y == 1) {
+        if (p.nblk == 1) {
             if (p.db[0] && cnt > 0) gl_put4((T*)p.db[0] + n, sg, cnt);
             if (p.db[1] && cnt > 0) gl_put4((T*)p.db[1] + n, su, cnt);
         } else {
@@ -479,23 +514,33 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p) {
     }
 }
 
-// db[n] = sum of the row blocks' partial sums: 64 columns (16 groups of 4) x 16 lanes per block, lanes joined in order
-template <typename T>
-__global__ __launch_bounds__(256) void k_gated_colsum(const float* colpart, int nblk, int64_t ldg, T* dbg, T* dbu, int N) {
-    __shared__ f32x4 red[16][16];
+// db[n] = sum of the row blocks' partial sums: a workgroup has 64 columns (16 groups of 4) of one plane and THREADS / 16 lanes, lanes
+// joined in order.  Workgroups [0, n) of it, the last ones of a launch of both products where there is one (2 to 5 us of a launch saved).
+struct GlColsum {
+    const float* colpart;
+    void* db[2];
+    int64_t ldg;
+    int nblk, N, n;
+};
+template <typename T, int THREADS> __device__ __forceinline__ void gl_colsum(const GlColsum& p, int b, f32x4 (*red)[16]) {
     const int c = threadIdx.x & 15, y = threadIdx.x >> 4;
-    const int n = blockIdx.x * 64 + c * 4, pl = blockIdx.y, cnt = N - n;
+    const int n = (b >> 1) * 64 + c * 4, pl = b & 1, cnt = p.N - n;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (cnt > 0)
 #pragma unroll 8
-        for (int b = y; b < nblk; b += 16) s += *(const f32x4*)(colpart + ((int64_t)b * 2 + pl) * ldg + n);
+        for (int k = y; k < p.nblk; k += THREADS / 16) s += *(const f32x4*)(p.colpart + ((int64_t)k * 2 + pl) * p.ldg + n);
     red[y][c] = s;
     __syncthreads();
-    T* const out = pl ? dbu : dbg;
+    T* const out = (T*)p.db[pl];
     if (y == 0 && cnt > 0 && out) {
-        for (int k = 1; k < 16; ++k) s += red[k][c];
+        for (int k = 1; k < THREADS / 16; ++k) s += red[k][c];
         gl_put4(out + n, s, cnt);
     }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_colsum(GlColsum p) {
+    __shared__ f32x4 red[16][16];
+    gl_colsum<T, 256>(p, blockIdx.x, red);
 }
 
 template <typename T>

@@ -169,9 +169,10 @@ __global__ __launch_bounds__(GF_THREADS) void k_gated_f32(GtArgs q) {
     gf_product<MODE, T, VEC>(q, blockIdx.x, gridDim.x, smem);
 }
 template <int T, bool VEC>
-__global__ __launch_bounds__(GF_THREADS) void k_gated_f32_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+__global__ __launch_bounds__(GF_THREADS) void k_gated_f32_both(GtArgs dx, GtArgs dw, int n0, int dx_first, GlColsum cs) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
+    const int b = blockIdx.x, all = gridDim.x - cs.n, first = b < n0, at = first ? b : b - n0, count = first ? n0 : all - n0;
+    if (b >= all) return gl_colsum<float, GF_THREADS>(cs, b - all, (f32x4(*)[16])smem);
     if (first == dx_first) gf_product<GL_DX, T, VEC>(dx, at, count, smem);
     else gf_product<GL_DW, T, VEC>(dw, at, count, smem);
 }

@@ -71,31 +71,4 @@ template <int MODE> __device__ __forceinline__ void gt_tile(const GtArgs& q, int
     tj = __builtin_amdgcn_readfirstlane(in / rows_here);
 }
 
-// copies of up to three matrices whose rows are not 16-byte aligned: [rows][ldd], columns C..ldd - 1 zero
-struct GlPack {
-    struct { const void* src; void* dst; int64_t ld, rows; } m[3];
-    int64_t ldd;
-    int C, n;
-};
-template <typename T>
-__global__ __launch_bounds__(256) void k_gated_pack(GlPack p) {
-    constexpr int E = 16 / sizeof(T);
-    const int64_t per = p.ldd / E;
-    int64_t total = 0;
-    for (int i = 0; i < p.n; ++i) total += p.m[i].rows * per;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-        int64_t r = t / per;
-        const int64_t c = (t - r * per) * E;
-        int i = 0;
-        while (r >= p.m[i].rows) r -= p.m[i++].rows;
-        const T* const src = (const T*)p.m[i].src + r * p.m[i].ld + c;
-        T v[E];
-        if (c + E <= p.C) __builtin_memcpy(v, src, 16);
-        else
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = c + e < p.C ? src[e] : (T)0;
-        __builtin_memcpy(__builtin_assume_aligned((T*)p.m[i].dst + r * p.ldd + c, 16), v, 16);
-    }
-}
-
 }  // namespace dp

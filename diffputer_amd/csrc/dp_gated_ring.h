@@ -235,10 +235,12 @@ __global__ __launch_bounds__(GS_THREADS, 2) void k_gated_ring(GtArgs q) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     gs_product<MODE>(q, blockIdx.x, gridDim.x, smem);
 }
-// both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, [n0, gridDim) the other
-__global__ __launch_bounds__(GS_THREADS, 2) static void k_gated_ring_both(GtArgs dx, GtArgs dw, int n0, int dx_first) {
+// both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, then the
+// other, then the column sums
+__global__ __launch_bounds__(GS_THREADS, 2) static void k_gated_ring_both(GtArgs dx, GtArgs dw, int n0, int dx_first, GlColsum cs) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int b = blockIdx.x, first = b < n0, at = first ? b : b - n0, count = first ? n0 : gridDim.x - n0;
+    const int b = blockIdx.x, all = gridDim.x - cs.n, first = b < n0, at = first ? b : b - n0, count = first ? n0 : all - n0;
+    if (b >= all) return gl_colsum<bf16_t, GS_THREADS>(cs, b - all, (f32x4(*)[16])smem);
     if (first == dx_first) gs_product<GL_DX>(dx, at, count, smem);
     else gs_product<GL_DW>(dw, at, count, smem);
 }
