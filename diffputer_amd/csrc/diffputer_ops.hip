@@ -413,8 +413,8 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     if (w.tx == 48) w.tx = 64;
     const int64_t cols = ceil_div<int64_t>(w.ldg, w.tx * 4);
     const int ty = 256 / w.tx;
-    // about 1024 workgroups, at least 4 rows per row lane
-    w.rows = (int)std::max<int64_t>(4 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 1024 / cols)));
+    // about 1024 workgroups, at least 2 rows per row lane
+    w.rows = (int)std::max<int64_t>(2 * ty, ceil_div<int64_t>(M, std::max<int64_t>(1, 1024 / cols)));
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
     w.dgu = c.take((size_t)2 * M * w.ldg * (w.plane == DP_DTYPE_BF16 ? 2 : 4));
     w.colpart = (float*)c.take(w.nblk > 1 ? (size_t)w.nblk * 2 * w.ldg * 4 : 0);

@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256) void k_gated_dgu(GlDgu p, GlPack pack) {
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
     if (n < p.ldg) gl_with_act(p.act, [&](auto act) {
         // R rows at a time, all their loads before the first store (which could hit what is loaded, as far as the compiler knows)
-        constexpr int R = 4;
+        constexpr int R = 2;
         for (int64_t m0 = r0 + ry; m0 < r1; m0 += R * ty) {
             f32x4 g[R], u[R], d[R];
 #pragma unroll
