@@ -166,7 +166,7 @@ static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
     const int64_t want = std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), nk / 8, (int64_t)(64 << 20) / std::max<int64_t>(gl_part_bytes(s), 1), 64});
     return gl_shape(s, 0, GG_K, (int)std::max<int64_t>(want, 1));
 }
-// both backward products: in one launch on a tile kernel, or two plans of their own
+// both backward products, in one launch if they take kernels of one kind and fit a grid
 static GlPlan gl_plan(const GlShape& s, int dtype, bool tile);
 static bool gl_plan_both_new(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
     if (tile && forced_kernel() != 1) {
@@ -174,7 +174,7 @@ static bool gl_plan_both_new(const GlShape s[2], int dtype, bool tile, GlPlan pl
         if (gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]) && pl[0].wgs + pl[1].wgs < (int64_t)1 << 22) return true;
     }
     for (int i = 0; i < 2; ++i) pl[i] = gl_plan(s[i], dtype, tile);
-    return false;
+    return pl[0].T == 0 && pl[1].T == 0 && gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]);
 }
 // A choice takes a microsecond or two and is asked for several times per call (workspace query, check, launch): the last ones are
 // remembered by everything that they depend on, sizes and settings.
@@ -237,6 +237,7 @@ static GtArgs gl_args(GlArgs a, const GlShape& s, const GlPlan& c) {
     a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
     return {a, (int)c.ti, (int)c.tj, 8};
 }
+static GgArgs gg_args(const GlArgs& a, const GlShape& s, const GlPlan& c) { return {gl_args(a, s, c).g, (int)c.ti, (int)c.tj, (int)c.wgs}; }
 static unsigned gl_join_grid(const GlShape& s) { return (unsigned)std::min<int64_t>(ceil_div<int64_t>(s.I * s.planes * ceil_div<int64_t>(s.J, 4), 256), 4096); }
 
 template <typename T, int MT, int CB>
@@ -262,7 +263,9 @@ static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, h
     int rc;
     if (c.T == GL_ROWS) return MODE == GL_FWD ? gr_rows<T>(q.g, st) : DP_EINVAL;
     if (c.T == 0) {
-        hipLaunchKernelGGL((k_gated_mm<T, typename GlPlane<T, MODE>::V, MODE>), dim3((unsigned)c.ti, (unsigned)c.tj, (unsigned)(s.planes * c.splits)), dim3(256), 0, st, q.g);
+        if (c.wgs > INT32_MAX) return fail(DP_EINVAL, "gated projection: %lld tiles", (long long)c.wgs);
+        const unsigned across = (unsigned)std::min<int64_t>(c.wgs, 1 << 20);
+        hipLaunchKernelGGL((k_gated_mm<T, typename GlPlane<T, MODE>::V, MODE>), dim3(across, (unsigned)ceil_div<int64_t>(c.wgs, across)), dim3(256), 0, st, gg_args(a, s, c));
         DP_LAUNCH_CHECK("k_gated_mm");
     } else if ((rc = gt_ready()) || (rc = gt_launch<MODE>(q, c, sizeof(T) == 2, vec, st))) return rc;
     if (c.splits > 1) {
@@ -276,11 +279,12 @@ static int gl_mm(const GlArgs& a, const GlShape& s, const GlPlan& c, bool vec, h
 template <typename T>
 static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], const GlColsum& cs, bool vec, hipStream_t st) {
     int rc;
-    if ((rc = gt_ready())) return rc;
+    if (c[0].T && (rc = gt_ready())) return rc;
     const GtArgs dx = gl_args(a[0], s[0], c[0]), dw = gl_args(a[1], s[1], c[1]);
     const int dx_first = c[0].kt_per >= c[1].kt_per, n0 = (int)c[dx_first ? 0 : 1].wgs;
     const dim3 grid((unsigned)(c[0].wgs + c[1].wgs + cs.n));
-    if (sizeof(T) == 2) {
+    if (c[0].T == 0) hipLaunchKernelGGL((k_gated_mm_both<T>), grid, dim3(256), 0, st, gg_args(a[0], s[0], c[0]), gg_args(a[1], s[1], c[1]), cs);
+    else if (sizeof(T) == 2) {
         if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, grid, dim3(GT_THREADS), GT_LDS, st, dx, dw, n0, dx_first, cs);
         else hipLaunchKernelGGL(k_gated_ring_both, grid, dim3(GS_THREADS), GS_LDS, st, dx, dw, n0, dx_first, cs);
     } else if (c[0].T == 128) {
@@ -290,7 +294,7 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], con
         if (vec) hipLaunchKernelGGL((k_gated_f32_both<64, true>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first, cs);
         else hipLaunchKernelGGL((k_gated_f32_both<64, false>), grid, dim3(GF_THREADS), GfShape<64>::LDS, st, dx, dw, n0, dx_first, cs);
     }
-    DP_LAUNCH_CHECK("gated tile kernel");
+    DP_LAUNCH_CHECK("gated products");
     const unsigned jx = c[0].splits > 1 ? gl_join_grid(s[0]) : 0, jw = c[1].splits > 1 ? gl_join_grid(s[1]) : 0;
     if (jx + jw) {
         hipLaunchKernelGGL((k_gated_join_both<T>), dim3(jx + jw), dim3(256), 0, st, dx.g, dw.g, (int)jx);

@@ -225,18 +225,25 @@ template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs&
 // TA: type of A.  bf16 layers' dg and du are float32 here and multiplied as bf16 hi + lo, two products: small layers, where
 // one product or two is the same time, then have no rounding between the gradient of h and the sums.
 constexpr int GG_T = 64, GG_K = 32;
+struct GgArgs {
+    GlArgs g;
+    int ti, tj, wgs;           // tiles along I and J; workgroups: tiles x slices x planes
+};
+template <typename T> struct GgShape {
+    static constexpr int LD = sizeof(T) == 2 ? GG_K + 8 : GG_K + 1, PART = GG_T * LD;         // row stride; elements of an operand
+};
 template <typename T, typename TA, int MODE>
-__global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
+__device__ __forceinline__ void gg_product(const GgArgs& q, int block, T* smem) {
     constexpr bool BF = sizeof(T) == 2, HILO = BF && sizeof(TA) == 4;
-    constexpr int LD = BF ? GG_K + 8 : GG_K + 1;
+    constexpr int LD = GgShape<T>::LD;
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
-    __shared__ __attribute__((aligned(16))) T sa[GG_T * LD];
-    __shared__ __attribute__((aligned(16))) T sb[GG_T * LD];
-    __shared__ __attribute__((aligned(16))) T slo[HILO ? GG_T * LD : 1];
+    T *const sa = smem, *const sb = smem + GgShape<T>::PART, *const slo = smem + 2 * GgShape<T>::PART;
+    const GlArgs& p = q.g;
+    const int bx = block % q.ti, by = block / q.ti % q.tj, bz = block / q.ti / q.tj;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-    const int64_t i0 = (int64_t)blockIdx.x * GG_T;
-    const int j0 = blockIdx.y * (MODE == GL_FWD ? GG_T / 2 : GG_T);
-    const int slice = blockIdx.z % p.splits, plane = p.zfirst + blockIdx.z / p.splits;
+    const int64_t i0 = (int64_t)bx * GG_T;
+    const int j0 = by * (MODE == GL_FWD ? GG_T / 2 : GG_T);
+    const int slice = bz % p.splits, plane = p.zfirst + bz / p.splits;
     const int segs = MODE == GL_DX ? 2 : 1;
     const int64_t nk = ceil_div<int64_t>(p.C, GG_K);
     const int64_t kt0 = (int64_t)slice * p.kt_per, kt1 = kt0 + p.kt_per < nk * segs ? kt0 + p.kt_per : nk * segs;
@@ -366,6 +373,13 @@ __global__ __launch_bounds__(256) void k_gated_mm(GlArgs p) {
                 }
         }
     }
+}
+
+template <typename T, typename TA, int MODE>
+__global__ __launch_bounds__(256) void k_gated_mm(GgArgs q) {
+    __shared__ __attribute__((aligned(16))) T smem[3 * GgShape<T>::PART];
+    const int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (b < q.wgs) gg_product<T, TA, MODE>(q, (int)b, smem);
 }
 
 // Joins the slices of a split launch, in order: 4 columns of one row per step.
@@ -541,6 +555,16 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_gated_colsum(GlColsum p) {
     __shared__ f32x4 red[16][16];
     gl_colsum<T, 256>(p, blockIdx.x, red);
+}
+
+// both backward products of a small layer, and the column sums
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_mm_both(GgArgs dx, GgArgs dw, GlColsum cs) {
+    __shared__ __attribute__((aligned(16))) T smem[3 * GgShape<T>::PART];
+    const int b = blockIdx.x;
+    if (b < dx.wgs) gg_product<T, float, GL_DX>(dx, b, smem);
+    else if (b < dx.wgs + dw.wgs) gg_product<T, float, GL_DW>(dw, b - dx.wgs, smem);
+    else gl_colsum<T, 256>(cs, b - dx.wgs - dw.wgs, (f32x4(*)[16])smem);
 }
 
 template <typename T>

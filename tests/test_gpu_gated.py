@@ -408,6 +408,24 @@ def test_offsets_past_32_bits():
     torch.cuda.empty_cache()
 
 
+@torch.no_grad()
+def test_general_kernel_more_than_2_20_tiles(tune):
+    """A grid that is folded: equal rows give equal results everywhere, the last rows their own."""
+    from diffputer_amd.gated import gated_linear
+    M, K, N, tail = 270_000, 64, 8192, 70
+    x, wg, wu, bg, bu, dh = make(tail, K, N, "bf16", seed=29)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    big = torch.full((M, K), 0.5, dtype=torch.bfloat16, device=DEV)
+    big[-tail:] = x.to(DEV)
+    tune(1, 0)
+    h = gated_linear(big, *[t.to(DEV) for t in (wg, wu, bg, bu)])
+    close(h[-tail:], ref.h, ref.eh, "h")
+    for a in range(0, M - tail, 30_000):
+        assert torch.equal(h[a:min(a + 30_000, M - tail)], h[:1].expand(min(30_000, M - tail - a), N))
+    del h, big
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_two_threads(dtype):
     """Two threads, each with a stream of its own, at the same time."""
