@@ -216,11 +216,12 @@ static bool gl_plan_both(const GlShape s[2], int dtype, bool tile, GlPlan pl[2])
 }
 static size_t gl_split_bytes(const GlShape& s, const GlPlan& c) { return c.splits > 1 ? gl_part_bytes(s) * c.splits : 0; }
 
+static unsigned gt_grid(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 256); }        // a CU has room for one workgroup, which walks on
 template <int MODE>
 static int gt_launch(const GtArgs& q, const GlPlan& pl, bool bf, bool vec, hipStream_t st) {
     const dim3 grid((unsigned)pl.wgs);
     if (bf) {
-        if (pl.T == 256) hipLaunchKernelGGL((k_gated_tile<MODE>), grid, dim3(GT_THREADS), GT_LDS, st, q);
+        if (pl.T == 256) hipLaunchKernelGGL((k_gated_tile<MODE>), dim3(gt_grid(pl.wgs)), dim3(GT_THREADS), GT_LDS, st, q);
         else hipLaunchKernelGGL((k_gated_ring<MODE>), grid, dim3(GS_THREADS), GS_LDS, st, q);
     } else if (pl.T == 128) {
         if (vec) hipLaunchKernelGGL((k_gated_f32<MODE, 128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, q);
@@ -235,7 +236,7 @@ static int gt_launch(const GtArgs& q, const GlPlan& pl, bool bf, bool vec, hipSt
 
 static GtArgs gl_args(GlArgs a, const GlShape& s, const GlPlan& c) {
     a.I = s.I; a.J = s.J; a.C = s.C; a.kt_per = c.kt_per; a.splits = c.splits; a.ldp = gl_ldp(s.J);
-    return {a, (int)c.ti, (int)c.tj, 8};
+    return {a, (int)c.ti, (int)c.tj, 8, (int)c.wgs};
 }
 static GgArgs gg_args(const GlArgs& a, const GlShape& s, const GlPlan& c) { return {gl_args(a, s, c).g, (int)c.ti, (int)c.tj, (int)c.wgs}; }
 static unsigned gl_join_grid(const GlShape& s) { return (unsigned)std::min<int64_t>(ceil_div<int64_t>(s.I * s.planes * ceil_div<int64_t>(s.J, 4), 256), 4096); }
@@ -285,7 +286,7 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], con
     const dim3 grid((unsigned)(c[0].wgs + c[1].wgs + cs.n));
     if (c[0].T == 0) hipLaunchKernelGGL((k_gated_mm_both<T>), grid, dim3(256), 0, st, gg_args(a[0], s[0], c[0]), gg_args(a[1], s[1], c[1]), cs);
     else if (sizeof(T) == 2) {
-        if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, grid, dim3(GT_THREADS), GT_LDS, st, dx, dw, n0, dx_first, cs);
+        if (c[0].T == 256) hipLaunchKernelGGL(k_gated_tile_both, dim3(gt_grid(c[0].wgs + c[1].wgs) + cs.n), dim3(GT_THREADS), GT_LDS, st, dx, dw, dx_first, cs);
         else hipLaunchKernelGGL(k_gated_ring_both, grid, dim3(GS_THREADS), GS_LDS, st, dx, dw, n0, dx_first, cs);
     } else if (c[0].T == 128) {
         if (vec) hipLaunchKernelGGL((k_gated_f32_both<128, true>), grid, dim3(GF_THREADS), GfShape<128>::LDS, st, dx, dw, n0, dx_first, cs);

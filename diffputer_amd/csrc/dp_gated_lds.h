@@ -12,6 +12,7 @@ struct GtArgs {
     GlArgs g;
     int nti, ntj;              // tiles along I and J
     int group;                 // tile rows that are walked together (shared B panels stay in the XCD's L2)
+    int wgs;                   // tiles x slices x planes
 };
 
 __device__ __forceinline__ unsigned gt_lds(const void* p) { return (unsigned)(size_t)(DP_LDS_AS const char*)p; }   // LDS byte address

@@ -32,9 +32,9 @@ constexpr int GT_HR = GT_T / 2, GT_HB = GT_HR * 128;                       // ro
 constexpr int GT_MI = GT_HR / 32, GT_NJ = GT_HR / GT_WN / 16;              // 16 x 16 tiles of a wave's quadrant
 constexpr int GT_LDS = 8 * GT_HB;
 
-// workgroup `b` of the launch's `count` that run this product: its tile and slice, neighbouring tiles on one XCD
+// tiles (and slices) b, b + step, .. of the product, neighbouring ones on one XCD; returns how far behind its end the walk is
 template <int MODE>
-__device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, char* smem) {
+__device__ __forceinline__ int gt_product(const GtArgs& q, int b, int step, char* smem) {
     constexpr bool A_ROW = MODE != GL_DW, B_ROW = MODE == GL_FWD;
     constexpr int HR = GT_HR, HB = GT_HB, MI = GT_MI, NJ = GT_NJ, NW = GT_NW, WN = GT_WN;
     constexpr unsigned OUTSIDE = 0x80000000u;                              // an offset behind every buffer
@@ -44,17 +44,22 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     const int wm = wave / WN, wn = wave % WN;
 
     const bool split = p.splits > 1;
-    int slice, plane, ti, tj;
-    gt_tile<MODE>(q, b, count, slice, plane, ti, tj);
-    const int64_t i0 = (int64_t)ti * GT_T;
-    const int j0 = tj * (MODE == GL_FWD ? HR : GT_T);
-
     const int nk = (int)((p.C + 63) >> 6);                                 // K-tiles of a segment
-    const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
+    struct Tile { int slice, plane, j0, kt0, kt1; int64_t i0; };
+    auto locate = [&](int at) {
+        Tile t;
+        int ti, tj;
+        gt_tile<MODE>(q, at, q.wgs, t.slice, t.plane, ti, tj);
+        t.i0 = (int64_t)ti * GT_T;
+        t.j0 = tj * (MODE == GL_FWD ? HR : GT_T);
+        t.kt0 = t.slice * p.kt_per;
+        t.kt1 = min(t.kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
+        return t;
+    };
 
     // ---- loads: a wave moves pieces `wave` and `wave + NW` (1 KiB each) of every half-tile ----
     //   row layout: piece = 8 rows x 128 B; column layout: piece = 4 k rows x 256 B
-    const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
+    const int64_t lda = p.A[0].ld * 2, ldb = p.B[0].ld * 2;                // bytes (both planes and both weights have the same)
     auto g_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
     const int r8 = lane >> 3, c8 = (lane & 7) ^ r8;                        // row layout: row of the piece, chunk of memory
     unsigned va[2], vb[2];
@@ -70,12 +75,12 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     // the K-tile.  Column layout: a K-tile has 64 k rows, the segment's last one `last` bytes.
     struct Stream { u32x4 at; unsigned full, last; int kt; };
     auto seg_of = [&](int kt) { return MODE == GL_DX && kt >= nk ? 1 : 0; };
-    auto open = [&](bool is_b, int h, int kt) {
+    auto open = [&](const Tile& t, bool is_b, int h, int kt) {
         const bool row = is_b ? B_ROW : A_ROW;
         const int seg = seg_of(kt);
-        const GlOp& op = is_b ? p.B[MODE == GL_FWD ? h : seg] : p.A[MODE == GL_DX ? seg : MODE == GL_DW ? plane : 0];
+        const GlOp& op = is_b ? p.B[MODE == GL_FWD ? h : seg] : p.A[MODE == GL_DX ? seg : MODE == GL_DW ? t.plane : 0];
         const int64_t ld = op.ld * 2, size = is_b ? p.J : p.I, kk = kt - seg * nk;
-        const int64_t first = (is_b ? j0 : i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);        // first row / column of the half
+        const int64_t first = (is_b ? t.j0 : t.i0) + (MODE == GL_FWD && is_b ? 0 : h * HR);        // first row / column of the half
         Stream st;
         st.at = gl_buffer((const char*)op.p + (row ? first * ld + kk * 128 : kk * 64 * ld + first * 2));
         st.full = gl_clip(row ? (size - 1 - first) * ld + op.cols * 2 : 63 * ld + (op.cols - first) * 2);
@@ -84,14 +89,15 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         st.kt = kt;
         return st;
     };
-    Stream sa[2] = {open(false, 0, kt0), open(false, 1, kt0)}, sb[2] = {open(true, 0, kt0), open(true, 1, kt0)};
+    Stream sa[2], sb[2];
+    Tile in;                                                               // the tile that is loaded
     const int64_t step_a = A_ROW ? 128 : 64 * lda, step_b = B_ROW ? 128 : 64 * ldb;
     const unsigned lds0 = gt_lds(smem);
     auto stage = [&](bool is_b, int h) {                                   // the next K-tile of a half; past the last one: no bytes
         Stream& st = is_b ? sb[h] : sa[h];
         const bool last = st.kt - seg_of(st.kt) * nk == nk - 1;
-        st.at[2] = st.kt >= kt1 ? 0u : last ? st.last : st.full;
-        const unsigned dst = lds0 + (unsigned)((((st.kt - kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024);
+        st.at[2] = st.kt >= in.kt1 ? 0u : last ? st.last : st.full;
+        const unsigned dst = lds0 + (unsigned)((((st.kt - in.kt0) & 1) * 4 + (is_b ? 2 : 0) + h) * HB + wave * 1024);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             unsigned vo = is_b ? vb[s] : va[s];
@@ -102,7 +108,7 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         gl_advance(st.at, is_b ? step_b : step_a);
         if (MODE == GL_DX && __builtin_expect(st.kt == nk, 0)) {
             asm volatile("");                                              // a branch, not a selection computed every time
-            st = open(is_b, h, st.kt);
+            st = open(in, is_b, h, st.kt);
         }
     };
 
@@ -134,15 +140,6 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
     };
 
     f32x4 acc[2][MI][2][NJ];                                               // [A half][m-tile][B half][n-tile]
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[a][i][b][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
 #define GT_MFMA(ha, hb, bfr)                                                                                    \
     do {                                                                                                        \
         asm volatile("" ::: "memory");                                                                          \
@@ -159,97 +156,121 @@ __device__ __forceinline__ void gt_product(const GtArgs& q, int b, int count, ch
         asm volatile("" ::: "memory");                                                                          \
     } while (0)
 
-    stage(true, 1); stage(false, 0); stage(true, 0); stage(false, 1);
-    stage(true, 1); stage(false, 0); stage(true, 0);
-    GT_VMCNT(8);                                                           // B1, A0, B0 of the first K-tile
-    __builtin_amdgcn_s_barrier();
-    if (wm == 1) __builtin_amdgcn_s_barrier();                             // the lower half runs one barrier behind
-    asm volatile("" ::: "memory");
-    read_b(b1, lds0, 1);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    unsigned par = 0;
+    // The first loads of a tile: where there is one before it, they are in flight while that one's results are stored.
+    auto begin = [&](int at) {
+        in = locate(at);
+        for (int h = 0; h < 2; ++h) {
+            sa[h] = open(in, false, h, in.kt0);
+            sb[h] = open(in, true, h, in.kt0);
+        }
+        stage(true, 1); stage(false, 0); stage(true, 0); stage(false, 1);
+        stage(true, 1); stage(false, 0); stage(true, 0);
+    };
+    if (b < q.wgs) begin(b);
+    bool first = true;
 #pragma clang loop unroll(disable)
-    for (int kt = kt0; kt < kt1; ++kt, par ^= 4 * HB) {
-        const unsigned buf = lds0 + par, nbuf = lds0 + (par ^ 4 * HB);
-        read_b(b0, buf, 0);                                                // c0
-        read_a(buf, 0);
-        GT_MFMA(0, 0, b0);
-        stage(false, 1);                                                   // c1: A1(t+1), B1(t+2)
-        stage(true, 1);
-        GT_VMCNT(10);
-        GT_MFMA(0, 1, b1);
-        read_a(buf, 1);                                                    // c2
-        stage(false, 0);
-        GT_VMCNT(10);
-        GT_MFMA(1, 1, b1);
-        read_b(b1, nbuf, 1);                                               // c3
-        stage(true, 0);
-        GT_VMCNT(8);
-        GT_MFMA(1, 0, b0);
-    }
-    if (wm == 0) __builtin_amdgcn_s_barrier();                 // as many barriers as the lower half
-    GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
-#undef GT_MFMA
-
-    // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
-    const int cl = wn * NJ * 16 + (lane >> 4) * 4;
-    const int64_t mrow = i0 + wm * (HR / 2) + (lane & 15);
-    if (split) {
+    for (; b < q.wgs; b += step, first = false) {
+        const Tile cur = in;
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                const int64_t m = mrow + a * HR + i * 16;
-                if (m >= p.I) continue;
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        const int n = j0 + (MODE == GL_FWD ? 0 : b * HR) + cl + j * 16, pl = MODE == GL_FWD ? b : plane;
-                        // ldp is a multiple of 4: four columns that start inside a row end inside its padding
-                        if (n < p.J) *(f32x4*)(p.part + (((int64_t)slice * 2 + pl) * p.I + m) * p.ldp + n) = acc[a][i][b][j];
-                    }
-            }
-        return;
+                    for (int j = 0; j < NJ; ++j) acc[a][i][b][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+        if (first) GT_VMCNT(8);                                                // B1, A0, B0 of the first K-tile
+        else GT_VMCNT(0);                                                      // (the last tile's stores are behind them)
+        __builtin_amdgcn_s_barrier();
+        if (wm == 1) __builtin_amdgcn_s_barrier();                             // the lower half runs one barrier behind
+        asm volatile("" ::: "memory");
+        read_b(b1, lds0, 1);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        unsigned par = 0;
+#pragma clang loop unroll(disable)
+        for (int kt = cur.kt0; kt < cur.kt1; ++kt, par ^= 4 * HB) {
+            const unsigned buf = lds0 + par, nbuf = lds0 + (par ^ 4 * HB);
+            read_b(b0, buf, 0);                                                // c0
+            read_a(buf, 0);
+            GT_MFMA(0, 0, b0);
+            stage(false, 1);                                                   // c1: A1(t+1), B1(t+2)
+            stage(true, 1);
+            GT_VMCNT(10);
+            GT_MFMA(0, 1, b1);
+            read_a(buf, 1);                                                    // c2
+            stage(false, 0);
+            GT_VMCNT(10);
+            GT_MFMA(1, 1, b1);
+            read_b(b1, nbuf, 1);                                               // c3
+            stage(true, 0);
+            GT_VMCNT(8);
+            GT_MFMA(1, 0, b0);
+        }
+        if (wm == 0) __builtin_amdgcn_s_barrier();                 // as many barriers as the lower half
+        GT_VMCNT(0);                                                           // nothing may land in LDS behind the workgroup's end
+        if (b + step < q.wgs) begin(b + step);
+
+        // ---- epilogue: lane holds row (lane & 15), columns 4 (lane >> 4) + 0..3 of each 16 x 16 tile ----
+        const int cl = wn * NJ * 16 + (lane >> 4) * 4;
+        const int64_t mrow = cur.i0 + wm * (HR / 2) + (lane & 15);
+        if (split) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const int64_t m = mrow + a * HR + i * 16;
+                    if (m >= p.I) continue;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) {
+                            const int n = cur.j0 + (MODE == GL_FWD ? 0 : b * HR) + cl + j * 16, pl = MODE == GL_FWD ? b : cur.plane;
+                            // ldp is a multiple of 4: four columns that start inside a row end inside its padding
+                            if (n < p.J) *(f32x4*)(p.part + (((int64_t)cur.slice * 2 + pl) * p.I + m) * p.ldp + n) = acc[a][i][b][j];
+                        }
+                }
+        } else if constexpr (MODE == GL_FWD) {
+            gl_with_act(p.act, [&](auto act) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = cur.j0 + cl + j * 16, cnt = p.J - n;
+                    if (cnt <= 0) continue;
+                    f32x4 bg, bu;
+                    gl_bias<bf16_t>(p, n, cnt, bg, bu);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            const int64_t m = mrow + a * HR + i * 16;
+                            if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[a][i][0][j] + bg, acc[a][i][1][j] + bu);
+                        }
+                }
+            });
+        } else {
+            bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? cur.plane : 0];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int n = cur.j0 + b * HR + cl + j * 16, cnt = p.J - n;
+                    if (cnt <= 0) continue;
+#pragma unroll
+                    for (int a = 0; a < 2; ++a)
+#pragma unroll
+                        for (int i = 0; i < MI; ++i) {
+                            const int64_t m = mrow + a * HR + i * 16;
+                            if (m < p.I) gl_put4(out + m * p.ldo + n, acc[a][i][b][j], cnt);
+                        }
+                }
+        }
     }
-    if constexpr (MODE == GL_FWD) {
-        gl_with_act(p.act, [&](auto act) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int n = j0 + cl + j * 16, cnt = p.J - n;
-                if (cnt <= 0) continue;
-                f32x4 bg, bu;
-                gl_bias<bf16_t>(p, n, cnt, bg, bu);
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        const int64_t m = mrow + a * HR + i * 16;
-                        if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[a][i][0][j] + bg, acc[a][i][1][j] + bu);
-                    }
-            }
-        });
-    } else {
-        bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? plane : 0];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int n = j0 + b * HR + cl + j * 16, cnt = p.J - n;
-                if (cnt <= 0) continue;
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) {
-                        const int64_t m = mrow + a * HR + i * 16;
-                        if (m < p.I) gl_put4(out + m * p.ldo + n, acc[a][i][b][j], cnt);
-                    }
-            }
-    }
+#undef GT_MFMA
+    return b - q.wgs;
 }
 
 template <int MODE>
@@ -257,14 +278,14 @@ __global__ __launch_bounds__(GT_THREADS) void k_gated_tile(GtArgs q) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     gt_product<MODE>(q, blockIdx.x, gridDim.x, smem);
 }
-// both backward products in one launch, the longer contraction first: workgroups [0, n0) the one, then the
-// other, then the column sums
-__global__ __launch_bounds__(GT_THREADS) static void k_gated_tile_both(GtArgs dx, GtArgs dw, int n0, int dx_first, GlColsum cs) {
+// both backward products in one launch, the longer contraction first, and the column sums
+__global__ __launch_bounds__(GT_THREADS) static void k_gated_tile_both(GtArgs dx, GtArgs dw, int dx_first, GlColsum cs) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int b = blockIdx.x, all = gridDim.x - cs.n, first = b < n0, at = first ? b : b - n0, count = first ? n0 : all - n0;
-    if (b >= all) return gl_colsum<bf16_t, GT_THREADS>(cs, b - all, (f32x4(*)[16])smem);
-    if (first == dx_first) gt_product<GL_DX>(dx, at, count, smem);
-    else gt_product<GL_DW>(dw, at, count, smem);
+    const int step = gridDim.x - cs.n;
+    int b = blockIdx.x;
+    if (b >= step) return gl_colsum<bf16_t, GT_THREADS>(cs, b - step, (f32x4(*)[16])smem);
+#pragma clang loop unroll(disable)
+    for (int k = 0; k < 2; ++k) b = (k == 0) == (dx_first != 0) ? gt_product<GL_DX>(dx, b, step, smem) : gt_product<GL_DW>(dw, b, step, smem);
 }
 
 }  // namespace dp
