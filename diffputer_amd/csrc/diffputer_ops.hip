@@ -323,7 +323,7 @@ static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void*
     o.vec = x_in && w_in;
     o.pack_x = o.pack_w = false;
     o.ldk = round_up<int64_t>(K, chunk);
-    const bool large = M * N * K >= GT_PACK_LEAST;
+    const bool large = (double)M * N * K >= (double)GT_PACK_LEAST;
     o.tile = forced != 1 && (bf ? forced || (o.vec && short_rows) || large : short_rows || large);
     if (o.tile && (bf || large || !short_rows)) {
         o.pack_x = !x_in || ldx > GT_MAX_LD || K % chunk;

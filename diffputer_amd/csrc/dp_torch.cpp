@@ -230,6 +230,11 @@ PyObject* py_grads(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const Tensor norm = at::empty({}, first->options().dtype(at::kFloat).requires_grad(false));
         const size_t need = dp_grad_workspace_bytes((int)count);
         const Tensor ws = bytes_like(*first, need);
+        if (clip)                                                // written in place: a graph that kept one of them notices
+            for (Py_ssize_t i = 0; i < count; ++i) {
+                const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            }
         if (clip) check(dp_clip_grads((int)count, ptrs.data(), numel.data(), dtypes.data(), (int)kind, (float)limit, (float*)norm.data_ptr(), ws.data_ptr(), need, stream_of(norm)), "dp_clip_grads");
         else check(dp_grad_norm((int)count, (const void* const*)ptrs.data(), numel.data(), dtypes.data(), (int)kind, (float*)norm.data_ptr(), ws.data_ptr(), need, stream_of(norm)), "dp_grad_norm");
         return THPVariable_Wrap(norm);

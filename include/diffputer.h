@@ -286,7 +286,7 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  *   act          0 = none, 1 = SiLU, 2 = GELU (g Phi(g), not its tanh approximation); a NaN of x or w reaches every element that depends on it
  *   pre          NULL, or dp_gated_linear_pre_bytes(dtype, M, N) bytes (16-byte aligned) that receive both projections for the
  *                backward pass (float32; for bf16 20 bits of it each); the layout is the library's own
- * Any strides, element-aligned pointers, 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
+ * Any strides, element-aligned pointers, outputs that overlap no input; 0 <= M < 2^29, 1 <= N, K <= 2^20.  M = 0 does nothing.  Rows are independent of
  * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
  * (workspace >= dp_gated_linear_workspace_bytes(.., grads) for the same arguments, grads = DP_GATED_FORWARD, or the DP_GATED_D.. that dp_gated_linear_bwd is asked for, 256-byte aligned; calls that may
  * overlap in time need workspaces of their own), and may be captured into a graph.  bf16 is fastest where x and the weights

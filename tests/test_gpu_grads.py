@@ -218,3 +218,22 @@ def test_m_step_clips():
     assert len(seen) == 12 and all(before > 1e-3 and after <= 1e-3 * (1 + 1e-5) for before, after in seen)
     assert all(torch.equal(a, b) for a, b in zip(runs[0][0].values(), runs[2][0].values())) and math.isfinite(runs[1][1])
     assert grads.clip_grads is plain
+
+
+def test_a_graph_that_kept_a_gradient_notices():
+    """Clipping writes in place: a graph that saved the tensor before must not use it afterwards."""
+    from diffputer_amd.grads import clip_grads, grad_norm
+    g = torch.randn(100, device=DEV)
+    w = torch.randn(100, device=DEV, requires_grad=True)
+    y = (w * g).sum()
+    grad_norm([g])
+    z = (w * g).sum()
+    torch.autograd.grad(y, w)
+    clip_grads([g], 0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z, w)
+    with torch.inference_mode():
+        g = torch.full((100,), 3.0, device=DEV)
+        clip_grads([g], 1.0)
+    # coefficient 1 / (30 + 1e-6) in float32, one product: 2^-23 of 0.1
+    assert abs(float(g[0]) - 3.0 / (30.0 + 1e-6)) <= 2.0 ** -22 * 0.1
