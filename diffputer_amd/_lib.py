@@ -54,7 +54,7 @@ SIGNATURES = {
     "dp_gated_linear_bwd": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "dp_grad_workspace_bytes": (_sz, [_i]),
     "dp_grad_norm": (_i, [_i, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(_i), _i, _vp, _vp, _sz, _vp]),
-    "dp_clip_grads": (_i, [_i, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(_i), _i, _f, _vp, _vp, _sz, _vp]),
+    "dp_clip_grads": (_i, [_i, C.POINTER(_vp), C.POINTER(_i64), C.POINTER(_i), _i, C.c_double, _vp, _vp, _sz, _vp]),
     "dp_noise_field": (_i, [_vp, _i64, _i, _u64, _u64, _i, _u32, _i, _vp]),
 }
 

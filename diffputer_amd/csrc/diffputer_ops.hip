@@ -643,11 +643,11 @@ int dp_grad_norm(int n, const void* const* g, const int64_t* numel, const int* d
     return DP_OK;
 }
 
-int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, float limit, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, double limit, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = gn_check("dp_clip_grads", n, g, numel, dtype, norm_type, workspace, workspace_bytes);
     if (rc) return rc;
     if (!norm) return fail(DP_EINVAL, "dp_clip_grads: null pointer");
-    if (!(limit >= 0.0f)) return fail(DP_EINVAL, "dp_clip_grads: the limit has to be a number of at least 0");
+    if (!(limit >= 0.0)) return fail(DP_EINVAL, "dp_clip_grads: the limit has to be a number of at least 0");
     try {                                                        // no two tensors may share memory: they are scaled in place
         std::vector<std::pair<uint64_t, uint64_t>> span;
         span.reserve(n);

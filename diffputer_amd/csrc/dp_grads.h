@@ -132,12 +132,12 @@ __global__ __launch_bounds__(GN_THREADS) void k_grad_total(const double* part, i
 
 // The table names the tensors from the last to the first, and a tensor's chunks are taken from its end: the end of what
 // k_grad_norm read is what the caches still hold.
-__global__ __launch_bounds__(GN_THREADS) void k_grad_clip(GradTable t, const double* part, int nparts, int inf, float limit, float* norm) {
+__global__ __launch_bounds__(GN_THREADS) void k_grad_clip(GradTable t, const double* part, int nparts, int inf, double limit, float* norm) {
     __shared__ double red[GN_THREADS / 64];
     const GnFirst first(t);
     const double total = gn_total(part, nparts, inf, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
-    const double cd = (double)limit / (total + 1e-6);
+    const double cd = limit / (total + 1e-6);
     if (cd >= 1.0) return;                                       // within the limit (a NaN coefficient goes on, and marks every element)
     const float coef = (float)cd;
     if (coef == 1.0f) return;

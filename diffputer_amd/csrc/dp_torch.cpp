@@ -235,7 +235,7 @@ PyObject* py_grads(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(args[0], i));
                 if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
             }
-        if (clip) check(dp_clip_grads((int)count, ptrs.data(), numel.data(), dtypes.data(), (int)kind, (float)limit, (float*)norm.data_ptr(), ws.data_ptr(), need, stream_of(norm)), "dp_clip_grads");
+        if (clip) check(dp_clip_grads((int)count, ptrs.data(), numel.data(), dtypes.data(), (int)kind, limit, (float*)norm.data_ptr(), ws.data_ptr(), need, stream_of(norm)), "dp_clip_grads");
         else check(dp_grad_norm((int)count, (const void* const*)ptrs.data(), numel.data(), dtypes.data(), (int)kind, (float*)norm.data_ptr(), ws.data_ptr(), need, stream_of(norm)), "dp_grad_norm");
         return THPVariable_Wrap(norm);
     });

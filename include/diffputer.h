@@ -329,7 +329,7 @@ int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gat
 size_t dp_grad_workspace_bytes(int n);
 int dp_grad_norm(int n, const void* const* g, const int64_t* numel, const int* dtype, int norm_type, float* norm,
                  void* workspace, size_t workspace_bytes, void* stream);
-int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, float limit, float* norm,
+int dp_clip_grads(int n, void* const* g, const int64_t* numel, const int* dtype, int norm_type, double limit, float* norm,
                   void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
