@@ -448,6 +448,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_gated_pack(GlPack p) { gl_pack<T>(p, blockIdx.x, gridDim.x); }
 
 // ---- backward, elementwise: du = dh act(g), dg = dh u act'(g), and their column sums ------------------------------------
+// Bound by memory: 11 bytes per element in bf16 (5 of pre, 2 of dh, 4 of dg and du), 16384 x 8192 in 300 us = 4.9 TB/s.
 // Block = tx column groups of 4 x (256 / tx) row lanes, `rows` rows; blocks behind the last row block make the copies that the
 // products read (one launch for both: 1537 x 777 x 1203 in bf16, copies in a launch of their own, 5.8 us).  dgu: two planes [M][ldg] of TD, columns N..ldg - 1
 // zero.  db: the column sums of the unrounded values: written here if one block has all rows, else left as partial sums

@@ -4,9 +4,11 @@
 // Such launches give a CU one or two workgroups and are bound by the latency of a K-step, not by the matrix pipes: nothing of a
 // step waits for itself.  While a step's products run, the fragments of the next one are read into a second set of registers
 // and the loads of the step five ahead go out, interleaved with the products; the only waits are one per step, for loads
-// that went out four steps before and for reads whose latency the products have covered, and one barrier.  Against the
-// four-phase schedule of the 256 x 256 kernel at this tile: 64 k's take 0.51 instead of 0.92 us with one workgroup on a CU in
-// four, 0.59 instead of 1.02 with one on each, 1.24 instead of 1.20 with two on each (64-byte row segments: half a cache line per request).
+// that went out four steps before and for reads whose latency the products have covered, and one barrier.  64 k's take 0.46 us
+// with one workgroup on a CU in four (the four-phase schedule of the 256 x 256 kernel at this tile: 0.92), 0.55 with one on
+// each (1.02), 1.16 with two on each (1.20), where LDS is the bound: a pair of workgroups reads 64 KiB of fragments and receives
+// 32 KiB of tiles per 32 k's, 768 cycles at 128 bytes each, and the matrix pipes need 512.  Both backward products of 4096 x 1024 x 2048, 512
+// workgroups: 68 us (1 010 TFLOP/s).
 //   step s:   { load step s + 5 into the slot of step s ; read fragments of s + 1 ; products of s ; wait ; barrier }
 //   RAW  step s + 1 was loaded in step s - 4 and waited for (all but the three newest steps' loads) at the end of step s - 1;
 //   WAR  the slot of step s was read in step s - 1, whose end every wave has passed with its reads done.

@@ -6,7 +6,9 @@
 // of 64 k's in bf16, 32 in float32, in turn, so that neighbouring bytes of a row are read at the same time), each lane loads
 // 16 bytes of a weight row straight into the matrix instruction's layout, and the waves' sums are added in order through LDS.
 // CB = 16: 16 gate and 16 up rows, two fragments; CB = 8 (narrow layers, twice the workgroups): 8 gate and 8 up rows in one.
-// x is read by every workgroup, from the L2.
+// x is read by every workgroup, from the L2.  The next round's weights are in flight under this one's products.
+// Measured, bf16: 24 x 4096 x 8192 30 us, 134 MB of weights at 4.5 TB/s (a large copy moves 4.7); 1 x 1024 x 2048 4.2 us, of which
+// about 3 are a launch's own.
 #pragma once
 #include "dp_gated_lds.h"
 

@@ -4,7 +4,9 @@
 //   coef = min(1, limit / (norm + 1e-6)),  g <- g coef  (in place; nothing is written when coef is 1)
 //
 // Two passes over memory: k_grad_norm leaves one partial per workgroup, k_grad_clip reduces the partials (each workgroup
-// for itself, in one fixed order: same bits everywhere) and scales.  Sums are float64; squares are added up in float32 within pairs
+// for itself, in one fixed order: same bits everywhere) and scales.  Bound by memory, in small sets by the two launches: 0.8 GB of float32
+// within the limit 135 us (5.9 TB/s), 2^27 bf16 numbers in 301 tensors clipped in 158 us (0.27 GB read, then read and written:
+// 5.1 TB/s), 42 MB in 14 tensors in 25.6 us, 0.3 MB in 10.  Sums are float64; squares are added up in float32 within pairs
 // (float32) or fours (bf16, whose squares are exact), two roundings at most, and only those go to float64: one conversion per
 // element held the kernel to 1.25 elements per ps, 2.5 TB/s in bf16.  A group outside [2^-96, inf) takes the long way, element
 // by element in float64: no square overflows or vanishes.
@@ -33,7 +35,8 @@ constexpr int GN_THREADS = 256;
 // change nothing there and lose 1 to 2 us at 0.3 MB and 42 MB.
 constexpr int GN_MAX_BLOCKS = 2048;
 
-// The entry that holds a chunk: lane l keeps the first chunks of entries l, l + 64 and l + 128 and the wave counts those that are not
+// The entry that holds a chunk (a walk along the table, 40 entries per chunk where 301 tensors share a launch or two, took 30 us
+// of 185): lane l keeps the first chunks of entries l, l + 64 and l + 128 and the wave counts those that are not
 // behind it.
 struct GnFirst {
     uint32_t c[(GN_MAX + 63) / 64];
