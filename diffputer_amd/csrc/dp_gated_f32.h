@@ -13,7 +13,7 @@
 //   With G = 64 / (T / 4) lane groups of T / 4 lanes, a lane reads four k's of its row or column, the group's 4 (G g + group) ..
 //   + 3: step s of the four multiplies the G k's 4 (G g + group) + s (both operands agree on that, and a sum over k does not
 //   ask for more).
-//   row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7), one ds_read_b128;
+//   row layout (k contiguous): LDS rows of 128 bytes, 16-byte chunk c of row r at c ^ ((r >> 1) & 7), one ds_read_b128;
 //   column layout: LDS holds k rows of 4 T bytes as they are in memory, four ds_read_b32; the bytes of k row k are stored with
 //   their place xor'ed by T * ((k / 4) % G), so that the G k's of a read use all banks.
 #pragma once
@@ -64,7 +64,7 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
         const int byte = (wave * NL + n) * 64 * EL + lane * EL;
-        const int r = byte >> 7, in_r = (((byte >> 4) & 7) ^ (r & 7)) * 16 + (byte & 15);      // row layout: row, byte within the row
+        const int r = byte >> 7, in_r = (((byte >> 4) & 7) ^ ((r >> 1) & 7)) * 16 + (byte & 15);      // row layout: row, byte within the row
         const int k = byte / (4 * T), in_k = (byte % (4 * T)) ^ (((k >> 2) & (G - 1)) * T);    // column layout: k, byte within the k row
         va[n] = A_ROW ? (unsigned)(r * lda + in_r) : (unsigned)(k * lda + in_k);
         vb[n] = B_ROW ? (unsigned)((r & (MODE == GL_FWD ? T / 2 - 1 : T - 1)) * ldb + in_r) : (unsigned)(k * ldb + in_k);
@@ -115,11 +115,11 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int ra = wm * (T / 2) + i * TS + r, rb = i * (T / 2) + wn * TS + r;
-                if (A_ROW) av[i] = *(const f32x4*)(sa + ra * 128 + (((G * g + grp) ^ (r & 7)) << 4));
+                if (A_ROW) av[i] = *(const f32x4*)(sa + ra * 128 + (((G * g + grp) ^ ((r >> 1) & 7)) << 4));
                 else
 #pragma unroll
                     for (int s = 0; s < 4; ++s) av[i][s] = *(const float*)(sa + (4 * (G * g + grp) + s) * (4 * T) + ((ra * 4) ^ (grp * T)));
-                if (B_ROW) bv[i] = *(const f32x4*)(sb + rb * 128 + (((G * g + grp) ^ (r & 7)) << 4));
+                if (B_ROW) bv[i] = *(const f32x4*)(sb + rb * 128 + (((G * g + grp) ^ ((r >> 1) & 7)) << 4));
                 else
 #pragma unroll
                     for (int s = 0; s < 4; ++s) bv[i][s] = *(const float*)(sb + (4 * (G * g + grp) + s) * (4 * T) + ((rb * 4) ^ (grp * T)));

@@ -42,12 +42,15 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
     const int kt0 = slice * p.kt_per, kt1 = min(kt0 + p.kt_per, nk * (MODE == GL_DX ? 2 : 1));
 
     // ---- loads: a wave moves pieces wave, wave + 4, .. (1 KiB) of each operand's T x 32 image ----
-    //   row layout: piece = 16 rows x 64 B, 16-byte chunk c of row r at c ^ ((r >> 2) & 3)
+    //   row layout: piece = 16 rows x 64 B, 16-byte chunk c of row r at c ^ turn(r / 4 % 4)
     //   column layout: k rows of 2 T bytes, piece = 512 / T of them, 32-byte slot s of k row k at s ^ g(k)
     const int64_t lda = p.A[MODE == GL_DW ? plane : 0].ld * 2, ldb = p.B[0].ld * 2;            // bytes
     constexpr int KR = 512 / T, CH = T / 8;                                // k rows of a piece, 16-byte chunks of a k row
     auto g_of = [](int k) { return (k & 3) | ((k >> 3) & 1) << 2; };
-    const int r16 = lane >> 2, c4 = (lane & 3) ^ ((lane >> 4) & 3);
+    // ds_read_b128 takes lanes 0-3, 12-15, 20-23 and 24-27 at a time (and 4-7, 8-11, 16-19, 28-31; the upper half alike): with 0, 2, 3, 1 their
+    // 16 chunks lie in 16 places, with 0, 1, 2, 3 in 8
+    auto turn = [](int x) { return ((x ^ x >> 1) & 1) << 1 | x >> 1; };
+    const int r16 = lane >> 2, c4 = (lane & 3) ^ turn(lane >> 4);
     unsigned va[NP], vb[NP];
 #pragma unroll
     for (int s = 0; s < NP; ++s) {
@@ -113,7 +116,7 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
     };
 
     // ---- fragment reads: an LDS byte address (column layout: the tile's number is xor'ed into the slot bits), and constant offsets ----
-    const unsigned foff = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) << 4);
+    const unsigned foff = (lane & 15) * 64 + (((lane >> 4) ^ turn((lane >> 2) & 3)) << 4);
     const int krow = (lane >> 4) * 8 + ((lane >> 2) & 3);
     const unsigned fc = krow * T * 2 + (g_of(krow) << 5) + (lane & 3) * 8;
     const unsigned fa = A_ROW ? foff + wm * MI * 1024 : fc ^ (wm * MI << 5), fb = B_ROW ? foff + wn * NJ * 1024 : fc ^ (wn * NJ << 5);
