@@ -6,8 +6,8 @@
 // and the loads of the step five ahead go out, interleaved with the products; the only waits are one per step, for loads
 // that went out four steps before and for reads whose latency the products have covered, and one barrier.  64 k's take 0.46 us
 // with one workgroup on a CU in four (the four-phase schedule of the 256 x 256 kernel at this tile: 0.92), 0.55 with one on
-// each (1.02), 1.16 with two on each (1.20), where LDS is the bound: a pair of workgroups reads 64 KiB of fragments and receives
-// 32 KiB of tiles per 32 k's, 768 cycles at 128 bytes each, and the matrix pipes need 512.  Both backward products of 4096 x 1024 x 2048, 512
+// each (1.02), 1.16 with two on each (1.20).  There the tiles' way into LDS is the bound: 64 KiB per 64 k's and pair of
+// workgroups, 1024 cycles at 64 bytes each, as long as the products; with loads of no bytes the same steps take 0.73.  Both backward products of 4096 x 1024 x 2048, 512
 // workgroups: 68 us (1 010 TFLOP/s).
 //   step s:   { load step s + 5 into the slot of step s ; read fragments of s + 1 ; products of s ; wait ; barrier }
 //   RAW  step s + 1 was loaded in step s - 4 and waited for (all but the three newest steps' loads) at the end of step s - 1;
