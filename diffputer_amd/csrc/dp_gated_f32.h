@@ -131,8 +131,7 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
 #pragma unroll
                     for (int h = 0; h < 2; ++h) acc[i][h] = Acc::mul(bv[h][s], av[i][s], acc[i][h]);
         }
-        GT_VMCNT(0);
-        __builtin_amdgcn_s_barrier();
+        GL_SYNC(0);                                              // the next tile is there, and this one's slot has been read by every wave
     }
 
     // lane: row r, columns 8 e + 4 grp + 0..3 of each TS x TS tile
