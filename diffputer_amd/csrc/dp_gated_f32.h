@@ -134,20 +134,31 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
         GL_SYNC(0);                                              // the next tile is there, and this one's slot has been read by every wave
     }
 
-    // lane: row r, columns 8 e + 4 grp + 0..3 of each TS x TS tile
+    // A lane holds row r, columns 8 e + 4 grp + 0..3 of each TS x TS tile: 32 bytes of a row side by side.  The tiles go through the wave's
+    // own part of LDS and leave by whole rows of 4 TS bytes.
+    constexpr int ROWB = TS * 4 + 16, LPR = TS / 4, RP = 64 / LPR;         // bytes of a row there; lanes of a row; rows at a time
+    static_assert(4 * 2 * TS * ROWB <= S::LDS, "the tiles of all waves fit");
+    char* const mine = smem + wave * 2 * TS * ROWB;
     float* const out = (float*)p.out[MODE == GL_DW ? plane : 0];
+    const int cl = wn * TS + lane % LPR * 4;
+    f32x4 bg, bu;
+    if (MODE == GL_FWD && !split && j0 + cl < p.J) gl_bias<float>(p, j0 + cl, p.J - j0 - cl, bg, bu);
 #pragma unroll
-    for (int e = 0; e < TS * TS / 256; ++e) {
-        const int cl = wn * TS + 8 * e + 4 * grp;
-        f32x4 bg, bu;
-        if (MODE == GL_FWD && !split && j0 + cl < p.J) gl_bias<float>(p, j0 + cl, p.J - j0 - cl, bg, bu);
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t m = i0 + wm * (T / 2) + i * TS + r;
-            if (m >= p.I) continue;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < TS * TS / 256; ++e)
+                *(f32x4*)(mine + (h * TS + r) * ROWB + (8 * e + 4 * grp) * 4) = (f32x4){acc[i][h][4 * e], acc[i][h][4 * e + 1], acc[i][h][4 * e + 2], acc[i][h][4 * e + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+        for (int k = 0; k < TS / RP; ++k) {
+            const int row = k * RP + lane / LPR;
+            const int64_t m = i0 + wm * (T / 2) + i * TS + row;
             f32x4 v[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) v[h] = (f32x4){acc[i][h][4 * e], acc[i][h][4 * e + 1], acc[i][h][4 * e + 2], acc[i][h][4 * e + 3]};
+            for (int h = 0; h < 2; ++h) v[h] = *(const f32x4*)(mine + (h * TS + row) * ROWB + lane % LPR * 16);
+            if (m >= p.I) continue;
             if (MODE == GL_FWD && !split) {
                 if (j0 + cl < p.J)
                     gl_with_act(p.act, [&](auto act) { gl_fwd_put<float, decltype(act)::value>(p, m, j0 + cl, p.J - j0 - cl, v[0] + bg, v[1] + bu); });
@@ -161,6 +172,7 @@ __device__ __forceinline__ void gf_product(const GtArgs& q, int b, int count, ch
                 else gl_put4(out + m * p.ldo + n, v[h], p.J - n);
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
 
