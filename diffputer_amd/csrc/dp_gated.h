@@ -154,7 +154,9 @@ template <typename T> __device__ __forceinline__ void gl_bias(const GlArgs& p, i
 // The projections g and u as the forward pass leaves them for the backward pass, by groups of 4 columns (G = N / 4 rounded up):
 //   float32   g[4], u[4]: two planes [M][G] of 16 bytes
 //   bf16      20 bits of each (sign, exponent, 11 bits of the fraction; rounded, half away from zero): a plane [M][G] of 16 bytes with the
-//             upper 16 bits of g[4] and u[4], and a plane [M][G] of 4 bytes with the next 4 bits of each.
+//             upper 16 bits of g[4] and u[4], and a plane [M][G] of 4 bytes with the next 4 bits of each, whole blocks of 8 groups
+//             in the order 0 4 1 5 2 6 3 7: a lane of the tile kernels has groups q and q + 4 and stores both at once (with 16 bytes
+//             per row and store the forward product of 4096 x 1024 x 2048 wrote 69 MB to memory, for 59 of results).
 // Half a step of 20 bits is 2^-12: dg = dh u act'(g) is off by a sixteenth of the rounding to bf16 that it gets as an operand
 // anyway, and neither range nor inf and NaN are lost, as they would be in 16 bits of either kind.  Against float32 planes the
 // forward pass writes and the backward pass reads 20 instead of 32 bytes per group.
@@ -174,26 +176,44 @@ template <> struct GlPre<float> {
 };
 template <> struct GlPre<bf16_t> {
     static __host__ __device__ int64_t bytes(int64_t M, int64_t G) { return M * G * 20; }
-    static __device__ __forceinline__ void put(void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4 g, f32x4 u) {
+    static __device__ __forceinline__ uint32_t* low(const void* pre, int64_t M, int64_t G, int64_t m, int g) {
+        const int block = g & ~7;
+        return (uint32_t*)((char*)pre + M * G * 16) + m * G + (block + 8 <= G ? block | (g & 3) << 1 | (g >> 2 & 1) : g);
+    }
+    // stores the upper bits, returns the next ones
+    static __device__ __forceinline__ uint32_t put_high(void* pre, int64_t G, int64_t m, int n, f32x4 g, f32x4 u) {
         uint32_t b[8], low = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             b[e] = __builtin_bit_cast(uint32_t, e < 4 ? g[e] : u[e - 4]) + 0x800u;             // carries into the exponent as a rounding does
             low |= ((b[e] >> 12) & 15u) << (4 * e);
         }
-        const int64_t at = m * G + (n >> 2);
         uint4 hi;
         hi.x = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
         hi.y = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
         hi.z = __builtin_amdgcn_perm(b[5], b[4], 0x07060302u);
         hi.w = __builtin_amdgcn_perm(b[7], b[6], 0x07060302u);
-        ((uint4*)pre)[at] = hi;
-        ((uint32_t*)((char*)pre + M * G * 16))[at] = low;
+        ((uint4*)pre)[m * G + (n >> 2)] = hi;
+        return low;
+    }
+    static __device__ __forceinline__ void put(void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4 g, f32x4 u) {
+        *low(pre, M, G, m, n >> 2) = put_high(pre, G, m, n, g, u);
+    }
+    // columns n .. and n + 16 .., n in the first half of a block of 32
+    static __device__ __forceinline__ void put2(void* pre, int64_t M, int64_t G, int64_t m, int n, const f32x4 (&g)[2], const f32x4 (&u)[2]) {
+        const uint32_t l[2] = {put_high(pre, G, m, n, g[0], u[0]), put_high(pre, G, m, n + 16, g[1], u[1])};
+        const int first = n >> 2;
+        uint32_t* const at = low(pre, M, G, m, first);
+        if ((first & ~7) + 8 <= G) __builtin_memcpy(at, l, 8);
+        else {
+            at[0] = l[0];
+            at[4] = l[1];
+        }
     }
     static __device__ __forceinline__ void get(const void* pre, int64_t M, int64_t G, int64_t m, int n, f32x4& g, f32x4& u) {
         const int64_t at = m * G + (n >> 2);
         const uint4 hi = ((const uint4*)pre)[at];
-        const uint32_t low = ((const uint32_t*)((const char*)pre + M * G * 16))[at];
+        const uint32_t low = *GlPre::low(pre, M, G, m, n >> 2);
         const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -211,6 +231,21 @@ template <typename T, int ACT> __device__ __forceinline__ void gl_fwd_put(const 
     for (int r = 0; r < 4; ++r) v[r] = gl_act<T, ACT>(g[r]) * u[r];
     T* const h = (T*)p.out[0];
     gl_put4(h + m * p.ldo + n, v, cnt);
+}
+// the same of columns n .. and n + 16 .. (bf16 tile kernels), n < J in the first half of a block of 32
+template <int ACT> __device__ __forceinline__ void gl_fwd_put2(const GlArgs& p, int64_t m, int n, const f32x4 (&g)[2], const f32x4 (&u)[2]) {
+    const bool both = n + 16 < p.J;
+    if (p.pre) {
+        if (both) GlPre<bf16_t>::put2(p.pre, p.I, (p.J + 3) >> 2, m, n, g, u);
+        else GlPre<bf16_t>::put(p.pre, p.I, (p.J + 3) >> 2, m, n, g[0], u[0]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = gl_act<bf16_t, ACT>(g[j][r]) * u[j][r];
+        if (j == 0 || both) gl_put4((bf16_t*)p.out[0] + m * p.ldo + n + 16 * j, v, p.J - n - 16 * j);
+    }
 }
 template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs& p, int64_t m, int n, int cnt, f32x4 g, f32x4 u) {
     f32x4 bg, bu;

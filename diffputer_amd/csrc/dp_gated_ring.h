@@ -204,18 +204,17 @@ __device__ __forceinline__ void gs_product(const GtArgs& q, int b, int count, ch
                 }
         }
     } else if constexpr (MODE == GL_FWD) {
-        gl_with_act(p.act, [&](auto act) {
+        static_assert(NJ == 2, "two tiles side by side");
+        const int n = j0 + cl;
+        if (n < p.J) gl_with_act(p.act, [&](auto act) {
+            f32x4 bg[2], bu[2];
+            gl_bias<bf16_t>(p, n, p.J - n, bg[0], bu[0]);
+            gl_bias<bf16_t>(p, n + 16, p.J - n - 16, bg[1], bu[1]);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int n = j0 + cl + j * 16, cnt = p.J - n;
-                if (cnt <= 0) continue;
-                f32x4 bg, bu;
-                gl_bias<bf16_t>(p, n, cnt, bg, bu);
-#pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    const int64_t m = mrow + i * 16;
-                    if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[i][j] + bg, acc[i][NJ + j] + bu);
-                }
+            for (int i = 0; i < MI; ++i) {
+                const int64_t m = mrow + i * 16;
+                const f32x4 g[2] = {acc[i][0] + bg[0], acc[i][1] + bg[1]}, u[2] = {acc[i][NJ] + bu[0], acc[i][NJ + 1] + bu[1]};
+                if (m < p.I) gl_fwd_put2<decltype(act)::value>(p, m, n, g, u);
             }
         });
     } else {

@@ -242,21 +242,20 @@ __device__ __forceinline__ int gt_product(const GtArgs& q, int b, int step, char
                         }
                 }
         } else if constexpr (MODE == GL_FWD) {
-            gl_with_act(p.act, [&](auto act) {
+            static_assert(NJ == 2, "two tiles side by side");
+            const int n = cur.j0 + cl;
+            if (n < p.J) gl_with_act(p.act, [&](auto act) {
+                f32x4 bg[2], bu[2];
+                gl_bias<bf16_t>(p, n, p.J - n, bg[0], bu[0]);
+                gl_bias<bf16_t>(p, n + 16, p.J - n - 16, bg[1], bu[1]);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int n = cur.j0 + cl + j * 16, cnt = p.J - n;
-                    if (cnt <= 0) continue;
-                    f32x4 bg, bu;
-                    gl_bias<bf16_t>(p, n, cnt, bg, bu);
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int i = 0; i < MI; ++i) {
-                            const int64_t m = mrow + a * HR + i * 16;
-                            if (m < p.I) gl_fwd_put<bf16_t, decltype(act)::value>(p, m, n, cnt, acc[a][i][0][j] + bg, acc[a][i][1][j] + bu);
-                        }
-                }
+                    for (int i = 0; i < MI; ++i) {
+                        const int64_t m = mrow + a * HR + i * 16;
+                        const f32x4 g[2] = {acc[a][i][0][0] + bg[0], acc[a][i][0][1] + bg[1]}, u[2] = {acc[a][i][1][0] + bu[0], acc[a][i][1][1] + bu[1]};
+                        if (m < p.I) gl_fwd_put2<decltype(act)::value>(p, m, n, g, u);
+                    }
             });
         } else {
             bf16_t* const out = (bf16_t*)p.out[MODE == GL_DW ? cur.plane : 0];
