@@ -9,7 +9,8 @@
 // bytes a lane where rows start on 16 bytes, else 4: element-wise loads are four times the instructions and still fit under
 // the products.
 //   Measured: T = 128 takes 3.8 us for a K-tile of two workgroups on every CU, 141 TFLOP/s of the pipe's 157 (a library product of
-//   4096^3: 140, 8192^3: 153); both backward products of 8192 x 1024 x 4096 2.0 ms (136 TFLOP/s), of 4096 x 1024 x 2048 0.49 to 0.56 ms.
+//   4096^3: 140, 8192^3: 153); both backward products of 8192 x 1024 x 4096 2.0 ms (136 TFLOP/s), of 4096 x 1024 x 2048 0.49 to
+//   0.56 ms.  Results leave through LDS by whole rows: stores of 32 bytes a row wrote 212 MB to memory for 101 MB of results.
 //   With G = 64 / (T / 4) lane groups of T / 4 lanes, a lane reads four k's of its row or column, the group's 4 (G g + group) ..
 //   + 3: step s of the four multiplies the G k's 4 (G g + group) + s (both operands agree on that, and a sum over k does not
 //   ask for more).

@@ -22,7 +22,7 @@
 //   * Bound by the matrix pipes, and on a full chip by the power that they may draw: a K-tile takes 1.07 us with 64 workgroups
 //     and 1.36 with 256, 0.85 being the pipes' own time at 2.4 GHz.  256 tiles of K = 4096 take 98 us (1 403 TFLOP/s; a
 //     library product of 8192^3 reaches 1 404), both backward products of 16384 x 4096 x 8192 3.1 ms (1 420 TFLOP/s), the
-//     forward product there 1.8 ms (1 220) with h and the projections for the backward pass, 0.94 GB, written beside it.
+//     forward product there 1.75 ms (1 260) with h and the projections for the backward pass, 0.94 GB, written beside it.
 //   * Why 128 x 64 per wave: 24 fragments are read from LDS for 64 matrix instructions, three quarters of what LDS delivers
 //     meanwhile (64 x 64 per wave: all of it).  128 x 128 per wave (4 waves, accumulators in AGPRs) has the same K-loop and
 //     takes 16.5 us beyond it instead of 11.
