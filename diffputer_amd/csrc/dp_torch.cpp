@@ -12,6 +12,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/util/Exception.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -77,6 +78,23 @@ Tensor forward_of(const Tensor& x, const Tensor& wg, const Tensor& wu, const Ten
     return h;
 }
 
+// A leaf's accumulation node belongs to the stream on which its first graph was made, and lives as long as any graph of the leaf.  A
+// backward pass under capture whose gradients go on to a node of another stream would have that stream wait, which is no part of
+// the capture, and end the process: whether one of the node's gradients goes to such a node.
+bool goes_elsewhere(const torch::autograd::Node& node, c10::DeviceIndex device) {
+    const auto here = c10::hip::getCurrentHIPStream(device).id();
+    for (const auto& edge : node.next_edges()) {
+        if (!edge.function) continue;
+        const auto stream = edge.function->stream();
+        if (stream && stream->id() != here) return true;
+    }
+    return false;
+}
+bool capturing(const Tensor& t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing((hipStream_t)stream_of(t), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+
 struct GatedLinear : public torch::autograd::Function<GatedLinear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::optional<Tensor>& b_gate,
                           const std::optional<Tensor>& b_up, int64_t act) {
@@ -93,6 +111,9 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const int64_t act = ctx->saved_data["act"].toInt(), biases = ctx->saved_data["biases"].toInt();
+        const auto node = torch::autograd::get_current_node();
+        if (node && capturing(saved[0]) && goes_elsewhere(*node, saved[0].device().index()))
+            throw LibraryError("gated_linear: this backward pass is captured while a graph of its inputs that was made on another stream is alive; drop that graph before the capture");
         const Tensor x = rows_of(saved[0]), &pre = saved[3];
         Tensor wg = saved[1], wu = saved[2];
         weights_of(wg, wu);
@@ -253,7 +274,16 @@ PyObject* py_set_errors(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+PyObject* py_goes_elsewhere(PyObject*, PyObject* o) {
+    return guarded([&]() -> PyObject* {
+        Tensor t;
+        if (!tensor_arg(o, t) || !t.defined() || !t.grad_fn()) Py_RETURN_NONE;
+        return PyBool_FromLong(goes_elsewhere(*t.grad_fn(), t.device().index()));
+    });
+}
+
 PyMethodDef g_methods[] = {
+    {"goes_elsewhere", py_goes_elsewhere, METH_O, "whether a gradient of the node that made a tensor goes to a node of another stream than the current one"},
     {"gated_linear", (PyCFunction)(void (*)(void))py_gated_linear, METH_FASTCALL, "gated_linear(x, w_gate, w_up, b_gate, b_up, act)"},
     {"grads", (PyCFunction)(void (*)(void))py_grads, METH_FASTCALL, "grads(tensors, norm_type, limit)"},
     {"set_errors", (PyCFunction)(void (*)(void))py_set_errors, METH_FASTCALL, "classes of the library's errors and of the allocator's"},

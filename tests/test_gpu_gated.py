@@ -529,6 +529,62 @@ def test_captured_and_replayed(dtype, M):
             assert all(torch.equal(a, b) for a, b in zip(want, out)), it
 
 
+def test_graphs_of_two_streams_are_seen():
+    """A leaf's accumulation node stays with the stream of its first graph as long as a graph of the leaf lives."""
+    from diffputer_amd import _lib
+    from diffputer_amd.gated import gated_linear
+    elsewhere = _lib.torch_side().goes_elsewhere
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(70, 96, 72, "bf16", seed=51)]
+    leaves = [t.requires_grad_() for t in (wg, wu, bg, bu)]
+    h = gated_linear(x, *leaves)
+    assert elsewhere(h) is False
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        k = gated_linear(x, *leaves)
+        assert elsewhere(k) is True
+        del k
+        other = gated_linear(x.detach().requires_grad_(), *[t.detach().requires_grad_() for t in leaves])
+        assert elsewhere(other) is False
+    torch.cuda.current_stream().wait_stream(s)
+    del h
+    with torch.cuda.stream(s):
+        k = gated_linear(x, *leaves)
+        assert elsewhere(k) is False
+    torch.cuda.synchronize()
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """A backward pass is not captured while an eager graph of the same leaves lives; the process goes on, and without that
+    graph the capture works, with .backward() too."""
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(70, 96, 72, "bf16", seed=52)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    eager = gated_linear(*leaves)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="drop that graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+    want = [g.clone() for g in torch.autograd.grad(eager, leaves, dh)]
+    del eager
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        gated_linear(*leaves).backward(dh)
+    torch.cuda.current_stream().wait_stream(s)
+    for t in leaves:
+        t.grad.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gated_linear(*leaves).backward(dh)
+    for _ in range(3):
+        for t in leaves:
+            t.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
 def test_module_and_denoiser_training_step():
     """A denoiser of gated layers inside model.Model: loss, gradients, clipping and Adam's step on the GPU against the same
     modules on the CPU in float64 (the draws replayed)."""
