@@ -179,6 +179,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!x.defined() || !w[0].defined() || !w[1].defined() || !x.is_cuda() || code_of(x) < 0 || x.dim() < 1 || w[0].dim() != 2 || w[1].sizes() != w[0].sizes()) Py_RETURN_NONE;
         const int64_t N = w[0].size(0), K = w[0].size(1);
         if (N < 1 || K < 1 || x.size(-1) != K) Py_RETURN_NONE;
+        if (N > 1 << 20 || K > 1 << 20) throw LibraryError("gated_linear: N = " + std::to_string(N) + ", K = " + std::to_string(K) + ": both are limited to 2^20");
         bool grad = x.requires_grad();
         for (const Tensor* t : {&w[0], &w[1], &b[0], &b[1]}) {
             if (!t->defined()) continue;

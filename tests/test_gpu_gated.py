@@ -529,6 +529,17 @@ def test_captured_and_replayed(dtype, M):
             assert all(torch.equal(a, b) for a, b in zip(want, out)), it
 
 
+@pytest.mark.parametrize("N,K", [((1 << 20) + 1, 1), ((1 << 32) + 5, 1), (1, (1 << 20) + 8), (3, (1 << 32) + 7)])
+def test_too_wide_is_refused(N, K):
+    """Sizes that the C ABI does not take, beyond 32 bits among them (nothing is allocated: expanded tensors)."""
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.gated import gated_linear
+    one = torch.ones(1, 1, dtype=torch.bfloat16, device=DEV)
+    for grad in (False, True):
+        with pytest.raises(DiffputerError, match="2\\^20"):
+            gated_linear(one.expand(2, K).detach().requires_grad_(grad), one.expand(N, K), one.expand(N, K))
+
+
 def test_graphs_of_two_streams_are_seen():
     """A leaf's accumulation node stays with the stream of its first graph as long as a graph of the leaf lives."""
     from diffputer_amd import _lib
