@@ -153,9 +153,19 @@ static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
 }
 static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < (int64_t)1 << 22; }
 
+// The kernel for few rows reads x once per workgroup: with many rows that takes longer than the weights do, and a tile kernel,
+// which pads the rows, is faster (us, few-row kernel / tile kernel).  bf16: 4096 x 8192 (K x N) at 24 rows 34 / 34, 32 rows
+// 38 to 41 / 37, 64 rows 51 / 38; 1024 x 8192 at 32 rows 10.1 / 10.6, 33 rows 11.3 / 10.9, 64 rows 14.1 / 11.5; 1024 x 4096 at 64 rows
+// 8.5 / 11.1.  float32: 4096 x 8192 at 32 rows 79 / 84, 33 rows 98 / 82, 64 rows 126 / 90; 2048 x 2048 at 64 rows
+// 21.7 / 19.0; 512 x 1024 at 64 rows 7.5 / 11.0.
+static int gr_columns(int J) { return J >= 16 * 256 ? 16 : 8; }                          // columns of a workgroup: narrow layers take twice as many workgroups
+static bool gr_slower(const GlShape& s, int dtype) {
+    if (dtype == DP_DTYPE_F32) return s.I > 32 && (int64_t)s.J * s.C >= (int64_t)1 << 21;
+    return s.I > 32 ? (int64_t)s.J * s.C >= (int64_t)1 << 23 : s.I > 16 && s.I * s.C * 2 * ceil_div(s.J, gr_columns(s.J)) >= (int64_t)1 << 27;
+}
 static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
     const int forced = forced_kernel();
-    if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0) return {GL_ROWS, 0, 1, 1, 1, 1};
+    if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0 && !(tile && gr_slower(s, dtype))) return {GL_ROWS, 0, 1, 1, 1, 1};
     if (tile && forced != 1) {
         GlPlan pl;
         gl_choose(&s, 1, dtype, &pl);
@@ -249,7 +259,7 @@ static int gr_launch(const GlArgs& a, hipStream_t st) {
 }
 template <typename T>
 static int gr_rows(const GlArgs& a, hipStream_t st) {
-    const bool wide = a.J >= 16 * 256;                            // narrower: 8 columns per workgroup, twice as many workgroups
+    const bool wide = gr_columns(a.J) == 16;
     if (a.I <= 16) return wide ? gr_launch<T, 1, 16>(a, st) : gr_launch<T, 1, 8>(a, st);
     if (a.I <= 32) return wide ? gr_launch<T, 2, 16>(a, st) : gr_launch<T, 2, 8>(a, st);
     return wide ? gr_launch<T, 4, 16>(a, st) : gr_launch<T, 4, 8>(a, st);
@@ -380,7 +390,8 @@ static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
     // the float32 forward product (both operands row laid out) loses 5 to 10 % to 4-byte loads, less than copies take
     if (dtype == DP_DTYPE_F32 && in.o.short_rows && (in.o.pack_x || in.o.pack_w)) in.o.pack_x = in.o.pack_w = in.o.vec = false;
     w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1};
-    w.plan = gl_plan(w.s, dtype, in.o.tile);
+    // few rows: copies of the weights would cost more than a tile kernel gains
+    w.plan = gl_plan(w.s, dtype, in.o.tile && !(in.M <= GR_MAX_ROWS && (in.o.pack_x || in.o.pack_w)));
     if (w.plan.T == GL_ROWS) {                                    // reads rows of any alignment
         in.o.pack_x = in.o.pack_w = false;
         w.s.C = in.K;

@@ -677,3 +677,10 @@ def test_every_bf16_gate(kernel, act, tune):
     close(h, a, (e + step) * 1.01 * a.abs() + tail, "h")
     eda = e * (1 + g.to(F8).abs() * (1 - torch.sigmoid(g.to(F8)).clamp(max=1))) * torch.sigmoid(g.to(F8)) if act == "silu" else e * (0.5 * torch.erfc(-g.to(F8) / math.sqrt(2)) + g.to(F8).abs() * torch.exp(-g.to(F8) ** 2 / 2))
     close(dx, da, (eda + 2 * step * da.abs()) * 1.02 + tail, "dx")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(32, 4096, 8192), (33, 2048, 4104), (40, 1024, 8200), (64, 4096, 2056), (47, 2056, 4097), (64, 1032, 2100), (33, 1027, 2048)])
+def test_some_rows_of_large_layers(M, K, N, dtype):
+    """Where the kernel for few rows and the tile kernels take turns."""
+    check(*make(M, K, N, dtype, seed=M + N), act="silu", train=M != 32)
