@@ -93,12 +93,12 @@ static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
 // 64 K-tiles: a K-step of `depth` takes `one` where a workgroup has its CU to itself and `full` where the CU holds `per_cu` of
 // them; `fixed` is what a launch takes beyond its K-steps, `round` what every further round of workgroups adds to that (`full_fwd`,
 // `round_fwd`: the forward product, whose operands are both row laid out and whose results are activated).  A split launch pays for
-// its partial sums, written and read at about 4.5 TB/s (forward 10 and 0.7 us per slice: most of them are still in the caches),
+// its partial sums, written and read at about 4.5 TB/s (forward 10 and `slice` for each slice: most of them are still in the caches),
 // and a launch more.  Over 180 sizes drawn at random (70 to 16384 rows, K 64 to 4096, N 64 to 8192, both types) the choice is on
 // average as fast as the best single tile with 1 to 8 slices for everything, at worst 16 % (forward) and 7 % (backward) behind it.
-struct GlRate { int T, depth, per_cu; double one, full, full_fwd, fixed, round, round_fwd; };
-static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.36, 1.36, 1.36, 11.0, 5.0, 5.0}, {128, 32, 2, 0.28, 0.50, 0.68, 5.5, 1.0, 2.5}};
-static const GlRate GL_RATES_F32[] = {{128, GF_K, 2, 2.10, 3.80, 3.80, 9.0, 4.0, 4.0}, {64, GF_K, 4, 0.70, 2.05, 2.05, 4.0, 1.0, 1.0}};
+struct GlRate { int T, depth, per_cu; double one, full, full_fwd, fixed, round, round_fwd, slice; };
+static const GlRate GL_RATES_BF16[] = {{256, 64, 1, 1.36, 1.36, 1.36, 11.0, 5.0, 5.0, 0.7}, {128, 32, 2, 0.28, 0.50, 0.68, 5.5, 1.0, 2.5, 0.7}};
+static const GlRate GL_RATES_F32[] = {{128, GF_K, 2, 2.10, 3.80, 3.80, 9.0, 4.0, 4.0, 0.3}, {64, GF_K, 4, 0.70, 2.05, 2.05, 4.0, 1.0, 1.0, 0.3}};
 // (by the fullest CU: 315 workgroups of the float32 tile of 64, 2190 x 1235 x 279, take 58.0 us; in three slices 46.0)
 static double gl_step(const GlRate& r, double full, double wgs) {
     const double here = std::min(ceil(wgs / 256.0), (double)r.per_cu);
@@ -113,7 +113,7 @@ static double gl_cost(const GlRate& r, const GlPlan* pl, const GlShape* s, int n
         if (pl[i].kt_per > pl[longer].kt_per) longer = i;
         if (pl[i].splits > 1) {
             const double bytes = (double)s[i].I * s[i].J * (s[i].mode == GL_DX ? 1 : 2) * 4 * 2 * pl[i].splits;
-            join = std::max(join, 5.0) + (s[i].mode == GL_FWD ? 0.7 * pl[i].splits + bytes / 10e6 : bytes / 4.5e6);
+            join = std::max(join, 5.0) + (s[i].mode == GL_FWD ? r.slice * pl[i].splits + bytes / 10e6 : bytes / 4.5e6);
         }
     }
     const double full = s[0].mode == GL_FWD ? r.full_fwd : r.full, slots = 256.0 * r.per_cu, most = pl[longer].kt_per, least = n > 1 ? pl[1 - longer].kt_per : most;
