@@ -401,7 +401,7 @@ static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
     if (dtype == DP_DTYPE_F32 && in.o.short_rows && (in.o.pack_x || in.o.pack_w)) in.o.pack_x = in.o.pack_w = in.o.vec = false;
     w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1};
     // few rows: copies of the weights would cost more than a tile kernel gains
-    w.plan = gl_plan(w.s, dtype, in.o.tile && !(in.M <= GR_MAX_ROWS && (in.o.pack_x || in.o.pack_w)));
+    w.plan = gl_plan(w.s, dtype, in.o.tile && !(in.M <= GR_MAX_ROWS && (in.o.pack_x || in.o.pack_w) && forced_kernel() == 0));
     if (w.plan.T == GL_ROWS) {                                    // reads rows of any alignment
         in.o.pack_x = in.o.pack_w = false;
         w.s.C = in.K;
