@@ -50,6 +50,7 @@ SIGNATURES = {
     "dp_mstep_fwd_bwd": (_i, [_i, _i, _i64, _vp, _vp, _vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), _vp, _vp, _vp, _sz, _vp]),
     "dp_gated_linear_pre_bytes": (_sz, [_i, _i64, _i]),
     "dp_gated_linear_workspace_bytes": (_sz, [_i, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _i]),
+    "dp_gated_linear_plan": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _i64, _i, _i, _i, C.POINTER(_i)]),
     "dp_gated_linear": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "dp_gated_linear_bwd": (_i, [_i, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _vp, _sz, _vp]),
     "dp_grad_workspace_bytes": (_sz, [_i]),

@@ -127,8 +127,12 @@ static double gl_cost(const GlRate& r, const GlPlan* pl, const GlShape* s, int n
     return r.fixed + (s[0].mode == GL_FWD ? r.round_fwd : r.round) * std::max(0.0, ceil(wgs / slots) - 1.0) + t + join;
 }
 
-// The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass).
-static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
+// A grid has fewer than 2^32 threads; the kernel of 256 tiles launches a workgroup per CU, which walk on by an int.
+static int64_t gl_most(int T) { return T == 256 ? (int64_t)1 << 30 : (int64_t)1 << 22; }
+static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < gl_most(pl.T); }
+
+// The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass); false if no tile's grid fits.
+static bool gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
     const bool bf = dtype == DP_DTYPE_BF16;
     const int forced = forced_kernel();
     static const int slices[] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
@@ -153,6 +157,7 @@ static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
                 fits = fits && (pl[i].splits == 1 || gl_part_bytes(s[i]) * pl[i].splits <= (size_t)128 << 20);
             }
             if (!fits && a > 1) continue;
+            if (!gl_grid_ok(pl[0]) || (n > 1 && (!gl_grid_ok(pl[1]) || pl[0].wgs + pl[1].wgs >= gl_most(r.T)))) continue;
             const double c = gl_cost(r, pl, s, n);
             if (c < least) {
                 least = c;
@@ -160,8 +165,8 @@ static void gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
             }
         }
     }
+    return least < 1e300;
 }
-static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < (int64_t)1 << 22; }
 
 // The kernel for few rows reads x once per workgroup: with many rows that takes longer than the weights do, and a tile kernel,
 // which pads the rows, is faster (us, few-row kernel / tile kernel).  bf16: 4096 x 8192 (K x N) at 24 rows 34 / 34, 32 rows
@@ -178,8 +183,7 @@ static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
     if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0 && !(tile && gr_slower(s, dtype))) return {GL_ROWS, 0, 1, 1, 1, 1};
     if (tile && forced != 1) {
         GlPlan pl;
-        gl_choose(&s, 1, dtype, &pl);
-        if (gl_grid_ok(pl)) return pl;
+        if (gl_choose(&s, 1, dtype, &pl)) return pl;
     }
     // general kernel: slices until there are about two workgroups per CU, as long as a slice keeps 8 K-tiles
     const int64_t nk = ceil_div<int64_t>(s.C, GG_K) * (s.mode == GL_DX ? 2 : 1), tiles = gl_shape(s, 0, GG_K, 1).wgs;
@@ -189,10 +193,7 @@ static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
 // both backward products, in one launch if they take kernels of one kind and fit a grid
 static GlPlan gl_plan(const GlShape& s, int dtype, bool tile);
 static bool gl_plan_both_new(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
-    if (tile && forced_kernel() != 1) {
-        gl_choose(s, 2, dtype, pl);
-        if (gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]) && pl[0].wgs + pl[1].wgs < (int64_t)1 << 22) return true;
-    }
+    if (tile && forced_kernel() != 1 && gl_choose(s, 2, dtype, pl)) return true;
     for (int i = 0; i < 2; ++i) pl[i] = gl_plan(s[i], dtype, tile);
     return pl[0].T == 0 && pl[1].T == 0 && gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]);
 }
@@ -431,6 +432,17 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     GlBwd w;
     // small layers take the general kernel, whose dg and du are not rounded: with few of them their roundings do not average out
     if (dtype == DP_DTYPE_BF16 && M * N < GL_EXACT_BELOW && forced_kernel() == 0) in.o.tile = in.o.pack_x = in.o.pack_w = false;
+    w.s[0] = {GL_DX, M, K, N, 1};
+    w.s[1] = {GL_DW, N, K, M, planes ? planes : 2};
+    for (;;) {
+        w.both = false;
+        if (want_dx && planes == 2) w.both = gl_plan_both(w.s, dtype, in.o.tile, w.plan);
+        else for (int i = 0; i < 2; ++i) w.plan[i] = gl_plan(w.s[i], dtype, in.o.tile);
+        // The general kernel reads planes of float32, a bf16 tile kernel planes of bf16: where a product that is asked for has no tile
+        // whose grid fits, the call takes the general kernel for all of them.
+        if (dtype == DP_DTYPE_F32 || !in.o.tile || ((!want_dx || w.plan[0].T) && (!planes || w.plan[1].T))) break;
+        in.o.tile = in.o.pack_x = in.o.pack_w = false;
+    }
     w.plane = in.o.tile ? dtype : DP_DTYPE_F32;
     Carver c = {(char*)base};
     in.carve(c);
@@ -444,11 +456,6 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     w.nblk = (int)ceil_div<int64_t>(std::max<int64_t>(M, 1), w.rows);
     w.dgu = c.take((size_t)2 * M * w.ldg * (w.plane == DP_DTYPE_BF16 ? 2 : 4));
     w.colpart = (float*)c.take(w.nblk > 1 ? (size_t)w.nblk * 2 * w.ldg * 4 : 0);
-    w.s[0] = {GL_DX, M, K, N, 1};
-    w.s[1] = {GL_DW, N, K, M, planes ? planes : 2};
-    w.both = false;
-    if (want_dx && planes == 2) w.both = gl_plan_both(w.s, dtype, in.o.tile, w.plan);
-    else for (int i = 0; i < 2; ++i) w.plan[i] = gl_plan(w.s[i], dtype, in.o.tile);
     for (int i = 0; i < 2; ++i) w.part[i] = (float*)c.take((i ? planes > 0 : want_dx) ? gl_split_bytes(w.s[i], w.plan[i]) : 0);
     w.bytes = c.off;
     return w;
@@ -597,6 +604,28 @@ size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, co
     GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
     if (grads == DP_GATED_FORWARD) return std::max<size_t>(gl_fwd_carve(dtype, in, nullptr).bytes, 256);
     return std::max<size_t>(gl_bwd_carve(dtype, in, ((grads & DP_GATED_DW_GATE) != 0) + ((grads & DP_GATED_DW_UP) != 0), (grads & DP_GATED_DX) != 0, nullptr).bytes, 256);
+}
+
+int dp_gated_linear_plan(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, int64_t M, int N, int K, int grads, int kernel[3]) {
+    const int rc = gl_check("dp_gated_linear_plan", dtype, M, N, K, 0);
+    if (rc) return rc;
+    if (grads < 0 || grads > 15) return fail(DP_EINVAL, "dp_gated_linear_plan: grads %d", grads);
+    if (!kernel) return fail(DP_EINVAL, "dp_gated_linear_plan: null pointer");
+    kernel[0] = kernel[1] = kernel[2] = -1;
+    if (M == 0) return DP_OK;
+    auto name = [](int T) { return T == 0 ? 1 : T == GL_ROWS ? 2 : T; };
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
+    if (grads == DP_GATED_FORWARD) {
+        kernel[0] = name(gl_fwd_carve(dtype, in, nullptr).plan.T);
+        return DP_OK;
+    }
+    const int planes = ((grads & DP_GATED_DW_GATE) != 0) + ((grads & DP_GATED_DW_UP) != 0);
+    const bool dx = (grads & DP_GATED_DX) != 0;
+    const GlBwd w = gl_bwd_carve(dtype, in, planes, dx, nullptr);
+    if (dx) kernel[0] = name(w.plan[0].T);
+    if (planes) kernel[1] = name(w.plan[1].T);
+    kernel[2] = w.plane;
+    return DP_OK;
 }
 
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,

@@ -305,6 +305,12 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
 size_t dp_gated_linear_pre_bytes(int dtype, int64_t M, int N);
 size_t dp_gated_linear_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw,
                                        int64_t M, int N, int K, int grads);
+/* How a call with these arguments runs under the current dp_tune settings (the library's own choice, without a GPU; for profiles and
+ * tests): kernel[0] = the forward product's kernel, or with grads != DP_GATED_FORWARD kernel[0] = dx's, kernel[1] = the weight gradients',
+ * kernel[2] = the type (DP_DTYPE_..) of dg and du between them.  1 = general kernel, 2 = kernel for few rows, 64 / 128 / 256 = tile
+ * kernel, -1 = nothing to run. */
+int dp_gated_linear_plan(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw,
+                         int64_t M, int N, int K, int grads, int kernel[3]);
 int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* b_gate, const void* b_up,
                     void* h, int64_t ldh, void* pre, int64_t M, int N, int K, int act, void* workspace, size_t workspace_bytes, void* stream);
 int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,

@@ -131,6 +131,60 @@ def test_gated_sizes():
     assert lib.dp_gated_linear_pre_bytes(0, 1 << 20, 4096) == 2 * (1 << 20) * 4096 * 4
 
 
+@pytest.fixture
+def tune():
+    lib = _lib.load()
+
+    def put(kernel, splits=0):
+        _lib.check(lib.dp_tune(b"gated_kernel", kernel), "dp_tune")
+        _lib.check(lib.dp_tune(b"gated_splits", splits), "dp_tune")
+
+    yield put
+    put(0)
+
+
+def _plan(dtype, M, N, K, grads, at=FAKE):
+    k = (C.c_int * 3)()
+    assert _lib.load().dp_gated_linear_plan(dtype, at, K, at, at, K, M, N, K, grads, k) == 0, _err(_lib.load())
+    return list(k)
+
+
+DX, DWG, DWU, DB = 1, 2, 4, 8
+
+
+@pytest.mark.parametrize("kernel", [0, 1, 128, 256])
+@pytest.mark.parametrize("M,N,K", [(1 << 28, 8, 136), ((1 << 29) - 1, 8, 8), (1 << 28, 136, 8), ((1 << 29) - 1, 8, 200), ((1 << 29) - 1, 1 << 20, 1 << 20), (1 << 20, 1 << 18, 1 << 18),
+                                   (4096, 2048, 1024), (1537, 1203, 777), (100, 64, 9), (1, 8, 8)])
+def test_planes_are_of_the_type_that_their_reader_takes(tune, kernel, M, N, K):
+    """The general kernel (1) reads dg and du as float32, the tile kernels in the layer's own type: also where a tile kernel's grid
+    would not fit (2^22 workgroups), a choice that the largest layers come to."""
+    tune(kernel)
+    for at in (FAKE, FAKE + 2):
+        for grads in range(1, 16):
+            dx, dw, plane = _plan(1, M, N, K, grads, at)
+            assert (dx == -1) == (not grads & DX) and (dw == -1) == (not grads & (DWG | DWU))
+            for k in (dx, dw):
+                assert k in (-1, 1, 128, 256)
+                assert k != 1 or plane == 0, (M, N, K, grads, dx, dw, plane)
+                assert k < 64 or plane == 1, (M, N, K, grads, dx, dw, plane)
+
+
+def test_large_layers_keep_tile_kernels():
+    """Where the cheaper tile's grid does not fit, the other tile's does."""
+    assert _plan(1, 1 << 28, 8, 136, DX)[0] == 256
+    assert _plan(1, (1 << 29) - 1, 8, 8, DX | DWG | DWU)[0] == 256
+    assert _plan(1, 4096, 2048, 1024, DX | DWG | DWU) == [128, 128, 1]
+    assert _plan(1, 32768, 2048, 2048, 0)[0] == 256 and _plan(1, 1, 2048, 1024, 0)[0] == 2 and _plan(0, 1, 2048, 1024, 0) == [2, -1, -1]
+
+
+def test_plan_refuses():
+    lib = _lib.load()
+    k = (C.c_int * 3)()
+    for args in ((2, FAKE, 8, FAKE, FAKE, 8, 5, 8, 8, 0, k), (1, FAKE, 8, FAKE, FAKE, 8, -1, 8, 8, 0, k), (1, FAKE, 8, FAKE, FAKE, 8, 5, 8, 8, 16, k), (1, FAKE, 8, FAKE, FAKE, 8, 5, 8, 8, 0, None)):
+        assert lib.dp_gated_linear_plan(*args) == -1 and "dp_gated_linear_plan" in _err(lib)
+    assert _plan(1, 0, 8, 8, 1) == [-1, -1, -1]
+
+
 def _table(ptrs, numel, dtypes):
     n = len(ptrs)
     return n, (C.c_void_p * n)(*ptrs), (C.c_int64 * n)(*numel), (C.c_int * n)(*dtypes)
