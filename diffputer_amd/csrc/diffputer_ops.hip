@@ -37,7 +37,9 @@ static int gl_check(const char* who, int dtype, int64_t M, int N, int K, int act
 // tile kernel of that tile (the nearest one that the type has); "gated_splits" 0 = by the rule, n = that many slices of the
 // contraction (as many as there are K-tiles at most)
 std::atomic<int> g_gated_kernel{0}, g_gated_splits{0};
-static int forced_kernel() { return g_gated_kernel.load(std::memory_order_relaxed); }
+// read once by an entry point: everything that a call decides (operands, planes, plans, workspace, launches) is decided by one pair of values
+struct GlTune { int kernel, splits; };
+static GlTune gl_tune() { return {g_gated_kernel.load(std::memory_order_relaxed), g_gated_splits.load(std::memory_order_relaxed)}; }
 
 // dynamic LDS of the tile kernels, once per device
 template <int MODE> static hipError_t gt_attributes() {
@@ -70,7 +72,7 @@ static int gt_ready() {
 // ---- how a product runs: by the general kernel (T = 0), a tile kernel (T = 64, 128 or 256) or the kernel for few rows
 // (GL_ROWS, forward only), and in how many slices of the contraction ----
 constexpr int GL_ROWS = 1;
-struct GlShape { int mode; int64_t I; int J; int64_t C; int planes; };
+struct GlShape { int mode; int64_t I; int J; int64_t C; int planes; GlTune tune; };
 struct GlPlan { int T, kt_per, splits; int64_t ti, tj, wgs; };
 static int64_t gl_ldp(int J) { return round_up<int64_t>(J, 4); }
 static size_t gl_part_bytes(const GlShape& s) { return (size_t)2 * s.I * gl_ldp(s.J) * 4; }       // one slice: two planes
@@ -82,7 +84,7 @@ static GlPlan gl_shape(const GlShape& s, int T, int kdepth, int want) {
     pl.T = T;
     pl.ti = ceil_div<int64_t>(s.I, t);
     pl.tj = ceil_div<int64_t>(s.J, s.mode == GL_FWD ? t / 2 : t);
-    if (const int f = g_gated_splits.load(std::memory_order_relaxed)) want = f;
+    if (s.tune.splits) want = s.tune.splits;
     pl.kt_per = (int)ceil_div<int64_t>(nk, std::max<int64_t>(1, std::min<int64_t>(want, nk)));
     pl.splits = (int)ceil_div<int64_t>(nk, pl.kt_per);
     pl.wgs = pl.ti * pl.tj * s.planes * pl.splits;
@@ -134,7 +136,7 @@ static bool gl_grid_ok(const GlPlan& pl) { return pl.wgs < gl_most(pl.T); }
 // The cheapest tile and slices for a launch of `n` products (one, or both of the backward pass); false if no tile's grid fits.
 static bool gl_choose(const GlShape* s, int n, int dtype, GlPlan* best) {
     const bool bf = dtype == DP_DTYPE_BF16;
-    const int forced = forced_kernel();
+    const int forced = s[0].tune.kernel;
     static const int slices[] = {1, 2, 3, 4, 6, 8, 12, 16, 32, 64};
     double least = 1e300;
     for (int k = 0; k < 2; ++k) {
@@ -179,7 +181,7 @@ static bool gr_slower(const GlShape& s, int dtype) {
     return s.I > 32 ? (int64_t)s.J * s.C >= (int64_t)1 << 23 : s.I > 16 && s.I * s.C * 2 * ceil_div(s.J, gr_columns(s.J)) >= (int64_t)1 << 27;
 }
 static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
-    const int forced = forced_kernel();
+    const int forced = s.tune.kernel;
     if (s.mode == GL_FWD && s.I <= GR_MAX_ROWS && forced == 0 && !(tile && gr_slower(s, dtype))) return {GL_ROWS, 0, 1, 1, 1, 1};
     if (tile && forced != 1) {
         GlPlan pl;
@@ -193,7 +195,7 @@ static GlPlan gl_plan_new(const GlShape& s, int dtype, bool tile) {
 // both backward products, in one launch if they take kernels of one kind and fit a grid
 static GlPlan gl_plan(const GlShape& s, int dtype, bool tile);
 static bool gl_plan_both_new(const GlShape s[2], int dtype, bool tile, GlPlan pl[2]) {
-    if (tile && forced_kernel() != 1 && gl_choose(s, 2, dtype, pl)) return true;
+    if (tile && s[0].tune.kernel != 1 && gl_choose(s, 2, dtype, pl)) return true;
     for (int i = 0; i < 2; ++i) pl[i] = gl_plan(s[i], dtype, tile);
     return pl[0].T == 0 && pl[1].T == 0 && gl_grid_ok(pl[0]) && gl_grid_ok(pl[1]);
 }
@@ -209,7 +211,7 @@ struct GlKey {
 struct GlMemo { GlKey key; GlPlan pl[2]; bool one; };
 static GlMemo& gl_memo(const GlShape& s, int dtype, bool tile, int both, bool& known) {
     static thread_local GlMemo memo[64];
-    const GlKey k = {s.I, s.C, s.J, s.mode + 1, s.planes, dtype, tile, forced_kernel(), g_gated_splits.load(std::memory_order_relaxed), both};
+    const GlKey k = {s.I, s.C, s.J, s.mode + 1, s.planes, dtype, tile, s.tune.kernel, s.tune.splits, both};
     GlMemo& m = memo[((uint64_t)(s.I * 31 + s.C) * 31 + (uint64_t)s.J * 7 + (uint64_t)(s.mode * 5 + both * 3 + dtype)) % 64];
     known = m.key == k;
     m.key = k;
@@ -334,13 +336,12 @@ constexpr int64_t GL_EXACT_BELOW = 8192;                         // M N
 constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
 constexpr int64_t GT_MAX_LD = 1 << 21;                           // 128 rows of float32 stay within 2^30 bytes
 struct GtOperands { bool tile, vec, short_rows, pack_x, pack_w; int64_t ldk; };   // ldk: row stride of the copies
-static GtOperands gt_operands(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
+static GtOperands gt_operands(int forced, int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
     GtOperands o;
     const bool bf = dtype == DP_DTYPE_BF16;
     const int chunk = bf ? 8 : 4;
     const bool x_in = gt_direct(x, ldx, K, chunk), w_in = gt_direct(wg, ldw, K, chunk) && gt_direct(wu, ldw, K, chunk);
     const bool short_rows = o.short_rows = ldx <= GT_MAX_LD && ldw <= GT_MAX_LD;
-    const int forced = forced_kernel();
     o.vec = x_in && w_in;
     o.pack_x = o.pack_w = false;
     o.ldk = round_up<int64_t>(K, chunk);
@@ -364,6 +365,7 @@ struct GlIn {
     int64_t M;
     int N, K;
     size_t es;
+    GlTune tune;
     GtOperands o;
     char *px, *pw;
     void carve(Carver& c) {
@@ -391,7 +393,8 @@ struct GlIn {
     int64_t fwd_c() const { return o.pack_x && o.pack_w ? o.ldk : K; }
 };
 static GlIn gl_in(int dtype, const void* x, int64_t ldx, const void* wg, const void* wu, int64_t ldw, int64_t M, int N, int K) {
-    return {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, dtype == DP_DTYPE_BF16 ? (size_t)2 : (size_t)4, gt_operands(dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
+    const GlTune tune = gl_tune();
+    return {{x, ldx, K}, {wg, ldw, K}, {wu, ldw, K}, M, N, K, dtype == DP_DTYPE_BF16 ? (size_t)2 : (size_t)4, tune, gt_operands(tune.kernel, dtype, x, ldx, wg, wu, ldw, M, N, K), nullptr, nullptr};
 }
 
 // forward workspace: copies, partial sums
@@ -400,9 +403,9 @@ static GlFwd gl_fwd_carve(int dtype, GlIn& in, void* base) {
     GlFwd w;
     // the float32 forward product (both operands row laid out) loses 5 to 10 % to 4-byte loads, less than copies take
     if (dtype == DP_DTYPE_F32 && in.o.short_rows && (in.o.pack_x || in.o.pack_w)) in.o.pack_x = in.o.pack_w = in.o.vec = false;
-    w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1};
+    w.s = {GL_FWD, in.M, in.N, in.fwd_c(), 1, in.tune};
     // few rows: copies of the weights would cost more than a tile kernel gains
-    w.plan = gl_plan(w.s, dtype, in.o.tile && !(in.M <= GR_MAX_ROWS && (in.o.pack_x || in.o.pack_w) && forced_kernel() == 0));
+    w.plan = gl_plan(w.s, dtype, in.o.tile && !(in.M <= GR_MAX_ROWS && (in.o.pack_x || in.o.pack_w) && in.tune.kernel == 0));
     if (w.plan.T == GL_ROWS) {                                    // reads rows of any alignment
         in.o.pack_x = in.o.pack_w = false;
         w.s.C = in.K;
@@ -431,9 +434,9 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     const int N = in.N, K = in.K;
     GlBwd w;
     // small layers take the general kernel, whose dg and du are not rounded: with few of them their roundings do not average out
-    if (dtype == DP_DTYPE_BF16 && M * N < GL_EXACT_BELOW && forced_kernel() == 0) in.o.tile = in.o.pack_x = in.o.pack_w = false;
-    w.s[0] = {GL_DX, M, K, N, 1};
-    w.s[1] = {GL_DW, N, K, M, planes ? planes : 2};
+    if (dtype == DP_DTYPE_BF16 && M * N < GL_EXACT_BELOW && in.tune.kernel == 0) in.o.tile = in.o.pack_x = in.o.pack_w = false;
+    w.s[0] = {GL_DX, M, K, N, 1, in.tune};
+    w.s[1] = {GL_DW, N, K, M, planes ? planes : 2, in.tune};
     for (;;) {
         w.both = false;
         if (want_dx && planes == 2) w.both = gl_plan_both(w.s, dtype, in.o.tile, w.plan);
@@ -462,8 +465,7 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
 }
 
 template <typename T>
-static int gl_forward(GlArgs a, GlIn& in, void* ws, hipStream_t st) {
-    const GlFwd w = gl_fwd_carve(sizeof(T) == 2 ? DP_DTYPE_BF16 : DP_DTYPE_F32, in, ws);
+static int gl_forward(GlArgs a, GlIn& in, const GlFwd& w, hipStream_t st) {
     int blocks;
     const GlPack copies = in.copies(true, true, &blocks);
     if (blocks) {
@@ -484,20 +486,20 @@ static int gl_zero(void* p, int64_t n, hipStream_t st) {
 }
 
 template <typename T>
-static int gl_backward(int dtype, GlIn& in, const void* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2], int act, void* ws, hipStream_t st) {
-    const int64_t M = in.M;
-    const int N = in.N, K = in.K;
+static int gl_no_rows(T* dw[2], T* db[2], int N, int K, hipStream_t st) {      // the sums are empty
     int rc;
-    if (M == 0) {                                                // no rows: the sums are empty
-        for (int z = 0; z < 2; ++z) {
-            if (dw[z] && (rc = gl_zero<T>(dw[z], (int64_t)N * K, st))) return rc;
-            if (db[z] && (rc = gl_zero<T>(db[z], N, st))) return rc;
-        }
-        return DP_OK;
+    for (int z = 0; z < 2; ++z) {
+        if (dw[z] && (rc = gl_zero<T>(dw[z], (int64_t)N * K, st))) return rc;
+        if (db[z] && (rc = gl_zero<T>(db[z], N, st))) return rc;
     }
-    const int planes = (dw[0] != nullptr) + (dw[1] != nullptr);
-    const GlBwd w = gl_bwd_carve(dtype, in, planes, dx != nullptr, ws);
-    int blocks;
+    return DP_OK;
+}
+
+template <typename T>
+static int gl_backward(int dtype, GlIn& in, const GlBwd& w, const void* pre, const GlOp& dh, T* dx, T* dw[2], T* db[2], int act, hipStream_t st) {
+    const int64_t M = in.M;
+    const int N = in.N, K = in.K, planes = (dw[0] != nullptr) + (dw[1] != nullptr);
+    int rc, blocks;
     const GlPack copies = in.copies(planes > 0, dx != nullptr, &blocks);
     const GlDgu e = {pre, dh.p, w.dgu, w.colpart, {db[0], db[1]}, dh.ld, w.ldg, M, N, act, w.tx, w.rows, w.nblk};
     const unsigned across = (unsigned)ceil_div<int64_t>(w.ldg, w.tx * 4);
@@ -639,7 +641,9 @@ int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, c
     for (const void* p : {x, w_gate, w_up, b_gate, b_up, (const void*)h})
         if (!aligned(p, es)) return fail(DP_EINVAL, "dp_gated_linear: a pointer is not aligned to its element");
     if (!aligned(pre, 16)) return fail(DP_EINVAL, "dp_gated_linear: pre must be 16-byte aligned");
-    const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, 0);
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
+    const GlFwd w = gl_fwd_carve(dtype, in, workspace);
+    const size_t need = std::max<size_t>(w.bytes, 256);
     if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
     GlArgs a;
     memset(&a, 0, sizeof a);
@@ -648,8 +652,7 @@ int dp_gated_linear(int dtype, const void* x, int64_t ldx, const void* w_gate, c
     a.bias[0] = b_gate; a.bias[1] = b_up;
     a.act = act;
     hipStream_t st = (hipStream_t)stream;
-    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
-    return dtype == DP_DTYPE_BF16 ? gl_forward<bf16_t>(a, in, workspace, st) : gl_forward<float>(a, in, workspace, st);
+    return dtype == DP_DTYPE_BF16 ? gl_forward<bf16_t>(a, in, w, st) : gl_forward<float>(a, in, w, st);
 }
 
 int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gate, const void* w_up, int64_t ldw, const void* pre, const void* dh, int64_t lddh,
@@ -662,21 +665,19 @@ int dp_gated_linear_bwd(int dtype, const void* x, int64_t ldx, const void* w_gat
         if (!x || !w_gate || !w_up || !pre || !dh) return fail(DP_EINVAL, "dp_gated_linear_bwd: null pointer");
         if (ldx < K || ldw < K || lddh < N) return fail(DP_EINVAL, "dp_gated_linear_bwd: row strides ldx=%lld ldw=%lld lddh=%lld are shorter than a row (K=%d, N=%d)", (long long)ldx, (long long)ldw, (long long)lddh, K, N);
         if (!aligned(pre, 16)) return fail(DP_EINVAL, "dp_gated_linear_bwd: pre must be 16-byte aligned");
-        const int grads = (dx ? DP_GATED_DX : 0) | (dw_gate ? DP_GATED_DW_GATE : 0) | (dw_up ? DP_GATED_DW_UP : 0) | DP_GATED_DB;
-        const size_t need = dp_gated_linear_workspace_bytes(dtype, x, ldx, w_gate, w_up, ldw, M, N, K, grads);
-        if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear_bwd: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
     }
     for (const void* p : {x, w_gate, w_up, dh, (const void*)dx, (const void*)dw_gate, (const void*)dw_up, (const void*)db_gate, (const void*)db_up})
         if (!aligned(p, es)) return fail(DP_EINVAL, "dp_gated_linear_bwd: a pointer is not aligned to its element");
-    const GlOp od = {dh, lddh, N};
-    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == DP_DTYPE_BF16) {
-        bf16_t *dw[2] = {(bf16_t*)dw_gate, (bf16_t*)dw_up}, *db[2] = {(bf16_t*)db_gate, (bf16_t*)db_up};
-        return gl_backward<bf16_t>(dtype, in, pre, od, (bf16_t*)dx, dw, db, act, workspace, st);
-    }
-    float *dw[2] = {(float*)dw_gate, (float*)dw_up}, *db[2] = {(float*)db_gate, (float*)db_up};
-    return gl_backward<float>(dtype, in, pre, od, (float*)dx, dw, db, act, workspace, st);
+    bf16_t *dw16[2] = {(bf16_t*)dw_gate, (bf16_t*)dw_up}, *db16[2] = {(bf16_t*)db_gate, (bf16_t*)db_up};
+    float *dw32[2] = {(float*)dw_gate, (float*)dw_up}, *db32[2] = {(float*)db_gate, (float*)db_up};
+    if (M == 0) return dtype == DP_DTYPE_BF16 ? gl_no_rows<bf16_t>(dw16, db16, N, K, st) : gl_no_rows<float>(dw32, db32, N, K, st);
+    GlIn in = gl_in(dtype, x, ldx, w_gate, w_up, ldw, M, N, K);
+    const GlBwd w = gl_bwd_carve(dtype, in, (dw_gate != nullptr) + (dw_up != nullptr), dx != nullptr, workspace);
+    const size_t need = std::max<size_t>(w.bytes, 256);
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 256)) return fail(DP_EWORKSPACE, "dp_gated_linear_bwd: workspace of %zu bytes, need %zu (256-byte aligned)", workspace_bytes, need);
+    const GlOp od = {dh, lddh, N};
+    return dtype == DP_DTYPE_BF16 ? gl_backward<bf16_t>(dtype, in, w, pre, od, (bf16_t*)dx, dw16, db16, act, st) : gl_backward<float>(dtype, in, w, pre, od, (float*)dx, dw32, db32, act, st);
 }
 
 size_t dp_grad_workspace_bytes(int n) { return n < 0 ? 0 : (size_t)(gn_cap(n) * gn_launches(n) + 1) * sizeof(double); }

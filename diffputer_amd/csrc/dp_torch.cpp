@@ -42,6 +42,19 @@ void check(int rc, const char* what) {
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 Tensor bytes_like(const Tensor& t, size_t n) { return at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)); }
 
+// A call with a workspace of the size that is asked for right before it: where another thread's dp_tune comes in between and the
+// call needs more, both are made again.
+template <typename Size, typename Call> void with_workspace(const Tensor& like, const char* who, Size size, Call call) {
+    for (int again = 8;; --again) {
+        const size_t need = size();
+        if (need == 0) check(DP_EINVAL, who);
+        const Tensor ws = bytes_like(like, need);
+        const int rc = call(ws.data_ptr(), need);
+        if (rc == DP_EWORKSPACE && again) continue;
+        return check(rc, who);
+    }
+}
+
 int code_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? DP_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? DP_DTYPE_BF16 : -1; }
 
 // ---- gated projection ----------------------------------------------------------------------------------------------------
@@ -70,11 +83,12 @@ Tensor forward_of(const Tensor& x, const Tensor& wg, const Tensor& wu, const Ten
     if (pre) *pre = bytes_like(x, dp_gated_linear_pre_bytes(code_of(x), M, (int)N));
     if (M == 0) return h;
     const int dt = code_of(x);
-    const size_t need = dp_gated_linear_workspace_bytes(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), M, (int)N, (int)K, 0);
-    if (need == 0) check(DP_EINVAL, "dp_gated_linear_workspace_bytes");
-    const Tensor ws = bytes_like(x, need);
-    check(dp_gated_linear(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), ptr(bg), ptr(bu), h.data_ptr(), N, pre ? pre->data_ptr() : nullptr, M, (int)N, (int)K, act,
-                          ws.data_ptr(), need, stream_of(x)), "dp_gated_linear");
+    with_workspace(
+        x, "dp_gated_linear", [&] { return dp_gated_linear_workspace_bytes(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), M, (int)N, (int)K, 0); },
+        [&](void* ws, size_t n) {
+            return dp_gated_linear(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), ptr(bg), ptr(bu), h.data_ptr(), N, pre ? pre->data_ptr() : nullptr, M, (int)N, (int)K, act,
+                                   ws, n, stream_of(x));
+        });
     return h;
 }
 
@@ -125,11 +139,12 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         auto out = [&](bool given, at::IntArrayRef size) { return given && ctx->needs_input_grad(edge++) ? at::empty(size, opt) : Tensor(); };
         Tensor dx = out(true, {M, K}), dwg = out(true, {N, K}), dwu = out(true, {N, K}), dbg = out(biases & 1, {N}), dbu = out(biases & 2, {N});
         const int dt = code_of(x), flags = (dx.defined() ? DP_GATED_DX : 0) | (dwg.defined() ? DP_GATED_DW_GATE : 0) | (dwu.defined() ? DP_GATED_DW_UP : 0) | DP_GATED_DB;
-        const size_t need = dp_gated_linear_workspace_bytes(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), M, (int)N, (int)K, flags);
-        if (need == 0) check(DP_EINVAL, "dp_gated_linear_workspace_bytes");
-        const Tensor ws = bytes_like(x, need);
-        check(dp_gated_linear_bwd(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), pre.data_ptr(), dh.data_ptr(), ld_of(dh), ptr(dx), ptr(dwg), ptr(dwu), ptr(dbg), ptr(dbu),
-                                  M, (int)N, (int)K, (int)act, ws.data_ptr(), need, stream_of(x)), "dp_gated_linear_bwd");
+        with_workspace(
+            x, "dp_gated_linear_bwd", [&] { return dp_gated_linear_workspace_bytes(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), M, (int)N, (int)K, flags); },
+            [&](void* ws, size_t n) {
+                return dp_gated_linear_bwd(dt, x.data_ptr(), ld_of(x), wg.data_ptr(), wu.data_ptr(), ld_of(wg), pre.data_ptr(), dh.data_ptr(), ld_of(dh), ptr(dx), ptr(dwg), ptr(dwu), ptr(dbg), ptr(dbu),
+                                           M, (int)N, (int)K, (int)act, ws, n, stream_of(x));
+            });
         variable_list res = {dx, dwg, dwu, dbg, dbu, Tensor()};
         if (at::GradMode::is_enabled()) {                        // create_graph: first derivatives only, said when a second one is asked for
             variable_list given;

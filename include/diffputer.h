@@ -21,7 +21,10 @@
  *     once under a lock in dp_plan_create and read-only afterwards; dp_last_error is thread-local).  ONE plan must not be
  *     used from two threads at once (its profiling slots and scratch embedding rows are unsynchronised).  dp_tune values
  *     are process-wide atomics read at every evaluation: changing one while another thread is inside a sampler call gives
- *     that call a mix of old and new settings ("fold_proj" changes the rounding sequence, the others do not change bits).
+ *     that call a mix of old and new settings ("fold_proj" changes the rounding sequence, "gated_kernel" and "gated_splits" the
+ *     order of sums and where bf16 gradients are rounded, the others do not change bits).  dp_gated_linear and its backward
+ *     read "gated_kernel" and "gated_splits" once per call; a workspace sized under other settings than the call's own is
+ *     refused (DP_EWORKSPACE) where it is too small.
  */
 #ifndef DIFFPUTER_H
 #define DIFFPUTER_H

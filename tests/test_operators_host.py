@@ -2,6 +2,7 @@
 every argument before the first HIP call)."""
 import ctypes as C
 import math
+import sys
 
 import pytest
 import torch
@@ -175,6 +176,59 @@ def test_large_layers_keep_tile_kernels():
     assert _plan(1, (1 << 29) - 1, 8, 8, DX | DWG | DWU)[0] == 256
     assert _plan(1, 4096, 2048, 1024, DX | DWG | DWU) == [128, 128, 1]
     assert _plan(1, 32768, 2048, 2048, 0)[0] == 256 and _plan(1, 1, 2048, 1024, 0)[0] == 2 and _plan(0, 1, 2048, 1024, 0) == [2, -1, -1]
+
+
+def test_settings_that_change_during_a_call(tune):
+    """A thread changes the tuning knobs while another plans calls: every plan and workspace is one that some setting gives, and none of
+    them is kept for another setting."""
+    import threading
+    lib = _lib.load()
+    settings = [(k, s) for k in (0, 1, 128, 256) for s in (0, 5)]
+    sizes = [(100 + 37 * i, 64 + 40 * (i % 11), 64 + 24 * (i % 17), at) for i in range(90) for at in (FAKE, FAKE + 2)]
+
+    def query(M, N, K, at):
+        k = (C.c_int * 3)()
+        lib.dp_gated_linear_plan(1, at, K, at, at, K, M, N, K, DX | DWG | DWU, k)
+        return tuple(k)
+
+    def workspace(M, N, K, at):
+        return tuple(lib.dp_gated_linear_workspace_bytes(1, at, K, at, at, K, M, N, K, g) for g in (0, DX | DWG | DWU))
+
+    plans, spaces = {}, {}
+    for t in settings:
+        tune(*t)
+        for z in sizes:
+            plans.setdefault(z, set()).add(query(*z))
+            for i, b in enumerate(workspace(*z)):
+                spaces.setdefault((z, i), set()).add(b)
+    tune(0)
+    serial = {z: (query(*z), workspace(*z)) for z in sizes}
+    stop, n = threading.Event(), [0]
+
+    def change():
+        while not stop.is_set():
+            for k, s in settings:
+                lib.dp_tune(b"gated_kernel", k)
+                lib.dp_tune(b"gated_splits", s)
+            n[0] += 1
+
+    t = threading.Thread(target=change)
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)                                    # so that both threads are inside the library most of the time
+    t.start()
+    try:
+        for _ in range(150):
+            for z in sizes:
+                assert query(*z) in plans[z], z
+                for i, b in enumerate(workspace(*z)):
+                    assert b in spaces[z, i], (z, i)
+    finally:
+        stop.set()
+        t.join()
+        sys.setswitchinterval(interval)
+    assert n[0] > 100
+    tune(0)
+    assert {z: (query(*z), workspace(*z)) for z in sizes} == serial
 
 
 def test_plan_refuses():
