@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/util/Exception.h>
@@ -37,6 +38,13 @@ struct LibraryError : std::runtime_error {
 };
 void check(int rc, const char* what) {
     if (rc != DP_OK) throw LibraryError(std::string(what) + " failed (code " + std::to_string(rc) + "): " + dp_last_error());
+}
+
+// Forward-mode derivatives: the kernels read values only, so a tangent would be dropped without a word.  (torch itself raises where
+// the call makes an autograd node.)
+void refuse_tangent(const Tensor& t, const char* who) {
+    if (t.defined() && t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        throw LibraryError(std::string(who) + " has no forward-mode derivatives (a tensor carries a tangent)");
 }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -191,6 +199,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != 6 || !tensor_arg(args[0], x) || !tensor_arg(args[1], w[0]) || !tensor_arg(args[2], w[1]) || !tensor_arg(args[3], b[0]) || !tensor_arg(args[4], b[1])) Py_RETURN_NONE;
         const long act = PyLong_AsLong(args[5]);
         if (act == -1 && PyErr_Occurred()) return nullptr;
+        for (const Tensor* t : {&x, &w[0], &w[1], &b[0], &b[1]}) refuse_tangent(*t, "gated_linear");
         if (!x.defined() || !w[0].defined() || !w[1].defined() || !x.is_cuda() || code_of(x) < 0 || x.dim() < 1 || w[0].dim() != 2 || w[1].sizes() != w[0].sizes()) Py_RETURN_NONE;
         const int64_t N = w[0].size(0), K = w[0].size(1);
         if (N < 1 || K < 1 || x.size(-1) != K) Py_RETURN_NONE;
@@ -244,6 +253,8 @@ PyObject* py_grads(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const double limit = clip ? PyFloat_AsDouble(args[2]) : 0.0;
         if (clip && limit == -1.0 && PyErr_Occurred()) return nullptr;
         if (count < 1 || count > (1 << 24)) Py_RETURN_NONE;
+        for (Py_ssize_t i = 0; i < count; ++i)
+            if (THPVariable_Check(PyList_GET_ITEM(args[0], i))) refuse_tangent(THPVariable_Unpack(PyList_GET_ITEM(args[0], i)), clip ? "clip_grads" : "grad_norm");
         std::vector<void*> ptrs(count);
         std::vector<int64_t> numel(count);
         std::vector<int> dtypes(count);

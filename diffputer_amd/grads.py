@@ -68,7 +68,8 @@ def _call(grads, kind, limit, what):
 
 def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
     """Norm of all elements of `grads` (a tensor, or an iterable of them: float32 / bfloat16, one device) as a 0-dim float32
-    tensor on that device; norm_type 2 or inf.  NaN and infinities propagate."""
+    tensor on that device; norm_type 2 or inf.  NaN and infinities propagate.  The norm itself has no derivatives (a tensor with
+    a forward-mode tangent is refused)."""
     return _call(_list(grads), _kind(norm_type), None, "grad_norm")
 
 

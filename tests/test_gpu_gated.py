@@ -684,3 +684,24 @@ def test_every_bf16_gate(kernel, act, tune):
 def test_some_rows_of_large_layers(M, K, N, dtype):
     """Where the kernel for few rows and the tile kernels take turns."""
     check(*make(M, K, N, dtype, seed=M + N), act="silu", train=M != 32)
+
+
+def test_no_tangent_is_lost():
+    """Forward-mode derivatives on the device: refused with and without gradients, through the module too."""
+    from torch.autograd import forward_ad
+
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.gated import GatedLinear, gated_linear
+    from diffputer_amd.grads import clip_grads, grad_norm
+    layer = GatedLinear(8, 16).to(DEV)
+    x = torch.randn(3, 8, device=DEV)
+    want = layer(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (layer, lambda t: gated_linear(t, layer.gate.weight.detach(), layer.up.weight.detach()), lambda t: grad_norm([t]), lambda t: clip_grads([t], 1e-3)):
+            with pytest.raises(DiffputerError, match="forward-mode"):
+                call(dual)
+        assert torch.equal(layer(x), want)
+        with torch.inference_mode():
+            assert torch.equal(layer(x), want)
+    assert torch.equal(layer(x), want)

@@ -58,6 +58,29 @@ def test_grads_refuse():
             clip_grads([g], limit)
 
 
+def _calls():
+    """Every entry point that takes tensors, as a function of one tensor (on the CPU: what is refused is refused before the device)."""
+    w = torch.randn(5, 4)
+    return [lambda t: gated_linear(t, w, w), lambda t: gated_linear(w[:3], t.expand(5, 4), w), lambda t: gated_linear(w, w, w, t[0, :1].expand(5)),
+            lambda t: gated_linear(w, w, w, None, t[0, :1].expand(5)), lambda t: grad_norm([w, t]), lambda t: clip_grads([w, t], 1.0)]
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_tangents_are_refused(i):
+    """Forward-mode derivatives would be dropped without a word: a dual tensor is refused wherever it comes in."""
+    from torch.autograd import forward_ad
+    call, x = _calls()[i], torch.randn(1, 4)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            base = x.clone().requires_grad_(grad)
+            with pytest.raises(_lib.DiffputerError, match="forward-mode"):
+                call(forward_ad.make_dual(base, torch.ones_like(x)))
+            with torch.no_grad(), pytest.raises(_lib.DiffputerError, match="forward-mode"):
+                call(forward_ad.make_dual(base, torch.ones_like(x)))
+        with pytest.raises(_lib.DiffputerError, match="no CPU fallback"):
+            call(x)                                                  # no tangent: as ever
+
+
 def test_module_on_the_cpu():
     torch.manual_seed(1)
     for act, f in (("silu", torch.nn.functional.silu), ("gelu", torch.nn.functional.gelu), ("none", lambda t: t)):
