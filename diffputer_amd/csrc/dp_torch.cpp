@@ -11,12 +11,15 @@
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/util/Exception.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
@@ -45,6 +48,16 @@ void check(int rc, const char* what) {
 void refuse_tangent(const Tensor& t, const char* who) {
     if (t.defined() && t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
         throw LibraryError(std::string(who) + " has no forward-mode derivatives (a tensor carries a tangent)");
+}
+
+// Tracers (torch.jit.trace, make_fx, fake and functional tensors) record torch's operations: of a call that would be the
+// allocation of its output, and a traced function that returns memory which nothing has filled.  (torch.compile breaks its graph here.)
+void refuse_trace(const char* who) {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    bool on = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    if (c10::impl::TorchDispatchModeTLS::any_modes_set())
+        for (const Mode m : {Mode::PROXY, Mode::FAKE, Mode::FUNCTIONAL}) on = on || c10::impl::TorchDispatchModeTLS::get_mode(m).has_value();
+    if (on) throw LibraryError(std::string(who) + " cannot be traced (torch.jit.trace, make_fx, fake tensors): its kernels are not torch operations");
 }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -199,6 +212,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != 6 || !tensor_arg(args[0], x) || !tensor_arg(args[1], w[0]) || !tensor_arg(args[2], w[1]) || !tensor_arg(args[3], b[0]) || !tensor_arg(args[4], b[1])) Py_RETURN_NONE;
         const long act = PyLong_AsLong(args[5]);
         if (act == -1 && PyErr_Occurred()) return nullptr;
+        refuse_trace("gated_linear");
         for (const Tensor* t : {&x, &w[0], &w[1], &b[0], &b[1]}) refuse_tangent(*t, "gated_linear");
         if (!x.defined() || !w[0].defined() || !w[1].defined() || !x.is_cuda() || code_of(x) < 0 || x.dim() < 1 || w[0].dim() != 2 || w[1].sizes() != w[0].sizes()) Py_RETURN_NONE;
         const int64_t N = w[0].size(0), K = w[0].size(1);
@@ -253,6 +267,7 @@ PyObject* py_grads(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const double limit = clip ? PyFloat_AsDouble(args[2]) : 0.0;
         if (clip && limit == -1.0 && PyErr_Occurred()) return nullptr;
         if (count < 1 || count > (1 << 24)) Py_RETURN_NONE;
+        refuse_trace(clip ? "clip_grads" : "grad_norm");
         for (Py_ssize_t i = 0; i < count; ++i)
             if (THPVariable_Check(PyList_GET_ITEM(args[0], i))) refuse_tangent(THPVariable_Unpack(PyList_GET_ITEM(args[0], i)), clip ? "clip_grads" : "grad_norm");
         std::vector<void*> ptrs(count);

@@ -705,3 +705,22 @@ def test_no_tangent_is_lost():
         with torch.inference_mode():
             assert torch.equal(layer(x), want)
     assert torch.equal(layer(x), want)
+
+
+def test_traces_on_the_device():
+    """Tracers are refused; a mode that only watches, and torch.compile, which breaks its graph, run the kernels."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.gated import GatedLinear
+    layer = GatedLinear(8, 16).to(DEV).requires_grad_(False)
+    x = torch.randn(3, 8, device=DEV)
+    want = layer(x)
+    for trace in (lambda: torch.jit.trace(layer, (x,)), lambda: make_fx(layer)(x)):
+        with pytest.raises(DiffputerError, match="traced"):
+            trace()
+    with FlopCounterMode(display=False):
+        assert torch.equal(layer(x), want)
+    assert torch.equal(torch.compile(layer, backend="eager")(x), want)
+    assert torch.equal(layer(x), want)

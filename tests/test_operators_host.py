@@ -81,6 +81,25 @@ def test_tangents_are_refused(i):
             call(x)                                                  # no tangent: as ever
 
 
+@pytest.mark.parametrize("i", range(6))
+@pytest.mark.parametrize("how", ["jit", "make_fx", "make_fx_symbolic", "make_fx_pre_dispatch", "fake"])
+def test_traces_are_refused(how, i):
+    """A trace would record the output's allocation and nothing that fills it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = _calls()[i], torch.randn(1, 4)
+    run = {"jit": lambda: torch.jit.trace(call, (x,)), "make_fx": lambda: make_fx(call)(x), "make_fx_symbolic": lambda: make_fx(call, tracing_mode="symbolic", _allow_non_fake_inputs=True)(x),
+           "make_fx_pre_dispatch": lambda: make_fx(call, pre_dispatch=True)(x)}
+    with pytest.raises(_lib.DiffputerError, match="traced"):
+        if how == "fake":
+            with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+                call(mode.from_tensor(x))
+        else:
+            run[how]()
+    with pytest.raises(_lib.DiffputerError, match="no CPU fallback"):
+        call(x)
+
+
 def test_module_on_the_cpu():
     torch.manual_seed(1)
     for act, f in (("silu", torch.nn.functional.silu), ("gelu", torch.nn.functional.gelu), ("none", lambda t: t)):
