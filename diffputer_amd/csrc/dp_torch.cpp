@@ -79,13 +79,17 @@ template <typename Size, typename Call> void with_workspace(const Tensor& like, 
 int code_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? DP_DTYPE_F32 : t.scalar_type() == at::kBFloat16 ? DP_DTYPE_BF16 : -1; }
 
 // ---- gated projection ----------------------------------------------------------------------------------------------------
-// [rows, cols] with contiguous rows that do not overlap: `t` itself, or a copy
+// [rows, cols] with contiguous rows that do not overlap: `t` itself, or a copy (also of a tensor whose negation is a bit, which its
+// memory does not show)
 Tensor rows_of(const Tensor& t) {
+    if (t.is_neg()) return t.resolve_neg().contiguous();
     if (t.is_contiguous() || ((t.stride(1) == 1 || t.size(1) == 1) && (t.stride(0) >= t.size(1) || t.size(0) == 1))) return t;
     return t.contiguous();
 }
 int64_t ld_of(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }           // a single row's stride says nothing
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+Tensor bias_of(const Tensor& t) { return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
 
 // the kernels take both weights with one row stride
 void weights_of(Tensor& wg, Tensor& wu) {
@@ -135,7 +139,7 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
                           const std::optional<Tensor>& b_up, int64_t act) {
         Tensor wg = w_gate, wu = w_up, pre;
         weights_of(wg, wu);
-        const Tensor xr = rows_of(x), bg = b_gate ? b_gate->contiguous() : Tensor(), bu = b_up ? b_up->contiguous() : Tensor();
+        const Tensor xr = rows_of(x), bg = b_gate ? bias_of(*b_gate) : Tensor(), bu = b_up ? bias_of(*b_up) : Tensor();
         const Tensor h = forward_of(xr, wg, wu, bg, bu, (int)act, &pre);
         ctx->save_for_backward({x, w_gate, w_up, pre});
         ctx->saved_data["act"] = act;
@@ -239,7 +243,7 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
             const at::NoGradGuard off;
             weights_of(w[0], w[1]);
             for (Tensor& t : b)
-                if (t.defined()) t = t.contiguous();
+                if (t.defined()) t = bias_of(t);
             h = forward_of(rows_of(x2), w[0], w[1], b[0], b[1], (int)act, nullptr);
         }
         if (!flat) {

@@ -724,3 +724,35 @@ def test_traces_on_the_device():
         assert torch.equal(layer(x), want)
     assert torch.equal(torch.compile(layer, backend="eager")(x), want)
     assert torch.equal(layer(x), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("which", [0, 1, 2, 3, 4, 5])
+def test_lazily_negated_tensors(which, dtype):
+    """A tensor whose negation is a bit (as the imaginary part of a conjugate has it) is read with its sign, dense or not."""
+    from diffputer_amd.gated import gated_linear
+    sets = [t.to(DEV) for t in make(9, 16, 8, dtype, seed=60 + which)]
+
+    lazy, plain = list(sets), list(sets)
+    lazy[which], plain[which] = torch._neg_view(sets[which]), -sets[which]
+    assert lazy[which].is_neg() and not plain[which].is_neg()
+    others = [i for i in range(5) if i != which]
+
+    def once(t):
+        leaves = [v.detach().requires_grad_(i in others) for i, v in enumerate(t[:5])]
+        h = gated_linear(*leaves)
+        return [h.detach(), *torch.autograd.grad(h, [leaves[i] for i in others], t[5])]
+
+    assert all(torch.equal(a, b) for a, b in zip(once(lazy), once(plain)))
+    with torch.no_grad():
+        assert torch.equal(gated_linear(*lazy[:5]), gated_linear(*plain[:5]))
+
+
+def test_lazily_negated_column():
+    """A column of one imaginary part per row: strided, and one element wide."""
+    from diffputer_amd.gated import gated_linear
+    z = torch.randn(20, 1, dtype=torch.complex64, device=DEV)
+    w = torch.randn(8, 1, device=DEV)
+    lazy = z.conj().imag
+    assert lazy.is_neg()
+    assert torch.equal(gated_linear(lazy, w, w), gated_linear(-z.imag.clone(), w, w))

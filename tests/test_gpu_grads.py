@@ -237,3 +237,21 @@ def test_a_graph_that_kept_a_gradient_notices():
         clip_grads([g], 1.0)
     # coefficient 1 / (30 + 1e-6) in float32, one product: 2^-23 of 0.1
     assert abs(float(g[0]) - 3.0 / (30.0 + 1e-6)) <= 2.0 ** -22 * 0.1
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_lazily_negated_tensors(dtype):
+    """A tensor whose negation is a bit: scaled in place through the bit, and the memory behind it with it."""
+    from diffputer_amd.grads import clip_grads, grad_norm
+    base = torch.randn(1000, device=DEV).to(dtype)
+    keep, lazy = base.clone(), torch._neg_view(base)
+    other = torch.randn(77, device=DEV)
+    norm = norm_of([keep, other])
+    assert abs(float(grad_norm([lazy, other])) - norm) <= 2.0 ** -23 * norm
+    want = [(-keep).clone(), other.clone()]
+    clip_grads(want, 0.3)
+    got = [lazy, other]
+    n = clip_grads(got, 0.3)
+    assert abs(float(n) - norm) <= 2.0 ** -23 * norm
+    assert lazy.is_neg() and all(torch.equal(a.resolve_neg(), b) for a, b in zip(got, want))
+    assert torch.equal(base, -want[0])
