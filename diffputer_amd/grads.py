@@ -43,6 +43,85 @@ def _refuse(grads, what):
     raise ValueError(f"{what} takes dense (strided) tensors")
 
 
+# ---- whether strided tensors share memory, exactly and without the GPU -------------------------------------------------------
+# A place of a tensor is base + sum x_k stride_k, 0 <= x_k < n_k, so two tensors meet where a sum of terms with bounded counts takes
+# one value.  The largest step first, the counts that are left are those between which the smaller steps can make up the rest: one
+# or two at each step where dimensions nest, as a view's do.
+_MOST_TRIES = 20_000
+
+
+def _solutions(terms, total, need):
+    """How many ways, up to `need`, there are to write `total` as sum x_k step_k with 0 <= x_k <= most_k; `need` where that takes
+    too long to find out.  terms: [(step >= 1, most >= 1)]."""
+    terms = sorted(terms, reverse=True)
+    reach, common = [0], [0]                                     # of the terms from k on: largest sum, common divisor
+    for step, most in reversed(terms):
+        reach.append(reach[-1] + step * most)
+        common.append(math.gcd(common[-1], step))
+    reach, common = reach[::-1], common[::-1]
+    tries = 0
+
+    def count(k, left, need):
+        nonlocal tries
+        tries += 1
+        if tries > _MOST_TRIES:
+            return need
+        if k == len(terms):
+            return int(left == 0)
+        if left < 0 or left > reach[k] or left % common[k]:
+            return 0
+        step, most = terms[k]
+        found = 0
+        for x in range(max(0, -((reach[k + 1] - left) // step)), min(most, left // step) + 1):
+            found += count(k + 1, left - x * step, need - found)
+            if found >= need:
+                return need
+        return found
+
+    return count(0, total, need)
+
+
+def _dims(t):
+    return [(s * t.element_size(), n - 1) for s, n in zip(t.stride(), t.shape) if n > 1]
+
+
+def _meets_itself(t):
+    """Whether two elements of t have one place."""
+    dims = _dims(t) if t.numel() else []
+    if any(s == 0 for s, _ in dims):
+        return True
+    # differences of two indexes, moved up by n - 1: equal indexes are one solution
+    return _solutions([(s, 2 * n) for s, n in dims], sum(s * n for s, n in dims), 2) > 1
+
+
+def _meet(a, b):
+    """Whether a and b, neither of them empty, share a byte."""
+    ends = [[(1, t.element_size() - 1)] if t.element_size() > 1 else [] for t in (a, b)]
+    back = _dims(b) + ends[1]                                    # counted from b's end
+    total = b.data_ptr() - a.data_ptr() + sum(s * n for s, n in back)
+    terms = {}
+    for s, n in [*_dims(a), *ends[0], *back]:
+        if s:
+            terms[s] = terms.get(s, 0) + n
+    return _solutions(list(terms.items()), total, 1) > 0
+
+
+def _refuse_shared(grads, what):
+    """The error of tensors that cannot be scaled in place, each element once."""
+    for i, t in enumerate(grads):
+        if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)) and t.numel():
+            raise ValueError(f"{what}: tensor {i} is expanded: its elements share memory")
+        if not t.is_contiguous() and _meets_itself(t):
+            raise ValueError(f"{what}: tensor {i} overlaps itself: its elements share memory")
+    spans = sorted(((t.data_ptr(), t.data_ptr() + sum(s * n for s, n in _dims(t)) + t.element_size(), t) for t in grads if t.numel()), key=lambda e: e[:2])
+    open_ = []                                                   # spans that reach behind the start of the next one
+    for start, end, t in spans:
+        open_ = [e for e in open_ if e[0] > start]
+        if any(_meet(o, t) for _, o in open_):
+            raise _lib.DiffputerError(f"{what}: two of the tensors share memory")
+        open_.append((end, t))
+
+
 def _call(grads, kind, limit, what):
     """The norm; `grads` are clipped in place if there is a limit."""
     call = _lib.torch_side().grads
@@ -50,12 +129,10 @@ def _call(grads, kind, limit, what):
     if norm is None:
         _refuse(grads, what)
     if isinstance(norm, int):                                    # tensor number `norm` does not fill one range of memory: copies
-        flat = []
+        if limit is not None:
+            _refuse_shared(grads, what)                          # (of dense tensors only, the library sees it)
         with torch.no_grad():
-            for i, g in enumerate(grads):
-                if limit is not None and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-                    raise ValueError(f"{what}: tensor {i} is expanded: its elements share memory")
-                flat.append(g if i < norm or g.is_contiguous() else g.contiguous())
+            flat = [g if i < norm or g.is_contiguous() else g.contiguous() for i, g in enumerate(grads)]
             norm = call(flat, kind, limit)
             if not isinstance(norm, torch.Tensor):
                 _refuse(grads, what)
@@ -78,8 +155,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, error_if_nonfinit
     their device; nothing waits for the GPU).  The rule of torch.nn.utils.clip_grad_norm_, on gradients instead of
     parameters: `clip_grads([p.grad for p in params if p.grad is not None], 1.0)`.
 
-    float32 and bfloat16 mix freely; every tensor has to own its elements once (an expanded tensor, or two that share
-    memory, are refused).  error_if_nonfinite: wait for the norm, and raise RuntimeError before anything is scaled if it is
+    float32 and bfloat16 mix freely; every tensor has to own its elements once (an expanded tensor, one that overlaps itself, or
+    two that share memory, are refused; views that interleave without a common element are not).  error_if_nonfinite: wait for the norm, and raise RuntimeError before anything is scaled if it is
     NaN or infinite (not inside a graph capture)."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -255,3 +255,20 @@ def test_lazily_negated_tensors(dtype):
     assert abs(float(n) - norm) <= 2.0 ** -23 * norm
     assert lazy.is_neg() and all(torch.equal(a.resolve_neg(), b) for a, b in zip(got, want))
     assert torch.equal(base, -want[0])
+
+
+def test_shared_memory_of_tensors_with_gaps():
+    """Overlaps of tensors that are not dense are refused before anything is scaled; views that interleave are scaled once each."""
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.grads import clip_grads
+    a = torch.randn(300, 8, device=DEV)
+    keep = a.clone()
+    for ts in ([a[:, :3], a[:, :3]], [a[:, :3], a[:, 2:5]], [a[:, :3], a[:, 1:]], [a.view(-1)[16:24], a[:, :2]], [a, a[:, :2]], [a.t()[:3], a[:, 2:]]):
+        with pytest.raises(DiffputerError, match="share memory"):
+            clip_grads(ts, 0.1)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grads([torch.as_strided(a, (3, 2), (1, 1))], 0.1)
+    assert torch.equal(a, keep)
+    check([a[:, ::2], a[:, 1:4:2], a[:, 5::2]], 0.1)
+    a.copy_(keep)
+    check([a[:, :3], a[:, 3:], torch.randn(5, device=DEV)], 0.1)

@@ -58,6 +58,84 @@ def test_grads_refuse():
             clip_grads([g], limit)
 
 
+class _Binding:
+    """Stands for csrc/dp_torch.so on the CPU: what clip_grads hands over, checked as the library checks it."""
+
+    @staticmethod
+    def grads(tensors, kind, limit):
+        for i, t in enumerate(tensors):
+            if not t.is_contiguous():
+                return i
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+        if limit is not None and any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise _lib.DiffputerError("two of the tensors share memory")
+        norm = torch.stack([t.float().square().sum() for t in tensors]).sum().sqrt()
+        if limit is not None:
+            for t in tensors:
+                t.mul_(min(1.0, limit / (float(norm) + 1e-6)))
+        return norm
+
+
+def _strided(base, size, stride, offset=0):
+    return torch.as_strided(base, size, stride, offset)
+
+
+def test_overlaps_of_tensors_with_gaps_are_refused(monkeypatch):
+    """clip_grads refuses tensors that share memory, also where they are not dense and would be scaled as copies."""
+    monkeypatch.setattr(_lib, "torch_side", lambda: _Binding)
+    a, b = torch.arange(1.0, 41).reshape(5, 8), torch.arange(1.0, 41).reshape(5, 8)
+    keep = a.clone()
+    flat = a.view(-1)
+    for ts in ([a[:, :3], a[:, :3]], [a[:, :3], a[:, 2:5]], [a[:, :3], a[:, 1:]], [flat[16:24], a[:, :2]], [a[:, :2], flat[16:24]], [b[:, :2], a[:, 1:4], b[:, 4:], a[:, 3:5]],
+               [a[:, ::2], a[:, 4:5]], [a[::2, ::2], a[2:3]], [a, a[:, :2]], [a.t()[:3], a[:, 2:]], [a[:, 3], a[2]], [a[:, :2], a.view(torch.bfloat16)[:, 3:5]]):
+        with pytest.raises(_lib.DiffputerError, match="share memory"):
+            clip_grads(ts, 1.0)
+        assert torch.equal(a, keep)
+        assert abs(float(grad_norm(ts)) - math.sqrt(sum(float(t.double().square().sum()) for t in ts))) < 1e-3 * float(grad_norm(ts))      # reading twice is fine
+    for t in (_strided(flat, (3, 2), (1, 1)), _strided(flat, (4, 3), (2, 1)), _strided(flat, (3, 5), (4, 2)), _strided(flat, (2, 3, 4), (1, 2, 3)), a[:, :1].expand(5, 4)):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grads([torch.ones(3), t], 1.0)
+        assert torch.equal(a, keep)
+    for ts in ([a[:, :3], a[:, 3:]], [a[:, ::2], a[:, 1::2]], [a[:, :2], a[:, 4:6], a[:, 2:4], a[:, 6:]], [a[::2], a[1::2, :5], a[1::2, 5:]], [a.t()[:3], a.t()[3:]], [flat[:8], a[1:, :2], a[1:, 2:]],
+               [_strided(flat, (2, 3), (3, 2)), flat[10:12]], [a[:, :1], torch.ones(0), a[:, 1:3]], [a[:, :2], a.view(torch.bfloat16)[:, 4:6]]):
+        a.copy_(keep)
+        want = [t.clone() for t in ts]
+        norm = clip_grads(ts, 1.0)
+        for t, w in zip(ts, want):
+            assert torch.allclose(t, w * min(1.0, 1.0 / (float(norm) + 1e-6)), rtol=2e-2 if t.dtype == torch.bfloat16 else 1e-5)
+    a.copy_(keep)
+
+
+def test_overlaps_against_enumeration():
+    """The host's answer against all addresses of small tensors."""
+    import random
+
+    from diffputer_amd import grads
+    r = random.Random(5)
+    base = torch.zeros(4000)
+    seen = [0, 0, 0, 0]
+
+    def some():
+        n = r.randint(1, 4)
+        return _strided(base, [r.randint(1, 4) for _ in range(n)], [r.choice([1, 2, 3, 4, 5, 7, 8, 12, 16, 30, 60]) for _ in range(n)], r.randint(0, 60))
+
+    def places(t):
+        where = torch.zeros(1, dtype=torch.int64)
+        for n, s in zip(t.shape, t.stride()):
+            where = (where[:, None] + torch.arange(n) * s).reshape(-1)
+        return (where + t.storage_offset()).tolist()
+
+    for _ in range(3000):
+        t, u = some(), some()
+        p, q = places(t), places(u)
+        for v, w in ((t, p), (u, q)):
+            assert grads._meets_itself(v) == (len(set(w)) < len(w)), (v.shape, v.stride())
+            seen[len(set(w)) < len(w)] += 1
+        assert grads._meet(t, u) == bool(set(p) & set(q)), (t.shape, t.stride(), t.storage_offset(), u.shape, u.stride(), u.storage_offset())
+        seen[2 + bool(set(p) & set(q))] += 1
+    assert min(seen) > 300
+
+
 def _calls():
     """Every entry point that takes tensors, as a function of one tensor (on the CPU: what is refused is refused before the device)."""
     w = torch.randn(5, 4)
