@@ -200,6 +200,15 @@ def test_m_step_limit_on_the_cpu():
     assert math.isfinite(best)
 
 
+def test_build_takes_its_argument():
+    """build(force=True) is how a rebuild was asked for; it is one of build()'s calls still."""
+    import inspect
+
+    import __graft_entry__ as entry
+    for args in ({}, {"force": True}, {"force": False}):
+        inspect.signature(entry.build).bind(**args)
+
+
 FAKE = 1 << 12                                                     # an aligned address that nothing reads: every call below is refused first
 
 
