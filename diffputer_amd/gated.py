@@ -49,7 +49,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     x [..., K]; w_gate, w_up [N, K]; b_gate, b_up [N] or None each; all of one dtype (float32 or bfloat16) on one CUDA (ROCm)
     device.  act: "silu", "gelu" (g Phi(g), not its tanh approximation) or "none".  Row strides are used as they are (a column range
     of a wider table is not copied); other layouts are copied.  Runs on torch's current stream of x's device; first
-    derivatives only, and by backward passes only (a tensor with a forward-mode tangent is refused); not for tracers
+    derivatives only (autocast does not convert its arguments; GatedLinear does), and by backward passes only (a tensor with a forward-mode tangent is refused); not for tracers
     (torch.jit.trace, make_fx, torch.export), which are refused, while torch.compile breaks its graph here; a backward pass under graph capture is refused while an eager graph of the same leaves, made on another
     stream, is alive.  A row of h depends on its own row of x only."""
     code = _ACTS.get(act)
@@ -61,7 +61,11 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
 
 class GatedLinear(nn.Module):
     """`act(gate(x)) * up(x)` with `gate`, `up` two Linear layers in_features -> out_features: a gated layer for denoisers that
-    `model.Precond` / `model.Model` take as `denoise_fn`.  State-dict keys `gate.weight`, `gate.bias`, `up.weight`, `up.bias`."""
+    `model.Precond` / `model.Model` take as `denoise_fn`.  State-dict keys `gate.weight`, `gate.bias`, `up.weight`, `up.bias`.
+
+    Under autocast it converts as nn.Linear does: to bf16, or to float32 where autocast asks for float16 (the kernels have no
+    float16).  Without autocast x has to be of the parameters' type: `model.Precond` gives its denoiser float32, so a bf16 layer inside
+    it needs a denoiser that casts, or autocast."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, act: str = "silu"):
         super().__init__()
@@ -73,7 +77,11 @@ class GatedLinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.is_cuda:
-            return gated_linear(x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias, act=self.act)
+            args = [x, self.gate.weight, self.up.weight, self.gate.bias, self.up.bias]
+            if torch.is_autocast_enabled("cuda"):
+                to = torch.bfloat16 if torch.get_autocast_dtype("cuda") == torch.bfloat16 else torch.float32
+                args = [t if t is None or t.dtype == torch.float64 else t.to(to) for t in args]
+            return gated_linear(*args, act=self.act)
         g = self.gate(x)
         g = nn.functional.silu(g) if self.act == "silu" else nn.functional.gelu(g) if self.act == "gelu" else g
         return g * self.up(x)

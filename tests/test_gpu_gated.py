@@ -756,3 +756,34 @@ def test_lazily_negated_column():
     lazy = z.conj().imag
     assert lazy.is_neg()
     assert torch.equal(gated_linear(lazy, w, w), gated_linear(-z.imag.clone(), w, w))
+
+
+@pytest.mark.parametrize("act", ["silu", "none"])
+def test_module_under_autocast(act):
+    """GatedLinear converts under autocast as the Linear layers that it has on the CPU do: bf16 there, float32 where autocast asks for
+    float16, which the kernels do not have; gradients arrive in the parameters' own type."""
+    from diffputer_amd.gated import GatedLinear, gated_linear
+    torch.manual_seed(2)
+    layer = GatedLinear(24, 40, act=act).to(DEV)
+    x = torch.randn(50, 24, device=DEV)
+    params = list(layer.parameters())
+    plain = layer(x)
+    low = [t.detach().bfloat16().requires_grad_() for t in (x, layer.gate.weight, layer.up.weight, layer.gate.bias, layer.up.bias)]
+    want = gated_linear(*low, act=act)
+    dh = torch.randn(50, 40, device=DEV).bfloat16()
+    grads = torch.autograd.grad(want, [low[1], low[3], low[2], low[4], low[0]], dh)
+    for given in (x.clone(), x.bfloat16()):
+        given.requires_grad_()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            h = layer(given)
+        assert h.dtype == torch.bfloat16 and torch.equal(h, want)
+        got = torch.autograd.grad(h, [*params, given], dh)
+        assert all(g.dtype == p.dtype and torch.equal(g, w.to(p.dtype)) for g, p, w in zip(got, [*params, given], grads))
+    with torch.autocast("cuda", dtype=torch.float16):
+        assert torch.equal(layer(x), plain) and torch.equal(layer(x.half()), layer(x.half().float()))
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.autocast("cuda", enabled=False):
+        assert torch.equal(layer(x), plain)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert torch.equal(layer(x), plain)
+    with pytest.raises(ValueError, match="float64"), torch.autocast("cuda", dtype=torch.bfloat16):
+        layer(x.double())
