@@ -129,9 +129,29 @@ bool goes_elsewhere(const torch::autograd::Node& node, c10::DeviceIndex device) 
     }
     return false;
 }
-bool capturing(const Tensor& t) {
+// the capture that a stream is part of (a stream that was forked from a captured one is), 0 = none
+unsigned long long capture_of(hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    return hipStreamIsCapturing((hipStream_t)stream_of(t), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) return 0;
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}
+// whether this is captured and one of the node's gradients goes to a node of a stream outside the capture
+bool leaves_capture(const torch::autograd::Node& node, c10::DeviceIndex device) {
+    if (!goes_elsewhere(node, device)) return false;
+    const auto here = c10::hip::getCurrentHIPStream(device);
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(here.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return false;
+    const auto capture = capture_of(here.stream());
+    for (const auto& edge : node.next_edges()) {
+        if (!edge.function) continue;
+        const auto stream = edge.function->stream();
+        if (!stream || stream->id() == here.id()) continue;
+        const hipStream_t other = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *stream).stream();
+        // (the null stream takes part in no capture, and may not be asked during one)
+        if (!capture || !other || stream->device_index() != device || capture_of(other) != capture) return true;
+    }
+    return false;
 }
 
 struct GatedLinear : public torch::autograd::Function<GatedLinear> {
@@ -151,8 +171,8 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
         const auto saved = ctx->get_saved_variables();
         const int64_t act = ctx->saved_data["act"].toInt(), biases = ctx->saved_data["biases"].toInt();
         const auto node = torch::autograd::get_current_node();
-        if (node && capturing(saved[0]) && goes_elsewhere(*node, saved[0].device().index()))
-            throw LibraryError("gated_linear: this backward pass is captured while a graph of its inputs that was made on another stream is alive; drop that graph before the capture");
+        if (node && leaves_capture(*node, saved[0].device().index()))
+            throw LibraryError("gated_linear: this backward pass is captured while a graph of its inputs that was made on a stream outside the capture is alive; drop that graph before the capture");
         const Tensor x = rows_of(saved[0]), &pre = saved[3];
         Tensor wg = saved[1], wu = saved[2];
         weights_of(wg, wu);

@@ -50,8 +50,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     device.  act: "silu", "gelu" (g Phi(g), not its tanh approximation) or "none".  Row strides are used as they are (a column range
     of a wider table is not copied); other layouts are copied.  Runs on torch's current stream of x's device; first
     derivatives only (autocast does not convert its arguments; GatedLinear does), and by backward passes only (a tensor with a forward-mode tangent is refused); not for tracers
-    (torch.jit.trace, make_fx, torch.export), which are refused, while torch.compile breaks its graph here; a backward pass under graph capture is refused while an eager graph of the same leaves, made on another
-    stream, is alive.  A row of h depends on its own row of x only."""
+    (torch.jit.trace, make_fx, torch.export), which are refused, while torch.compile breaks its graph here; a backward pass under graph capture is refused while a graph of the same leaves, made on a stream
+    outside the capture, is alive.  A row of h depends on its own row of x only."""
     code = _ACTS.get(act)
     h = None if code is None else _lib.torch_side().gated_linear(x, w_gate, w_up, b_gate, b_up, code)
     if h is None:

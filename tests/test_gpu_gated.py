@@ -787,3 +787,63 @@ def test_module_under_autocast(act):
         assert torch.equal(layer(x), plain)
     with pytest.raises(ValueError, match="float64"), torch.autocast("cuda", dtype=torch.bfloat16):
         layer(x.double())
+
+
+def test_captured_backward_over_a_forked_stream():
+    """A stream that is forked inside the capture is part of it: gradients may go to a node that was made there."""
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(70, 96, 72, "f32", seed=54)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    side = torch.cuda.Stream()
+
+    def once():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            w = leaves[1] * 2                                       # its node, and the leaf's, belong to the side stream
+        main.wait_stream(side)
+        h = gated_linear(leaves[0], w, *leaves[2:])
+        return [h.detach(), *torch.autograd.grad(h, leaves, dh)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = [t.clone() for t in once()]
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = once()
+    for _ in range(4):
+        for t in out:
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        torch.randn(1 << 16, device=DEV).sum()
+
+
+def test_capture_beside_a_graph_of_a_side_stream_is_refused():
+    """The same with a living graph of the leaves on a stream that is no part of the capture; the process goes on."""
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(70, 96, 72, "bf16", seed=55)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        eager = gated_linear(*leaves)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="drop that graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+    with torch.cuda.stream(s):
+        want = torch.autograd.grad(eager, leaves, dh)
+    torch.cuda.synchronize()
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(gated_linear(*leaves), leaves, dh)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
