@@ -847,3 +847,72 @@ def test_capture_beside_a_graph_of_a_side_stream_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_threads_every_result(dtype):
+    """Two threads on streams of their own: h and every gradient of every call, with sizes that are copied to aligned rows, split into
+    slices and joined, and small ones, so that workspaces of both threads are written at the same time."""
+    import threading
+
+    from diffputer_amd.gated import gated_linear
+    sizes = [[(300, 513, 520), (200, 4096, 96), (40, 72, 33)], [(600, 1032, 264), (310, 511, 500), (129, 64, 65)]]
+    sets = [[[t.to(DEV) for t in make(*z, dtype, seed=70 + 10 * i + j)] for j, z in enumerate(s)] for i, s in enumerate(sizes)]
+
+    def once(s):
+        leaves = [t.detach().requires_grad_() for t in s[:5]]
+        h = gated_linear(*leaves)
+        return [h.detach(), *torch.autograd.grad(h, leaves, s[5])]
+
+    want = [[once(s) for s in per] for per in sets]
+    torch.cuda.synchronize()
+    wrong, errors = [None, None], []
+    together = threading.Barrier(2)
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                bad = torch.zeros((), dtype=torch.int64, device=DEV)
+                together.wait(60)
+                for _ in range(40):
+                    for s, w in zip(sets[i], want[i]):
+                        for a, b in zip(once(s), w):
+                            bad += (a != b).sum()
+                wrong[i] = int(bad)
+        except Exception as e:                                      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert wrong == [0, 0]
+
+
+def test_float32_offsets_past_32_bits():
+    """More than 2^31 elements of h in float32, and planes of 9 GB between the backward pass's products: the last rows against the
+    formula, and weight gradients that only they contribute to."""
+    from diffputer_amd.gated import gated_linear
+    M, K, N, tail = 2_100_000, 16, 1032, 70
+    x, wg, wu, bg, bu, dh = make(tail, K, N, "f32", seed=24)
+    ref = Ref(x, wg, wu, bg, bu, dh, "silu")
+    big = torch.full((M, K), 0.5, device=DEV)
+    big[-tail:] = x.to(DEV)
+    leaves = [big.requires_grad_(), *[t.to(DEV).requires_grad_() for t in (wg, wu, bg, bu)]]
+    h = gated_linear(*leaves)
+    assert h.numel() > 1 << 31
+    close(h[-tail:], ref.h, ref.eh, "h")
+    assert torch.equal(h[:1000], h[:1].expand(1000, N)) and torch.equal(h[M // 2:M // 2 + 1000], h[:1].expand(1000, N))
+    d = torch.zeros((M, N), device=DEV)
+    d[-tail:] = dh.to(DEV)
+    grads = torch.autograd.grad(h, leaves, d)
+    close(grads[0][-tail:], ref.dx, ref.edx, "dx")
+    assert not grads[0][:-tail].any()
+    for name, g in zip(("wg", "wu", "bg", "bu"), grads[1:]):
+        # sums of M terms, all but `tail` of them zero: the bound counts additions, of zeros too
+        more = gamma(M) / gamma(tail)
+        close(g, getattr(ref, "d" + name), more * getattr(ref, "ed" + name), "d" + name)
+    del h, d, grads, big, leaves
+    torch.cuda.empty_cache()
