@@ -332,6 +332,11 @@ static int gl_both(const GlArgs a[2], const GlShape s[2], const GlPlan c[2], con
 // 4-byte loads of rows that start anywhere, 540 with copies).  Smaller products run on the general kernel in bf16, and with 4-byte
 // loads in float32.  The kernel for few rows takes rows of any alignment.
 static bool gt_direct(const void* p, int64_t ld, int64_t cols, int chunk) { return aligned(p, 16) && ld % chunk == 0 && cols % chunk == 0; }
+// Backward passes of bf16 layers below this M N keep dg and du in float32 (general kernel, bf16 hi + lo).  Rounded, their roundings
+// come into each gradient once per term: its error against float64 is 1.35 to 1.6 times that of gradients rounded only at the end, at
+// 1 row as at 16384; unrounded 1.00.  What that costs, general / tile kernel in us (M x K x N): 64 x 1024 x 64 11.4 / 9.3,
+// 16 x 1024 x 256 17.9 / 11.6, 1 x 1024 x 8000 49 / 32, 8 x 4096 x 1000 32 / 23; with K in the thousands beside M or N in the thousands
+// it costs more (1 x 16384 x 8000 652 / 314).  In larger layers it would be the second product's whole time: those are rounded.
 constexpr int64_t GL_EXACT_BELOW = 8192;                         // M N
 constexpr int64_t GT_PACK_LEAST = (int64_t)1 << 26;              // M N K
 constexpr int64_t GT_MAX_LD = 1 << 21;                           // 128 rows of float32 stay within 2^30 bytes
@@ -433,7 +438,7 @@ static GlBwd gl_bwd_carve(int dtype, GlIn& in, int planes, bool want_dx, void* b
     const int64_t M = in.M;
     const int N = in.N, K = in.K;
     GlBwd w;
-    // small layers take the general kernel, whose dg and du are not rounded: with few of them their roundings do not average out
+    // small layers take the general kernel, whose dg and du are not rounded
     if (dtype == DP_DTYPE_BF16 && M * N < GL_EXACT_BELOW && in.tune.kernel == 0) in.o.tile = in.o.pack_x = in.o.pack_w = false;
     w.s[0] = {GL_DX, M, K, N, 1, in.tune};
     w.s[1] = {GL_DW, N, K, M, planes ? planes : 2, in.tune};

@@ -103,7 +103,7 @@ struct GlArgs {
     int J;                     // columns of C (of one plane)
     int64_t C;                 // contraction length of one segment
     int kt_per, splits;        // K-tiles per slice, slices
-    int zfirst;                // GL_DW: first plane of this launch (planes = gridDim.z / splits)
+    int zfirst;                // GL_DW: first plane of this launch (0, or 1 where only the up weight's gradient is asked for)
     // outputs
     void* out[2];              // GL_FWD: h in out[0]; GL_DX: dx; GL_DW: dWg, dWu
     int64_t ldo;
@@ -158,7 +158,8 @@ template <typename T> __device__ __forceinline__ void gl_bias(const GlArgs& p, i
 //             in the order 0 4 1 5 2 6 3 7: a lane of the tile kernels has groups q and q + 4 and stores both at once (with 16 bytes
 //             per row and store the forward product of 4096 x 1024 x 2048 wrote 69 MB to memory, for 59 of results).
 // Half a step of 20 bits is 2^-12: dg = dh u act'(g) is off by a sixteenth of the rounding to bf16 that it gets as an operand
-// anyway, and neither range nor inf and NaN are lost, as they would be in 16 bits of either kind.  Against float32 planes the
+// anyway, and neither float32's exponents nor inf and NaN are lost, as they would be in 16 bits of either kind (numbers within 2^-13
+// of float32's largest become inf).  Against float32 planes the
 // forward pass writes and the backward pass reads 20 instead of 32 bytes per group.
 template <typename T> struct GlPre;
 template <> struct GlPre<float> {
@@ -257,8 +258,8 @@ template <typename T> __device__ __forceinline__ void gl_fwd_store(const GlArgs&
 // 64 x 64 x 32 tile, 4 waves of 32 x 32, operands through registers into LDS as [row][k] (element loads with bounds checks).
 // GL_FWD: columns 0..31 of the tile are 32 gate columns, 32..63 the up columns of the same places, so that one lane ends
 // with g and u of the same elements.
-// TA: type of A.  bf16 layers' dg and du are float32 here and multiplied as bf16 hi + lo, two products: small layers, where
-// one product or two is the same time, then have no rounding between the gradient of h and the sums.
+// TA: type of A.  bf16 layers' dg and du are float32 here and multiplied as bf16 hi + lo, two products, so that there is no rounding
+// between the gradient of h and the sums.
 constexpr int GG_T = 64, GG_K = 32;
 struct GgArgs {
     GlArgs g;

@@ -1,8 +1,9 @@
-// bf16 products of the gated projection with fewer than 256 tiles of 256 x 256 (dp_gated.h has the three products and their
-// operands): 128 x 128 tile, 4 waves of 64 x 64, K-steps of 32 in a ring of five LDS slots, two workgroups per CU.
+// bf16 products of the gated projection in 128 x 128 tiles (dp_gated.h has the three products and their operands): 4 waves of
+// 64 x 64, K-steps of 32 in a ring of five LDS slots, two workgroups per CU.
 //
-// Such launches give a CU one or two workgroups and are bound by the latency of a K-step, not by the matrix pipes: nothing of a
-// step waits for itself.  While a step's products run, the fragments of the next one are read into a second set of registers
+// Made for products with fewer than 256 tiles of 256 x 256, and taken wherever the host's estimate says it is faster (whole rounds
+// of 256 tiles that end badly, layers narrower than such a tile).  With one or two workgroups on a CU it is bound by the latency of a
+// K-step, not by the matrix pipes: nothing of a step waits for itself.  While a step's products run, the fragments of the next one are read into a second set of registers
 // and the loads of the step five ahead go out, interleaved with the products; the only waits are one per step, for loads
 // that went out four steps before and for reads whose latency the products have covered, and one barrier.  64 k's take 0.46 us
 // with one workgroup on a CU in four (the four-phase schedule of the 256 x 256 kernel at this tile: 0.92), 0.55 with one on

@@ -293,12 +293,14 @@ int dp_noise_field(float* out, int64_t n_rows, int d_in, uint64_t seed, uint64_t
  * each other; memory outside [M, N] of h is not written.  Deterministic, asynchronous on `stream`, allocates nothing
  * (workspace >= dp_gated_linear_workspace_bytes(.., grads) for the same arguments, grads = DP_GATED_FORWARD, or the DP_GATED_D.. that dp_gated_linear_bwd is asked for, 256-byte aligned; calls that may
  * overlap in time need workspaces of their own), and may be captured into a graph.  bf16 is fastest where x and the weights
- * have rows that start on 16 bytes and K % 8 == 0: other rows are first copied to the workspace.
+ * have rows that start on 16 bytes, are at most 2^21 elements apart, and K % 8 == 0.  Other rows are copied to the workspace first
+ * where M N K >= 2^26, and run on the general kernel below that; the kernel for few rows (at most 64, by size) takes any rows.
  *
  * dp_gated_linear_bwd: gradients for a given dh [M, N] (row stride lddh).  dx [M, K], dw_gate, dw_up [N, K], db_gate,
  * db_up [N]: contiguous, overwritten, each may be NULL (not wanted).  M = 0 writes zeros to the weights' gradients.
- * bf16: dg and du are rounded to bf16 once, as the operands of the three products (not in small layers, M N < 8192); bias
- * gradients sum them unrounded.
+ * bf16: dg and du are rounded to bf16 once, as the operands of the three products, except where the general kernel runs: layers with
+ * M N < 8192, and layers whose x or weights are not laid out as above with M N K < 2^26.  Rounded, the gradients' error is
+ * about 1.4 times that of gradients that are rounded only at the end.  Bias gradients sum dg and du unrounded.
  */
 #define DP_GATED_FORWARD 0
 #define DP_GATED_DX      1
