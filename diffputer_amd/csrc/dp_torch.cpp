@@ -249,8 +249,11 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
             grad = grad || t->requires_grad();
         }
         if (x.layout() != at::kStrided) Py_RETURN_NONE;
-        for (const Tensor& t : b)
-            if (t.defined() && (t.dim() != 1 || t.size(0) != N)) Py_RETURN_NONE;
+        for (const Tensor& t : b) {
+            if (!t.defined()) continue;
+            if (t.dim() != 1 || t.size(0) != N) Py_RETURN_NONE;
+            if (!t.data_ptr()) throw LibraryError("gated_linear: a bias has no memory of its own (a wrapper of other tensors?)");     // a null pointer is no bias
+        }
         const bool flat = x.dim() == 2;
         int64_t M = 1;
         for (int64_t d = 0; d + 1 < x.dim(); ++d) M *= x.size(d);

@@ -916,3 +916,26 @@ def test_float32_offsets_past_32_bits():
         close(g, getattr(ref, "d" + name), more * getattr(ref, "ed" + name), "d" + name)
     del h, d, grads, big, leaves
     torch.cuda.empty_cache()
+
+
+def test_bias_without_memory_is_refused():
+    """A tensor that stands for others and has no memory of its own (a wrapper subclass) is no absent bias."""
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.gated import gated_linear
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError(func)
+
+    x, w, b = torch.randn(3, 8, device=DEV), torch.randn(16, 8, device=DEV), torch.randn(16, device=DEV)
+    for i in range(5):
+        args = [x, w, w, b, b]
+        args[i] = Wrapper(args[i])
+        with pytest.raises((DiffputerError, RuntimeError), match="memory|null pointer"):
+            gated_linear(*args)
+    assert torch.isfinite(gated_linear(x, w, w, b, b)).all()
