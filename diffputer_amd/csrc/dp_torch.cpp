@@ -133,7 +133,10 @@ bool goes_elsewhere(const torch::autograd::Node& node, c10::DeviceIndex device) 
 unsigned long long capture_of(hipStream_t stream) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     unsigned long long id = 0;
-    if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) return 0;
+    if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();                                 // which the next launch would report as its own
+        return 0;
+    }
     return status == hipStreamCaptureStatusActive ? id : 0;
 }
 // whether this is captured and one of the node's gradients goes to a node of a stream outside the capture
