@@ -173,6 +173,8 @@ struct GatedLinear : public torch::autograd::Function<GatedLinear> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const int64_t act = ctx->saved_data["act"].toInt(), biases = ctx->saved_data["biases"].toInt();
+        refuse_trace("gated_linear's backward pass");
+        for (const Tensor* t : {&saved[0], &saved[1], &saved[2], (const Tensor*)&grads[0]}) refuse_tangent(*t, "gated_linear's backward pass");
         const auto node = torch::autograd::get_current_node();
         if (node && leaves_capture(*node, saved[0].device().index()))
             throw LibraryError("gated_linear: this backward pass is captured while a graph of its inputs that was made on a stream outside the capture is alive; drop that graph before the capture");

@@ -939,3 +939,23 @@ def test_bias_without_memory_is_refused():
         with pytest.raises((DiffputerError, RuntimeError), match="memory|null pointer"):
             gated_linear(*args)
     assert torch.isfinite(gated_linear(x, w, w, b, b)).all()
+
+
+def test_backward_loses_no_tangent_and_no_trace():
+    """A gradient that comes in with a tangent, or under a tracer, is refused as the forward call's arguments are."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from diffputer_amd._lib import DiffputerError
+    from diffputer_amd.gated import gated_linear
+    x, wg, wu, bg, bu, dh = [t.to(DEV) for t in make(9, 16, 8, "f32", seed=58)]
+    leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
+    h = gated_linear(*leaves)
+    want = torch.autograd.grad(h, leaves, dh, retain_graph=True)
+    with forward_ad.dual_level():
+        with pytest.raises((DiffputerError, RuntimeError), match="forward-mode"):
+            torch.autograd.grad(h, leaves, forward_ad.make_dual(dh, torch.ones_like(dh)), retain_graph=True)
+    with pytest.raises((DiffputerError, RuntimeError), match="traced"):
+        make_fx(lambda d: torch.autograd.grad(h, leaves, d, retain_graph=True))(dh)
+    got = torch.autograd.grad(h, leaves, dh)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
