@@ -5,8 +5,8 @@
 //
 // Two passes over memory: k_grad_norm leaves one partial per workgroup, k_grad_clip reduces the partials (each workgroup
 // for itself, in one fixed order: same bits everywhere) and scales.  Bound by memory, in small sets by the two launches: 0.8 GB of float32
-// within the limit 135 us (5.9 TB/s), 2^27 bf16 numbers in 301 tensors clipped in 158 us (0.27 GB read, then read and written:
-// 5.1 TB/s), 42 MB in 14 tensors in 25.6 us, 0.3 MB in 10.  Sums are float64; squares are added up in float32 within pairs
+// within the limit 135 us (5.9 TB/s), 2^27 bf16 numbers in 301 tensors clipped in 156 to 170 us on three cards (0.27 GB read,
+// then read and written: 4.7 to 5.1 TB/s), 42 MB in 14 tensors in 25.6 us, 0.3 MB in 10.  Sums are float64; squares are added up in float32 within pairs
 // (float32) or fours (bf16, whose squares are exact), two roundings at most, and only those go to float64: one conversion per
 // element held the kernel to 1.25 elements per ps, 2.5 TB/s in bf16.  A group outside [2^-96, inf) takes the long way, element
 // by element in float64: no square overflows or vanishes.

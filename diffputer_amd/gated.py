@@ -1,7 +1,8 @@
 """Gated projection on the HIP kernels: `h = act(x Wg^T + bg) * (x Wu^T + bu)` (`dp_gated_linear`, include/diffputer.h).
 
 The gated counterpart of `sampler.linear` (act(A W^T + bias)) and of the Linear + SiLU pairs of `model.MLPDiffusion`, for
-denoisers built from gated layers: both products, the activation and the gating are one kernel, few rows (a request of one)
+denoisers built from gated layers, which train inside `model.Model` (`em.m_step`, `em.run_em` and the sampler's plans run MLPDiffusion
+only): both products, the activation and the gating are one kernel, few rows (a request of one)
 have a form of their own, and autograd gets the gradients of x, both weights and both biases from `dp_gated_linear_bwd`.
 
 float32 or bfloat16 throughout; sums, the saved projections and the bias gradients' sums are float32.  There is no CPU
