@@ -134,6 +134,43 @@ def test_overlaps_against_enumeration():
         assert grads._meet(t, u) == bool(set(p) & set(q)), (t.shape, t.stride(), t.storage_offset(), u.shape, u.stride(), u.storage_offset())
         seen[2 + bool(set(p) & set(q))] += 1
     assert min(seen) > 300
+    for _ in range(1500):
+        pitch = r.choice([6, 8, 15])
+        ts = [_strided(base, (r.randint(2, 4), r.randint(1, 3)), (pitch, r.choice([1, 2])), r.randint(0, 20)) for _ in range(r.randint(2, 5))]
+        if any(grads._meets_itself(t) for t in ts):
+            continue
+        all_ = [x for t in ts for x in places(t)]
+        try:
+            grads._refuse_shared(ts, "x")
+            assert len(set(all_)) == len(all_)
+        except _lib.DiffputerError:
+            assert len(set(all_)) < len(all_)
+
+
+def test_many_views_of_one_table(monkeypatch):
+    """Column ranges of one table are told apart without a look at every pair; one that meets another is found."""
+    from diffputer_amd import grads
+    pairs, meet = [], grads._meet
+    monkeypatch.setattr(grads, "_meet", lambda o, t: pairs.append(1) or meet(o, t))
+    a = torch.zeros(40, 1200)
+    views = [a[:, 3 * i:3 * i + 3] for i in range(400)]
+    rows = [a[i::7, ::2] for i in range(7)] + [a[i::7, 1::2] for i in range(7)]
+    grads._refuse_shared(views, "x")
+    grads._refuse_shared(views[::-1] + [torch.zeros(3, 4)[:, :2]], "x")
+    assert not pairs
+    grads._refuse_shared(rows, "x")
+    assert pairs
+    for more in (a[5:9, 1100:1102], a[::2, 7:8], a.view(-1)[17:18], a[:, 1199:]):
+        with pytest.raises(_lib.DiffputerError, match="share memory"):
+            grads._refuse_shared([*views, more], "x")
+    # a range that wraps round the end of the table's row, beside one that it meets and one that it does not
+    flat = a.view(-1)
+    wrap = _strided(flat, (39, 4), (1200, 1), 1198)
+    grads._refuse_shared([wrap, a[:, 2:1198]], "x")
+    with pytest.raises(_lib.DiffputerError, match="share memory"):
+        grads._refuse_shared([wrap, a[:, 1:5]], "x")
+    with pytest.raises(_lib.DiffputerError, match="share memory"):
+        grads._refuse_shared([wrap, a[:, 1199:]], "x")
 
 
 def _calls():
