@@ -221,7 +221,8 @@ int dp_linear(int dtype, const void* A, const void* W, const float* bias, void* 
  *                   bit-identical results.
  *   "gated_kernel"  which kernel runs the products of dp_gated_linear and its backward: 0 (default) = by size and alignment, 1 = the
  *                   general kernel (any size, stride and type), 64 / 128 / 256 = the tile kernel of that tile
- *                   (bf16 has 128 and 256, float32 64 and 128: the nearest).
+ *                   (bf16 has 128 and 256, float32 64 and 128: the nearest).  1 also keeps bf16 layers' dg and du unrounded in the
+ *                   backward pass, whatever the size.
  *   "gated_splits"  slices of the contraction of those products: 0 (default) = by size, else that many (at most one per K-tile).  The
  *                   order of sums, and with it the last bits, depend on it.
  */
